@@ -414,6 +414,89 @@ int qx_decode_attention_noalloc(const void* q, const void* k_cache, const void* 
                                 int sink, int window, int64_t count, float softmax_scale,
                                 qx_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Head norm and rotation of a prompt chunk (or of one decode position) in one
+ * pass.  qkv fp16 [tokens, q_heads + 2 kv_heads, head_dim] (the fused q|k|v
+ * projection's output); q and k heads are RMSNorm'd over head_dim (fp16
+ * result) and rotated (rotate-half RoPE in fp32, one fp16 rounding); the v
+ * heads are copied.  cos / sin fp32 [rope_rows, head_dim]: token t reads row
+ * t % rope_rows, rope_rows dividing tokens (tokens = batch x chunk in that
+ * order: rope_rows = chunk for one set of positions, = tokens for each
+ * sequence's own).  q_out [tokens, q_heads, head_dim], k_out and v_out
+ * [tokens, kv_heads, head_dim].  head_dim in {64, 128, 256}; every tensor
+ * 16-byte aligned; outputs must not overlap inputs.  Bit-identical to
+ * qx_fused_rmsnorm over the heads followed by fp32 x cos + rot(x) sin.  New
+ * component (the reference runs these as separate torch ops).
+ * ---------------------------------------------------------------------- */
+int qx_qk_norm_rope(const void* qkv, int64_t tokens, int q_heads, int kv_heads, int head_dim,
+                    const void* q_norm_w, const void* k_norm_w, float eps, const float* cos,
+                    const float* sin, int64_t rope_rows, void* q_out, void* k_out, void* v_out,
+                    qx_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * The StreamingLLM ring held in 4 bits.  New component (the reference's ring
+ * holds fp16); slot rules, counts and masks are those of the fp16 ring above.
+ *
+ * Storage of a layer, keys and values each:
+ *   codes  uint8  [batch, kv_heads, slots, head_dim / 2]
+ *   params uint16 [batch, kv_heads, slots, head_dim / group]
+ * with slots = qx_ring_q4_slots(sink, window) (sink + window rounded up to
+ * 64) and group in {32, 64, 128}, at most head_dim, in {64, 128}.  A group of
+ * consecutive head dimensions stands for s (c - z), c its 4-bit codes; its
+ * param is the fp16 s, of 7 significant bits, with z (0..15) in the four low
+ * bits.  s (c - z) is a fp16 number exactly.  The order of the codes within a
+ * row is private to the library; all entry points agree on it.
+ * Quantisation: s = the smallest such number >= (max(x, 0) - min(x, 0)) / 15,
+ * z = rint(-min(x, 0) / s), c = rint(x / s) + z: |x - s (c - z)| <= s / 2 (at
+ * most s where the value would pass 65504).  A group that holds a NaN or an
+ * infinity reads as NaN.  Slots past the valid ones may hold anything.
+ *
+ * count / counts: tokens written before this call; counts = NULL: `count` for
+ * every sequence, else int64 [batch] in device memory, each sequence's own
+ * (>= 0, below 2^62; read when the kernel runs, so a captured graph follows it).
+ * Every tensor 16-byte aligned.
+ * ---------------------------------------------------------------------- */
+int64_t qx_ring_q4_slots(int sink, int window);
+
+/* Quantises new_k, new_v fp16 [batch, tokens, kv_heads, head_dim] into the
+ * slots of positions count .. count + tokens - 1, later tokens winning a
+ * slot; other slots are left as they were. */
+int qx_ring_append_q4(void* k_codes, void* k_params, void* v_codes, void* v_params, const void* new_k,
+                      const void* new_v, int batch, int tokens, int kv_heads, int head_dim, int group,
+                      int sink, int window, int64_t count, const int64_t* counts, qx_stream_t stream);
+
+/* K and V in logical order as fp16 [batch, valid_length(count), kv_heads, head_dim]
+ * (qx_ring_gather's order): the values the attention multiplies, exactly. */
+int qx_ring_gather_q4(const void* k_codes, const void* k_params, const void* v_codes,
+                      const void* v_params, void* k_out, void* v_out, int batch, int kv_heads,
+                      int head_dim, int group, int sink, int window, int64_t count, qx_stream_t stream);
+
+/* qx_decode_attention over the 4-bit ring: q, out fp16 [batch, q_heads,
+ * head_dim], count including the current token, q_heads / kv_heads <= 16.  A
+ * sequence without tokens gets zeros.  Workspace: the matching size function's
+ * bytes (0 for some shapes: NULL then), 16-byte aligned, no initialisation,
+ * not shared by calls that may overlap. */
+size_t qx_decode_attention_q4_workspace_size(int batch, int q_heads, int kv_heads, int head_dim, int sink,
+                                             int window);
+int qx_decode_attention_q4(const void* q, const void* k_codes, const void* k_params, const void* v_codes,
+                           const void* v_params, void* out, int batch, int q_heads, int kv_heads,
+                           int head_dim, int group, int sink, int window, int64_t count,
+                           const int64_t* counts, float softmax_scale, void* workspace,
+                           size_t workspace_bytes, qx_stream_t stream);
+
+/* qx_prefill_attention over the 4-bit ring: q, out fp16 [batch, n, q_heads,
+ * head_dim], k_new / v_new fp16 [batch, n, kv_heads, head_dim] (attended as
+ * given, appended by the caller afterwards), the ring after count tokens,
+ * q_heads / kv_heads <= 16.  Keys hidden from a query do not reach its row,
+ * whatever they hold.  Workspace as above. */
+size_t qx_prefill_attention_q4_workspace_size(int batch, int n, int q_heads, int kv_heads, int head_dim,
+                                              int sink, int window);
+int qx_prefill_attention_q4(const void* q, const void* k_new, const void* v_new, const void* k_codes,
+                            const void* k_params, const void* v_codes, const void* v_params, void* out,
+                            int batch, int n, int q_heads, int kv_heads, int head_dim, int group, int sink,
+                            int window, int64_t count, const int64_t* counts, float softmax_scale,
+                            void* workspace, size_t workspace_bytes, qx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,7 +29,9 @@ import torch
 from . import _lib, _workspace
 
 __all__ = ["fused_rmsnorm", "fused_swiglu", "w4a16_gemv", "w4a16_lora_gemv",
-           "RingBufferKVCache", "decode_attention", "ring_slot_indices"]
+           "RingBufferKVCache", "decode_attention", "ring_slot_indices", "qk_norm_rope",
+           "RingBufferKVCacheQ4", "ring_q4_storage", "ring_append_q4", "ring_gather_q4",
+           "decode_attention_q4", "prefill_attention_q4"]
 
 _LIB = _lib.load()  # fail at import time if the native library is absent
 _SUPPORTED_RANKS = (8, 16, 32, 48, 64, 128)
@@ -585,6 +587,192 @@ def prefill_attention(q, k_new, v_new, k_cache, v_cache, count: int, sink: int, 
     return out
 
 
+# ------------------------------------------- head norm + rotation, 4-bit ring --
+def _launch(dev: torch.device, what: str, fn, *args):
+    """``fn(*args, stream)`` on the current stream of ``dev``."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc < 0:
+        _lib.check(rc, what)
+
+
+def _same_device(what: str, *tensors):
+    dev = tensors[0].device
+    if any(t.device != dev for t in tensors):
+        raise RuntimeError(f"{what}: tensors must be on one device")
+    return dev
+
+
+def qk_norm_rope(qkv: torch.Tensor, q_heads: int, kv_heads: int, q_norm: torch.Tensor, k_norm: torch.Tensor,
+                 eps: float, cos: torch.Tensor, sin: torch.Tensor):
+    """Head norm and rotation of a chunk in one pass: ``qkv`` fp16 ``[B, T,
+    (q_heads + 2 kv_heads) D]`` (the fused projection's output), ``cos`` / ``sin``
+    fp32 ``[T, D]`` (the chunk's positions) or ``[B, T, D]`` (each sequence's
+    own).  Returns q ``[B, T, q_heads, D]`` and k ``[B, T, kv_heads, D]``, RMSNorm'd
+    over D and rotated, and v ``[B, T, kv_heads, D]``.  Bit-identical to
+    ``fused_rmsnorm`` over the heads followed by rotate-half RoPE in fp32 (new
+    component: the reference runs them as separate torch ops)."""
+    for t, n in ((qkv, "qkv"), (q_norm, "q_norm"), (k_norm, "k_norm")):
+        _check_input(t, n)
+        _check_fp16(t, n)
+    D = q_norm.numel()
+    if q_heads < 1 or kv_heads < 1 or qkv.dim() != 3 or k_norm.numel() != D or \
+            qkv.size(2) != (q_heads + 2 * kv_heads) * D:
+        raise RuntimeError("qk_norm_rope: qkv must be [B, T, (q_heads + 2 kv_heads) * head_dim]")
+    B, T = qkv.size(0), qkv.size(1)
+    for t, n in ((cos, "cos"), (sin, "sin")):
+        _check_input(t, n)
+        if t.dtype != torch.float32 or tuple(t.shape) not in ((T, D), (B, T, D)) or t.shape != cos.shape:
+            raise RuntimeError(f"{n} must be float32 [{T}, {D}] or [{B}, {T}, {D}]")
+    dev = _same_device("qk_norm_rope", qkv, q_norm, k_norm, cos, sin)
+    q = torch.empty(B, T, q_heads, D, dtype=torch.float16, device=dev)
+    k = torch.empty(B, T, kv_heads, D, dtype=torch.float16, device=dev)
+    v = torch.empty_like(k)
+    _launch(dev, "qk_norm_rope", _LIB.qx_qk_norm_rope, qkv.data_ptr(), B * T, q_heads, kv_heads, D,
+            q_norm.data_ptr(), k_norm.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(),
+            max(1, cos.numel() // D), q.data_ptr(), k.data_ptr(), v.data_ptr())
+    return q, k, v
+
+
+def ring_q4_slots(sink: int, window: int) -> int:
+    """Slots of a 4-bit ring's storage: ``sink + window`` rounded up to 64."""
+    return _lib.check(_LIB.qx_ring_q4_slots(int(sink), int(window)), "ring_q4_slots")
+
+
+def ring_q4_storage(batch: int, kv_heads: int, head_dim: int, sink: int, window: int, group_size: int = 64,
+                    device="cuda"):
+    """Zeroed storage of one layer's 4-bit ring: ``codes`` uint8 ``[2, B, Hkv,
+    slots, D / 2]`` and ``params`` int16 ``[2, B, Hkv, slots, D / group_size]``
+    (0: keys, 1: values), the form every ``*_q4`` op takes."""
+    if head_dim not in (64, 128) or group_size not in (32, 64, 128) or group_size > head_dim:
+        raise RuntimeError("ring_q4_storage: head_dim must be 64 or 128, group_size 32, 64 or 128 and at most head_dim")
+    shape = (2, batch, kv_heads, ring_q4_slots(sink, window))
+    return (torch.zeros(*shape, head_dim // 2, dtype=torch.uint8, device=device),
+            torch.zeros(*shape, head_dim // group_size, dtype=torch.int16, device=device))
+
+
+def _ring_q4(what, codes, params, count, sink, window, *others):
+    """Checks a layer's 4-bit ring and returns (device, B, Hkv, D, group, the four
+    storage pointers, the count arguments)."""
+    for t, n, dt in ((codes, "codes", torch.uint8), (params, "params", torch.int16)):
+        _check_input(t, n)
+        if t.dtype != dt or t.dim() != 5 or t.size(0) != 2:
+            raise RuntimeError(f"{what}: codes must be uint8 [2, B, Hkv, slots, D / 2] and params int16 "
+                               "[2, B, Hkv, slots, D / group]")
+    _, B, Hkv, slots, half = codes.shape
+    if params.shape[:4] != codes.shape[:4] or slots != ring_q4_slots(sink, window):
+        raise RuntimeError(f"{what}: codes and params must have {ring_q4_slots(sink, window)} slots "
+                           f"(sink + window rounded up to 64), got {list(codes.shape)} and {list(params.shape)}")
+    D, groups = 2 * half, params.size(4)
+    if groups < 1 or D % groups:
+        raise RuntimeError(f"{what}: {groups} groups do not divide head_dim {D}")
+    if isinstance(count, torch.Tensor):
+        _check_input(count, "count")
+        if count.dtype != torch.int64 or tuple(count.shape) != (B,):
+            raise RuntimeError(f"{what}: a count tensor must be int64 [{B}]")
+        others += (count,)
+        counts = (0, count.data_ptr())
+    else:
+        counts = (int(count), None)
+    for t in others:
+        _check_input(t, f"{what}: every tensor")
+    dev = _same_device(what, codes, params, *others)
+    kc, kp = codes.data_ptr(), params.data_ptr()
+    ptrs = (kc, kp, kc + codes.numel() // 2, kp + params.numel())  # int16: half the elements are numel bytes
+    return dev, B, Hkv, D, D // groups, ptrs, counts
+
+
+def _check_new_kv(what, new_k, new_v, B, Hkv, D, tokens=None):
+    for t, n in ((new_k, "new_k"), (new_v, "new_v")):
+        _check_input(t, n)
+        _check_fp16(t, n)
+    if new_k.dim() != 4 or new_k.shape != new_v.shape or new_k.size(0) != B or \
+            tuple(new_k.shape[2:]) != (Hkv, D) or (tokens is not None and new_k.size(1) != tokens):
+        raise RuntimeError(f"{what}: new keys and values must be [{B}, {'T' if tokens is None else tokens}, {Hkv}, {D}], "
+                           f"got {list(new_k.shape)} and {list(new_v.shape)}")
+
+
+def ring_append_q4(new_k: torch.Tensor, new_v: torch.Tensor, codes: torch.Tensor, params: torch.Tensor,
+                   count: int | torch.Tensor, sink: int, window: int) -> None:
+    """Quantises ``new_k`` / ``new_v`` fp16 ``[B, T, Hkv, D]`` to 4 bits into the
+    ring slots of positions ``count ..`` (in place; later tokens win a slot).
+    ``count``: tokens written before, for all sequences or int64 ``[B]`` on the
+    device, each sequence's own."""
+    dev, B, Hkv, D, group, ptrs, counts = _ring_q4("ring_append_q4", codes, params, count, sink, window, new_k, new_v)
+    _check_new_kv("ring_append_q4", new_k, new_v, B, Hkv, D)
+    _launch(dev, "ring_append_q4", _LIB.qx_ring_append_q4, *ptrs, new_k.data_ptr(), new_v.data_ptr(), B,
+            new_k.size(1), Hkv, D, group, sink, window, *counts)
+
+
+def ring_gather_q4(codes: torch.Tensor, params: torch.Tensor, count: int, sink: int, window: int):
+    """(K, V) of a 4-bit ring in logical order, fp16 ``[B, valid, Hkv, D]``: the
+    values the attention multiplies, exactly."""
+    if isinstance(count, torch.Tensor):
+        raise RuntimeError("ring_gather_q4: count must be a number (it gives the output's length)")
+    dev, B, Hkv, D, group, ptrs, (n, _) = _ring_q4("ring_gather_q4", codes, params, count, sink, window)
+    valid = min(n, sink) + max(0, min(n - sink, window))
+    k = torch.empty(B, max(valid, 0), Hkv, D, dtype=torch.float16, device=dev)
+    v = torch.empty_like(k)
+    _launch(dev, "ring_gather_q4", _LIB.qx_ring_gather_q4, *ptrs, k.data_ptr(), v.data_ptr(), B, Hkv, D, group, sink,
+            window, n)
+    return k, v
+
+
+def _scratch(dev: torch.device, nbytes: int):
+    """Scratch of one call, from torch's allocator: calls on different streams
+    and captured graphs never share it."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def decode_attention_q4(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, count: int | torch.Tensor,
+                        sink: int, window: int, softmax_scale: float | None = None) -> torch.Tensor:
+    """``decode_attention`` over a 4-bit ring, read in place: ``q`` fp16 ``[B,
+    Hq, D]``, ``count`` tokens written (the current one included), for all
+    sequences or int64 ``[B]`` on the device; a sequence without tokens gets
+    zeros."""
+    dev, B, Hkv, D, group, ptrs, counts = _ring_q4("decode_attention_q4", codes, params, count, sink, window, q)
+    _check_input(q, "q")
+    _check_fp16(q, "q")
+    if q.dim() != 3 or q.size(0) != B or q.size(2) != D:
+        raise RuntimeError(f"decode_attention_q4: q must be [{B}, Hq, {D}], got {list(q.shape)}")
+    Hq = q.size(1)
+    out = torch.empty_like(q)
+    with torch.cuda.device(dev):
+        need = _LIB.qx_decode_attention_q4_workspace_size(B, Hq, Hkv, D, sink, window)
+        ws = _scratch(dev, need)
+        _launch(dev, "decode_attention_q4", _LIB.qx_decode_attention_q4, q.data_ptr(), *ptrs, out.data_ptr(), B, Hq,
+                Hkv, D, group, sink, window, *counts, float(softmax_scale or 0.0), _ptr(ws), need)
+    return out
+
+
+def prefill_attention_q4(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, codes: torch.Tensor,
+                         params: torch.Tensor, count: int | torch.Tensor, sink: int, window: int,
+                         softmax_scale: float | None = None) -> torch.Tensor:
+    """``prefill_attention`` over a 4-bit ring: a chunk ``q`` fp16 ``[B, n, Hq,
+    D]`` at positions ``count ..`` over the ring's ``count`` tokens and its own
+    ``k_new`` / ``v_new`` fp16 ``[B, n, Hkv, D]`` (attended as given; append them
+    afterwards).  Causal, sinks + the last ``window`` positions visible."""
+    dev, B, Hkv, D, group, ptrs, counts = _ring_q4("prefill_attention_q4", codes, params, count, sink, window, q,
+                                                   k_new, v_new)
+    _check_input(q, "q")
+    _check_fp16(q, "q")
+    if q.dim() != 4 or q.size(0) != B or q.size(3) != D:
+        raise RuntimeError(f"prefill_attention_q4: q must be [{B}, n, Hq, {D}], got {list(q.shape)}")
+    n, Hq = q.size(1), q.size(2)
+    _check_new_kv("prefill_attention_q4", k_new, v_new, B, Hkv, D, n)
+    out = torch.empty_like(q)
+    with torch.cuda.device(dev):
+        need = _LIB.qx_prefill_attention_q4_workspace_size(B, n, Hq, Hkv, D, sink, window)
+        ws = _scratch(dev, need)
+        _launch(dev, "prefill_attention_q4", _LIB.qx_prefill_attention_q4, q.data_ptr(), k_new.data_ptr(),
+                v_new.data_ptr(), *ptrs, out.data_ptr(), B, n, Hq, Hkv, D, group, sink, window, *counts,
+                float(softmax_scale or 0.0), _ptr(ws), need)
+    return out
+
+
 class RingBufferKVCache:
     """StreamingLLM sink + ring-window KV cache (reference:
     ``csrc/include/ring_buffer.h:32-77``, ``csrc/kv_cache/ring_buffer.cu``).
@@ -688,4 +876,77 @@ class RingBufferKVCache:
             q = q.unsqueeze(0)
         out = decode_attention(q, self.k[layer_idx], self.v[layer_idx], self._write_count,
                                self.sink_size, self.window_size, softmax_scale)
+        return out[0] if squeeze else out
+
+
+class RingBufferKVCacheQ4(RingBufferKVCache):
+    """``RingBufferKVCache`` held in 4 bits: same methods and counts, about 0.27
+    of the memory.  Every ``group_size`` (32, 64 or 128) consecutive values of a
+    head share a scale and a zero point (``ring_append_q4``).
+
+    Storage: ``codes`` uint8 ``[num_layers, 2, batch, kv_heads, slots, head_dim / 2]``
+    and ``params`` int16 ``[num_layers, 2, batch, kv_heads, slots, head_dim /
+    group_size]``, ``slots`` = sink + window rounded up to 64.
+    """
+
+    def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, sink_size: int = 4,
+                 window_size: int = 4092, batch: int = 1, device=None, group_size: int = 64):
+        if window_size < 1 or sink_size < 0:
+            raise RuntimeError("sink_size must be >= 0 and window_size >= 1")
+        if head_dim not in (64, 128) or group_size not in (32, 64, 128) or group_size > head_dim:
+            raise RuntimeError("RingBufferKVCacheQ4: head_dim must be 64 or 128, group_size 32, 64 or 128 and at "
+                               "most head_dim")
+        self.num_layers, self.num_kv_heads, self.head_dim = num_layers, num_kv_heads, head_dim
+        self.sink_size, self.window_size = sink_size, window_size
+        self.total_size = sink_size + window_size
+        self.batch, self.group_size = batch, group_size
+        dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        if dev.type != "cuda":
+            raise RuntimeError("RingBufferKVCacheQ4 lives on a CUDA device")
+        self.device = dev
+        shape = (num_layers, 2, batch, num_kv_heads, ring_q4_slots(sink_size, window_size))
+        self.codes = torch.zeros(*shape, head_dim // 2, dtype=torch.uint8, device=dev)
+        self.params = torch.zeros(*shape, head_dim // group_size, dtype=torch.int16, device=dev)
+        self._write_count = 0
+
+    @property
+    def k(self) -> torch.Tensor:
+        """the keys' codes"""
+        return self.codes[:, 0]
+
+    @property
+    def v(self) -> torch.Tensor:
+        """the values' codes"""
+        return self.codes[:, 1]
+
+    def _layer(self, layer_idx: int):
+        if not 0 <= layer_idx < self.num_layers:
+            raise RuntimeError(f"layer_idx {layer_idx} out of range")
+        return self.codes[layer_idx], self.params[layer_idx]
+
+    def append(self, new_k: torch.Tensor, new_v: torch.Tensor, layer_idx: int) -> None:
+        """``new_k``/``new_v``: ``[H, D]`` (one token, batch 1), ``[T, H, D]``
+        (batch 1) or ``[B, T, H, D]``."""
+        codes, params = self._layer(layer_idx)
+        if new_k.dim() not in (2, 3, 4) or new_k.shape != new_v.shape:
+            raise RuntimeError("new_k and new_v must both be [H, D], [T, H, D] or [B, T, H, D]")
+        lead = (1,) * (4 - new_k.dim())
+        new_k, new_v = new_k.reshape(lead + new_k.shape), new_v.reshape(lead + new_v.shape)
+        ring_append_q4(new_k, new_v, codes, params, self._write_count, self.sink_size, self.window_size)
+        if layer_idx == self.num_layers - 1:
+            self._write_count += new_k.size(1)
+
+    def get_kv(self, layer_idx: int):
+        """(K, V) in logical order as fp16: ``[valid, H, D]`` for batch 1, else
+        ``[B, valid, H, D]``."""
+        k, v = ring_gather_q4(*self._layer(layer_idx), self._write_count, self.sink_size, self.window_size)
+        return (k[0], v[0]) if self.batch == 1 else (k, v)
+
+    def decode_attention(self, q: torch.Tensor, layer_idx: int,
+                         softmax_scale: float | None = None) -> torch.Tensor:
+        squeeze = q.dim() == 2
+        if squeeze:
+            q = q.unsqueeze(0)
+        out = decode_attention_q4(q, *self._layer(layer_idx), self._write_count, self.sink_size, self.window_size,
+                                  softmax_scale)
         return out[0] if squeeze else out

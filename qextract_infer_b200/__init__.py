@@ -13,9 +13,16 @@ __version__ = "0.1.0"
 try:
     from ._C import (  # noqa: F401
         RingBufferKVCache,
+        RingBufferKVCacheQ4,
         decode_attention,
+        decode_attention_q4,
         fused_rmsnorm,
         fused_swiglu,
+        prefill_attention_q4,
+        qk_norm_rope,
+        ring_append_q4,
+        ring_gather_q4,
+        ring_q4_storage,
         w4a16_gemv,
         w4a16_lora_gemv,
     )

@@ -86,6 +86,21 @@ SIGNATURES = {
     "qx_decode_attention_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                             c_int, c_int, c_int, c_int, c_int64, c_float,
                                             c_void_p]),
+    "qx_qk_norm_rope": (c_int, [c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p,
+                                c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "qx_ring_q4_slots": (c_int64, [c_int, c_int]),
+    "qx_ring_append_q4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                  c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p, c_void_p]),
+    "qx_ring_gather_q4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                  c_int, c_int, c_int, c_int, c_int64, c_void_p]),
+    "qx_decode_attention_q4_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "qx_decode_attention_q4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                       c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p, c_float, c_void_p,
+                                       c_size_t, c_void_p]),
+    "qx_prefill_attention_q4_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "qx_prefill_attention_q4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                        c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                        c_int64, c_void_p, c_float, c_void_p, c_size_t, c_void_p]),
 }
 
 

@@ -4,8 +4,9 @@
 Same constructor, ``append`` / ``get_kv`` / ``valid_length`` /
 ``max_capacity`` / ``memory_usage_bytes`` / ``reset`` / ``repr``.  Unlike the
 reference there is no pure-PyTorch fallback: without the native library the
-constructor raises.  Additions: ``batch``, multi-token ``append`` and
-``decode_attention``.
+constructor raises.  Additions: ``batch``, multi-token ``append``,
+``decode_attention`` and ``bits=4`` (K and V held in 4 bits, a scale and a zero
+point for every ``group_size`` values; what goes in and comes out stays fp16).
 """
 
 from __future__ import annotations
@@ -16,11 +17,13 @@ import torch
 class QExtractKVCache:
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, sink_size: int = 4,
                  window_size: int = 4092, device: str = "cuda", dtype: torch.dtype = torch.float16,
-                 batch: int = 1):
+                 batch: int = 1, bits: int = 16, group_size: int = 64):
+        if bits not in (4, 16):
+            raise RuntimeError(f"QExtractKVCache holds K/V in 16 or 4 bits, not {bits}")
         if dtype != torch.float16:
             raise RuntimeError("QExtractKVCache stores float16 K/V")
         try:
-            from ._C import RingBufferKVCache
+            from ._C import RingBufferKVCache, RingBufferKVCacheQ4
         except ImportError as e:  # no silent fallback
             raise RuntimeError("QExtractKVCache needs the native library "
                                "(python -m qextract_infer_b200.build)") from e
@@ -33,8 +36,13 @@ class QExtractKVCache:
         self.device = device
         self.dtype = dtype
         self.batch = batch
-        self._backend = RingBufferKVCache(num_layers, num_kv_heads, head_dim, sink_size,
-                                          window_size, batch=batch, device=device)
+        self.bits = bits
+        if bits == 4:
+            self._backend = RingBufferKVCacheQ4(num_layers, num_kv_heads, head_dim, sink_size, window_size,
+                                                batch=batch, device=device, group_size=group_size)
+        else:
+            self._backend = RingBufferKVCache(num_layers, num_kv_heads, head_dim, sink_size,
+                                              window_size, batch=batch, device=device)
 
     @property
     def write_count(self) -> int:
@@ -70,7 +78,9 @@ class QExtractKVCache:
 
     def memory_usage_bytes(self) -> int:
         """``L * (S + W) * H * D * 2 bytes * 2 (K, V)`` per sequence
-        (``qextract/kv_cache.py:159-163``)."""
+        (``qextract/kv_cache.py:159-163``); the storage's own size at 4 bits."""
+        if self.bits == 4:
+            return sum(t.numel() * t.element_size() for t in (self._backend.codes, self._backend.params))
         return self.num_layers * self.total_size * self.num_kv_heads * self.head_dim * 2 * 2 * self.batch
 
     def reset(self) -> None:

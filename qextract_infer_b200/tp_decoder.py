@@ -66,6 +66,8 @@ class DecoderConfig:
     sink: int = 4
     window: int = 4092
     init_std: float = 0.02  # embeddings, norms, lm_head ~ N(0, std)
+    kv_bits: int = 16  # the ring's K and V: fp16, or 4 bits with a scale and zero point
+    kv_group: int = 64  # for every kv_group values of a head
 
 
 class ShardedQuantLinear:
@@ -213,8 +215,14 @@ class TPDecoder:
             )
             del q, k, v, gate, up
             self.layers.append(L)
-        self.cache = _C.RingBufferKVCache(cfg.num_layers, self.hkv, D, cfg.sink, cfg.window,
-                                          batch=batch, device=dev)
+        if cfg.kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 16 or 4, not {cfg.kv_bits}")
+        if cfg.kv_bits == 4:
+            self.cache = _C.RingBufferKVCacheQ4(cfg.num_layers, self.hkv, D, cfg.sink, cfg.window, batch=batch,
+                                                device=dev, group_size=cfg.kv_group)
+        else:
+            self.cache = _C.RingBufferKVCache(cfg.num_layers, self.hkv, D, cfg.sink, cfg.window,
+                                              batch=batch, device=dev)
         # q/k norm + RoPE + append fused into the attention kernel for a few
         # sequences (one launch fewer per layer, same time); for many, the
         # separate append kernel is faster (32 sequences: 86 vs 96 us per layer)
@@ -256,16 +264,6 @@ class TPDecoder:
             return self.ar.add_rmsnorm(partial, x, w, self.cfg.rms_eps)
         return _C.add_rmsnorm(x, self._allreduce(partial), w, self.cfg.rms_eps)
 
-    def _rope(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
-        """x [..., T, heads, D] fp16; cos/sin [T, D] fp32 -> rotated fp16 (HF rotate_half)."""
-        xf = x.float()
-        half = x.size(-1) // 2
-        rot = torch.cat([-xf[..., half:], xf[..., :half]], dim=-1)
-        return (xf * cos[:, None, :] + rot * sin[:, None, :]).half()
-
-    def _head_norm(self, t: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
-        return _C.fused_rmsnorm(t.contiguous(), w, self.cfg.rms_eps)
-
     def _mlp(self, L, h: torch.Tensor) -> torch.Tensor:
         return self._allreduce(L["down"](L["gate_up"].swiglu(h)))
 
@@ -277,7 +275,7 @@ class TPDecoder:
         cfg, B, D = self.cfg, self.batch, self.cfg.head_dim
         eps = cfg.rms_eps
         pos = self.cache.get_total_written()
-        cos, sin = self.cos[pos], self.sin[pos]
+        cos, sin = (self.cos[pos:pos + 1], self.sin[pos:pos + 1]) if cfg.kv_bits == 4 else (self.cos[pos], self.sin[pos])
         x = self.embed.index_select(0, tokens)  # [B, H], the residual stream
         h = _C.fused_rmsnorm(x, self.layers[0]["in_norm"], eps)
         n = len(self.layers)
@@ -293,7 +291,13 @@ class TPDecoder:
                 x, xo = xo, x
             else:
                 qkv = L["qkv"](h)
-            if self.fused_attention:
+            if cfg.kv_bits == 4:
+                q, k, v = _C.qk_norm_rope(qkv.view(B, 1, -1), self.hq, self.hkv, L["q_norm"], L["k_norm"], eps,
+                                          cos, sin)
+                ring = (self.cache.codes[li], self.cache.params[li])
+                _C.ring_append_q4(k, v, *ring, pos, cfg.sink, cfg.window)
+                att = _C.decode_attention_q4(q.view(B, self.hq, D), *ring, pos + 1, cfg.sink, cfg.window)
+            elif self.fused_attention:
                 att = _C.decode_attention_qkv(qkv, self.hq, self.hkv, L["q_norm"], L["k_norm"], eps,
                                               cos, sin, self.cache.k[li], self.cache.v[li], cfg.sink,
                                               cfg.window, pos)
@@ -353,15 +357,15 @@ class TPDecoder:
             x = self.embed.index_select(0, tc.reshape(-1)).view(B * n, cfg.hidden)
             for li, L in enumerate(self.layers):
                 h = _C.fused_rmsnorm(x, L["in_norm"], cfg.rms_eps)
-                qp, kp, vp = L["qkv"](h).split(L["qkv"].splits, dim=-1)
-                q = self._head_norm(qp.reshape(B * n * self.hq, D), L["q_norm"])
-                k = self._head_norm(kp.reshape(B * n * self.hkv, D), L["k_norm"])
-                v = vp.reshape(B, n, self.hkv, D).contiguous()
-                q = self._rope(q.view(B, n, self.hq, D), cos, sin)
-                k = self._rope(k.view(B, n, self.hkv, D), cos, sin)
+                q, k, v = _C.qk_norm_rope(L["qkv"](h).view(B, n, -1), self.hq, self.hkv, L["q_norm"], L["k_norm"],
+                                          cfg.rms_eps, cos, sin)
                 # the chunk over the ring (read in place) and its own keys, then the append
-                att = _C.prefill_attention(q, k.contiguous(), v, self.cache.k[li], self.cache.v[li], c,
-                                           cfg.sink, cfg.window)  # [B, n, hq, D]
+                if cfg.kv_bits == 4:
+                    att = _C.prefill_attention_q4(q, k, v, self.cache.codes[li], self.cache.params[li], c, cfg.sink,
+                                                  cfg.window)
+                else:
+                    att = _C.prefill_attention(q, k, v, self.cache.k[li], self.cache.v[li], c,
+                                               cfg.sink, cfg.window)  # [B, n, hq, D]
                 self.cache.append(k, v, li)
                 att = att.reshape(B * n, self.hq * D)
                 x = x + self._allreduce(L["o"](att))
