@@ -5,9 +5,27 @@
 // positions its write rule gives them.  New component (the reference gathers
 // the cache, qextract/kv_cache.py:96-112, and attends over the copy).
 //
-// Flash-attention form: one CTA = 4 warps = 64 query positions of one query
-// head; key tiles of 64 (ring slots made fp16 on the way to shared memory,
-// then the chunk's), S = Q K^T and O += P V on mma.sync with an online softmax.
+// Flash-attention form on the tcgen05 tensor cores.  A CTA owns 256 rows of one
+// KV head in two tiles of 128; a row is (query position, query head of the
+// group), positions outermost, so the group's heads share every key tile and
+// the rows of a CTA see nearly the same keys.  Tiles of 128 keys: the ring's
+// that any of its rows sees, then the chunk's up to the last row.
+//   warps 0-3, 4-7  softmax of row tile 0 and 1, one thread a row: S from TMEM,
+//                   the running maximum and sum in fp32, P in fp16 back to TMEM
+//                   over S.  O (fp32, TMEM) is rescaled only when the row's
+//                   maximum grew by more than 2^4, so P carries 2^11 at the
+//                   maximum last used and at most 2^15; both cancel in O / l.
+//   warps 8-11      loaders: ring rows are made fp16 (exactly: kv4.cuh) on the
+//                   way to the 128-byte-swizzled K (K-major) and V (MN-major)
+//                   tiles, the chunk's rows copied; two stages each
+//   warp 12         one thread issues tcgen05.mma: S = Q K^T (both operands in
+//                   shared memory) and O += P V (P from TMEM).  The two row tiles
+//                   alternate: while one's softmax runs the other's products do.
+// TMEM: S/P of both tiles and O of both, 512 columns of the SM's 512.
+// Few rows (a short chunk after a long context): CTAs split the key tiles and a
+// second kernel joins their fp32 results.
+// Every wait is bounded (kWaitLimitNs, then QX_DEVERR_MBAR_TIMEOUT; the CTA's
+// later waits give up at once).
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -18,7 +36,25 @@
 namespace qx {
 namespace pattn4 {
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, QROWS = WARPS * 16, KT = 64;
+constexpr int ROWS = 128;        // rows of a tile: tcgen05's M
+constexpr int KT = 128;          // keys of a tile
+constexpr int STAGES = 2;
+constexpr int SOFTMAX_WARPS = 8, LOAD_WARPS = 4, MMA_WARP = SOFTMAX_WARPS + LOAD_WARPS;
+constexpr int THREADS = (MMA_WARP + 1) * 32;
+constexpr float GROW = 4.f;      // log2 growth of a row's maximum that O is rescaled for
+constexpr float PSHIFT = 11.f;   // P carries 2^11: at most 2^15 with GROW, subnormal below 2^-25 of the maximum
+constexpr int MAX_SPLITS = 32;
+
+// barriers (8 bytes each)
+enum { FULL_K, EMPTY_K = FULL_K + STAGES, FULL_V = EMPTY_K + STAGES, EMPTY_V = FULL_V + STAGES,
+       S_FULL = EMPTY_V + STAGES, P_FULL = S_FULL + 2, O_FULL = P_FULL + 2, Q_FULL = O_FULL + 2, NBARS };
+
+template <int D>
+struct Smem {
+  static constexpr int TILE = ROWS * D * 2;  // bytes of a Q, K or V tile
+  static constexpr int Q = 0, K = 2 * TILE, V = K + STAGES * TILE, BARS = V + STAGES * TILE;
+  static constexpr int TMEM = BARS + NBARS * 8, GAVE_UP = TMEM + 4, BYTES = GAVE_UP + 4 + 1024;  // + alignment slack
+};
 
 struct Params {
   const __half* q;   // [B][n][Hq][D]
@@ -29,22 +65,121 @@ struct Params {
   const unsigned char* vc;
   const uint16_t* vp;
   __half* out;
+  float* part_o;    // [nsplit][B][n][Hq][D]
+  float2* part_ml;  // [nsplit][B][n][Hq]
   const int64_t* counts;
   int64_t count, cap;
-  int n, hq, hkv, G, sink, window;
+  int batch, n, hq, hkv, G, sink, window, nsplit;
   float scale_log2;
 };
 
+// Sticky device-side error word of this file's kernels (QX_DEVERR_* bits),
+// merged into qx_get_device_error.
+static __device__ unsigned g_prefill4_error = 0;
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+__device__ __forceinline__ void bar_init(uint32_t b, uint32_t n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n) : "memory");
 }
-__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+__device__ __forceinline__ void bar_arrive(uint32_t b) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(b) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred P; mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 P, [%1], %2; "
+      "selp.u32 %0, 1, 0, P; }"
+      : "=r"(ok)
+      : "r"(b), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ void bar_wait_slow(uint32_t b, uint32_t parity, volatile unsigned* gave_up) {
+  uint64_t t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  while (!bar_try(b, parity)) {
+    if (*gave_up) return;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    if (t - t0 > kWaitLimitNs) {
+      *gave_up = 1;
+      atomicOr(&g_prefill4_error, QX_DEVERR_MBAR_TIMEOUT);
+      return;
+    }
+  }
+}
+__device__ __forceinline__ void bar_wait(uint32_t b, uint32_t parity, volatile unsigned* gave_up) {
+  if (!bar_try(b, parity)) bar_wait_slow(b, parity, gave_up);
+}
+
+// shared-memory operand of 128-byte-swizzled rows (64 values), 8-row atoms 1024 B
+// apart, tiles of 64 values `half` bytes apart.  K-major (Q, K): the rows are M
+// or N, `half` unused; MN-major (V): the rows are the product's K, `half` steps N.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t half) {
+  return uint64_t((saddr >> 4) & 0x3FFF) | (uint64_t(half >> 4) << 16) | (uint64_t(64) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+// kind::f16 instruction descriptor: D f32, A and B f16, M = 128; MN_B: B is MN-major
+template <int N, bool MN_B>
+constexpr uint32_t idesc() {
+  return (1u << 4) | (MN_B ? 1u << 16 : 0u) | (uint32_t(N >> 3) << 17) | (uint32_t(ROWS >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(b) : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+#define QX_R8(v, i) "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3]), "=f"(v[i + 4]), "=f"(v[i + 5]), "=f"(v[i + 6]), "=f"(v[i + 7])
+#define QX_W8(v, i) "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7])
+// 32 columns of the warp's 32 rows, a row a thread
+__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : QX_R8(v, 0), QX_R8(v, 8), QX_R8(v, 16), QX_R8(v, 24)
+      : "r"(addr));
+}
+// waits for the loads before it; the values pass through so that no use of them moves above it
+__device__ __forceinline__ void tmem_ld_wait(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : QX_W8(v, 0), QX_W8(v, 8), QX_W8(v, 16), QX_W8(v, 24)::"memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"f"(v[0]),
+      "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
+      "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]),
+      "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]),
+      "f"(v[29]), "f"(v[30]), "f"(v[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(v[0]),
+      "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
   __half2 h = __floats2half2_rn(a, b);
@@ -123,189 +258,542 @@ __device__ __noinline__ void redo_row(const Params& p, const Ring& ring, int b, 
   for (int e = 0; e < E; ++e) p.out[at + 32 * e] = __float2half_rn(acc[e] / l);
 }
 
-template <int D, int NG>
-__global__ void __launch_bounds__(THREADS) prefill_attn_q4_kernel(const Params p) {
-  pdl_trigger();
-  constexpr int NI = D / 32, LPR = D / 8, ROWB = D * 2;
-  __shared__ __align__(128) unsigned char s_k[KT * ROWB], s_v[KT * ROWB];
-  auto swz = [](int r, int ch) { return uint32_t(r * ROWB + ((ch ^ (r & 7)) << 4)); };
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = lane >> 2, c = lane & 3;
-  const int h = blockIdx.y, b = blockIdx.z, kvh = h / p.G;
-  const int r0 = blockIdx.x * QROWS;
-  const int rowA = r0 + warp * 16 + g, rowB = rowA + 8;
-  pdl_wait();
-  const Ring ring(kv4::count_of(p.counts, p.count, b), p.sink, p.window);
-  const int last = min(p.n, r0 + QROWS) - 1;
-  const int ncache = (ring.valid + KT - 1) / KT;
-  const int ntiles = ncache + last / KT + 1;
-  const uint32_t ks = smem_u32(s_k), vs = smem_u32(s_v);
-  const int64_t base = (int64_t(b) * p.hkv + kvh) * p.cap;
+// The key tiles that some row of [rmin, rmax] (chunk positions) may see, as
+// ranges of tile numbers: of the ring's slots the sinks, those up to the newest
+// token's and those after it (older, where the ring has wrapped), then of the
+// chunk's keys the sinks and the window.  Hidden from rmin is hidden from all
+// for the ring; a range starts after the one before it.
+struct Tiles {
+  int start[5], len[5], total;
+  __device__ Tiles(const Ring& r, int rmin, int rmax, int sink, int window) {
+    const int held = r.valid - sink;  // ring tokens (below zero: sinks only)
+    // visible to rmin: ring index w <= newest with w >= newest - window + 2 + rmin, or w > newest with w >= newest + 2 + rmin
+    const int lo1 = max(0, r.newest - window + 2 + rmin), lo2 = r.newest + 2 + rmin;
+    const int first[5] = {0, sink + lo1, sink + lo2, 0, max(0, rmin - window + 1)};
+    const int last[5] = {min(r.valid, sink) - 1, r.newest >= 0 ? sink + min(r.newest, held - 1) : -1,
+                         r.newest >= 0 ? sink + held - 1 : -1, min(r.sinks - 1, rmax), rmax};
+    int next = 0;
+    total = 0;
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {
+      if (k == 3) next = 0;
+      start[k] = max(next, first[k] / KT);
+      len[k] = last[k] >= first[k] ? max(0, last[k] / KT + 1 - start[k]) : 0;
+      if (len[k] > 0) next = start[k] + len[k];
+      total += len[k];
+    }
+  }
+  // tile t of the list: its number, and whether it is the ring's
+  __device__ int at(int t, bool& of_ring) const {
+    int idx = 0;
+    of_ring = true;
+    bool found = false;
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {
+      if (!found && t < len[k]) {
+        idx = start[k] + t;
+        of_ring = k < 3;
+        found = true;
+      }
+      t -= len[k];
+    }
+    return idx;
+  }
+};
 
-  uint32_t qa[D / 16][4];
-  {
-    const bool okA = rowA < p.n, okB = rowB < p.n;
-    const __half* qA = p.q + ((int64_t(b) * p.n + (okA ? rowA : 0)) * p.hq + h) * D;
-    const __half* qB = p.q + ((int64_t(b) * p.n + (okB ? rowB : 0)) * p.hq + h) * D;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      const int d0 = kk * 16 + 2 * c;
-      qa[kk][0] = okA ? *reinterpret_cast<const uint32_t*>(qA + d0) : 0u;
-      qa[kk][1] = okB ? *reinterpret_cast<const uint32_t*>(qB + d0) : 0u;
-      qa[kk][2] = okA ? *reinterpret_cast<const uint32_t*>(qA + d0 + 8) : 0u;
-      qa[kk][3] = okB ? *reinterpret_cast<const uint32_t*>(qB + d0 + 8) : 0u;
-    }
-  }
-  float o[D / 8][4];
-#pragma unroll
-  for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.f, 0.f};
-  const int mi = lane >> 3, ri = lane & 7;
+// does every row of [rmin, rmax] see every key of the tile?
+__device__ __forceinline__ bool all_seen(const Ring& r, bool of_ring, int k0, int rmin, int rmax, int sink, int window) {
+  const int k1 = k0 + KT - 1;
+  if (!of_ring) return k1 <= rmin && (k0 > rmax - window || k1 < r.sinks);
+  if (k1 >= r.valid) return false;
+  const int w0 = max(k0 - sink, 0), w1 = k1 - sink;
+  if (w1 < 0) return true;
+  if (w0 <= r.newest && w0 < r.newest - window + 2 + rmax) return false;
+  return w1 <= r.newest || max(w0, r.newest + 1) >= r.newest + 2 + rmax;
+}
 
-  for (int t = 0; t < ntiles; ++t) {
-    __syncthreads();
-    const bool cache = t < ncache;
-    const int k0 = cache ? t * KT : (t - ncache) * KT;
-    for (int idx = tid; idx < KT * LPR; idx += THREADS) {
-      const int r = idx / LPR, ch = idx % LPR;
-      uint4 kv = make_uint4(0u, 0u, 0u, 0u), vv = kv;
-      if (cache) {
-        if (k0 + r < ring.valid) {
-          const int64_t row = base + k0 + r;
-          const int cc = ch & 3, i = ch >> 2;
-          const uint16_t* vr = reinterpret_cast<const uint16_t*>(p.vc) + row * (2 * LPR);
-          const uint32_t kw = *(reinterpret_cast<const uint32_t*>(p.kc) + row * LPR + cc * NI + i);
-          const uint32_t vw = uint32_t(vr[2 * cc * NI + i]) | (uint32_t(vr[(2 * cc + 1) * NI + i]) << 16);
-          const uint32_t kq = p.kp[row * NG + i * NG / NI], vq = p.vp[row * NG + i * NG / NI];
-          uint32_t w[4];
-          kv4::dequant_word(kw, kv4::group_scale(kq | (kq << 16)), w);
-          kv = make_uint4(w[0], w[1], w[2], w[3]);
-          kv4::dequant_word(vw, kv4::group_scale(vq | (vq << 16)), w);
-          vv = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      } else if (k0 + r < p.n) {
-        const int64_t off = ((int64_t(b) * p.n + k0 + r) * p.hkv + kvh) * D + ch * 8;
-        kv = *reinterpret_cast<const uint4*>(p.kn + off);
-        vv = *reinterpret_cast<const uint4*>(p.vn + off);
+// bits of [lo, hi) within [base, base + 32)
+__device__ __forceinline__ uint32_t bits(int lo, int hi, int base) {
+  lo = min(max(lo - base, 0), 32);
+  hi = min(max(hi - base, 0), 32);
+  if (hi <= lo) return 0u;
+  return (0xFFFFFFFFu >> (32 - (hi - lo))) << lo;  // hi > lo: lo < 32 and the width is 1 to 32
+}
+
+// A loader lane's share of a key tile: a quarter (c) of rows 8 pass + its own, the
+// 8-value blocks 4 i + c, as 16-byte chunks of the swizzled tile.  The rows of
+// a warp's store turn are four apart in pairs, so that eight lanes write eight
+// different 16-byte columns.
+template <int D>
+__device__ __forceinline__ void put_block(unsigned char* tile, int row, int c, int i, uint4 v) {
+  *reinterpret_cast<uint4*>(tile + (i >> 1) * (KT * 128) + row * 128 + (((4 * (i & 1) + c) ^ (row & 7)) << 4)) = v;
+}
+
+// A lane's codes and params of one tile of the ring's keys or values, on their way:
+// loaded a tile ahead, stored as fp16 when the stage is free.
+template <int D, int NG, bool VALUES>
+struct RingTile {
+  static constexpr int NI = D / 32, PASSES = KT / (LOAD_WARPS * 8), PW = NG == 4 ? 2 : 1;
+  uint32_t w[PASSES][NI], pr[PASSES][PW];
+
+  __device__ __forceinline__ void load(const Params& p, int64_t base, int k0, int valid, int warp, int lane) {
+    const unsigned char* codes = VALUES ? p.vc : p.kc;
+    const uint16_t* params = VALUES ? p.vp : p.kp;
+    const int c = lane & 3, q = lane >> 2, r8 = (q >> 1) | ((q & 1) << 2);
+#pragma unroll
+    for (int s = 0; s < PASSES; ++s) {
+      // a free slot reads the last valid one's row (the tile may end behind the storage)
+      const int64_t row = base + min(k0 + s * (LOAD_WARPS * 8) + warp * 8 + r8, valid - 1);
+      if constexpr (NI == 4) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(codes + row * (D / 2)) + c);
+        w[s][0] = v.x, w[s][1] = v.y, w[s][2] = v.z, w[s][3] = v.w;
+      } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(codes + row * (D / 2)) + c);
+        w[s][0] = v.x, w[s][1] = v.y;
       }
-      *reinterpret_cast<uint4*>(s_k + swz(r, ch)) = kv;
-      *reinterpret_cast<uint4*>(s_v + swz(r, ch)) = vv;
-    }
-    __syncthreads();
-    float s[8][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-#pragma unroll
-      for (int j2 = 0; j2 < 4; ++j2) {
-        uint32_t bk[4];
-        ldsm_x4(bk, ks + swz(j2 * 16 + 8 * (mi >> 1) + ri, 2 * kk + (mi & 1)));
-        mma_16816(s[2 * j2], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], bk[0], bk[1]);
-        mma_16816(s[2 * j2 + 1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], bk[2], bk[3]);
-      }
-    }
-    float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-#pragma unroll
-      for (int e1 = 0; e1 < 2; ++e1) {
-        const int key = k0 + j * 8 + 2 * c + e1;
-        bool vA, vB;
-        if (cache) {
-          vA = key < ring.valid && ring.sees(key, rowA, p.sink, p.window);
-          vB = key < ring.valid && ring.sees(key, rowB, p.sink, p.window);
-        } else {
-          vA = key < p.n && ring.sees_new(key, rowA, p.window);
-          vB = key < p.n && ring.sees_new(key, rowB, p.window);
-        }
-        s[j][e1] = vA ? s[j][e1] * p.scale_log2 : -INFINITY;
-        s[j][2 + e1] = vB ? s[j][2 + e1] * p.scale_log2 : -INFINITY;
-        mx0 = fmaxf(mx0, s[j][e1]);
-        mx1 = fmaxf(mx1, s[j][2 + e1]);
-      }
-    }
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-    const float mn0 = fmaxf(m_r[0], mx0), mn1 = fmaxf(m_r[1], mx1);
-    const float mb0 = mn0 == -INFINITY ? 0.f : mn0, mb1 = mn1 == -INFINITY ? 0.f : mn1;
-    const float al0 = exp2f(m_r[0] - mb0), al1 = exp2f(m_r[1] - mb1);
-    m_r[0] = mn0;
-    m_r[1] = mn1;
-    float ls0 = 0.f, ls1 = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      s[j][0] = exp2f(s[j][0] - mb0 + 14.f);
-      s[j][1] = exp2f(s[j][1] - mb0 + 14.f);
-      s[j][2] = exp2f(s[j][2] - mb1 + 14.f);
-      s[j][3] = exp2f(s[j][3] - mb1 + 14.f);
-      ls0 += s[j][0] + s[j][1];
-      ls1 += s[j][2] + s[j][3];
-    }
-    l_r[0] = l_r[0] * al0 + ls0;
-    l_r[1] = l_r[1] * al1 + ls1;
-#pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      o[j][0] *= al0;
-      o[j][1] *= al0;
-      o[j][2] *= al1;
-      o[j][3] *= al1;
-    }
-#pragma unroll
-    for (int kq = 0; kq < 4; ++kq) {
-      const uint32_t pa0 = pack_h2(s[2 * kq][0], s[2 * kq][1]);
-      const uint32_t pa1 = pack_h2(s[2 * kq][2], s[2 * kq][3]);
-      const uint32_t pa2 = pack_h2(s[2 * kq + 1][0], s[2 * kq + 1][1]);
-      const uint32_t pa3 = pack_h2(s[2 * kq + 1][2], s[2 * kq + 1][3]);
-#pragma unroll
-      for (int jj = 0; jj < D / 16; ++jj) {
-        uint32_t bv[4];
-        ldsm_x4_t(bv, vs + swz(kq * 16 + 8 * (mi & 1) + ri, 2 * jj + (mi >> 1)));
-        mma_16816(o[2 * jj], pa0, pa1, pa2, pa3, bv[0], bv[1]);
-        mma_16816(o[2 * jj + 1], pa0, pa1, pa2, pa3, bv[2], bv[3]);
+      if constexpr (NG == 4) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(params + row * NG));
+        pr[s][0] = v.x, pr[s][1] = v.y;
+      } else if constexpr (NG == 2) {
+        pr[s][0] = __ldg(reinterpret_cast<const uint32_t*>(params + row * NG));
+      } else {
+        pr[s][0] = __ldg(params + row);
       }
     }
   }
-  uint32_t redo = 0;  // bit r: row r of the warp's 16
+  __device__ __forceinline__ void store(unsigned char* tile, int warp, int lane) const {
+    const int c = lane & 3, q = lane >> 2, r8 = (q >> 1) | ((q & 1) << 2);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    l_r[k] += __shfl_xor_sync(0xffffffffu, l_r[k], 1);
-    l_r[k] += __shfl_xor_sync(0xffffffffu, l_r[k], 2);
-    const int row = k ? rowB : rowA;
-    const float inv = 1.f / l_r[k];
-    bool fine = true;
+    for (int s = 0; s < PASSES; ++s) {
+      const int row = s * (LOAD_WARPS * 8) + warp * 8 + r8;
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      const float x = o[j][2 * k] * inv, y = o[j][2 * k + 1] * inv;
-      fine = fine && fabsf(x) <= 65504.f && fabsf(y) <= 65504.f;
-      if (row < p.n)
-        *reinterpret_cast<uint32_t*>(p.out + ((int64_t(b) * p.n + row) * p.hq + h) * D + 8 * j + 2 * c) = pack_h2(x, y);
+      for (int n = 0; n < NG; ++n) {
+        const uint32_t pair = NG == 1 ? pr[s][0] * 0x10001u : prmt(pr[s][n >> 1], 0u, (n & 1) ? 0x3232u : 0x1010u);
+        const kv4::GroupScale gs = kv4::group_scale(pair);
+#pragma unroll
+        for (int i = n * NI / NG; i < (n + 1) * NI / NG; ++i) {
+          const uint32_t word = VALUES ? prmt(w[s][i >> 1], w[s][NI / 2 + (i >> 1)], (i & 1) ? 0x7632u : 0x5410u) : w[s][i];
+          uint32_t o[4];
+          kv4::dequant_word(word, gs, o);
+          put_block<D>(tile, row, c, i, make_uint4(o[0], o[1], o[2], o[3]));
+        }
+      }
     }
-    const uint32_t bad = __ballot_sync(0xffffffffu, !fine && row < p.n);
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-      if ((bad >> (4 * r)) & 15u) redo |= 1u << (8 * k + r);
   }
-  __syncwarp();
-  for (; redo; redo &= redo - 1) redo_row<D, NG>(p, ring, b, h, r0 + warp * 16 + __ffs(redo) - 1, lane);
+};
+
+// one tile of the chunk's keys or values, rows past the chunk zero
+template <int D>
+__device__ __forceinline__ void copy_new_tile(const __half* src, int64_t first, int64_t stride, int k0, int n,
+                                              uint32_t tile, int warp, int lane) {
+  constexpr int LPR = D / 8;
+#pragma unroll 4
+  for (int r = warp * (32 / LPR) + lane / LPR; r < KT; r += LOAD_WARPS * (32 / LPR)) {
+    const int ch = lane % LPR, key = k0 + r;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                     tile + (ch >> 3) * (KT * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
+                 "l"(src + first + min(key, n - 1) * stride + ch * 8), "r"(key < n ? 16 : 0));
+  }
+  asm volatile("cp.async.commit_group;");
 }
 
 template <int D, int NG>
-cudaError_t launch(const Params& p, int batch, cudaStream_t st) {
-  return launch_pdl(prefill_attn_q4_kernel<D, NG>, dim3((p.n + QROWS - 1) / QROWS, p.hq, batch), dim3(THREADS), 0, st, p);
+__global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __grid_constant__ Params p) {
+  using L = Smem<D>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sb = smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  volatile unsigned* gave_up = reinterpret_cast<volatile unsigned*>(smem + L::GAVE_UP);
+  auto bar = [&](int i) { return sb + L::BARS + 8 * i; };
+  if (tid == 0) {
+    *gave_up = 0;
+    for (int i = 0; i < STAGES; ++i) {
+      bar_init(bar(FULL_K + i), LOAD_WARPS);
+      bar_init(bar(EMPTY_K + i), 1);
+      bar_init(bar(FULL_V + i), LOAD_WARPS);
+      bar_init(bar(EMPTY_V + i), 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      bar_init(bar(S_FULL + x), 1);
+      bar_init(bar(P_FULL + x), 4);
+      bar_init(bar(O_FULL + x), 1);
+    }
+    bar_init(bar(Q_FULL), SOFTMAX_WARPS);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == MMA_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(sb + L::TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  // only now: a kernel launched early must not take TMEM columns that this one waits for
+  pdl_trigger();
+  pdl_wait();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::TMEM);
+
+  const int split = blockIdx.x % p.nsplit, block = blockIdx.x / p.nsplit;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int rows = p.n * p.G, row0 = block * 2 * ROWS;
+  const int last_row = min(rows, row0 + 2 * ROWS) - 1;
+  const int rmin = row0 / p.G, rmax = last_row / p.G;
+  const int ntile = last_row - row0 >= ROWS ? 2 : 1;  // row tiles with rows
+  const Ring ring(kv4::count_of(p.counts, p.count, b), p.sink, p.window);
+  const Tiles tiles(ring, rmin, rmax, p.sink, p.window);
+  const int t0 = int(int64_t(tiles.total) * split / p.nsplit), t1 = int(int64_t(tiles.total) * (split + 1) / p.nsplit);
+  const int T = t1 - t0;
+  const uint32_t tmem_s[2] = {tmem, tmem + KT}, tmem_o[2] = {tmem + 2 * KT, tmem + 2 * KT + D};
+
+  if (warp < SOFTMAX_WARPS) {
+    // --------------------------------------------------------------- softmax
+    const int x = warp >> 2, quad = warp & 3;
+    const uint32_t lanes = uint32_t(quad * 32) << 16;
+    {  // this warp's 32 rows of Q, D / 8 lanes a row
+      constexpr int LPR = D / 8;
+      for (int r = lane / LPR; r < 32; r += 32 / LPR) {
+        const int tr = quad * 32 + r, row = row0 + x * ROWS + tr, ch = lane % LPR;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows) {
+          const int pos = row / p.G, hg = row - pos * p.G;
+          v = __ldg(reinterpret_cast<const uint4*>(p.q + ((int64_t(b) * p.n + pos) * p.hq + kvh * p.G + hg) * D) + ch);
+        }
+        *reinterpret_cast<uint4*>(smem + L::Q + x * L::TILE + (ch >> 3) * (ROWS * 128) + tr * 128 +
+                                  (((ch & 7) ^ (tr & 7)) << 4)) = v;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(bar(Q_FULL));
+    }
+    const int row = row0 + x * ROWS + quad * 32 + lane;
+    const int pos = min(row, rows - 1) / p.G, hg = min(row, rows - 1) - pos * p.G;
+    const int64_t orow = (int64_t(b) * p.n + pos) * p.hq + kvh * p.G + hg;
+    float m_used = -INFINITY, l = 0.f;
+    if (x < ntile) {
+      const uint32_t ts = tmem_s[x] + lanes, to = tmem_o[x] + lanes;
+      for (int it = 0; it < T; ++it) {
+        bool of_ring;
+        const int k0 = tiles.at(t0 + it, of_ring) * KT;
+        const bool full = all_seen(ring, of_ring, k0, rmin, rmax, p.sink, p.window);
+        // the keys of the tile that this row sees, a bit each
+        uint32_t seen[KT / 32];
+        if (!full) {
+          if (of_ring) {
+            const int sk = p.sink - k0, nw = sk + ring.newest;  // from the tile's first slot: first ring slot, newest
+            const int end = ring.valid - k0;
+#pragma unroll
+            for (int j = 0; j < KT / 32; ++j)
+              seen[j] = bits(0, min(sk, end), 32 * j) |
+                        bits(max(sk, nw - p.window + 2 + pos), min(nw + 1, end), 32 * j) |
+                        bits(max(nw + 1, nw + 2 + pos), end, 32 * j);
+          } else {
+#pragma unroll
+            for (int j = 0; j < KT / 32; ++j)
+              seen[j] = bits(0, min(pos + 1, ring.sinks) - k0, 32 * j) | bits(pos - p.window + 1 - k0, pos + 1 - k0, 32 * j);
+          }
+        }
+        auto hide = [&](float (&v)[32], uint32_t m) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = (m >> e) & 1u ? v[e] : -INFINITY;
+        };
+        bar_wait(bar(S_FULL + x), it & 1, gave_up);
+        fence_after();
+        float v[2][32];
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tmem_ld(ts, v[0]);
+#pragma unroll
+        for (int j = 0; j < KT / 32; ++j) {
+          tmem_ld_wait(v[j & 1]);
+          if (j + 1 < KT / 32) tmem_ld(ts + 32 * (j + 1), v[(j + 1) & 1]);
+          if (!full) hide(v[j & 1], seen[j]);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], v[j & 1][e]);
+        }
+        tmem_ld(ts, v[0]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        const bool grew = top > m_used + GROW;
+        if (__any_sync(0xffffffffu, grew)) {
+          const float m_new = fmaxf(m_used, top);
+          const float mb = m_new == -INFINITY ? 0.f : m_new;
+          const float alpha = ex2(m_used - mb);
+          m_used = m_new;
+          l *= alpha;
+          if (it > 0) {  // P V of the tile before has ended: its commit came with this S
+            tmem_ld_wait(v[0]);
+            float o[32];
+#pragma unroll 1
+            for (int j = 0; j < D; j += 32) {
+              tmem_ld(to + j, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= alpha;
+              tmem_st32(to + j, o);
+            }
+          }
+        }
+        const float shift = PSHIFT - (m_used == -INFINITY ? 0.f : m_used);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KT / 32; ++j) {
+          tmem_ld_wait(v[j & 1]);
+          if (j + 1 < KT / 32) tmem_ld(ts + 32 * (j + 1), v[(j + 1) & 1]);
+          if (!full) hide(v[j & 1], seen[j]);
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float a = ex2(fmaf(v[j & 1][e], p.scale_log2, shift)), c = ex2(fmaf(v[j & 1][e + 1], p.scale_log2, shift));
+            sum[e & 2] += a;
+            sum[(e & 2) + 1] += c;
+            pk[e / 2] = pack_h2(a, c);
+          }
+          tmem_st16(ts + 16 * j, pk);  // columns 16 j .. of S, all read by now
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st_wait();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar(P_FULL + x));
+      }
+      // ------------------------------------------------------------- epilogue
+      if (T > 0) {
+        bar_wait(bar(O_FULL + x), 0, gave_up);
+        fence_after();
+      }
+      float v[32];
+      if (p.nsplit == 1) {
+        const float inv = 1.f / l;
+        bool fine = true;
+#pragma unroll 1
+        for (int j = 0; j < D; j += 32) {
+          tmem_ld(to + j, v);
+          tmem_ld_wait(v);
+          uint32_t h[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float a = v[e] * inv, c = v[e + 1] * inv;
+            fine = fine && fabsf(a) <= 65504.f && fabsf(c) <= 65504.f;
+            h[e / 2] = pack_h2(a, c);
+          }
+          if (row < rows)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<uint4*>(p.out + orow * D + j + 2 * e) = make_uint4(h[e], h[e + 1], h[e + 2], h[e + 3]);
+        }
+        uint32_t redo = __ballot_sync(0xffffffffu, !fine && row < rows);
+        for (; redo; redo &= redo - 1) {
+          const int r = row0 + x * ROWS + quad * 32 + __ffs(redo) - 1;
+          redo_row<D, NG>(p, ring, b, kvh * p.G + r % p.G, r / p.G, lane);
+        }
+      } else {
+        const int64_t part = int64_t(split) * p.batch * p.n * p.hq + orow;
+        if (row < rows) p.part_ml[part] = make_float2(m_used, l);
+        if (T > 0) {
+#pragma unroll 1
+          for (int j = 0; j < D; j += 32) {
+            tmem_ld(to + j, v);
+            tmem_ld_wait(v);
+            if (row < rows)
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<float4*>(p.part_o + part * D + j + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          }
+        }
+      }
+    }
+  } else if (warp < MMA_WARP) {
+    // --------------------------------------------------------------- loaders
+    const int lw = warp - SOFTMAX_WARPS;
+    const int64_t base = (int64_t(b) * p.hkv + kvh) * p.cap;
+    const int64_t first = (int64_t(b) * p.n * p.hkv + kvh) * D, stride = int64_t(p.hkv) * D;
+    RingTile<D, NG, false> kr;
+    RingTile<D, NG, true> vr;
+    bool of_ring = false;
+    int k0 = T > 0 ? tiles.at(t0, of_ring) * KT : 0;
+    if (of_ring) {
+      kr.load(p, base, k0, ring.valid, lw, lane);
+      vr.load(p, base, k0, ring.valid, lw, lane);
+    }
+    auto done = [&](int b_full) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(bar(b_full));
+    };
+    for (int it = 0; it < T; ++it) {
+      const int st = it % STAGES;
+      unsigned char* kt = smem + L::K + st * L::TILE;
+      unsigned char* vt = smem + L::V + st * L::TILE;
+      bool next_ring = false;
+      const int next = it + 1 < T ? tiles.at(t0 + it + 1, next_ring) * KT : 0;
+      if (it >= STAGES) bar_wait(bar(EMPTY_K + st), (it / STAGES - 1) & 1, gave_up);
+      if (of_ring) {
+        kr.store(kt, lw, lane);
+        done(FULL_K + st);
+        if (next_ring) kr.load(p, base, next, ring.valid, lw, lane);
+        if (it >= STAGES) bar_wait(bar(EMPTY_V + st), (it / STAGES - 1) & 1, gave_up);
+        vr.store(vt, lw, lane);
+        done(FULL_V + st);
+        if (next_ring) vr.load(p, base, next, ring.valid, lw, lane);
+      } else {
+        copy_new_tile<D>(p.kn, first, stride, k0, p.n, smem_u32(kt), lw, lane);
+        if (it >= STAGES) bar_wait(bar(EMPTY_V + st), (it / STAGES - 1) & 1, gave_up);
+        copy_new_tile<D>(p.vn, first, stride, k0, p.n, smem_u32(vt), lw, lane);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        done(FULL_K + st);
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        done(FULL_V + st);
+      }
+      of_ring = next_ring;
+      k0 = next;
+    }
+  } else if (lane == 0 && T > 0) {
+    // -------------------------------------------------------------- products
+    auto scores = [&](int x, int st) {  // S_x = Q_x K^T
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t at = (k >> 2) * (ROWS * 128) + (k & 3) * 32;
+        mma_ss(tmem_s[x], sw128_desc(sb + L::Q + x * L::TILE + at, 16), sw128_desc(sb + L::K + st * L::TILE + at, 16),
+               idesc<KT, false>(), k != 0);
+      }
+    };
+    bar_wait(bar(Q_FULL), 0, gave_up);
+    bar_wait(bar(FULL_K), 0, gave_up);
+    fence_after();
+    for (int x = 0; x < ntile; ++x) {
+      scores(x, 0);
+      mma_commit(bar(S_FULL + x));
+    }
+    mma_commit(bar(EMPTY_K));
+    for (int it = 0; it < T; ++it) {
+      const int st = it % STAGES, nst = (it + 1) % STAGES;
+      bar_wait(bar(FULL_V + st), (it / STAGES) & 1, gave_up);
+      for (int x = 0; x < ntile; ++x) {
+        bar_wait(bar(P_FULL + x), it & 1, gave_up);
+        fence_after();
+#pragma unroll
+        for (int k = 0; k < KT / 16; ++k)  // O_x += P_x V: 16 keys are 8 columns of P and 16 rows of V
+          mma_ts(tmem_o[x], tmem_s[x] + 8 * k, sw128_desc(sb + L::V + st * L::TILE + k * 2048, KT * 128),
+                 idesc<D, true>(), (it | k) != 0);
+        if (x == ntile - 1) mma_commit(bar(EMPTY_V + st));
+        if (it + 1 < T) {  // in order after P V: S_x overwrites P_x
+          if (x == 0) {
+            bar_wait(bar(FULL_K + nst), ((it + 1) / STAGES) & 1, gave_up);
+            fence_after();
+          }
+          scores(x, nst);
+          mma_commit(bar(S_FULL + x));
+          if (x == ntile - 1) mma_commit(bar(EMPTY_K + nst));
+        } else {
+          mma_commit(bar(O_FULL + x));
+        }
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// joins the splits of a row: one warp a row
+template <int D, int NG>
+__global__ void __launch_bounds__(128) prefill_attn_q4_merge_kernel(const __grid_constant__ Params p) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t total = int64_t(p.batch) * p.n * p.hq;
+  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (row >= total) return;
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < p.nsplit) ml = p.part_ml[lane * total + row];
+  const float m = warp_max(ml.x);
+  const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+  const float inv = 1.f / warp_sum(w * ml.y);
+  float acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float ws = __shfl_sync(0xffffffffu, w, s);
+    if (__shfl_sync(0xffffffffu, ml.x, s) == -INFINITY) continue;  // no key there: its O was not written, or is void
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(ws, p.part_o[(s * total + row) * D + 32 * e + lane], acc[e]);
+  }
+  bool fine = true;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    fine = fine && fabsf(acc[e] * inv) <= 65504.f;
+    p.out[row * D + 32 * e + lane] = __float2half_rn(acc[e] * inv);
+  }
+  if (__any_sync(0xffffffffu, !fine)) {
+    const int h = int(row % p.hq), b = int(row / p.hq / p.n), pos = int(row / p.hq % p.n);
+    const Ring ring(kv4::count_of(p.counts, p.count, b), p.sink, p.window);
+    redo_row<D, NG>(p, ring, b, h, pos, lane);
+  }
+}
+
+// CTAs that split the key tiles of a row block: where the row blocks leave SMs
+// idle, as many as fill them with at least two tiles each
+inline int splits(int batch, int n, int G, int kv_heads, int sink, int window) {
+  const int64_t ctas = (int64_t(n) * G + 2 * ROWS - 1) / (2 * ROWS) * kv_heads * batch;
+  const int64_t most = (kv4::capacity(sink, window) / KT + (n + KT - 1) / KT) / 2;
+  return int(std::max<int64_t>(1, std::min<int64_t>({device_sm_count() / ctas, most, MAX_SPLITS})));
+}
+inline size_t workspace_for(int batch, int n, int q_heads, int head_dim, int nsplit) {
+  return nsplit == 1 ? 0 : size_t(nsplit) * batch * n * q_heads * (size_t(head_dim) * sizeof(float) + sizeof(float2));
+}
+
+template <int D, int NG>
+cudaError_t launch(const Params& p, cudaStream_t st) {
+  {
+    static std::mutex mu;
+    static bool done[64] = {};
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!done[dev]) {
+      const cudaError_t a = cudaFuncSetAttribute(prefill_attn_q4_kernel<D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 Smem<D>::BYTES);
+      if (a != cudaSuccess) return a;
+      done[dev] = true;
+    }
+  }
+  const int blocks = (p.n * p.G + 2 * ROWS - 1) / (2 * ROWS);
+  const cudaError_t e = launch_pdl(prefill_attn_q4_kernel<D, NG>, dim3(unsigned(blocks * p.nsplit), unsigned(p.hkv), unsigned(p.batch)),
+                                   dim3(THREADS), Smem<D>::BYTES, st, p);
+  if (e != cudaSuccess || p.nsplit == 1) return e;
+  const int64_t rows = int64_t(p.batch) * p.n * p.hq;
+  return launch_pdl(prefill_attn_q4_merge_kernel<D, NG>, dim3(unsigned((rows + 3) / 4)), dim3(128), 0, st, p);
 }
 
 }  // namespace pattn4
+
+int prefill4_device_error(unsigned* code, int reset) {
+  QX_CUDA_TRY(cudaMemcpyFromSymbol(code, pattn4::g_prefill4_error, sizeof(unsigned)), "get_device_error: read");
+  if (reset) {
+    const unsigned zero = 0;
+    QX_CUDA_TRY(cudaMemcpyToSymbol(pattn4::g_prefill4_error, &zero, sizeof(unsigned)), "get_device_error: reset");
+  }
+  return QX_OK;
+}
+
 }  // namespace qx
 
 using namespace qx;
 
 extern "C" size_t qx_prefill_attention_q4_workspace_size(int batch, int n, int q_heads, int kv_heads, int head_dim,
                                                          int sink, int window) {
-  (void)batch, (void)n, (void)q_heads, (void)kv_heads, (void)head_dim, (void)sink, (void)window;
-  return 0;
+  if (batch <= 0 || n <= 0 || n >= (1 << 26) || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads ||
+      q_heads / kv_heads > 16 || (head_dim != 64 && head_dim != 128) || sink < 0 || window < 1 ||
+      kv4::capacity(sink, window) >= (int64_t(1) << 30))
+    return 0;
+  return pattn4::workspace_for(batch, n, q_heads, head_dim,
+                               pattn4::splits(batch, n, q_heads / kv_heads, kv_heads, sink, window));
 }
 
 extern "C" int qx_prefill_attention_q4(const void* q, const void* k_new, const void* v_new, const void* k_codes,
@@ -313,7 +801,6 @@ extern "C" int qx_prefill_attention_q4(const void* q, const void* k_new, const v
                                        int batch, int n, int q_heads, int kv_heads, int head_dim, int group, int sink,
                                        int window, int64_t count, const int64_t* counts, float softmax_scale,
                                        void* workspace, size_t workspace_bytes, qx_stream_t stream) {
-  (void)workspace, (void)workspace_bytes;
   const int rc = kv4::check_ring("prefill_attention_q4", batch, kv_heads, head_dim, group, sink, window);
   if (rc != QX_OK) return rc;
   QX_REQUIRE(n >= 0 && q_heads > 0 && q_heads % kv_heads == 0 && q_heads / kv_heads <= 16,
@@ -326,6 +813,10 @@ extern "C" int qx_prefill_attention_q4(const void* q, const void* k_new, const v
   QX_REQUIRE(aligned(q, 16) && aligned(k_new, 16) && aligned(v_new, 16) && aligned(k_codes, 16) &&
                  aligned(v_codes, 16) && aligned(k_params, 16) && aligned(v_params, 16) && aligned(out, 16),
              "prefill_attention_q4: tensors must be 16-byte aligned");
+  const int nsplit = pattn4::splits(batch, n, q_heads / kv_heads, kv_heads, sink, window);
+  const size_t need = pattn4::workspace_for(batch, n, q_heads, head_dim, nsplit);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(QX_ERR_WORKSPACE, "prefill_attention_q4: workspace needs %zu bytes, 16-byte aligned", need);
   pattn4::Params p{};
   p.q = static_cast<const __half*>(q);
   p.kn = static_cast<const __half*>(k_new);
@@ -335,24 +826,28 @@ extern "C" int qx_prefill_attention_q4(const void* q, const void* k_new, const v
   p.vc = static_cast<const unsigned char*>(v_codes);
   p.vp = static_cast<const uint16_t*>(v_params);
   p.out = static_cast<__half*>(out);
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + int64_t(nsplit) * batch * n * q_heads * head_dim);
   p.counts = counts;
   p.count = count;
   p.cap = kv4::capacity(sink, window);
+  p.batch = batch;
   p.n = n;
   p.hq = q_heads;
   p.hkv = kv_heads;
   p.G = q_heads / kv_heads;
   p.sink = sink;
   p.window = window;
+  p.nsplit = nsplit;
   p.scale_log2 = (softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf(float(head_dim))) * 1.4426950408889634f;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (head_dim == 64)
-    e = group == 32 ? pattn4::launch<64, 2>(p, batch, st) : pattn4::launch<64, 1>(p, batch, st);
+    e = group == 32 ? pattn4::launch<64, 2>(p, st) : pattn4::launch<64, 1>(p, st);
   else
-    e = group == 32   ? pattn4::launch<128, 4>(p, batch, st)
-        : group == 64 ? pattn4::launch<128, 2>(p, batch, st)
-                      : pattn4::launch<128, 1>(p, batch, st);
+    e = group == 32   ? pattn4::launch<128, 4>(p, st)
+        : group == 64 ? pattn4::launch<128, 2>(p, st)
+                      : pattn4::launch<128, 1>(p, st);
   QX_CUDA_TRY(e, "prefill_attention_q4: launch");
   return check_launch("prefill_attention_q4");
 }
