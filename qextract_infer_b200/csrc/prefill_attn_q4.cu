@@ -10,18 +10,24 @@
 // group), positions outermost, so the group's heads share every key tile and
 // the rows of a CTA see nearly the same keys.  Tiles of 128 keys: the ring's
 // that any of its rows sees, then the chunk's up to the last row.
-//   warps 0-3, 4-7  softmax of row tile 0 and 1, one thread a row: S from TMEM,
-//                   the running maximum and sum in fp32, P in fp16 back to TMEM
-//                   over S.  O (fp32, TMEM) is rescaled only when the row's
-//                   maximum grew by more than 2^4, so P carries 2^11 at the
-//                   maximum last used and at most 2^15; both cancel in O / l.
-//   warps 8-11      loaders: ring rows are made fp16 (exactly: kv4.cuh) on the
+//   warp 0          an elected lane issues tcgen05.mma: S = Q K^T (both operands in
+//                   shared memory) and O += P V (P from TMEM).  As the last warp
+//                   it lost its issue slots to the others and each of its waits
+//                   took 300 clocks longer.
+//   warps 1-3       loaders: ring rows are made fp16 (exactly: kv4.cuh) on the
 //                   way to the 128-byte-swizzled K (K-major) and V (MN-major)
 //                   tiles, the chunk's rows copied; two stages each
-//   warp 12         one thread issues tcgen05.mma: S = Q K^T (both operands in
-//                   shared memory) and O += P V (P from TMEM).  The two row tiles
-//                   alternate: while one's softmax runs the other's products do.
-// TMEM: S/P of both tiles and O of both, 512 columns of the SM's 512.
+//   warps 4-7, 8-11 softmax of row tile 0 and 1, one thread a row: S from TMEM,
+//                   the running maximum and sum in fp32, P in fp16 back to
+//                   TMEM.  O (fp32, TMEM) is rescaled only when the row's
+//                   maximum grew by more than 2^4, so P carries 2^11 at the
+//                   maximum last used and at most 2^15; both cancel in O / l.
+// The two row tiles alternate: while one's softmax runs, the other's P V and next
+// Q K^T do.  A softmax thread takes its row of S to registers, and P goes over S:
+// TMEM holds S/P of both row tiles (256 columns) and O of both (2 D), the SM's 512
+// at D = 128.  (Steps of 64 keys with an S, P and O apart overlap more on paper,
+// but their products read Q twice as often: shared memory is then the bound, and
+// every barrier wait queues behind it: 197 us for the 2048-token chunk.)
 // Few rows (a short chunk after a long context): CTAs split the key tiles and a
 // second kernel joins their fp32 results.
 // Every wait is bounded (kWaitLimitNs, then QX_DEVERR_MBAR_TIMEOUT; the CTA's
@@ -39,21 +45,25 @@ namespace pattn4 {
 constexpr int ROWS = 128;        // rows of a tile: tcgen05's M
 constexpr int KT = 128;          // keys of a tile
 constexpr int STAGES = 2;
-constexpr int SOFTMAX_WARPS = 8, LOAD_WARPS = 4, MMA_WARP = SOFTMAX_WARPS + LOAD_WARPS;
-constexpr int THREADS = (MMA_WARP + 1) * 32;
+constexpr int LOAD_WARPS = 3, SOFTMAX_WARP0 = 1 + LOAD_WARPS, SOFTMAX_WARPS = 8;
+constexpr int THREADS = (SOFTMAX_WARP0 + SOFTMAX_WARPS) * 32;
+constexpr int GROUPS = KT / 8;  // 8-row groups of a key tile, dealt to the loader warps in turn
+constexpr int PASSES = (GROUPS + LOAD_WARPS - 1) / LOAD_WARPS;
+static_assert(SOFTMAX_WARP0 % 4 == 0, "a softmax warp's TMEM lanes are 32 (warp % 4) ..");
 constexpr float GROW = 4.f;      // log2 growth of a row's maximum that O is rescaled for
 constexpr float PSHIFT = 11.f;   // P carries 2^11: at most 2^15 with GROW, subnormal below 2^-25 of the maximum
 constexpr int MAX_SPLITS = 32;
 
 // barriers (8 bytes each)
 enum { FULL_K, EMPTY_K = FULL_K + STAGES, FULL_V = EMPTY_K + STAGES, EMPTY_V = FULL_V + STAGES,
-       S_FULL = EMPTY_V + STAGES, P_FULL = S_FULL + 2, O_FULL = P_FULL + 2, Q_FULL = O_FULL + 2, NBARS };
+       S_FULL = EMPTY_V + STAGES, P_FULL = S_FULL + 2, PV_DONE = P_FULL + 2, O_FULL = PV_DONE + 2, Q_FULL = O_FULL + 2, NBARS };
 
 template <int D>
 struct Smem {
   static constexpr int TILE = ROWS * D * 2;  // bytes of a Q, K or V tile
   static constexpr int Q = 0, K = 2 * TILE, V = K + STAGES * TILE, BARS = V + STAGES * TILE;
-  static constexpr int TMEM = BARS + NBARS * 8, GAVE_UP = TMEM + 4, BYTES = GAVE_UP + 4 + 1024;  // + alignment slack
+  static constexpr int TMEM = BARS + NBARS * 8, GAVE_UP = TMEM + 4, LIST = GAVE_UP + 4;
+  static constexpr int BYTES = LIST + 128 + 1024;  // + alignment slack
 };
 
 struct Params {
@@ -114,57 +124,63 @@ __device__ __forceinline__ void bar_wait(uint32_t b, uint32_t parity, volatile u
 // shared-memory operand of 128-byte-swizzled rows (64 values), 8-row atoms 1024 B
 // apart, tiles of 64 values `half` bytes apart.  K-major (Q, K): the rows are M
 // or N, `half` unused; MN-major (V): the rows are the product's K, `half` steps N.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t half) {
-  return uint64_t((saddr >> 4) & 0x3FFF) | (uint64_t(half >> 4) << 16) | (uint64_t(64) << 32) | (uint64_t(1) << 46) |
-         (uint64_t(2) << 61);
-}
+// Only the low word holds the address.
+constexpr uint32_t DESC_HI = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t half) { return (saddr >> 4) | (half >> 4) << 16; }
 // kind::f16 instruction descriptor: D f32, A and B f16, M = 128; MN_B: B is MN-major
 template <int N, bool MN_B>
 constexpr uint32_t idesc() {
   return (1u << 4) | (MN_B ? 1u << 16 : 0u) | (uint32_t(N >> 3) << 17) | (uint32_t(ROWS >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t id, uint32_t acc) {
   asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(acc)
+      "{ .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p; }" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(id), "r"(acc), "r"(DESC_HI)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t id, uint32_t acc) {
   asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(acc)
+      "{ .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %4, 0;\n mov.b64 b, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p; }" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(id), "r"(acc), "r"(DESC_HI)
       : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint32_t b) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(b) : "memory");
 }
+// one lane of a converged warp (the same one every time)
+__device__ __forceinline__ bool elected() {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p; }" : "=r"(ok));
+  return ok != 0;
+}
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
 #define QX_R8(v, i) "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3]), "=f"(v[i + 4]), "=f"(v[i + 5]), "=f"(v[i + 6]), "=f"(v[i + 7])
-#define QX_W8(v, i) "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7])
-// 32 columns of the warp's 32 rows, a row a thread
-__device__ __forceinline__ void tmem_ld(uint32_t addr, float (&v)[32]) {
+// Columns of the warp's 32 rows, a row a thread.  Load and wait are one statement:
+// between them a value still on its way could be copied or spilled.
+__device__ __forceinline__ void tmem_ld64(uint32_t addr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+      "}, [%64];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : QX_R8(v, 0), QX_R8(v, 8), QX_R8(v, 16), QX_R8(v, 24), QX_R8(v, 32), QX_R8(v, 40), QX_R8(v, 48), QX_R8(v, 56)
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;"
       : QX_R8(v, 0), QX_R8(v, 8), QX_R8(v, 16), QX_R8(v, 24)
-      : "r"(addr));
-}
-// waits for the loads before it; the values pass through so that no use of them moves above it
-__device__ __forceinline__ void tmem_ld_wait(float (&v)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" : QX_W8(v, 0), QX_W8(v, 8), QX_W8(v, 16), QX_W8(v, 24)::"memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"f"(v[0]),
-      "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
-      "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]),
-      "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]),
-      "f"(v[29]), "f"(v[30]), "f"(v[31]), "r"(addr)
+      : "r"(addr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
@@ -174,12 +190,48 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]
       "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : QX_R8(v, 0), QX_R8(v, 8)
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const float (&v)[16]) {
+  uint32_t u[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[i]);
+  tmem_st16(addr, u);
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// two fp32 operations an instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{ .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      "fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x; }"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{ .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n"
+      "mov.b64 {%0, %1}, x; }"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));  // NaN if one is
+  return d;
 }
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
   __half2 h = __floats2half2_rn(a, b);
@@ -259,58 +311,58 @@ __device__ __noinline__ void redo_row(const Params& p, const Ring& ring, int b, 
 }
 
 // The key tiles that some row of [rmin, rmax] (chunk positions) may see, as
-// ranges of tile numbers: of the ring's slots the sinks, those up to the newest
-// token's and those after it (older, where the ring has wrapped), then of the
-// chunk's keys the sinks and the window.  Hidden from rmin is hidden from all
-// for the ring; a range starts after the one before it.
+// ranges of tile numbers: of the ring's slots the sinks (0), those up to the
+// newest token's (1) and those after it (2: older, where the ring has wrapped),
+// then of the chunk's keys the sinks (3) and the window (4).  What the ring hides
+// from rmin it hides from all; a range starts after the one before it.  And the
+// keys [lo, hi) of each part that all of the rows see.  Made once, in shared memory.
 struct Tiles {
-  int start[5], len[5], total;
-  __device__ Tiles(const Ring& r, int rmin, int rmax, int sink, int window) {
-    const int held = r.valid - sink;  // ring tokens (below zero: sinks only)
-    // visible to rmin: ring index w <= newest with w >= newest - window + 2 + rmin, or w > newest with w >= newest + 2 + rmin
-    const int lo1 = max(0, r.newest - window + 2 + rmin), lo2 = r.newest + 2 + rmin;
-    const int first[5] = {0, sink + lo1, sink + lo2, 0, max(0, rmin - window + 1)};
-    const int last[5] = {min(r.valid, sink) - 1, r.newest >= 0 ? sink + min(r.newest, held - 1) : -1,
-                         r.newest >= 0 ? sink + held - 1 : -1, min(r.sinks - 1, rmax), rmax};
+  int start[5], end[5], lo[5], hi[5], total;
+
+  __device__ void make(const Ring& r, int rmin, int rmax, int sink, int window) {
+    const int held = r.valid - sink, last = min(r.newest, held - 1);  // ring tokens (below zero: sinks only)
+    const bool some = r.newest >= 0;
+    // row p sees ring index w <= newest from newest - window + 2 + p, w > newest from newest + 2 + p
+    const int from = r.newest - window + 2;
+    const int first[5] = {0, sink + max(0, from + rmin), sink + r.newest + 2 + rmin, 0, max(0, rmin - window + 1)};
+    const int stop[5] = {min(r.valid, sink), some ? sink + last + 1 : 0, some ? r.valid : 0, min(r.sinks, rmax + 1), rmax + 1};
     int next = 0;
     total = 0;
-#pragma unroll
     for (int k = 0; k < 5; ++k) {
       if (k == 3) next = 0;
       start[k] = max(next, first[k] / KT);
-      len[k] = last[k] >= first[k] ? max(0, last[k] / KT + 1 - start[k]) : 0;
-      if (len[k] > 0) next = start[k] + len[k];
-      total += len[k];
+      end[k] = stop[k] > first[k] ? max(start[k], (stop[k] - 1) / KT + 1) : start[k];
+      if (end[k] > start[k]) next = end[k];
+      total += end[k] - start[k];
     }
-  }
-  // tile t of the list: its number, and whether it is the ring's
-  __device__ int at(int t, bool& of_ring) const {
-    int idx = 0;
-    of_ring = true;
-    bool found = false;
-#pragma unroll
-    for (int k = 0; k < 5; ++k) {
-      if (!found && t < len[k]) {
-        idx = start[k] + t;
-        of_ring = k < 3;
-        found = true;
-      }
-      t -= len[k];
-    }
-    return idx;
+    lo[0] = 0, hi[0] = stop[0];
+    lo[1] = sink + max(0, from + rmax), hi[1] = stop[1];
+    lo[2] = sink + r.newest + 2 + rmax, hi[2] = stop[2];
+    lo[3] = 0, hi[3] = min(r.sinks, rmin + 1);
+    lo[4] = max(0, rmax - window + 1), hi[4] = rmin + 1;
+    if (lo[1] <= hi[0] && hi[1] > hi[0]) hi[0] = hi[1];  // the sinks and the window meet
+    if (lo[4] <= hi[3] && hi[4] > hi[3]) hi[3] = hi[4];
   }
 };
 
-// does every row of [rmin, rmax] see every key of the tile?
-__device__ __forceinline__ bool all_seen(const Ring& r, bool of_ring, int k0, int rmin, int rmax, int sink, int window) {
-  const int k1 = k0 + KT - 1;
-  if (!of_ring) return k1 <= rmin && (k0 > rmax - window || k1 < r.sinks);
-  if (k1 >= r.valid) return false;
-  const int w0 = max(k0 - sink, 0), w1 = k1 - sink;
-  if (w1 < 0) return true;
-  if (w0 <= r.newest && w0 < r.newest - window + 2 + rmax) return false;
-  return w1 <= r.newest || max(w0, r.newest + 1) >= r.newest + 2 + rmax;
-}
+// a walk over the list from tile t on
+struct Walk {
+  int k, tile;
+  __device__ Walk(const Tiles& l, int t) : k(0) {
+    while (k < 4 && t >= l.end[k] - l.start[k]) {
+      t -= l.end[k] - l.start[k];
+      ++k;
+    }
+    tile = l.start[k] + t;
+  }
+  __device__ void next(const Tiles& l) {
+    if (++tile < l.end[k]) return;
+    while (++k < 5 && l.start[k] >= l.end[k]) {
+    }
+    if (k < 5) tile = l.start[k];
+  }
+  __device__ bool of_ring() const { return k < 3; }
+};
 
 // bits of [lo, hi) within [base, base + 32)
 __device__ __forceinline__ uint32_t bits(int lo, int hi, int base) {
@@ -333,7 +385,7 @@ __device__ __forceinline__ void put_block(unsigned char* tile, int row, int c, i
 // loaded a tile ahead, stored as fp16 when the stage is free.
 template <int D, int NG, bool VALUES>
 struct RingTile {
-  static constexpr int NI = D / 32, PASSES = KT / (LOAD_WARPS * 8), PW = NG == 4 ? 2 : 1;
+  static constexpr int NI = D / 32, PW = NG == 4 ? 2 : 1;
   uint32_t w[PASSES][NI], pr[PASSES][PW];
 
   __device__ __forceinline__ void load(const Params& p, int64_t base, int k0, int valid, int warp, int lane) {
@@ -343,7 +395,7 @@ struct RingTile {
 #pragma unroll
     for (int s = 0; s < PASSES; ++s) {
       // a free slot reads the last valid one's row (the tile may end behind the storage)
-      const int64_t row = base + min(k0 + s * (LOAD_WARPS * 8) + warp * 8 + r8, valid - 1);
+      const int64_t row = base + min(k0 + (s * LOAD_WARPS + warp) * 8 + r8, valid - 1);
       if constexpr (NI == 4) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(codes + row * (D / 2)) + c);
         w[s][0] = v.x, w[s][1] = v.y, w[s][2] = v.z, w[s][3] = v.w;
@@ -365,7 +417,8 @@ struct RingTile {
     const int c = lane & 3, q = lane >> 2, r8 = (q >> 1) | ((q & 1) << 2);
 #pragma unroll
     for (int s = 0; s < PASSES; ++s) {
-      const int row = s * (LOAD_WARPS * 8) + warp * 8 + r8;
+      if (s * LOAD_WARPS + warp >= GROUPS) break;
+      const int row = (s * LOAD_WARPS + warp) * 8 + r8;
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         const uint32_t pair = NG == 1 ? pr[s][0] * 0x10001u : prmt(pr[s][n >> 1], 0u, (n & 1) ? 0x3232u : 0x1010u);
@@ -404,7 +457,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sb = smem_u32(smem);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   volatile unsigned* gave_up = reinterpret_cast<volatile unsigned*>(smem + L::GAVE_UP);
   auto bar = [&](int i) { return sb + L::BARS + 8 * i; };
   if (tid == 0) {
@@ -418,12 +471,13 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
     for (int x = 0; x < 2; ++x) {
       bar_init(bar(S_FULL + x), 1);
       bar_init(bar(P_FULL + x), 4);
+      bar_init(bar(PV_DONE + x), 1);
       bar_init(bar(O_FULL + x), 1);
     }
     bar_init(bar(Q_FULL), SOFTMAX_WARPS);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == MMA_WARP) {
+  if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(sb + L::TMEM) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -442,26 +496,39 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
   const int rmin = row0 / p.G, rmax = last_row / p.G;
   const int ntile = last_row - row0 >= ROWS ? 2 : 1;  // row tiles with rows
   const Ring ring(kv4::count_of(p.counts, p.count, b), p.sink, p.window);
-  const Tiles tiles(ring, rmin, rmax, p.sink, p.window);
+  Tiles& tiles = *reinterpret_cast<Tiles*>(smem + L::LIST);
+  static_assert(sizeof(Tiles) <= 128, "room for the tile list");
+  if (tid == 0) tiles.make(ring, rmin, rmax, p.sink, p.window);
+  __syncthreads();
   const int t0 = int(int64_t(tiles.total) * split / p.nsplit), t1 = int(int64_t(tiles.total) * (split + 1) / p.nsplit);
   const int T = t1 - t0;
-  const uint32_t tmem_s[2] = {tmem, tmem + KT}, tmem_o[2] = {tmem + 2 * KT, tmem + 2 * KT + D};
+  // TMEM columns: S of row tile x, then its P, at 128 x; its O at 256 + D x
 
-  if (warp < SOFTMAX_WARPS) {
+  if (warp >= SOFTMAX_WARP0) {
     // --------------------------------------------------------------- softmax
-    const int x = warp >> 2, quad = warp & 3;
+    const int x = (warp - SOFTMAX_WARP0) >> 2, quad = warp & 3;
     const uint32_t lanes = uint32_t(quad * 32) << 16;
-    {  // this warp's 32 rows of Q, D / 8 lanes a row
-      constexpr int LPR = D / 8;
-      for (int r = lane / LPR; r < 32; r += 32 / LPR) {
-        const int tr = quad * 32 + r, row = row0 + x * ROWS + tr, ch = lane % LPR;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row < rows) {
-          const int pos = row / p.G, hg = row - pos * p.G;
-          v = __ldg(reinterpret_cast<const uint4*>(p.q + ((int64_t(b) * p.n + pos) * p.hq + kvh * p.G + hg) * D) + ch);
+    {  // this warp's 32 rows of Q, D / 8 lanes a row, eight loads in flight
+      constexpr int LPR = D / 8, TURNS = LPR;
+      const int ch = lane % LPR;
+#pragma unroll
+      for (int u0 = 0; u0 < TURNS; u0 += 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int row = row0 + x * ROWS + quad * 32 + (u0 + u) * (32 / LPR) + lane / LPR;
+          v[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (row < rows) {
+            const int pos = row / p.G, hg = row - pos * p.G;
+            v[u] = __ldg(reinterpret_cast<const uint4*>(p.q + ((int64_t(b) * p.n + pos) * p.hq + kvh * p.G + hg) * D) + ch);
+          }
         }
-        *reinterpret_cast<uint4*>(smem + L::Q + x * L::TILE + (ch >> 3) * (ROWS * 128) + tr * 128 +
-                                  (((ch & 7) ^ (tr & 7)) << 4)) = v;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int tr = quad * 32 + (u0 + u) * (32 / LPR) + lane / LPR;
+          *reinterpret_cast<uint4*>(smem + L::Q + x * L::TILE + (ch >> 3) * (ROWS * 128) + tr * 128 +
+                                    (((ch & 7) ^ (tr & 7)) << 4)) = v[u];
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -471,48 +538,45 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
     const int pos = min(row, rows - 1) / p.G, hg = min(row, rows - 1) - pos * p.G;
     const int64_t orow = (int64_t(b) * p.n + pos) * p.hq + kvh * p.G + hg;
     float m_used = -INFINITY, l = 0.f;
+    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
     if (x < ntile) {
-      const uint32_t ts = tmem_s[x] + lanes, to = tmem_o[x] + lanes;
+      const uint32_t ts = tmem + KT * x + lanes, to = tmem + 2 * KT + x * D + lanes;
+      Walk walk(tiles, t0);
+      int lo[5], hi[5];
+#pragma unroll
+      for (int k = 0; k < 5; ++k) lo[k] = tiles.lo[k], hi[k] = tiles.hi[k] - KT;
       for (int it = 0; it < T; ++it) {
-        bool of_ring;
-        const int k0 = tiles.at(t0 + it, of_ring) * KT;
-        const bool full = all_seen(ring, of_ring, k0, rmin, rmax, p.sink, p.window);
-        // the keys of the tile that this row sees, a bit each
-        uint32_t seen[KT / 32];
-        if (!full) {
-          if (of_ring) {
-            const int sk = p.sink - k0, nw = sk + ring.newest;  // from the tile's first slot: first ring slot, newest
-            const int end = ring.valid - k0;
-#pragma unroll
-            for (int j = 0; j < KT / 32; ++j)
-              seen[j] = bits(0, min(sk, end), 32 * j) |
-                        bits(max(sk, nw - p.window + 2 + pos), min(nw + 1, end), 32 * j) |
-                        bits(max(nw + 1, nw + 2 + pos), end, 32 * j);
-          } else {
-#pragma unroll
-            for (int j = 0; j < KT / 32; ++j)
-              seen[j] = bits(0, min(pos + 1, ring.sinks) - k0, 32 * j) | bits(pos - p.window + 1 - k0, pos + 1 - k0, 32 * j);
-          }
-        }
-        auto hide = [&](float (&v)[32], uint32_t m) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = (m >> e) & 1u ? v[e] : -INFINITY;
-        };
+        const bool of_ring = walk.of_ring();
+        const int k0 = walk.tile * KT;
+        walk.next(tiles);
+        // does every row see every key of the tile?
+        const bool full = of_ring ? (k0 >= lo[0] && k0 <= hi[0]) || (k0 >= lo[1] && k0 <= hi[1]) || (k0 >= lo[2] && k0 <= hi[2])
+                                  : (k0 >= lo[3] && k0 <= hi[3]) || (k0 >= lo[4] && k0 <= hi[4]);
         bar_wait(bar(S_FULL + x), it & 1, gave_up);
         fence_after();
-        float v[2][32];
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        tmem_ld(ts, v[0]);
+        float v[KT];
+        tmem_ld64(ts, v);
+        tmem_ld64(ts + 64, v + 64);
+        if (!full) {  // the keys of the tile that this row sees, a bit each
 #pragma unroll
-        for (int j = 0; j < KT / 32; ++j) {
-          tmem_ld_wait(v[j & 1]);
-          if (j + 1 < KT / 32) tmem_ld(ts + 32 * (j + 1), v[(j + 1) & 1]);
-          if (!full) hide(v[j & 1], seen[j]);
+          for (int j = 0; j < 4; ++j) {
+            uint32_t seen;
+            if (of_ring) {
+              const int sk = p.sink - k0, nw = sk + ring.newest;  // from the tile's first slot: first ring slot, newest
+              const int end = ring.valid - k0;
+              seen = bits(0, min(sk, end), 32 * j) | bits(max(sk, nw - p.window + 2 + pos), min(nw + 1, end), 32 * j) |
+                     bits(max(nw + 1, nw + 2 + pos), end, 32 * j);
+            } else {
+              seen = bits(0, min(pos + 1, ring.sinks) - k0, 32 * j) | bits(pos - p.window + 1 - k0, pos + 1 - k0, 32 * j);
+            }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], v[j & 1][e]);
+            for (int e = 0; e < 32; ++e) v[32 * j + e] = (seen >> e) & 1u ? v[32 * j + e] : -INFINITY;
+          }
         }
-        tmem_ld(ts, v[0]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < KT; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], v[e], v[e + 1]);
+        const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * p.scale_log2;
         const bool grew = top > m_used + GROW;
         if (__any_sync(0xffffffffu, grew)) {
           const float m_new = fmaxf(m_used, top);
@@ -520,37 +584,34 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
           const float alpha = ex2(m_used - mb);
           m_used = m_new;
           l *= alpha;
-          if (it > 0) {  // P V of the tile before has ended: its commit came with this S
-            tmem_ld_wait(v[0]);
-            float o[32];
+          if (it > 0) {  // P V of the tile before has ended: this S was computed after it
+            float o[16];
 #pragma unroll 1
-            for (int j = 0; j < D; j += 32) {
-              tmem_ld(to + j, o);
-              tmem_ld_wait(o);
+            for (int j = 0; j < D; j += 16) {
+              tmem_ld16(to + j, o);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] *= alpha;
-              tmem_st32(to + j, o);
+              for (int e = 0; e < 16; ++e) o[e] *= alpha;
+              tmem_st16(to + j, o);
             }
           }
         }
-        const float shift = PSHIFT - (m_used == -INFINITY ? 0.f : m_used);
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        // a NaN or +infinity among the scores makes the row NaN
+        const float shift = !(top < INFINITY) ? top - top : PSHIFT - (m_used == -INFINITY ? 0.f : m_used);
+        const float2 shift2 = make_float2(shift, shift);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int j = 0; j < KT / 32; ++j) {
-          tmem_ld_wait(v[j & 1]);
-          if (j + 1 < KT / 32) tmem_ld(ts + 32 * (j + 1), v[(j + 1) & 1]);
-          if (!full) hide(v[j & 1], seen[j]);
+        for (int j = 0; j < KT; j += 32) {
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float a = ex2(fmaf(v[j & 1][e], p.scale_log2, shift)), c = ex2(fmaf(v[j & 1][e + 1], p.scale_log2, shift));
-            sum[e & 2] += a;
-            sum[(e & 2) + 1] += c;
-            pk[e / 2] = pack_h2(a, c);
+            const float2 t = fma2(make_float2(v[j + e], v[j + e + 1]), scale2, shift2);
+            const float2 w = make_float2(ex2(t.x), ex2(t.y));
+            sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], w);
+            pk[e / 2] = pack_h2(w.x, w.y);
           }
-          tmem_st16(ts + 16 * j, pk);  // columns 16 j .. of S, all read by now
+          tmem_st16(ts + j / 2, pk);  // over S, which is in registers
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_st_wait();
         fence_before();
         __syncwarp();
@@ -567,8 +628,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
         bool fine = true;
 #pragma unroll 1
         for (int j = 0; j < D; j += 32) {
-          tmem_ld(to + j, v);
-          tmem_ld_wait(v);
+          tmem_ld32(to + j, v);
           uint32_t h[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
@@ -581,7 +641,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
             for (int e = 0; e < 16; e += 4)
               *reinterpret_cast<uint4*>(p.out + orow * D + j + 2 * e) = make_uint4(h[e], h[e + 1], h[e + 2], h[e + 3]);
         }
-        uint32_t redo = __ballot_sync(0xffffffffu, !fine && row < rows);
+        // a sum that is not finite has a visible score that is not: the whole row is NaN, and is so already
+        uint32_t redo = __ballot_sync(0xffffffffu, !fine && fabsf(l) < INFINITY && row < rows);
         for (; redo; redo &= redo - 1) {
           const int r = row0 + x * ROWS + quad * 32 + __ffs(redo) - 1;
           redo_row<D, NG>(p, ring, b, kvh * p.G + r % p.G, r / p.G, lane);
@@ -592,8 +653,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
         if (T > 0) {
 #pragma unroll 1
           for (int j = 0; j < D; j += 32) {
-            tmem_ld(to + j, v);
-            tmem_ld_wait(v);
+            tmem_ld32(to + j, v);
             if (row < rows)
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
@@ -602,15 +662,16 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
         }
       }
     }
-  } else if (warp < MMA_WARP) {
+  } else if (warp > 0) {
     // --------------------------------------------------------------- loaders
-    const int lw = warp - SOFTMAX_WARPS;
+    const int lw = warp - 1;
     const int64_t base = (int64_t(b) * p.hkv + kvh) * p.cap;
     const int64_t first = (int64_t(b) * p.n * p.hkv + kvh) * D, stride = int64_t(p.hkv) * D;
     RingTile<D, NG, false> kr;
     RingTile<D, NG, true> vr;
-    bool of_ring = false;
-    int k0 = T > 0 ? tiles.at(t0, of_ring) * KT : 0;
+    Walk walk(tiles, t0);
+    bool of_ring = T > 0 && walk.of_ring();
+    int k0 = walk.tile * KT;
     if (of_ring) {
       kr.load(p, base, k0, ring.valid, lw, lane);
       vr.load(p, base, k0, ring.valid, lw, lane);
@@ -624,8 +685,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
       const int st = it % STAGES;
       unsigned char* kt = smem + L::K + st * L::TILE;
       unsigned char* vt = smem + L::V + st * L::TILE;
-      bool next_ring = false;
-      const int next = it + 1 < T ? tiles.at(t0 + it + 1, next_ring) * KT : 0;
+      walk.next(tiles);
+      const bool next_ring = it + 1 < T && walk.of_ring();
+      const int next = walk.tile * KT;
       if (it >= STAGES) bar_wait(bar(EMPTY_K + st), (it / STAGES - 1) & 1, gave_up);
       if (of_ring) {
         kr.store(kt, lw, lane);
@@ -647,52 +709,63 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
       of_ring = next_ring;
       k0 = next;
     }
-  } else if (lane == 0 && T > 0) {
+  } else {
     // -------------------------------------------------------------- products
-    auto scores = [&](int x, int st) {  // S_x = Q_x K^T
+    // Every value here is the warp's own: what the products' operands are made of
+    // then stays in uniform registers (moved there for each product, from the
+    // lanes' registers, they held the issue up: 90 clocks a product instead of 50).
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const int n = __shfl_sync(0xffffffffu, T, 0), nx = __shfl_sync(0xffffffffu, ntile, 0);
+    const uint32_t q_lo = desc_lo(sb + L::Q, 16), k_lo = desc_lo(sb + L::K, 16), v_lo = desc_lo(sb + L::V, KT * 128);
+    auto scores = [&](int x, int it) {  // S_x = Q_x K^T of tile it
+      const uint32_t ql = q_lo + x * (L::TILE >> 4), kl = k_lo + it % STAGES * (L::TILE >> 4);
+      if (elected()) {
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t at = (k >> 2) * (ROWS * 128) + (k & 3) * 32;
-        mma_ss(tmem_s[x], sw128_desc(sb + L::Q + x * L::TILE + at, 16), sw128_desc(sb + L::K + st * L::TILE + at, 16),
-               idesc<KT, false>(), k != 0);
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t at = ((k >> 2) * (ROWS * 128) + (k & 3) * 32) >> 4;
+          mma_ss(tm + KT * x, ql + at, kl + at, idesc<KT, false>(), k != 0);
+        }
+        mma_commit(bar(S_FULL + x));
+        if (x == nx - 1) mma_commit(bar(EMPTY_K + it % STAGES));
       }
+      __syncwarp();
     };
-    bar_wait(bar(Q_FULL), 0, gave_up);
-    bar_wait(bar(FULL_K), 0, gave_up);
-    fence_after();
-    for (int x = 0; x < ntile; ++x) {
-      scores(x, 0);
-      mma_commit(bar(S_FULL + x));
+    auto values = [&](int x, int it) {  // O_x += P_x V of tile it: 16 keys are 8 columns of P and 16 rows of V
+      const uint32_t vl = v_lo + it % STAGES * (L::TILE >> 4);
+      if (elected()) {
+#pragma unroll
+        for (int k = 0; k < KT / 16; ++k)
+          mma_ts(tm + 2 * KT + x * D, tm + KT * x + 8 * k, vl + k * (2048 >> 4), idesc<D, true>(), (it | k) != 0);
+        mma_commit(bar(it + 1 < n ? PV_DONE + x : O_FULL + x));
+        if (x == nx - 1) mma_commit(bar(EMPTY_V + it % STAGES));
+      }
+      __syncwarp();
+    };
+    if (n > 0) {
+      bar_wait(bar(Q_FULL), 0, gave_up);
+      bar_wait(bar(FULL_K), 0, gave_up);
+      fence_after();
+      for (int x = 0; x < nx; ++x) scores(x, 0);
     }
-    mma_commit(bar(EMPTY_K));
-    for (int it = 0; it < T; ++it) {
+    for (int it = 0; it < n; ++it) {
       const int st = it % STAGES, nst = (it + 1) % STAGES;
       bar_wait(bar(FULL_V + st), (it / STAGES) & 1, gave_up);
-      for (int x = 0; x < ntile; ++x) {
+      for (int x = 0; x < nx; ++x) {
         bar_wait(bar(P_FULL + x), it & 1, gave_up);
         fence_after();
-#pragma unroll
-        for (int k = 0; k < KT / 16; ++k)  // O_x += P_x V: 16 keys are 8 columns of P and 16 rows of V
-          mma_ts(tmem_o[x], tmem_s[x] + 8 * k, sw128_desc(sb + L::V + st * L::TILE + k * 2048, KT * 128),
-                 idesc<D, true>(), (it | k) != 0);
-        if (x == ntile - 1) mma_commit(bar(EMPTY_V + st));
-        if (it + 1 < T) {  // in order after P V: S_x overwrites P_x
-          if (x == 0) {
-            bar_wait(bar(FULL_K + nst), ((it + 1) / STAGES) & 1, gave_up);
-            fence_after();
-          }
-          scores(x, nst);
-          mma_commit(bar(S_FULL + x));
-          if (x == ntile - 1) mma_commit(bar(EMPTY_K + nst));
-        } else {
-          mma_commit(bar(O_FULL + x));
-        }
+        values(x, it);
+        if (it + 1 == n) continue;
+        if (x == 0) bar_wait(bar(FULL_K + nst), ((it + 1) / STAGES) & 1, gave_up);
+        // the next S overwrites P: products with different accumulators need not run in the order of their issue
+        bar_wait(bar(PV_DONE + x), it & 1, gave_up);
+        fence_after();
+        scores(x, it + 1);
       }
     }
   }
   fence_before();
   __syncthreads();
-  if (warp == MMA_WARP) {
+  if (warp == 0) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
@@ -728,7 +801,7 @@ __global__ void __launch_bounds__(128) prefill_attn_q4_merge_kernel(const __grid
     fine = fine && fabsf(acc[e] * inv) <= 65504.f;
     p.out[row * D + 32 * e + lane] = __float2half_rn(acc[e] * inv);
   }
-  if (__any_sync(0xffffffffu, !fine)) {
+  if (__any_sync(0xffffffffu, !fine) && fabsf(inv) > 0.f) {  // 1 / l: 0 or NaN where a visible score is not finite
     const int h = int(row % p.hq), b = int(row / p.hq / p.n), pos = int(row / p.hq % p.n);
     const Ring ring(kv4::count_of(p.counts, p.count, b), p.sink, p.window);
     redo_row<D, NG>(p, ring, b, h, pos, lane);

@@ -27,6 +27,13 @@ def C():
     return _C
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out(C):
+    C.device_error()
+    yield
+    C.check_device_error("4-bit ring attention")
+
+
 def _check(got, ref, keys, D, msg=""):
     out, weight, size = ref
     got = got.astype(np.float64)
