@@ -68,47 +68,60 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const Params p) {
     s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
   }
   const bool lo = l < LPH / 2;  // first half of the head: its partner enters negated
+  const int vfirst = p.hq + p.hkv, warp_h = h0 - (threadIdx.x % 32) / LPH;
+  float ss[HPL];
 #pragma unroll
   for (int i = 0; i < HPL; ++i) {
-    const int h = h0 + i * HPP;
     const uint32_t xd[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-    float f[8], ss = 0.f;
+    ss[i] = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 t = h2_to_f2(xd[j]);
-      f[2 * j] = t.x;
-      f[2 * j + 1] = t.y;
-      ss = fmaf(t.x, t.x, ss);
-      ss = fmaf(t.y, t.y, ss);
+      ss[i] = fmaf(t.x, t.x, ss[i]);
+      ss[i] = fmaf(t.y, t.y, ss[i]);
     }
 #pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = 1.0f / sqrtf(ss * (1.0f / D) + p.eps);
+    for (int o = LPH / 2; o > 0; o >>= 1) ss[i] += __shfl_xor_sync(0xffffffffu, ss[i], o);
+  }
+  // the root and the division once: lane i of a group does head i's
+  float root = ss[0];
+#pragma unroll
+  for (int i = 1; i < HPL; ++i) root = l == i ? ss[i] : root;
+  root = 1.0f / sqrtf(root * (1.0f / D) + p.eps);
+#pragma unroll
+  for (int i = 0; i < HPL; ++i) {
+    const int h = h0 + i * HPP;
+    const float r = HPL == 1 ? root : __shfl_sync(0xffffffffu, root, i, LPH);
+    if (warp_h + i * HPP >= vfirst) {  // the warp's heads are values, or past the last
+      if (h < heads) p.v[(tok * p.hkv + (h - vfirst)) * LPH + l] = x[i];
+      continue;
+    }
+    const uint32_t xd[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
     const uint4 w = h < p.hq ? wq : wk;
     const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
     uint32_t yd[4], od[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 g = h2_to_f2(wd[j]);
-      const __half2 y = __floats2half2_rn((f[2 * j] * r) * g.x, (f[2 * j + 1] * r) * g.y);
+      const float2 f = h2_to_f2(xd[j]), g = h2_to_f2(wd[j]);
+      const __half2 y = __floats2half2_rn((f.x * r) * g.x, (f.y * r) * g.y);
       yd[j] = *reinterpret_cast<const uint32_t*>(&y);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t pd = __shfl_xor_sync(0xffffffffu, yd[j], LPH / 2);
+      uint32_t pd = __shfl_xor_sync(0xffffffffu, yd[j], LPH / 2);
+      pd ^= lo ? 0x80008000u : 0u;
       const float2 y = h2_to_f2(yd[j]), t = h2_to_f2(pd);
-      const float rx = lo ? -t.x : t.x, ry = lo ? -t.y : t.y;
       const __half2 o =
-          __floats2half2_rn(__fadd_rn(__fmul_rn(y.x, c[2 * j]), __fmul_rn(rx, s[2 * j])),
-                            __fadd_rn(__fmul_rn(y.y, c[2 * j + 1]), __fmul_rn(ry, s[2 * j + 1])));
+          __floats2half2_rn(__fadd_rn(__fmul_rn(y.x, c[2 * j]), __fmul_rn(t.x, s[2 * j])),
+                            __fadd_rn(__fmul_rn(y.y, c[2 * j + 1]), __fmul_rn(t.y, s[2 * j + 1])));
       od[j] = *reinterpret_cast<const uint32_t*>(&o);
     }
     if (h < p.hq)
       p.q[(tok * p.hq + h) * LPH + l] = make_uint4(od[0], od[1], od[2], od[3]);
-    else if (h < p.hq + p.hkv)
+    else if (h < vfirst)
       p.k[(tok * p.hkv + (h - p.hq)) * LPH + l] = make_uint4(od[0], od[1], od[2], od[3]);
     else if (h < heads)
-      p.v[(tok * p.hkv + (h - p.hq - p.hkv)) * LPH + l] = x[i];
+      p.v[(tok * p.hkv + (h - vfirst)) * LPH + l] = x[i];
   }
 }
 

@@ -11,15 +11,20 @@
 //       |s (c - z)| would pass the largest finite fp16 number
 // so |x - s (c - z)| <= s / 2 (clamping loses nothing more: hi <= 15 s + lo).
 // A group holding a NaN or an infinity gets the scale NaN: it reads as NaN.
-// s is found by rounding up in three steps (64-bit quotient to fp32 to fp16 to
-// 7 bits), which composes; x / s is the IEEE fp32 quotient of an 11-bit by a
-// 7-bit number: one that is no tie is at least 2^-12 away from any (near k + 1/2,
-// x - (k + 1/2) s is a whole multiple of the smaller of their units), so its rint
-// is the real quotient's.
+// s is found by rounding up in fp32 (hi - lo, then its fifteenth), to fp16, to 7
+// bits: a candidate s and 15 s are numbers of each of those formats, so each step
+// keeps which of them are large enough.  x / s (11 bits by 7 bits) is a tie or at
+// least 2^-12 away from one: near k + 1/2, x - (k + 1/2) s is a whole multiple of
+// the smaller of their units.  So x times the rounded 1 / s (off by less than
+// 2^-18) is rounded to a multiple of 2^-13 first: ties become exact ties, and
+// nothing else reaches one.
 //
 // Bound: HBM (2 bytes read per value, 0.53 written; the read-back the reverse).
-// D / 8 lanes hold one (token, head) row, 8 values each: the group's minimum and
-// maximum are butterflies over group / 8 lanes.
+// Four lanes hold one (token, head) row, lane c the blocks 4 i + c: its codes are
+// 16 bytes side by side in the cache (8 at D = 64), a group of 32 is one block of
+// each of the four lanes, and a row's loads are all in flight at once.  (With
+// D / 8 lanes a row, one block each, and 64-bit index divisions: append of 2048
+// tokens x 8 heads and read-back of 4096 slots 29.6 us.)
 #include <algorithm>
 
 #include "kv4.cuh"
@@ -28,148 +33,162 @@
 namespace qx {
 namespace ring4 {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, LANES = 4, ROWS = THREADS / LANES;  // rows of a CTA
 
 struct AppendParams {
-  uint32_t* codes[2];
+  unsigned char* codes[2];
   uint16_t* params[2];
-  const uint4* fresh[2];
+  const __half* fresh[2];
   const int64_t* counts;
-  int64_t count, rows;  // rows: batch * tokens * kv_heads
-  int tokens, kv_heads, sink, window;
-  int64_t cap;
+  int64_t count, cap;
+  int tokens, kv_heads, rows, sink, window;  // rows: tokens * kv_heads, of one sequence
 };
 
-// E (low half): codes of the even values of the lane's 8; O (high half): of the odd ones
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float s, int z) {
-  uint32_t w = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    int k = s > 0.f ? int(rintf(__fdiv_rn(x[e], s))) : 0;
-    int c = min(max(k + z, 0), 15);
-    k = c - z;
-    if (fabsf(float(k) * s) > 65504.f) c -= k > 0 ? 1 : -1;
-    w |= uint32_t(c) << ((e >> 1) * 4 + (e & 1) * 16);
-  }
-  return w;
+// nearest whole number to x / s, ties to even (see above); |x / s| <= 16
+__device__ __forceinline__ int nearest(float x, float inv_s) {
+  const float t = fmaf(x, inv_s, 1536.f) - 1536.f;  // fp32's step at 1024 .. 2048 is 2^-13
+  return __float_as_int(t + 12582912.f) - __float_as_int(12582912.f);
 }
 
 template <int D, int GROUP>
-__global__ void __launch_bounds__(THREADS) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(THREADS) append_kernel(const __grid_constant__ AppendParams p) {
   pdl_trigger();
   pdl_wait();
-  constexpr int LPR = D / 8;      // lanes per row
-  constexpr int LPG = GROUP / 8;  // lanes per group
-  constexpr int NI = D / 32;
-  const int l = threadIdx.x % LPR;
-  const int which = blockIdx.y;
-  const int64_t step = int64_t(gridDim.x) * (THREADS / LPR);
-  const int64_t first = int64_t(blockIdx.x) * (THREADS / LPR) + threadIdx.x / LPR;
-  // every lane of a warp runs every turn (the butterflies need them all)
-  const int64_t turns = (p.rows + step - 1) / step;
-  for (int64_t turn = 0; turn < turns; ++turn) {
-    const int64_t r = first + turn * step;
-    const bool in = r < p.rows;
-    const int64_t bt = in ? r / p.kv_heads : 0;
-    const int h = in ? int(r - bt * p.kv_heads) : 0;
-    const int b = int(bt / p.tokens), j = int(bt - int64_t(b) * p.tokens);
-    const int64_t count = kv4::count_of(p.counts, p.count, b);
-    const int64_t pos = count + j;
-    // a ring token that a later one of this chunk replaces is not stored
-    const bool keep = in && (pos < p.sink || j >= p.tokens - p.window);
-    const uint4 v = keep ? __ldg(p.fresh[which] + r * LPR + l) : make_uint4(0u, 0u, 0u, 0u);
-    const uint32_t vd[4] = {v.x, v.y, v.z, v.w};
-    float x[8], lo = 0.f, hi = 0.f;
-    bool fine = true;
+  constexpr int NI = D / 32, NG = D / GROUP, IPG = NI / NG;
+  const int c = threadIdx.x % LANES, b = blockIdx.y, which = blockIdx.z;
+  const int r = int(blockIdx.x) * ROWS + int(threadIdx.x) / LANES;
+  const int j = r / p.kv_heads, h = r - j * p.kv_heads;
+  const int64_t count = kv4::count_of(p.counts, p.count, b), pos = count + j;
+  // a ring token that a later one of this chunk replaces is not stored
+  const bool keep = r < p.rows && (pos < p.sink || j >= p.tokens - p.window);
+  uint4 v[NI];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = h2_to_f2(vd[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-      fine = fine && fabsf(f.x) <= 65504.f && fabsf(f.y) <= 65504.f;  // false for a NaN
-      lo = fminf(lo, fminf(f.x, f.y));
-      hi = fmaxf(hi, fmaxf(f.x, f.y));
-    }
-    int bad = fine ? 0 : 1;
+  for (int i = 0; i < NI; ++i)
+    v[i] = keep ? __ldg(reinterpret_cast<const uint4*>(p.fresh[which] + (int64_t(b) * p.rows + r) * D) + 4 * i + c)
+                : make_uint4(0u, 0u, 0u, 0u);
+  uint32_t word[NI], param[NG];
 #pragma unroll
-    for (int o = LPG / 2; o > 0; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+  for (int n = 0; n < NG; ++n) {
+    __half2 lo2 = __float2half2_rn(0.f), hi2 = lo2;
+#pragma unroll
+    for (int i = n * IPG; i < (n + 1) * IPG; ++i) {
+      const uint32_t d[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __half2 x = *reinterpret_cast<const __half2*>(&d[e]);
+        lo2 = __hmin2_nan(lo2, x);
+        hi2 = __hmax2_nan(hi2, x);
+      }
     }
-    uint32_t word = 0, param = kv4::NAN_PARAM;
-    if (!bad) {
-      const float least = __double2float_ru((double(hi) - double(lo)) / 15.0);
-      const uint32_t bits = (uint32_t(__half_as_ushort(__float2half_ru(least))) + 15u) & 0xFFF0u;
-      const float s = __half2float(__ushort_as_half(uint16_t(bits)));
-      const int z = s > 0.f ? int(rintf(__fdiv_rn(-lo, s))) : 0;
-      word = quantise8(x, s, z);
-      param = bits | uint32_t(z);
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) {
+      lo2 = __hmin2_nan(lo2, __shfl_xor_sync(0xffffffffu, lo2, o));
+      hi2 = __hmax2_nan(hi2, __shfl_xor_sync(0xffffffffu, hi2, o));
     }
-    const int c = l & 3, i = l >> 2;
-    if (which == 1) {
-      // values: the even halves of blocks (i, i + 1) share a word, and the odd ones
-      const uint32_t send = (i & 1) ? (word & 0xFFFFu) : (word >> 16);
-      const uint32_t got = __shfl_xor_sync(0xffffffffu, send, 4);
-      word = (i & 1) ? (got | (word & 0xFFFF0000u)) : ((word & 0xFFFFu) | (got << 16));
+    const float lo = __half2float(__hmin_nan(__low2half(lo2), __high2half(lo2)));
+    const float hi = __half2float(__hmax_nan(__low2half(hi2), __high2half(hi2)));
+    const bool fine = lo >= -65504.f && hi <= 65504.f;  // false for a NaN
+    const float least = __fdiv_ru(__fsub_ru(hi, lo), 15.f);
+    const uint32_t bits = (uint32_t(__half_as_ushort(__float2half_ru(least))) + 15u) & 0xFFF0u;
+    const float s = __half2float(__ushort_as_half(uint16_t(bits)));
+    const float inv = fine && s > 0.f ? __frcp_rn(s) : 0.f;
+    const int z = fine ? nearest(-lo, inv) : 0;
+    param[n] = fine ? bits | uint32_t(z) : kv4::NAN_PARAM;
+#pragma unroll
+    for (int i = n * IPG; i < (n + 1) * IPG; ++i) {
+      const uint32_t d[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      uint32_t w = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 x = h2_to_f2(d[e]);
+        int c0 = min(max(nearest(x.x, inv) + z, 0), 15), c1 = min(max(nearest(x.y, inv) + z, 0), 15);
+        if (s > 65504.f / 15.f) {  // only then can s (c - z) pass the largest finite number
+          if (fabsf(float(c0 - z) * s) > 65504.f) c0 -= c0 > z ? 1 : -1;
+          if (fabsf(float(c1 - z) * s) > 65504.f) c1 -= c1 > z ? 1 : -1;
+        }
+        w |= uint32_t(c0) << (4 * e) | uint32_t(c1) << (4 * e + 16);  // even values low, odd values high
+      }
+      word[i] = fine ? w : 0u;
     }
-    if (!keep) continue;
-    const int64_t slot = pos < p.sink ? pos : p.sink + (pos - p.sink) % p.window;
-    const int64_t row = (int64_t(b) * p.kv_heads + h) * p.cap + slot;
-    const int at = which == 0 ? c * NI + i : ((2 * c + (i & 1)) * NI + (i & ~1)) / 2;
-    p.codes[which][row * LPR + at] = word;
-    if (l % LPG == 0) p.params[which][row * (D / GROUP) + l / LPG] = uint16_t(param);
   }
+  if (!keep) return;
+  const int64_t slot = pos < p.sink ? pos : p.sink + (pos - p.sink) % p.window;
+  const int64_t row = (int64_t(b) * p.kv_heads + h) * p.cap + slot;
+  if (which == 1) {  // values: the even halves side by side, then the odd ones
+    uint32_t t[NI];
+#pragma unroll
+    for (int i = 0; i < NI; i += 2) {
+      t[i / 2] = prmt(word[i], word[i + 1], 0x5410u);
+      t[NI / 2 + i / 2] = prmt(word[i], word[i + 1], 0x7632u);
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i) word[i] = t[i];
+  }
+  unsigned char* dst = p.codes[which] + row * (D / 2) + c * (D / 8);
+  if constexpr (NI == 4)
+    *reinterpret_cast<uint4*>(dst) = make_uint4(word[0], word[1], word[2], word[3]);
+  else
+    *reinterpret_cast<uint2*>(dst) = make_uint2(word[0], word[1]);
+  uint16_t* pp = p.params[which] + row * NG;
+#pragma unroll
+  for (int n = 0; n < NG; ++n)
+    if (c == n) pp[n] = uint16_t(param[n]);
 }
 
 struct GatherParams {
-  const uint16_t* codes[2];
+  const unsigned char* codes[2];
   const uint16_t* params[2];
-  uint4* out[2];
-  int64_t count, rows;  // rows: batch * valid * kv_heads
-  int valid, kv_heads, sink, window;
+  __half* out[2];
   int64_t cap;
+  int start, kv_heads, rows, sink, window;  // start: the ring's oldest token; rows: valid * kv_heads
 };
 
 template <int D, int GROUP>
-__global__ void __launch_bounds__(THREADS) gather_kernel(const GatherParams p) {
+__global__ void __launch_bounds__(THREADS) gather_kernel(const __grid_constant__ GatherParams p) {
   pdl_trigger();
   pdl_wait();
-  constexpr int LPR = D / 8, NI = D / 32;
-  const int l = threadIdx.x % LPR, c = l & 3, i = l >> 2;
-  const int which = blockIdx.y;
-  const int64_t step = int64_t(gridDim.x) * (THREADS / LPR);
-  const int64_t f = p.count - p.sink;
-  const int64_t start = f <= p.window ? 0 : f % p.window;  // the ring's oldest token
-  for (int64_t r = int64_t(blockIdx.x) * (THREADS / LPR) + threadIdx.x / LPR; r < p.rows; r += step) {
-    const int64_t bi = r / p.kv_heads;
-    const int h = int(r - bi * p.kv_heads);
-    const int b = int(bi / p.valid), n = int(bi - int64_t(b) * p.valid);
-    const int64_t slot = n < p.sink ? n : p.sink + (start + (n - p.sink)) % p.window;
-    const int64_t row = (int64_t(b) * p.kv_heads + h) * p.cap + slot;
-    const uint16_t* cr = p.codes[which] + row * (2 * LPR);
-    const uint32_t word = which == 0 ? __ldg(reinterpret_cast<const uint32_t*>(cr) + c * NI + i)
-                                     : (uint32_t(__ldg(cr + 2 * c * NI + i)) |
-                                        (uint32_t(__ldg(cr + (2 * c + 1) * NI + i)) << 16));
-    const uint32_t param = __ldg(p.params[which] + row * (D / GROUP) + l / (GROUP / 8));
+  constexpr int NI = D / 32, NG = D / GROUP;
+  const int c = threadIdx.x % LANES, b = blockIdx.y, which = blockIdx.z;
+  const int r = int(blockIdx.x) * ROWS + int(threadIdx.x) / LANES;
+  if (r >= p.rows) return;
+  const int n = r / p.kv_heads, h = r - n * p.kv_heads;
+  int slot = n;
+  if (n >= p.sink) {
+    slot += p.start;  // below sink + 2 window
+    if (slot >= p.sink + p.window) slot -= p.window;
+  }
+  const int64_t row = (int64_t(b) * p.kv_heads + h) * p.cap + slot;
+  const unsigned char* src = p.codes[which] + row * (D / 2) + c * (D / 8);
+  uint32_t w[NI], param[NG];
+  if constexpr (NI == 4) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+    w[0] = v.x, w[1] = v.y;
+  }
+#pragma unroll
+  for (int g = 0; g < NG; ++g) param[g] = __ldg(p.params[which] + row * NG + g) * 0x10001u;
+  uint4* out = reinterpret_cast<uint4*>(p.out[which] + (int64_t(b) * p.rows + r) * D) + c;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const uint32_t word =
+        which == 0 ? w[i] : prmt(w[i >> 1], w[NI / 2 + (i >> 1)], (i & 1) ? 0x7632u : 0x5410u);
     uint32_t o[4];
-    kv4::dequant_word(word, kv4::group_scale(param | (param << 16)), o);
-    p.out[which][r * LPR + l] = make_uint4(o[0], o[1], o[2], o[3]);
+    kv4::dequant_word(word, kv4::group_scale(param[i * NG / NI]), o);
+    out[4 * i] = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
-inline unsigned grid_for(int64_t rows, int lanes_per_row) {
-  const int64_t per = THREADS / lanes_per_row;
-  return unsigned(std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, int64_t(device_sm_count()) * 16)));
-}
-
 template <int D, int GROUP>
-cudaError_t launch_append(const AppendParams& p, cudaStream_t st) {
-  return launch_pdl(append_kernel<D, GROUP>, dim3(grid_for(p.rows, D / 8), 2), dim3(THREADS), 0, st, p);
+cudaError_t launch_append(const AppendParams& p, int batch, cudaStream_t st) {
+  return launch_pdl(append_kernel<D, GROUP>, dim3(unsigned((p.rows + ROWS - 1) / ROWS), unsigned(batch), 2),
+                    dim3(THREADS), 0, st, p);
 }
 template <int D, int GROUP>
-cudaError_t launch_gather(const GatherParams& p, cudaStream_t st) {
-  return launch_pdl(gather_kernel<D, GROUP>, dim3(grid_for(p.rows, D / 8), 2), dim3(THREADS), 0, st, p);
+cudaError_t launch_gather(const GatherParams& p, int batch, cudaStream_t st) {
+  return launch_pdl(gather_kernel<D, GROUP>, dim3(unsigned((p.rows + ROWS - 1) / ROWS), unsigned(batch), 2),
+                    dim3(THREADS), 0, st, p);
 }
 
 }  // namespace ring4
@@ -193,16 +212,18 @@ extern "C" int qx_ring_append_q4(void* k_codes, void* k_params, void* v_codes, v
   QX_REQUIRE(aligned(k_codes, 16) && aligned(v_codes, 16) && aligned(k_params, 16) && aligned(v_params, 16) &&
                  aligned(new_k, 16) && aligned(new_v, 16),
              "ring_append_q4: tensors must be 16-byte aligned");
+  QX_REQUIRE(batch <= 65535 && int64_t(tokens) * kv_heads < (int64_t(1) << 31) - ring4::ROWS,
+             "ring_append_q4: batch=%d or tokens=%d too large", batch, tokens);
   ring4::AppendParams p{};
-  p.codes[0] = static_cast<uint32_t*>(k_codes);
-  p.codes[1] = static_cast<uint32_t*>(v_codes);
+  p.codes[0] = static_cast<unsigned char*>(k_codes);
+  p.codes[1] = static_cast<unsigned char*>(v_codes);
   p.params[0] = static_cast<uint16_t*>(k_params);
   p.params[1] = static_cast<uint16_t*>(v_params);
-  p.fresh[0] = static_cast<const uint4*>(new_k);
-  p.fresh[1] = static_cast<const uint4*>(new_v);
+  p.fresh[0] = static_cast<const __half*>(new_k);
+  p.fresh[1] = static_cast<const __half*>(new_v);
   p.counts = counts;
   p.count = count;
-  p.rows = int64_t(batch) * tokens * kv_heads;
+  p.rows = tokens * kv_heads;
   p.tokens = tokens;
   p.kv_heads = kv_heads;
   p.sink = sink;
@@ -211,11 +232,11 @@ extern "C" int qx_ring_append_q4(void* k_codes, void* k_params, void* v_codes, v
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (head_dim == 64)
-    e = group == 32 ? ring4::launch_append<64, 32>(p, st) : ring4::launch_append<64, 64>(p, st);
+    e = group == 32 ? ring4::launch_append<64, 32>(p, batch, st) : ring4::launch_append<64, 64>(p, batch, st);
   else
-    e = group == 32   ? ring4::launch_append<128, 32>(p, st)
-        : group == 64 ? ring4::launch_append<128, 64>(p, st)
-                      : ring4::launch_append<128, 128>(p, st);
+    e = group == 32   ? ring4::launch_append<128, 32>(p, batch, st)
+        : group == 64 ? ring4::launch_append<128, 64>(p, batch, st)
+                      : ring4::launch_append<128, 128>(p, batch, st);
   QX_CUDA_TRY(e, "ring_append_q4: launch");
   return check_launch("ring_append_q4");
 }
@@ -232,16 +253,17 @@ extern "C" int qx_ring_gather_q4(const void* k_codes, const void* k_params, cons
   QX_REQUIRE(aligned(k_codes, 16) && aligned(v_codes, 16) && aligned(k_params, 16) && aligned(v_params, 16) &&
                  aligned(k_out, 16) && aligned(v_out, 16),
              "ring_gather_q4: tensors must be 16-byte aligned");
+  QX_REQUIRE(batch <= 65535 && int64_t(valid) * kv_heads < (int64_t(1) << 31) - ring4::ROWS,
+             "ring_gather_q4: batch=%d or %d tokens too large", batch, valid);
   ring4::GatherParams p{};
-  p.codes[0] = static_cast<const uint16_t*>(k_codes);
-  p.codes[1] = static_cast<const uint16_t*>(v_codes);
+  p.codes[0] = static_cast<const unsigned char*>(k_codes);
+  p.codes[1] = static_cast<const unsigned char*>(v_codes);
   p.params[0] = static_cast<const uint16_t*>(k_params);
   p.params[1] = static_cast<const uint16_t*>(v_params);
-  p.out[0] = static_cast<uint4*>(k_out);
-  p.out[1] = static_cast<uint4*>(v_out);
-  p.count = count;
-  p.rows = int64_t(batch) * valid * kv_heads;
-  p.valid = valid;
+  p.out[0] = static_cast<__half*>(k_out);
+  p.out[1] = static_cast<__half*>(v_out);
+  p.start = count - sink <= window ? 0 : int((count - sink) % window);
+  p.rows = valid * kv_heads;
   p.kv_heads = kv_heads;
   p.sink = sink;
   p.window = window;
@@ -249,11 +271,11 @@ extern "C" int qx_ring_gather_q4(const void* k_codes, const void* k_params, cons
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (head_dim == 64)
-    e = group == 32 ? ring4::launch_gather<64, 32>(p, st) : ring4::launch_gather<64, 64>(p, st);
+    e = group == 32 ? ring4::launch_gather<64, 32>(p, batch, st) : ring4::launch_gather<64, 64>(p, batch, st);
   else
-    e = group == 32   ? ring4::launch_gather<128, 32>(p, st)
-        : group == 64 ? ring4::launch_gather<128, 64>(p, st)
-                      : ring4::launch_gather<128, 128>(p, st);
+    e = group == 32   ? ring4::launch_gather<128, 32>(p, batch, st)
+        : group == 64 ? ring4::launch_gather<128, 64>(p, batch, st)
+                      : ring4::launch_gather<128, 128>(p, batch, st);
   QX_CUDA_TRY(e, "ring_gather_q4: launch");
   return check_launch("ring_gather_q4");
 }
