@@ -10,25 +10,39 @@
 // 16).  tcgen05 would need 128 rows of M: the cache rows would have to pass
 // through shared memory as fp16, four times their bytes, for a product whose
 // arithmetic is a small part of the time.
-//   S^T = K Q^T   the codes enter as fp16 subnormals: a mask of a 32-bit word
-//                 is the pair c 2^-24 (or 16 c 2^-24, whose q comes divided by
-//                 16), exact, one instruction a pair.  Scale and zero point act
-//                 on the fp32 accumulator per token and group:
-//                 s (sum q c - z sum q).
-//   O^T = V^T P^T the token sits on the K side, so V's scale cannot act on the
-//                 accumulator; the pairs are made exact fp16 s (c - z) in three
-//                 instructions.  P^T comes from S^T's accumulator layout by
-//                 movmatrix, in fp16 scaled by 2^14 (its subnormals then start
-//                 at weights of 2^-28 of the largest), summed in fp32.
-// The online softmax keeps a running maximum and sum per warp and head in fp32.
+// The codes enter as fp16 subnormals: a mask of a 32-bit word is the pair c 2^-24
+// (or 16 c 2^-24), exact, one instruction a pair; the zero points take part as one
+// more product of the same kind.
+//   S^T = K Q^T   per group, sum q c - z sum q (sum q in two fp16 parts) in one
+//                 accumulator, then times the token's scale in fp32.  The q of the
+//                 codes that come as 16 c are divided by 16.
+//   O^T = V^T P^T the token sits on the K side, so the scale goes to the weight:
+//                 P s in fp16 per group.  P^T comes from S^T's accumulator layout
+//                 by movmatrix.
+// The online softmax keeps a running reference and sum per warp and head in fp32.
+// The reference is the maximum score plus the exponent E of the largest value scale
+// so far, and P carries 2^14: P s stays below 2^15 and its fp16 subnormals start
+// below 2^-28 of the largest.
 //
-// Loads go from global memory straight to the MMA fragments (the format puts
-// each lane's share of a row side by side), one step of 32 tokens ahead; no
-// shared memory until the four warps of a CTA join their results.  A warp takes
-// every (4 nsplit)-th step; with more than one split the CTAs write fp32 partial
-// results and a second kernel joins them.
+// What bounds it: at 8 sequences and more the instructions (about 250 a warp for
+// 16 tokens of a KV head), not HBM.  Made exact fp16 s (c - z) in registers, with
+// three instructions a pair of V, it took 352.
+//
+// Each warp streams its steps of 32 tokens through a ring of its own in shared
+// memory (STAGES deep, four bulk copies a step onto one mbarrier) and reads the
+// fragments from there; the format puts each lane's share of a row side by side.
+// (Loaded from global memory straight into the fragments, one step ahead, the bytes
+// in flight hung on the registers: 41 us for 32 sequences x 4096 slots.)  A warp
+// takes every (4 nsplit)-th step.  The warps of a CTA join their results in the
+// ring's memory; with more than one split the CTAs write fp32 partial results and a
+// second kernel joins them.
+//
+// Row g of an MMA is token g ^ (g / 2 & 1) of its eight: neighbouring rows, and the
+// rows that four quads read together, then lie in different halves of the banks.
+// Every wait is bounded (kWaitLimitNs, then QX_DEVERR_MBAR_TIMEOUT).
 #include <algorithm>
 #include <cmath>
+#include <mutex>
 
 #include "kv4.cuh"
 #include "qx_b200.h"
@@ -39,8 +53,22 @@ namespace dattn4 {
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int STEP = 32;          // tokens per warp step
-constexpr float PSHIFT = 14.f;    // P in fp16 carries 2^14
+constexpr float PSHIFT = 14.f;    // P carries 2^14
 constexpr int MAX_SPLITS = 64;
+constexpr int STAGES = 3;
+
+// bytes of a stage: codes of K and V, params of K and V
+template <int D, int NG>
+struct Stage {
+  static constexpr int CODES = STEP * D / 2, PARAMS = STEP * NG * 2, BYTES = 2 * (CODES + PARAMS);
+};
+// shared memory: the ring of every warp, or the warps' results; then the barriers
+template <int D, int NG, int NT>
+struct Smem {
+  static constexpr int RING = WARPS * STAGES * Stage<D, NG>::BYTES;
+  static constexpr int JOIN = WARPS * 8 * NT * (D + 1 + 2) * 4;
+  static constexpr int BARS = RING > JOIN ? RING : (JOIN + 15) / 16 * 16, BYTES = BARS + WARPS * STAGES * 8;
+};
 
 struct Params {
   const __half* q;
@@ -57,6 +85,38 @@ struct Params {
   float scale_log2;
 };
 
+// Sticky device-side error word of this file's kernels (QX_DEVERR_* bits),
+// merged into qx_get_device_error.
+static __device__ unsigned g_decode4_error = 0;
+
+__device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred P; mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 P, [%1], %2; "
+      "selp.u32 %0, 1, 0, P; }"
+      : "=r"(ok)
+      : "r"(b), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ bool bar_wait_slow(uint32_t b, uint32_t parity) {
+  uint64_t t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  while (!bar_try(b, parity)) {
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    if (t - t0 > kWaitLimitNs) {
+      atomicOr(&g_decode4_error, QX_DEVERR_MBAR_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar), "l"(policy)
+      : "memory");
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -72,89 +132,96 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 template <int WORDS>
-__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[WORDS]) {
+__device__ __forceinline__ void load_words(const unsigned char* p, uint32_t (&w)[WORDS]) {  // shared memory
   if constexpr (WORDS == 4) {
-    const uint4 v = ldg_stream_v4(p);
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
   } else if constexpr (WORDS == 2) {
-    const uint2 v = __ldcs(static_cast<const uint2*>(p));
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
     w[0] = v.x, w[1] = v.y;
   } else {
-    w[0] = __ldcs(static_cast<const unsigned*>(p));
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
 
-// what a lane holds of 16 tokens: K rows g and g + 8 (a quarter of each), V of
-// tokens 2c, 2c + 1, 2c + 8, 2c + 9 (an eighth of each), and their params
-template <int D, int NG>
-struct Frag {
-  static constexpr int NI = D / 32;
-  static constexpr int KPW = NG > 2 ? 2 : 1;  // 32-bit words of a K row's params
-  uint32_t k[2][NI];
-  uint32_t v[4][NI / 2];
-  uint32_t kp[2][KPW];
-  uint32_t vp[2][NG];  // token pairs (2c, 2c + 1) and (2c + 8, 2c + 9)
-
-  __device__ __forceinline__ void load(const unsigned char* kc, const uint16_t* kpar, const unsigned char* vc,
-                                       const uint16_t* vpar, int64_t row0, int g, int c) {
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int64_t row = row0 + g + 8 * r;
-      load_words<NI>(kc + row * (D / 2) + c * (D / 8), k[r]);
-      const uint16_t* pp = kpar + row * NG;
-      if constexpr (NG == 1)
-        kp[r][0] = __ldcs(pp);
-      else
-        load_words<KPW>(pp, kp[r]);
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-      load_words<NI / 2>(vc + (row0 + 2 * c + (t & 1) + (t >> 1) * 8) * (D / 2) + g * (D / 16), v[t]);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) load_words<NG>(vpar + (row0 + 2 * c + t * 8) * NG, vp[t]);
-  }
-  __device__ __forceinline__ uint32_t kparam(int r, int grp) const {
-    return NG == 1 ? kp[r][0] : (grp & 1) ? kp[r][grp >> 1] >> 16 : kp[r][grp >> 1] & 0xFFFFu;
-  }
-  // the pair's params of one group: token 2c in the low half
-  __device__ __forceinline__ uint32_t vparam(int t, int grp) const {
-    if constexpr (NG == 1) return vp[t][0];
-    return prmt(vp[t][grp >> 1], vp[t][NG / 2 + (grp >> 1)], (grp & 1) ? 0x7632u : 0x5410u);
+// the params of one token: NG 16-bit words
+template <int NG>
+struct RowParams {
+  static constexpr int W = NG > 2 ? 2 : 1;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const unsigned char* p) {
+    if constexpr (NG == 1)
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    else
+      load_words<W>(p, w);
   }
 };
+// the scale of group `grp` from a row's params
+template <int NG>
+__device__ __forceinline__ float scale_of(const RowParams<NG>& p, int grp) {
+  const uint32_t w = NG == 1 ? p.w[0] : (grp & 1) ? p.w[grp >> 1] >> 16 : p.w[grp >> 1];
+  return __half2float(__ushort_as_half(uint16_t(w & 0xFFF0u)));
+}
 
 template <int D, int NG, int NT>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kernel(const __grid_constant__ Params p) {
   pdl_trigger();
   constexpr int NI = D / 32, IPG = NI / NG;  // 32-value blocks of a row, and of a group
   constexpr int SROW = D + 1;                // odd: the column writes below meet no bank twice
-  __shared__ float s_o[WARPS][8 * NT][SROW];
-  __shared__ float s_m[WARPS][8 * NT], s_l[WARPS][8 * NT];
+  using St = Stage<D, NG>;
+  using Sm = Smem<D, NG, NT>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  float (*s_o)[8 * NT][SROW] = reinterpret_cast<float (*)[8 * NT][SROW]>(smem);
+  float (*s_m)[8 * NT] = reinterpret_cast<float (*)[8 * NT]>(s_o + WARPS);
+  float (*s_l)[8 * NT] = s_m + WARPS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-  const int64_t base = (int64_t(b) * p.hkv + kvh) * p.cap;
-  const unsigned char* kc = p.kc + base * (D / 2);
-  const unsigned char* vc = p.vc + base * (D / 2);
-  const uint16_t* kp = p.kp + base * NG;
-  const uint16_t* vp = p.vp + base * NG;
+  const unsigned char* ring = smem + warp * STAGES * St::BYTES;
+  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  const uint32_t bars = static_cast<uint32_t>(__cvta_generic_to_shared(smem + Sm::BARS)) + warp * STAGES * 8;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + 8 * i) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
   pdl_wait();
   const int valid = kv4::valid_slots(kv4::count_of(p.counts, p.count, b), p.sink, p.window);
   const int steps = (valid + STEP - 1) / STEP, stride = p.nsplit * WARPS;
   int step = split * WARPS + warp;
 
-  Frag<D, NG> nxt[2];
-  if (step < steps)
+  // (a step's rows all lie in the storage: it has a multiple of 64)
+  const int64_t row0 = (int64_t(b) * p.hkv + kvh) * p.cap;
+  uint64_t policy;  // read once
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  auto fetch = [&](int st, int t) {  // lane 0
+    const uint32_t dst = ring_at + st * St::BYTES, bar = bars + 8 * st;
+    const int64_t row = row0 + int64_t(t) * STEP;
+    asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(St::BYTES) : "memory");
+    bulk_copy(dst, p.kc + row * (D / 2), St::CODES, bar, policy);
+    bulk_copy(dst + 2 * St::CODES, p.kp + row * NG, St::PARAMS, bar, policy);
+    bulk_copy(dst + St::CODES, p.vc + row * (D / 2), St::CODES, bar, policy);
+    bulk_copy(dst + 2 * St::CODES + St::PARAMS, p.vp + row * NG, St::PARAMS, bar, policy);
+  };
+  if (lane == 0)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) nxt[u].load(kc, kp, vc, vp, int64_t(step) * STEP + u * 16, g, c);
+    for (int i = 0; i < STAGES; ++i)
+      if (step + i * stride < steps) fetch(i, step + i * stride);
+  // this lane's places in a stage: MMA row g is token tg of its eight
+  const int tg = g ^ ((g >> 1) & 1), odd = c & 1;
+  const int at_k = tg * (D / 2) + c * (D / 8), at_p = 2 * St::CODES + tg * NG * 2;
+  const int at_v[2] = {St::CODES + (2 * c + odd) * (D / 2) + g * (D / 16), St::CODES + (2 * c + 1 - odd) * (D / 2) + g * (D / 16)};
+  const int at_z = 2 * St::CODES + St::PARAMS + 2 * c * NG * 2;
+  const uint32_t sel_lo = odd ? 0x1054u : 0x5410u, sel_hi = odd ? 0x3276u : 0x7632u;  // a pair of tokens in MMA order
 
   // Q^T fragments: head g (of N tile nt), values 32 i + 8 c ..; a head is scaled by
-  // the power of two that brings its largest value to [2^10, 2^11), undone in
-  // hf: the second pair of each k step is divided by 16 (its codes come
-  // multiplied by 16), which then costs no bits that count.
+  // the power of two that brings its largest value to [2^4, 2^5), undone in hf: the
+  // second pair of each k step is divided by 16, which then costs no bits that count,
+  // and the sum over a group stays within fp16.
   uint32_t qb[NT][NI][4];
-  float qs[NT][NG][2];  // 2^-24 sum of the scaled q over a group, of heads 2c, 2c + 1
-  float hf[NT][2];      // accumulator -> log2 domain
+  uint32_t qz[NT][NG];  // minus the sum of the scaled q over a group, in two fp16 parts: k = 0, 1 of a product
+  float hf[NT][2];      // accumulator -> log2 domain, of heads 2c, 2c + 1
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int h = nt * 8 + g;
@@ -174,8 +241,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kerne
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int ex = top > 0.f && top <= 65504.f ? int(__float_as_uint(top) >> 23) - 127 : 10;
-    const float up = __uint_as_float(uint32_t(127 + 10 - ex) << 23), down = __uint_as_float(uint32_t(127 + ex - 10) << 23);
+    const int ex = top > 0.f && top <= 65504.f ? int(__float_as_uint(top) >> 23) - 127 : 4;
+    const float up = __uint_as_float(uint32_t(127 + 4 - ex) << 23), down = __uint_as_float(uint32_t(127 + ex - 4) << 23);
 #pragma unroll
     for (int n = 0; n < NG; ++n) sum[n] = 0.f;
 #pragma unroll
@@ -194,46 +261,63 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kerne
     for (int n = 0; n < NG; ++n) {
       sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
       sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
-      qs[nt][n][0] = __shfl_sync(0xffffffffu, sum[n], 8 * c) * 0x1p-24f;
-      qs[nt][n][1] = __shfl_sync(0xffffffffu, sum[n], 8 * c + 4) * 0x1p-24f;
+      const float big = __half2float(__float2half_rn(-sum[n]));
+      qz[nt][n] = c == 0 ? pack_h2(big, -sum[n] - big) : 0u;
     }
     const float k = down * 0x1p24f * p.scale_log2;
     hf[nt][0] = __shfl_sync(0xffffffffu, k, 8 * c);
     hf[nt][1] = __shfl_sync(0xffffffffu, k, 8 * c + 4);
   }
 
-  float o[NI][2][NT][4];
+  float o[NI][2][NT][4], oz[NG][NT][4];
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
+  for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int f = 0; f < 2; ++f)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) o[i][f][nt][0] = o[i][f][nt][1] = o[i][f][nt][2] = o[i][f][nt][3] = 0.f;
+      for (int f = 0; f < 2; ++f) o[i][f][nt][0] = o[i][f][nt][1] = o[i][f][nt][2] = o[i][f][nt][3] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NG; ++n) oz[n][nt][0] = oz[n][nt][1] = oz[n][nt][2] = oz[n][nt][3] = 0.f;
+  }
+  // m_r: the largest score; vexp: the exponent of the largest value scale (of its bits,
+  // biased); ref = m_r + vexp - 14 what the weights refer to
   float m_r[NT][2], l_r[NT][2];
+  int vexp = 0;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) m_r[nt][0] = m_r[nt][1] = -INFINITY, l_r[nt][0] = l_r[nt][1] = 0.f;
+  const uint32_t kz_mask = c == 0 ? 0x000F000Fu : 0u;
 
+  int st = 0;
+  uint32_t phase = 0;
   for (; step < steps; step += stride) {
-    Frag<D, NG> cur[2] = {nxt[0], nxt[1]};
-    if (step + stride < steps)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) nxt[u].load(kc, kp, vc, vp, int64_t(step + stride) * STEP + u * 16, g, c);
     const int left = valid - step * STEP;  // tokens of this step that exist
-
-    // scores: rows g, g + 8 (e >> 1) by heads 2c, 2c + 1 (e & 1)
+    const unsigned char* at = ring + st * St::BYTES;
+    if (!bar_try(bars + 8 * st, phase) && !bar_wait_slow(bars + 8 * st, phase)) {
+      for (int i = 1; i < STAGES && step + i * stride < steps; ++i)  // the copies behind it, too, before the memory goes
+        bar_wait_slow(bars + 8 * ((st + i) % STAGES), st + i >= STAGES ? phase ^ 1 : phase);
+      break;
+    }
+    // scores, over hf: rows g, g + 8 (e >> 1) by heads 2c, 2c + 1 (e & 1)
     float s[2][NT][4];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
+      uint32_t kc[2][NI];
+      RowParams<NG> kp[2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = 0.f;
+      for (int r = 0; r < 2; ++r) {
+        load_words<NI>(at + at_k + (u * 16 + 8 * r) * (D / 2), kc[r]);
+        kp[r].load(at + at_p + (u * 16 + 8 * r) * NG * 2);
+      }
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         float acc[NT][4];
+        const uint32_t sel = NG == 1 || !(n & 1) ? 0x1010u : 0x3232u;
+        const uint32_t z0 = prmt(kp[0].w[n >> 1], 0u, sel) & kz_mask, z1 = prmt(kp[1].w[n >> 1], 0u, sel) & kz_mask;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) mma_16816_zc(acc[nt], z0, z1, 0u, 0u, qz[nt][n], 0u);
 #pragma unroll
         for (int i = n * IPG; i < (n + 1) * IPG; ++i) {
-          const uint32_t w0 = cur[u].k[0][i], w1 = cur[u].k[1][i], h0 = w0 >> 8, h1 = w1 >> 8;
+          const uint32_t w0 = kc[0][i], w1 = kc[1][i], h0 = w0 >> 8, h1 = w1 >> 8;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma_16816(acc[nt], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qb[nt][i][0],
@@ -244,45 +328,45 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kerne
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t w = cur[u].kparam(r, n);
-          const float sc = __half2float(__ushort_as_half(uint16_t(w & 0xFFF0u)));
-          const float z = float(w & 15u);
+          const float sc = scale_of<NG>(kp[r], n);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            s[u][nt][2 * r] = fmaf(sc, fmaf(-z, qs[nt][n][0], acc[nt][2 * r]), s[u][nt][2 * r]);
-            s[u][nt][2 * r + 1] = fmaf(sc, fmaf(-z, qs[nt][n][1], acc[nt][2 * r + 1]), s[u][nt][2 * r + 1]);
-          }
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              s[u][nt][2 * r + k] = n == 0 ? sc * acc[nt][2 * r + k] : fmaf(sc, acc[nt][2 * r + k], s[u][nt][2 * r + k]);
         }
       }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[u][nt][e] *= hf[nt][e & 1];  // to the log2 domain
     }
-    if (left < STEP) {  // the last step: slots past the valid ones may hold anything
+    // the value scales of tokens g, g + 8, and the exponent of the largest
+    float vs[2][2][NG];
+    uint32_t top = 0;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        RowParams<NG> vp;
+        vp.load(at + at_p + St::PARAMS + (u * 16 + 8 * r) * NG * 2);
+        // a slot past the valid ones may hold anything: scale 0, for P is 0 there, and 0 times a NaN would not be
+        if (left < STEP && u * 16 + tg + 8 * r >= left) vp = RowParams<NG>{};
+#pragma unroll
+        for (int n = 0; n < NG; ++n) vs[u][r][n] = scale_of<NG>(vp, n);
+#pragma unroll
+        for (int w = 0; w < RowParams<NG>::W; ++w) top = __vmaxu2(top, vp.w[w]);
+      }
+    if (left < STEP) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (u * 16 + g + 8 * (e >> 1) >= left) s[u][nt][e] = -INFINITY;
-        // scale 0: P is 0 there, and 0 times a NaN would not be
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int t0 = u * 16 + 8 * t + 2 * c;
-          const uint32_t keep = (t0 < left ? 0xFFFFu : 0u) | (t0 + 1 < left ? 0xFFFF0000u : 0u);
-          if constexpr (NG == 1) {
-            cur[u].vp[t][0] &= keep;
-          } else {
-#pragma unroll
-            for (int n = 0; n < NG; ++n) cur[u].vp[t][n] &= n < NG / 2 ? (keep & 0xFFFFu) * 0x10001u : (keep >> 16) * 0x10001u;
-          }
-        }
-      }
+            if (u * 16 + tg + 8 * (e >> 1) >= left) s[u][nt][e] = -INFINITY;
     }
+    const int e_new = max(vexp, int(__reduce_max_sync(0xffffffffu, max(top >> 16, top & 0xFFFFu)) >> 10));
+    bool grew = e_new != vexp;
+    const float e_shift = float(e_new - vexp);
+    vexp = e_new;
     // online softmax
-    bool grew = false;
     float alpha[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -292,60 +376,80 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kerne
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float mn = fmaxf(m_r[nt][k], mx), mb = mn == -INFINITY ? 0.f : mn;
-        alpha[nt][k] = ex2(m_r[nt][k] - mb);
+        const float mn = fmaxf(m_r[nt][k], mx * hf[nt][k]), mb = mn == -INFINITY ? 0.f : mn;
+        alpha[nt][k] = ex2(m_r[nt][k] - mb - e_shift);
         grew = grew || mn != m_r[nt][k];
         m_r[nt][k] = mn;
+        const float shift = PSHIFT + 14.f - float(vexp) - mb;
         float sum = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            s[u][nt][2 * r + k] = ex2(s[u][nt][2 * r + k] - mb + PSHIFT);
+            s[u][nt][2 * r + k] = ex2(fmaf(s[u][nt][2 * r + k], hf[nt][k], shift));
             sum += s[u][nt][2 * r + k];
           }
         l_r[nt][k] = fmaf(l_r[nt][k], alpha[nt][k], sum);
       }
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int f = 0; f < 2; ++f)
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            o[i][f][nt][0] *= alpha[nt][0];
-            o[i][f][nt][1] *= alpha[nt][1];
-            o[i][f][nt][2] *= alpha[nt][0];
-            o[i][f][nt][3] *= alpha[nt][1];
+          for (int i = 0; i < NI; ++i) {
+            o[i][0][nt][e] *= alpha[nt][e & 1];
+            o[i][1][nt][e] *= alpha[nt][e & 1];
           }
+#pragma unroll
+          for (int n = 0; n < NG; ++n) oz[n][nt][e] *= alpha[nt][e & 1];
+        }
     }
-    // O^T += V^T P^T
+    // O^T += V^T (P s)^T
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      uint32_t pb[NT][2];
+      uint32_t vc[4][NI / 2], vz[2][NG];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        pb[nt][0] = transpose8x8(pack_h2(s[u][nt][0], s[u][nt][1]));
-        pb[nt][1] = transpose8x8(pack_h2(s[u][nt][2], s[u][nt][3]));
-      }
+      for (int t = 0; t < 4; ++t) load_words<NI / 2>(at + at_v[t & 1] + (u * 16 + (t >> 1) * 8) * (D / 2), vc[t]);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) load_words<NG>(at + at_z + (u * 16 + t * 8) * NG * 2, vz[t]);
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        const kv4::GroupScale ga = kv4::group_scale(cur[u].vparam(0, n)), gb = kv4::group_scale(cur[u].vparam(1, n));
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            pb[nt][r] = transpose8x8(pack_h2(s[u][nt][2 * r] * vs[u][r][n], s[u][nt][2 * r + 1] * vs[u][r][n]));
+        // the zero points of this lane's pairs of tokens, as fp16 z 2^-24
+        uint32_t z2[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          z2[t] = prmt(vz[t][n >> 1], NG == 1 ? vz[t][0] >> 16 : vz[t][NG / 2 + (n >> 1)], (n & 1) ? sel_hi : sel_lo) & 0x000F000Fu;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_16816(oz[n][nt], z2[0], z2[0], z2[1], z2[1], pb[nt][0], pb[nt][1]);
 #pragma unroll
         for (int i = n * IPG; i < (n + 1) * IPG; ++i) {
           const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;
-          uint32_t va[4], vb[4];
-          kv4::dequant_word(prmt(cur[u].v[0][i / 2], cur[u].v[1][i / 2], sel), ga, va);
-          kv4::dequant_word(prmt(cur[u].v[2][i / 2], cur[u].v[3][i / 2], sel), gb, vb);
+          const uint32_t a = prmt(vc[0][i / 2], vc[1][i / 2], sel), ah = a >> 8;
+          const uint32_t d = prmt(vc[2][i / 2], vc[3][i / 2], sel), dh = d >> 8;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_16816(o[i][0][nt], va[0], va[1], vb[0], vb[1], pb[nt][0], pb[nt][1]);
-            mma_16816(o[i][1][nt], va[2], va[3], vb[2], vb[3], pb[nt][0], pb[nt][1]);
+          for (int nt = 0; nt < NT; ++nt) {  // rows g: c 2^-24, rows g + 8: 16 c 2^-24
+            mma_16816(o[i][0][nt], a & 0x000F000Fu, a & 0x00F000F0u, d & 0x000F000Fu, d & 0x00F000F0u, pb[nt][0], pb[nt][1]);
+            mma_16816(o[i][1][nt], ah & 0x000F000Fu, ah & 0x00F000F0u, dh & 0x000F000Fu, dh & 0x00F000F0u, pb[nt][0],
+                      pb[nt][1]);
           }
         }
       }
     }
+    __syncwarp();  // every lane has read the stage
+    if (lane == 0 && step + STAGES * stride < steps) fetch(st, step + STAGES * stride);
+    if (++st == STAGES) {
+      st = 0;
+      phase ^= 1;
+    }
   }
+  __syncthreads();  // the rings are free
 
   // the warps' results to shared memory, joined per (head, value)
 #pragma unroll
@@ -357,14 +461,15 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kerne
       l += __shfl_xor_sync(0xffffffffu, l, 8);
       l += __shfl_xor_sync(0xffffffffu, l, 16);
       const int h = nt * 8 + 2 * c + k;
-      if (g == 0) s_m[warp][h] = m_r[nt][k], s_l[warp][h] = l;
+      if (g == 0) s_m[warp][h] = m_r[nt][k] + float(vexp), s_l[warp][h] = l;
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
           for (int r = 0; r < 2; ++r)
-            s_o[warp][h][32 * i + 8 * (g >> 1) + 2 * (2 * f + r) + (g & 1)] = o[i][f][nt][2 * r + k];
+            s_o[warp][h][32 * i + 8 * (g >> 1) + 2 * (2 * f + r) + (g & 1)] =
+                fmaf(o[i][f][nt][2 * r + k], r ? 0x1p20f : 0x1p24f, -0x1p24f * oz[i / IPG][nt][k]);
     }
   __syncthreads();
   for (int idx = tid; idx < p.G * D; idx += THREADS) {
@@ -424,7 +529,7 @@ __global__ void __launch_bounds__(32) decode_attn_q4_merge_kernel(const float* _
 // as long as each warp has a step
 inline int splits(int batch, int kv_heads, int valid) {
   const int pairs = batch * kv_heads;
-  const int want = (device_sm_count() * 3 + pairs - 1) / pairs;
+  const int want = (device_sm_count() * 6 + pairs - 1) / pairs;
   const int most = (valid + STEP * WARPS - 1) / (STEP * WARPS);
   return std::max(1, std::min({want, most, MAX_SPLITS}));
 }
@@ -435,8 +540,23 @@ inline size_t workspace_for(int batch, int q_heads, int head_dim, int nsplit) {
 
 template <int D, int NG, int NT>
 cudaError_t launch(const Params& p, int batch, cudaStream_t st) {
+  {
+    static std::mutex mu;
+    static bool done[64] = {};
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!done[dev]) {
+      const cudaError_t a = cudaFuncSetAttribute(decode_attn_q4_kernel<D, NG, NT>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D, NG, NT>::BYTES);
+      if (a != cudaSuccess) return a;
+      done[dev] = true;
+    }
+  }
   return launch_pdl(decode_attn_q4_kernel<D, NG, NT>, dim3(unsigned(p.nsplit), unsigned(p.hkv), unsigned(batch)),
-                    dim3(THREADS), 0, st, p);
+                    dim3(THREADS), Smem<D, NG, NT>::BYTES, st, p);
 }
 template <int D, int NG>
 cudaError_t launch(const Params& p, int batch, cudaStream_t st) {
@@ -444,6 +564,16 @@ cudaError_t launch(const Params& p, int batch, cudaStream_t st) {
 }
 
 }  // namespace dattn4
+
+int decode4_device_error(unsigned* code, int reset) {
+  QX_CUDA_TRY(cudaMemcpyFromSymbol(code, dattn4::g_decode4_error, sizeof(unsigned)), "get_device_error: read");
+  if (reset) {
+    const unsigned zero = 0;
+    QX_CUDA_TRY(cudaMemcpyToSymbol(dattn4::g_decode4_error, &zero, sizeof(unsigned)), "get_device_error: reset");
+  }
+  return QX_OK;
+}
+
 }  // namespace qx
 
 using namespace qx;

@@ -8,7 +8,10 @@ summed in fp32 over at most D/16 + 16 accumulations whose terms are at most
 15 steps of a group by |q|, under 4 times the largest sum of |q| |k| (a value's
 group reaches at least 7 steps on one side): each score is off by dS <= 4 size
 (D/16 + 16) 2^-23, a weight by a factor exp(2 dS); exp2's 2^-22 and the fp32
-sums over L / 16 steps of keys, 2^-23 each."""
+sums over L / 16 steps of keys, 2^-23 each.  Decode sums s P c and s P z apart
+before it subtracts them: with P at most 1 in all, terms of up to 15 s, and 15 s is
+at most (1 + 2^-6) of the group's span, which is at most twice its largest |v|:
+each of those fp32 steps is off by 2^-22 x 2.1 max |v| more."""
 
 import numpy as np
 import pytest
@@ -34,7 +37,8 @@ def no_wait_ran_out(C):
     C.check_device_error("4-bit ring attention")
 
 
-def _check(got, ref, keys, D, msg=""):
+def _check(got, ref, keys, D, msg="", apart=0.0):
+    """``apart``: the largest |value| where the codes' sums are kept apart."""
     out, weight, size = ref
     got = got.astype(np.float64)
     assert got.shape == out.shape
@@ -43,6 +47,7 @@ def _check(got, ref, keys, D, msg=""):
     vmax = np.nanmax(weight, initial=0.0)
     with np.errstate(invalid="ignore"):
         bound = (np.abs(out) * 2.0 ** -11 + 2.0 ** -25 + keys * 2.0 ** -39 * vmax +
+                 (keys / 16 + 16) * 2.0 ** -22 * 2.1 * apart +
                  weight * (2.0 ** -11 + np.expm1(2 * ds) + 2.0 ** -20 + (keys / 16 + 16) * 2.0 ** -22))
         bad = np.abs(got - out) > bound
     assert not bad.any(), (msg, int(bad.sum()), np.argwhere(bad)[0], got[bad][0], out[bad][0], bound[bad][0])
@@ -82,7 +87,7 @@ def _decode(C, B, Hq, Hkv, D, group, S, W, count, seed, scale=None, std=1.0, qst
     for b in range(B):
         k, v, pos = seqs[b]
         ref = attention64(q[b][None], k, v, np.ones((1, len(pos)), bool), scale)
-        _check(to_np(out)[b][None], ref, len(pos), D, f"b={b} count={counts[b]}")
+        _check(to_np(out)[b][None], ref, len(pos), D, f"b={b} count={counts[b]}", np.abs(v).max(initial=0.0))
     return q, codes, params, out
 
 
@@ -126,7 +131,7 @@ def test_decode_long(C):
     k, v = (to_np(t)[0] for t in C.ring_gather_q4(codes, params, S + W, S, W))
     out = C.decode_attention_q4(q, codes, params, S + W, S, W)
     ref = attention64(to_np(q), k, v, np.ones((1, S + W), bool))
-    _check(to_np(out), ref, S + W, D)
+    _check(to_np(out), ref, S + W, D, apart=np.abs(v.astype(np.float64)).max())
     counts = torch.full((1,), (1 << 40) + 5, dtype=torch.int64, device="cuda")  # the ring is full: every slot counts
     assert torch.equal(C.decode_attention_q4(q, codes, params, counts, S, W), out)
 
