@@ -34,6 +34,12 @@ __all__ = ["fused_rmsnorm", "fused_swiglu", "w4a16_gemv", "w4a16_lora_gemv",
            "decode_attention_q4", "prefill_attention_q4"]
 
 _LIB = _lib.load()  # fail at import time if the native library is absent
+try:
+    from . import _binding
+except ImportError as e:
+    raise ImportError(f"qextract_infer_b200: cannot load the native binding: {e}; run "
+                      "`python -m qextract_infer_b200.build`") from e
+_binding.set_error(_lib.QXError)
 _SUPPORTED_RANKS = (8, 16, 32, 48, 64, 128)
 
 
@@ -588,53 +594,17 @@ def prefill_attention(q, k_new, v_new, k_cache, v_cache, count: int, sink: int, 
 
 
 # ------------------------------------------- head norm + rotation, 4-bit ring --
-def _launch(dev: torch.device, what: str, fn, *args):
-    """``fn(*args, stream)`` on the current stream of ``dev``."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev))
-    if rc < 0:
-        _lib.check(rc, what)
-
-
-def _same_device(what: str, *tensors):
-    dev = tensors[0].device
-    if any(t.device != dev for t in tensors):
-        raise RuntimeError(f"{what}: tensors must be on one device")
-    return dev
-
-
+# (their argument checks, outputs and scratch are csrc/binding.cpp's)
 def qk_norm_rope(qkv: torch.Tensor, q_heads: int, kv_heads: int, q_norm: torch.Tensor, k_norm: torch.Tensor,
                  eps: float, cos: torch.Tensor, sin: torch.Tensor):
     """Head norm and rotation of a chunk in one pass: ``qkv`` fp16 ``[B, T,
     (q_heads + 2 kv_heads) D]`` (the fused projection's output), ``cos`` / ``sin``
     fp32 ``[T, D]`` (the chunk's positions) or ``[B, T, D]`` (each sequence's
-    own).  Returns q ``[B, T, q_heads, D]`` and k ``[B, T, kv_heads, D]``, RMSNorm'd
-    over D and rotated, and v ``[B, T, kv_heads, D]``.  Bit-identical to
-    ``fused_rmsnorm`` over the heads followed by rotate-half RoPE in fp32 (new
-    component: the reference runs them as separate torch ops)."""
-    for t, n in ((qkv, "qkv"), (q_norm, "q_norm"), (k_norm, "k_norm")):
-        _check_input(t, n)
-        _check_fp16(t, n)
-    D = q_norm.numel()
-    if q_heads < 1 or kv_heads < 1 or qkv.dim() != 3 or k_norm.numel() != D or \
-            qkv.size(2) != (q_heads + 2 * kv_heads) * D:
-        raise RuntimeError("qk_norm_rope: qkv must be [B, T, (q_heads + 2 kv_heads) * head_dim]")
-    B, T = qkv.size(0), qkv.size(1)
-    for t, n in ((cos, "cos"), (sin, "sin")):
-        _check_input(t, n)
-        if t.dtype != torch.float32 or tuple(t.shape) not in ((T, D), (B, T, D)) or t.shape != cos.shape:
-            raise RuntimeError(f"{n} must be float32 [{T}, {D}] or [{B}, {T}, {D}]")
-    dev = _same_device("qk_norm_rope", qkv, q_norm, k_norm, cos, sin)
-    q = torch.empty(B, T, q_heads, D, dtype=torch.float16, device=dev)
-    k = torch.empty(B, T, kv_heads, D, dtype=torch.float16, device=dev)
-    v = torch.empty_like(k)
-    _launch(dev, "qk_norm_rope", _LIB.qx_qk_norm_rope, qkv.data_ptr(), B * T, q_heads, kv_heads, D,
-            q_norm.data_ptr(), k_norm.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(),
-            max(1, cos.numel() // D), q.data_ptr(), k.data_ptr(), v.data_ptr())
-    return q, k, v
+    own), D 64, 128 or 256.  Returns q ``[B, T, q_heads, D]`` and k ``[B, T,
+    kv_heads, D]``, RMSNorm'd over D and rotated, and v ``[B, T, kv_heads, D]``.
+    Bit-identical to ``fused_rmsnorm`` over the heads followed by rotate-half RoPE
+    in fp32 (new component: the reference runs them as separate torch ops)."""
+    return _binding.qk_norm_rope(qkv, q_heads, kv_heads, q_norm, k_norm, eps, cos, sin)
 
 
 def ring_q4_slots(sink: int, window: int) -> int:
@@ -642,57 +612,20 @@ def ring_q4_slots(sink: int, window: int) -> int:
     return _lib.check(_LIB.qx_ring_q4_slots(int(sink), int(window)), "ring_q4_slots")
 
 
+def _check_q4_heads(what: str, head_dim: int, group_size: int):
+    if head_dim not in (64, 128) or group_size not in (32, 64, 128) or group_size > head_dim:
+        raise RuntimeError(f"{what}: head_dim must be 64 or 128, group_size 32, 64 or 128 and at most head_dim")
+
+
 def ring_q4_storage(batch: int, kv_heads: int, head_dim: int, sink: int, window: int, group_size: int = 64,
                     device="cuda"):
     """Zeroed storage of one layer's 4-bit ring: ``codes`` uint8 ``[2, B, Hkv,
     slots, D / 2]`` and ``params`` int16 ``[2, B, Hkv, slots, D / group_size]``
     (0: keys, 1: values), the form every ``*_q4`` op takes."""
-    if head_dim not in (64, 128) or group_size not in (32, 64, 128) or group_size > head_dim:
-        raise RuntimeError("ring_q4_storage: head_dim must be 64 or 128, group_size 32, 64 or 128 and at most head_dim")
+    _check_q4_heads("ring_q4_storage", head_dim, group_size)
     shape = (2, batch, kv_heads, ring_q4_slots(sink, window))
     return (torch.zeros(*shape, head_dim // 2, dtype=torch.uint8, device=device),
             torch.zeros(*shape, head_dim // group_size, dtype=torch.int16, device=device))
-
-
-def _ring_q4(what, codes, params, count, sink, window, *others):
-    """Checks a layer's 4-bit ring and returns (device, B, Hkv, D, group, the four
-    storage pointers, the count arguments)."""
-    for t, n, dt in ((codes, "codes", torch.uint8), (params, "params", torch.int16)):
-        _check_input(t, n)
-        if t.dtype != dt or t.dim() != 5 or t.size(0) != 2:
-            raise RuntimeError(f"{what}: codes must be uint8 [2, B, Hkv, slots, D / 2] and params int16 "
-                               "[2, B, Hkv, slots, D / group]")
-    _, B, Hkv, slots, half = codes.shape
-    if params.shape[:4] != codes.shape[:4] or slots != ring_q4_slots(sink, window):
-        raise RuntimeError(f"{what}: codes and params must have {ring_q4_slots(sink, window)} slots "
-                           f"(sink + window rounded up to 64), got {list(codes.shape)} and {list(params.shape)}")
-    D, groups = 2 * half, params.size(4)
-    if groups < 1 or D % groups:
-        raise RuntimeError(f"{what}: {groups} groups do not divide head_dim {D}")
-    if isinstance(count, torch.Tensor):
-        _check_input(count, "count")
-        if count.dtype != torch.int64 or tuple(count.shape) != (B,):
-            raise RuntimeError(f"{what}: a count tensor must be int64 [{B}]")
-        others += (count,)
-        counts = (0, count.data_ptr())
-    else:
-        counts = (int(count), None)
-    for t in others:
-        _check_input(t, f"{what}: every tensor")
-    dev = _same_device(what, codes, params, *others)
-    kc, kp = codes.data_ptr(), params.data_ptr()
-    ptrs = (kc, kp, kc + codes.numel() // 2, kp + params.numel())  # int16: half the elements are numel bytes
-    return dev, B, Hkv, D, D // groups, ptrs, counts
-
-
-def _check_new_kv(what, new_k, new_v, B, Hkv, D, tokens=None):
-    for t, n in ((new_k, "new_k"), (new_v, "new_v")):
-        _check_input(t, n)
-        _check_fp16(t, n)
-    if new_k.dim() != 4 or new_k.shape != new_v.shape or new_k.size(0) != B or \
-            tuple(new_k.shape[2:]) != (Hkv, D) or (tokens is not None and new_k.size(1) != tokens):
-        raise RuntimeError(f"{what}: new keys and values must be [{B}, {'T' if tokens is None else tokens}, {Hkv}, {D}], "
-                           f"got {list(new_k.shape)} and {list(new_v.shape)}")
 
 
 def ring_append_q4(new_k: torch.Tensor, new_v: torch.Tensor, codes: torch.Tensor, params: torch.Tensor,
@@ -700,31 +633,15 @@ def ring_append_q4(new_k: torch.Tensor, new_v: torch.Tensor, codes: torch.Tensor
     """Quantises ``new_k`` / ``new_v`` fp16 ``[B, T, Hkv, D]`` to 4 bits into the
     ring slots of positions ``count ..`` (in place; later tokens win a slot).
     ``count``: tokens written before, for all sequences or int64 ``[B]`` on the
-    device, each sequence's own."""
-    dev, B, Hkv, D, group, ptrs, counts = _ring_q4("ring_append_q4", codes, params, count, sink, window, new_k, new_v)
-    _check_new_kv("ring_append_q4", new_k, new_v, B, Hkv, D)
-    _launch(dev, "ring_append_q4", _LIB.qx_ring_append_q4, *ptrs, new_k.data_ptr(), new_v.data_ptr(), B,
-            new_k.size(1), Hkv, D, group, sink, window, *counts)
+    device, each sequence's own (read when the kernel runs: a captured graph
+    follows it)."""
+    _binding.ring_append_q4(new_k, new_v, codes, params, count, sink, window)
 
 
 def ring_gather_q4(codes: torch.Tensor, params: torch.Tensor, count: int, sink: int, window: int):
     """(K, V) of a 4-bit ring in logical order, fp16 ``[B, valid, Hkv, D]``: the
     values the attention multiplies, exactly."""
-    if isinstance(count, torch.Tensor):
-        raise RuntimeError("ring_gather_q4: count must be a number (it gives the output's length)")
-    dev, B, Hkv, D, group, ptrs, (n, _) = _ring_q4("ring_gather_q4", codes, params, count, sink, window)
-    valid = min(n, sink) + max(0, min(n - sink, window))
-    k = torch.empty(B, max(valid, 0), Hkv, D, dtype=torch.float16, device=dev)
-    v = torch.empty_like(k)
-    _launch(dev, "ring_gather_q4", _LIB.qx_ring_gather_q4, *ptrs, k.data_ptr(), v.data_ptr(), B, Hkv, D, group, sink,
-            window, n)
-    return k, v
-
-
-def _scratch(dev: torch.device, nbytes: int):
-    """Scratch of one call, from torch's allocator: calls on different streams
-    and captured graphs never share it."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    return _binding.ring_gather_q4(codes, params, count, sink, window)
 
 
 def decode_attention_q4(q: torch.Tensor, codes: torch.Tensor, params: torch.Tensor, count: int | torch.Tensor,
@@ -733,19 +650,7 @@ def decode_attention_q4(q: torch.Tensor, codes: torch.Tensor, params: torch.Tens
     Hq, D]``, ``count`` tokens written (the current one included), for all
     sequences or int64 ``[B]`` on the device; a sequence without tokens gets
     zeros."""
-    dev, B, Hkv, D, group, ptrs, counts = _ring_q4("decode_attention_q4", codes, params, count, sink, window, q)
-    _check_input(q, "q")
-    _check_fp16(q, "q")
-    if q.dim() != 3 or q.size(0) != B or q.size(2) != D:
-        raise RuntimeError(f"decode_attention_q4: q must be [{B}, Hq, {D}], got {list(q.shape)}")
-    Hq = q.size(1)
-    out = torch.empty_like(q)
-    with torch.cuda.device(dev):
-        need = _LIB.qx_decode_attention_q4_workspace_size(B, Hq, Hkv, D, sink, window)
-        ws = _scratch(dev, need)
-        _launch(dev, "decode_attention_q4", _LIB.qx_decode_attention_q4, q.data_ptr(), *ptrs, out.data_ptr(), B, Hq,
-                Hkv, D, group, sink, window, *counts, float(softmax_scale or 0.0), _ptr(ws), need)
-    return out
+    return _binding.decode_attention_q4(q, codes, params, count, sink, window, softmax_scale)
 
 
 def prefill_attention_q4(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, codes: torch.Tensor,
@@ -755,22 +660,7 @@ def prefill_attention_q4(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tens
     D]`` at positions ``count ..`` over the ring's ``count`` tokens and its own
     ``k_new`` / ``v_new`` fp16 ``[B, n, Hkv, D]`` (attended as given; append them
     afterwards).  Causal, sinks + the last ``window`` positions visible."""
-    dev, B, Hkv, D, group, ptrs, counts = _ring_q4("prefill_attention_q4", codes, params, count, sink, window, q,
-                                                   k_new, v_new)
-    _check_input(q, "q")
-    _check_fp16(q, "q")
-    if q.dim() != 4 or q.size(0) != B or q.size(3) != D:
-        raise RuntimeError(f"prefill_attention_q4: q must be [{B}, n, Hq, {D}], got {list(q.shape)}")
-    n, Hq = q.size(1), q.size(2)
-    _check_new_kv("prefill_attention_q4", k_new, v_new, B, Hkv, D, n)
-    out = torch.empty_like(q)
-    with torch.cuda.device(dev):
-        need = _LIB.qx_prefill_attention_q4_workspace_size(B, n, Hq, Hkv, D, sink, window)
-        ws = _scratch(dev, need)
-        _launch(dev, "prefill_attention_q4", _LIB.qx_prefill_attention_q4, q.data_ptr(), k_new.data_ptr(),
-                v_new.data_ptr(), *ptrs, out.data_ptr(), B, n, Hq, Hkv, D, group, sink, window, *counts,
-                float(softmax_scale or 0.0), _ptr(ws), need)
-    return out
+    return _binding.prefill_attention_q4(q, k_new, v_new, codes, params, count, sink, window, softmax_scale)
 
 
 class RingBufferKVCache:
@@ -893,9 +783,7 @@ class RingBufferKVCacheQ4(RingBufferKVCache):
                  window_size: int = 4092, batch: int = 1, device=None, group_size: int = 64):
         if window_size < 1 or sink_size < 0:
             raise RuntimeError("sink_size must be >= 0 and window_size >= 1")
-        if head_dim not in (64, 128) or group_size not in (32, 64, 128) or group_size > head_dim:
-            raise RuntimeError("RingBufferKVCacheQ4: head_dim must be 64 or 128, group_size 32, 64 or 128 and at "
-                               "most head_dim")
+        _check_q4_heads("RingBufferKVCacheQ4", head_dim, group_size)
         self.num_layers, self.num_kv_heads, self.head_dim = num_layers, num_kv_heads, head_dim
         self.sink_size, self.window_size = sink_size, window_size
         self.total_size = sink_size + window_size

@@ -12,6 +12,10 @@ rebuilt when their source or any header is newer.
 with per-CTA phase timestamps, recorded when ``qx_trace_launches`` is given a
 buffer (``bench.py --workload timeline`` reads them).  The package never loads
 it; the product library carries no trace code.
+
+Beside the library it builds ``_binding.so`` from ``csrc/binding.cpp`` with g++
+against torch's headers: the Python binding of the operators whose host side
+counts (it calls the library's C ABI).
 """
 
 from __future__ import annotations
@@ -32,6 +36,7 @@ BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libqx_b200.so")
 BUILD_TRACE = os.path.join(PKG, "_build_trace")
 LIB_TRACE = os.path.join(PKG, "libqx_b200_trace.so")
+BINDING = os.path.join(PKG, "_binding.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -88,7 +93,37 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None, trace: b
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, lib)
+    if not trace:
+        build_binding(force=force, verbose=verbose)
     return lib
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    """``_binding.so``, linked against ``libqx_b200.so`` beside it and torch."""
+    src = os.path.join(CSRC, "binding.cpp")
+    if not (force or _stale(BINDING, [src, os.path.join(INCLUDE, "qx_b200.h")])):
+        return BINDING
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    tmp = BINDING + f".tmp{os.getpid()}"
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE,
+           "-I", sysconfig.get_paths()["include"], "-I", os.path.join(cuda, "include")]
+    for d in cpp_extension.include_paths():
+        cmd += ["-isystem", d]
+    cmd += [src, "-o", tmp, "-L", PKG, "-l:libqx_b200.so", "-Wl,-rpath,$ORIGIN", "-L", lib, "-lc10", "-lc10_cuda",
+            "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
 
 
 def main(argv=None):
