@@ -20,26 +20,32 @@
 //                 P s in fp16 per group.  P^T comes from S^T's accumulator layout
 //                 by movmatrix.
 // The online softmax keeps a running reference and sum per warp and head in fp32.
-// The reference is the maximum score plus the exponent E of the largest value scale
-// so far, and P carries 2^14: P s stays below 2^15 and its fp16 subnormals start
-// below 2^-28 of the largest.
+// The reference is the largest score, to 2^4, plus the exponent of the largest value
+// scale so far, and P carries 2^10: P s stays below 2^15 and its fp16 subnormals
+// start below 2^-24 of the largest.
 //
 // What bounds it: at 8 sequences and more the instructions (about 250 a warp for
 // 16 tokens of a KV head), not HBM.  Made exact fp16 s (c - z) in registers, with
 // three instructions a pair of V, it took 352.
 //
 // Each warp streams its steps of 32 tokens through a ring of its own in shared
-// memory (STAGES deep, four bulk copies a step onto one mbarrier) and reads the
-// fragments from there; the format puts each lane's share of a row side by side.
-// (Loaded from global memory straight into the fragments, one step ahead, the bytes
-// in flight hung on the registers: 41 us for 32 sequences x 4096 slots.)  A warp
-// takes every (4 nsplit)-th step.  The warps of a CTA join their results in the
-// ring's memory; with more than one split the CTAs write fp32 partial results and a
-// second kernel joins them.
+// memory (STAGES deep, cp.async) and reads the fragments from there; the format puts
+// each lane's share of a row side by side.  (Loaded from global memory straight into
+// the fragments, one step ahead, the bytes in flight hung on the registers: 84 us for
+// one sequence of 131072 slots.  Four bulk copies a step, two of them of 128 bytes,
+// were bound by the number of copies: 47 us for 32 sequences x 4096 slots.)
+//
+// The work is cut into units of 128 tokens of one (sequence, KV head), and the CTAs,
+// as many as are resident at once, take equal runs of units in order, whatever pair
+// they belong to: with a grid of (split, KV head, sequence) the last wave of CTAs left
+// SMs idle (41 us for 32 sequences x 4096 slots at the best split).  The warps of a
+// CTA take a unit's four steps and join their results of a pair in the ring's
+// memory; a pair that one CTA did whole is finished there, the others' fp32 results
+// are joined by a second kernel (the results of CTA i for pair j are number i + j:
+// in the order of the runs each next one has a larger i or a larger j).
 //
 // Row g of an MMA is token g ^ (g / 2 & 1) of its eight: neighbouring rows, and the
 // rows that four quads read together, then lie in different halves of the banks.
-// Every wait is bounded (kWaitLimitNs, then QX_DEVERR_MBAR_TIMEOUT).
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -53,8 +59,9 @@ namespace dattn4 {
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int STEP = 32;          // tokens per warp step
-constexpr float PSHIFT = 14.f;    // P carries 2^14
-constexpr int MAX_SPLITS = 64;
+constexpr float GROW = 4.f;       // log2 growth of the largest score that the reference follows
+constexpr float PSHIFT = 14.f - GROW;  // what P carries: P s stays below 2^15
+constexpr int UNIT = WARPS * STEP;  // tokens
 constexpr int STAGES = 3;
 
 // bytes of a stage: codes of K and V, params of K and V
@@ -62,12 +69,12 @@ template <int D, int NG>
 struct Stage {
   static constexpr int CODES = STEP * D / 2, PARAMS = STEP * NG * 2, BYTES = 2 * (CODES + PARAMS);
 };
-// shared memory: the ring of every warp, or the warps' results; then the barriers
+// shared memory: the ring of every warp, or the warps' results
 template <int D, int NG, int NT>
 struct Smem {
   static constexpr int RING = WARPS * STAGES * Stage<D, NG>::BYTES;
   static constexpr int JOIN = WARPS * 8 * NT * (D + 1 + 2) * 4;
-  static constexpr int BARS = RING > JOIN ? RING : (JOIN + 15) / 16 * 16, BYTES = BARS + WARPS * STAGES * 8;
+  static constexpr int BYTES = RING > JOIN ? RING : JOIN;
 };
 
 struct Params {
@@ -77,46 +84,81 @@ struct Params {
   const unsigned char* vc;
   const uint16_t* vp;
   __half* out;
-  float* part_o;   // [batch][q_heads][nsplit][D]
-  float2* part_ml;  // [batch][q_heads][nsplit]
+  float* part_o;    // [piece][G][D]
+  float2* part_ml;  // [piece][G]
   const int64_t* counts;
   int64_t count, cap;
-  int hq, hkv, G, sink, window, nsplit;
+  int batch, hq, hkv, G, sink, window;
+  int ctas;  // of the first kernel
   float scale_log2;
 };
 
-// Sticky device-side error word of this file's kernels (QX_DEVERR_* bits),
-// merged into qx_get_device_error.
-static __device__ unsigned g_decode4_error = 0;
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ int valid_of(const Params& p, int b) {
+  return kv4::valid_slots(kv4::count_of(p.counts, p.count, b), p.sink, p.window);
+}
+__device__ __forceinline__ int units_of(const Params& p, int b) { return (valid_of(p, b) + UNIT - 1) / UNIT; }
+// first unit of CTA i
+__device__ __forceinline__ int first_unit(int total, int i, int ctas) {
+  return ctas > 0 ? int(int64_t(total) * i / ctas) : 0;
+}
+// the CTA that has unit u: the last one whose first unit is at most u
+__device__ __forceinline__ int cta_of(int u, int total, int ctas) { return int((int64_t(u + 1) * ctas - 1) / total); }
 
-__device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{ .reg .pred P; mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 P, [%1], %2; "
-      "selp.u32 %0, 1, 0, P; }"
-      : "=r"(ok)
-      : "r"(b), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __noinline__ bool bar_wait_slow(uint32_t b, uint32_t parity) {
-  uint64_t t0, t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  while (!bar_try(b, parity)) {
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (t - t0 > kWaitLimitNs) {
-      atomicOr(&g_decode4_error, QX_DEVERR_MBAR_TIMEOUT);
-      return false;
-    }
+// With a count for each sequence: how the units of all KV heads lie, found by a whole
+// block of T threads from the counts.  total: all of them; b, first: the sequence that
+// unit `u(total)` lies in and its first unit, or of sequence `want` where that is not
+// negative.  Up to T sequences take one pass over the counts.
+template <int T, class U>
+__device__ void place(const Params& p, int want, U u, int& total, int& b, int& first) {
+  __shared__ int s_warp[T / 32], s_b, s_first;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int head = tid < p.batch ? units_of(p, tid) * p.hkv : 0;  // of the first T sequences
+  int rest = 0;
+  for (int i = T + tid; i < p.batch; i += T) rest += units_of(p, i) * p.hkv;
+  total = 0;
+  if (p.batch > T) {
+    rest = __reduce_add_sync(0xffffffffu, rest);
+    if (lane == 0) s_warp[warp] = rest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < T / 32; ++w) total += s_warp[w];
+    __syncthreads();
   }
-  return true;
+  int at = 0;
+  for (int b0 = 0, before = 0;; b0 += T) {
+    const int mine = b0 == 0 ? head : b0 + tid < p.batch ? units_of(p, b0 + tid) * p.hkv : 0;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += t;
+    }
+    if (lane == 31) s_warp[warp] = upto;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < T / 32; ++w) {
+      if (w < warp) upto += s_warp[w];
+      all += s_warp[w];
+    }
+    if (b0 == 0) {
+      total += all;
+      at = u(total);
+    }
+    upto += before;
+    const bool here = want >= 0 ? b0 + tid == want : upto - mine <= at && at < upto;
+    if (here) s_b = b0 + tid, s_first = upto - mine;
+    before += all;
+    __syncthreads();
+    if ((want >= 0 ? want < b0 + T : at < before) || b0 + T >= p.batch) break;
+  }
+  b = s_b;
+  first = s_first;
 }
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(dst),
-      "l"(src), "r"(bytes), "r"(bar), "l"(policy)
-      : "memory");
-}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -163,8 +205,11 @@ __device__ __forceinline__ float scale_of(const RowParams<NG>& p, int grp) {
   return __half2float(__ushort_as_half(uint16_t(w & 0xFFF0u)));
 }
 
+// what their registers and rings allow
+constexpr int ctas_per_sm(int head_dim, int n_tiles) { return n_tiles > 1 ? 2 : head_dim == 64 ? 4 : 3; }
+
 template <int D, int NG, int NT>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_kernel(const __grid_constant__ Params p) {
   pdl_trigger();
   constexpr int NI = D / 32, IPG = NI / NG;  // 32-value blocks of a row, and of a group
   constexpr int SROW = D + 1;                // odd: the column writes below meet no bank twice
@@ -176,44 +221,61 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kerne
   float (*s_l)[8 * NT] = s_m + WARPS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, c = lane & 3;
-  const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
   const unsigned char* ring = smem + warp * STAGES * St::BYTES;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-  const uint32_t bars = static_cast<uint32_t>(__cvta_generic_to_shared(smem + Sm::BARS)) + warp * STAGES * 8;
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < STAGES; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + 8 * i) : "memory");
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __syncwarp();
   pdl_wait();
-  const int valid = kv4::valid_slots(kv4::count_of(p.counts, p.count, b), p.sink, p.window);
-  const int steps = (valid + STEP - 1) / STEP, stride = p.nsplit * WARPS;
-  int step = split * WARPS + warp;
+  // this CTA's units [u, u_end), and the sequence and its first unit that u lies in
+  int b, first, total, units = 0;
+  if (p.counts) {
+    place<THREADS>(p, -1, [&](int all) { return first_unit(all, min(int(blockIdx.x), min(p.ctas, all) - 1), min(p.ctas, all)); },
+                   total, b, first);
+  } else {
+    units = units_of(p, 0);
+    total = units * p.hkv * p.batch;
+  }
+  const int n = min(p.ctas, total);  // CTAs with work: none of them has an empty run
+  if (int(blockIdx.x) >= n) return;
+  int u = first_unit(total, blockIdx.x, n);
+  const int u_end = first_unit(total, blockIdx.x + 1, n);
+  if (p.counts) {
+    units = units_of(p, b);
+  } else {
+    b = u / (units * p.hkv);
+    first = b * units * p.hkv;
+  }
 
-  // (a step's rows all lie in the storage: it has a multiple of 64)
-  const int64_t row0 = (int64_t(b) * p.hkv + kvh) * p.cap;
-  uint64_t policy;  // read once
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-  auto fetch = [&](int st, int t) {  // lane 0
-    const uint32_t dst = ring_at + st * St::BYTES, bar = bars + 8 * st;
-    const int64_t row = row0 + int64_t(t) * STEP;
-    asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(St::BYTES) : "memory");
-    bulk_copy(dst, p.kc + row * (D / 2), St::CODES, bar, policy);
-    bulk_copy(dst + 2 * St::CODES, p.kp + row * NG, St::PARAMS, bar, policy);
-    bulk_copy(dst + St::CODES, p.vc + row * (D / 2), St::CODES, bar, policy);
-    bulk_copy(dst + 2 * St::CODES + St::PARAMS, p.vp + row * NG, St::PARAMS, bar, policy);
-  };
-  if (lane == 0)
+  // a step's rows to stage st, 16 bytes a lane and copy; they all lie in the storage: it has a multiple of 64
+  auto fetch = [&](int st, int64_t row) {
+    const uint32_t dst = ring_at + st * St::BYTES + lane * 16;
+    const unsigned char *kc = p.kc + row * (D / 2) + lane * 16, *vc = p.vc + row * (D / 2) + lane * 16;
 #pragma unroll
-    for (int i = 0; i < STAGES; ++i)
-      if (step + i * stride < steps) fetch(i, step + i * stride);
+    for (int i = 0; i < St::CODES / 512; ++i) {
+      copy16(dst + i * 512, kc + i * 512);
+      copy16(dst + St::CODES + i * 512, vc + i * 512);
+    }
+    const int l = lane & 15;  // params: K's by the first half of the warp, V's by the second
+    if (l < St::PARAMS / 16)
+      copy16(ring_at + st * St::BYTES + 2 * St::CODES + (lane >> 4) * St::PARAMS + l * 16,
+             reinterpret_cast<const unsigned char*>((lane >> 4 ? p.vp : p.kp) + row * NG) + l * 16);
+  };
   // this lane's places in a stage: MMA row g is token tg of its eight
   const int tg = g ^ ((g >> 1) & 1), odd = c & 1;
   const int at_k = tg * (D / 2) + c * (D / 8), at_p = 2 * St::CODES + tg * NG * 2;
   const int at_v[2] = {St::CODES + (2 * c + odd) * (D / 2) + g * (D / 16), St::CODES + (2 * c + 1 - odd) * (D / 2) + g * (D / 16)};
   const int at_z = 2 * St::CODES + St::PARAMS + 2 * c * NG * 2;
   const uint32_t sel_lo = odd ? 0x1054u : 0x5410u, sel_hi = odd ? 0x3276u : 0x7632u;  // a pair of tokens in MMA order
+
+  const uint32_t kz_mask = c == 0 ? 0x000F000Fu : 0u;
+  while (true) {  // a pair (sequence b, KV head kvh), or the part of it that is this CTA's
+  const int kvh = (u - first) / units, off = u - first - kvh * units, len = min(units - off, u_end - u);
+  const int valid = valid_of(p, b), steps = min((valid + STEP - 1) / STEP, (off + len) * WARPS);
+  const int64_t row0 = (int64_t(b) * p.hkv + kvh) * p.cap;
+  int step = off * WARPS + warp;
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) {
+    if (step + i * WARPS < steps) fetch(i, row0 + int64_t(step + i * WARPS) * STEP);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
 
   // Q^T fragments: head g (of N tile nt), values 32 i + 8 c ..; a head is scaled by
   // the power of two that brings its largest value to [2^4, 2^5), undone in hf: the
@@ -279,24 +341,17 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kerne
 #pragma unroll
     for (int n = 0; n < NG; ++n) oz[n][nt][0] = oz[n][nt][1] = oz[n][nt][2] = oz[n][nt][3] = 0.f;
   }
-  // m_r: the largest score; vexp: the exponent of the largest value scale (of its bits,
-  // biased); ref = m_r + vexp - 14 what the weights refer to
-  float m_r[NT][2], l_r[NT][2];
+  // m_r: the score and vexp: the exponent (of its bits, biased) of the value scale that the
+  // weights refer to
+  float m_r[NT][2], l_r[NT][2], shift[NT][2];
   int vexp = 0;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) m_r[nt][0] = m_r[nt][1] = -INFINITY, l_r[nt][0] = l_r[nt][1] = 0.f;
-  const uint32_t kz_mask = c == 0 ? 0x000F000Fu : 0u;
-
-  int st = 0;
-  uint32_t phase = 0;
-  for (; step < steps; step += stride) {
+  for (int nt = 0; nt < NT; ++nt) m_r[nt][0] = m_r[nt][1] = -INFINITY, l_r[nt][0] = l_r[nt][1] = shift[nt][0] = shift[nt][1] = 0.f;
+  for (int st = 0; step < steps; step += WARPS, st = st + 1 == STAGES ? 0 : st + 1) {
     const int left = valid - step * STEP;  // tokens of this step that exist
     const unsigned char* at = ring + st * St::BYTES;
-    if (!bar_try(bars + 8 * st, phase) && !bar_wait_slow(bars + 8 * st, phase)) {
-      for (int i = 1; i < STAGES && step + i * stride < steps; ++i)  // the copies behind it, too, before the memory goes
-        bar_wait_slow(bars + 8 * ((st + i) % STAGES), st + i >= STAGES ? phase ^ 1 : phase);
-      break;
-    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    __syncwarp();
     // scores, over hf: rows g, g + 8 (e >> 1) by heads 2c, 2c + 1 (e & 1)
     float s[2][NT][4];
 #pragma unroll
@@ -362,49 +417,60 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kerne
           for (int e = 0; e < 4; ++e)
             if (u * 16 + tg + 8 * (e >> 1) >= left) s[u][nt][e] = -INFINITY;
     }
-    const int e_new = max(vexp, int(__reduce_max_sync(0xffffffffu, max(top >> 16, top & 0xFFFFu)) >> 10));
-    bool grew = e_new != vexp;
-    const float e_shift = float(e_new - vexp);
-    vexp = e_new;
-    // online softmax
-    float alpha[NT][2];
+    // The reference (a score, m_r, and the exponent of the largest value scale, vexp) follows
+    // only where a score passes m_r by 2^GROW or a scale passes vexp; m_r starts at minus infinity.
+    float mx[NT][2];
+    bool grew = (max(top >> 16, top & 0xFFFFu) >> 10) > uint32_t(vexp);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        float mx = fmaxf(fmaxf(s[0][nt][k], s[0][nt][2 + k]), fmaxf(s[1][nt][k], s[1][nt][2 + k]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float mn = fmaxf(m_r[nt][k], mx * hf[nt][k]), mb = mn == -INFINITY ? 0.f : mn;
-        alpha[nt][k] = ex2(m_r[nt][k] - mb - e_shift);
-        grew = grew || mn != m_r[nt][k];
-        m_r[nt][k] = mn;
-        const float shift = PSHIFT + 14.f - float(vexp) - mb;
-        float sum = 0.f;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            s[u][nt][2 * r + k] = ex2(fmaf(s[u][nt][2 * r + k], hf[nt][k], shift));
-            sum += s[u][nt][2 * r + k];
-          }
-        l_r[nt][k] = fmaf(l_r[nt][k], alpha[nt][k], sum);
+        mx[nt][k] = fmaxf(fmaxf(s[0][nt][k], s[0][nt][2 + k]), fmaxf(s[1][nt][k], s[1][nt][2 + k])) * hf[nt][k];
+        grew = grew || mx[nt][k] > m_r[nt][k] + GROW;
       }
     if (__any_sync(0xffffffffu, grew)) {
+      const int e_new = max(vexp, int(__reduce_max_sync(0xffffffffu, max(top >> 16, top & 0xFFFFu)) >> 10));
+      const float e_shift = float(e_new - vexp);
+      vexp = e_new;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float alpha[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float m = mx[nt][k];
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          m = fmaxf(m, m_r[nt][k]);
+          const float mb = m == -INFINITY ? 0.f : m;
+          alpha[k] = ex2(m_r[nt][k] - mb - e_shift);
+          m_r[nt][k] = m;
+          l_r[nt][k] *= alpha[k];
+          shift[nt][k] = PSHIFT + 14.f - float(vexp) - mb;
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
 #pragma unroll
           for (int i = 0; i < NI; ++i) {
-            o[i][0][nt][e] *= alpha[nt][e & 1];
-            o[i][1][nt][e] *= alpha[nt][e & 1];
+            o[i][0][nt][e] *= alpha[e & 1];
+            o[i][1][nt][e] *= alpha[e & 1];
           }
 #pragma unroll
-          for (int n = 0; n < NG; ++n) oz[n][nt][e] *= alpha[nt][e & 1];
+          for (int n = 0; n < NG; ++n) oz[n][nt][e] *= alpha[e & 1];
         }
+      }
     }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            s[u][nt][2 * r + k] = ex2(fmaf(s[u][nt][2 * r + k], hf[nt][k], shift[nt][k]));
+            l_r[nt][k] += s[u][nt][2 * r + k];
+          }
     // O^T += V^T (P s)^T
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -443,11 +509,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kerne
       }
     }
     __syncwarp();  // every lane has read the stage
-    if (lane == 0 && step + STAGES * stride < steps) fetch(st, step + STAGES * stride);
-    if (++st == STAGES) {
-      st = 0;
-      phase ^= 1;
-    }
+    if (step + STAGES * WARPS < steps) fetch(st, row0 + int64_t(step + STAGES * WARPS) * STEP);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
   __syncthreads();  // the rings are free
 
@@ -485,61 +548,93 @@ __global__ void __launch_bounds__(THREADS, NT == 1 ? 3 : 2) decode_attn_q4_kerne
       acc = fmaf(a, s_o[w][h][d], acc);
       l = fmaf(a, s_l[w][h], l);
     }
-    const int64_t row = int64_t(b) * p.hq + int64_t(kvh) * p.G + h;
-    if (p.nsplit == 1) {
-      p.out[row * D + d] = __float2half_rn(valid > 0 ? acc / l : 0.f);
+    if (len == units) {
+      p.out[(int64_t(b) * p.hq + int64_t(kvh) * p.G + h) * D + d] = __float2half_rn(acc / l);
     } else {
-      p.part_o[(row * p.nsplit + split) * D + d] = acc;
-      if (d == 0) p.part_ml[row * p.nsplit + split] = make_float2(m, l);
+      const int64_t piece = (int64_t(blockIdx.x) + int64_t(b) * p.hkv + kvh) * p.G + h;
+      p.part_o[piece * D + d] = acc;
+      if (d == 0) p.part_ml[piece] = make_float2(m, l);
     }
   }
+  u += len;
+  if (u >= u_end) break;
+  if (off + len == units && kvh == p.hkv - 1) {  // the next sequence with tokens
+    first += units * p.hkv;
+    do units = units_of(p, ++b);
+    while (units == 0);
+  }
+  __syncthreads();  // the ring's memory back to the copies
+  }
 }
 
-// joins the splits of one (sequence, query head): one warp
-template <int D>
-__global__ void __launch_bounds__(32) decode_attn_q4_merge_kernel(const float* __restrict__ part_o,
-                                                                  const float2* __restrict__ part_ml,
-                                                                  __half* __restrict__ out, const int64_t* counts,
-                                                                  int64_t count, int hq, int nsplit) {
+// Joins the pieces of one (sequence, query head), PARTS groups of D threads taking
+// every PARTS-th; zeros where a sequence has no token.
+template <int D, int PARTS>
+__global__ void __launch_bounds__(PARTS * D) decode_attn_q4_merge_kernel(const __grid_constant__ Params p) {
   pdl_trigger();
   pdl_wait();
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x;
-  const int64_t row = blockIdx.x;
+  __shared__ float s_acc[PARTS][D], s_l[PARTS];
+  __shared__ int s_cta[2];
+  const int b = blockIdx.x / p.hq, h = blockIdx.x - b * p.hq, kvh = h / p.G, d = threadIdx.x % D, part = threadIdx.x / D;
+  const int units = units_of(p, b);
+  __half* out = p.out + (int64_t(b) * p.hq + h) * D + d;
+  if (units == 0) {
+    if (part == 0) *out = __float2half_rn(0.f);
+    return;
+  }
+  int first, total, at = b;
+  if (p.counts) {
+    place<PARTS * D>(p, b, [](int) { return 0; }, total, at, first);
+  } else {
+    total = units * p.hkv * p.batch;
+    first = b * units * p.hkv;
+  }
+  first += kvh * units;
+  if (threadIdx.x < 2)  // the CTAs of the first and of the last unit
+    s_cta[threadIdx.x] = cta_of(threadIdx.x == 0 ? first : first + units - 1, total, min(p.ctas, total));
+  __syncthreads();
+  const int i0 = s_cta[0], i1 = s_cta[1];
+  if (i0 == i1) return;  // one CTA's: finished there
+  const int64_t base = (int64_t(b) * p.hkv + kvh) * p.G + (h - kvh * p.G);  // piece i at base + i G
   float m = -INFINITY;
-  for (int s = lane; s < nsplit; s += 32) m = fmaxf(m, part_ml[row * nsplit + s].x);
+  for (int i = i0 + int(threadIdx.x) % 32; i <= i1; i += 32) m = fmaxf(m, p.part_ml[base + int64_t(i) * p.G].x);
   m = warp_max(m);
   const float mb = m == -INFINITY ? 0.f : m;
-  float acc[E], l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int s = 0; s < nsplit; ++s) {
-    const float2 ml = part_ml[row * nsplit + s];
+  float acc = 0.f, l = 0.f;
+#pragma unroll 8
+  for (int i = i0 + part; i <= i1; i += PARTS) {
+    const float2 ml = p.part_ml[base + int64_t(i) * p.G];
     const float a = ex2(ml.x - mb);
     l = fmaf(a, ml.y, l);
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(a, part_o[(row * nsplit + s) * D + e * 32 + lane], acc[e]);
+    acc = fmaf(a, p.part_o[(base + int64_t(i) * p.G) * D + d], acc);
   }
-  const bool some = kv4::count_of(counts, count, int(row / hq)) > 0;
+  if constexpr (PARTS > 1) {
+    s_acc[part][d] = acc;
+    if (d == 0) s_l[part] = l;
+    __syncthreads();
+    if (part > 0) return;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[row * D + e * 32 + lane] = __float2half_rn(some ? acc[e] / l : 0.f);
+    for (int k = 1; k < PARTS; ++k) acc += s_acc[k][d], l += s_l[k];
+  }
+  *out = __float2half_rn(acc / l);
 }
 
-// CTAs that split a KV head's slots: as many as keep every SM's three CTAs busy,
-// as long as each warp has a step
-inline int splits(int batch, int kv_heads, int valid) {
-  const int pairs = batch * kv_heads;
-  const int want = (device_sm_count() * 6 + pairs - 1) / pairs;
-  const int most = (valid + STEP * WARPS - 1) / (STEP * WARPS);
-  return std::max(1, std::min({want, most, MAX_SPLITS}));
+// CTAs of the first kernel: those resident at once, or one a unit of what the ring
+// can hold.  Not of what it holds, so that a call sums in the same order whether
+// its counts are known on the host or not.
+inline int64_t units_most(int batch, int kv_heads, int sink, int window) {
+  return (kv4::capacity(sink, window) + UNIT - 1) / UNIT * batch * kv_heads;
 }
-
-inline size_t workspace_for(int batch, int q_heads, int head_dim, int nsplit) {
-  return nsplit == 1 ? 0 : size_t(batch) * q_heads * nsplit * (size_t(head_dim) * sizeof(float) + sizeof(float2));
+inline int ctas(int batch, int q_heads, int kv_heads, int head_dim, int sink, int window) {
+  const int most = device_sm_count() * ctas_per_sm(head_dim, q_heads / kv_heads > 8 ? 2 : 1);
+  return int(std::min<int64_t>(most, units_most(batch, kv_heads, sink, window)));
+}
+inline size_t workspace_for(int batch, int q_heads, int kv_heads, int head_dim, int n) {
+  return (size_t(n) + size_t(batch) * kv_heads) * (q_heads / kv_heads) * (size_t(head_dim) * sizeof(float) + sizeof(float2));
 }
 
 template <int D, int NG, int NT>
-cudaError_t launch(const Params& p, int batch, cudaStream_t st) {
+cudaError_t launch(const Params& p, cudaStream_t st) {
   {
     static std::mutex mu;
     static bool done[64] = {};
@@ -555,25 +650,23 @@ cudaError_t launch(const Params& p, int batch, cudaStream_t st) {
       done[dev] = true;
     }
   }
-  return launch_pdl(decode_attn_q4_kernel<D, NG, NT>, dim3(unsigned(p.nsplit), unsigned(p.hkv), unsigned(batch)),
-                    dim3(THREADS), Smem<D, NG, NT>::BYTES, st, p);
+  const cudaError_t e = launch_pdl(decode_attn_q4_kernel<D, NG, NT>, dim3(unsigned(p.ctas)), dim3(THREADS),
+                                   Smem<D, NG, NT>::BYTES, st, p);
+  // where the runs end with pairs, known here without per-sequence counts, every pair is one CTA's
+  if (e != cudaSuccess || (!p.counts && p.count > 0 && p.batch * p.hkv % p.ctas == 0)) return e;
+  const dim3 grid(unsigned(p.batch) * unsigned(p.hq));
+  // many pieces a pair (one sequence: 32 and more) are loaded by four groups of threads: 8.3 instead of 9.5 us for
+  // one sequence of 4096 slots; a few by one: 512 threads a block and row cost 4 us more at 32 sequences
+  if (p.ctas >= 8 * p.batch * p.hkv)
+    return launch_pdl(decode_attn_q4_merge_kernel<D, 4>, grid, dim3(4 * D), 0, st, p);
+  return launch_pdl(decode_attn_q4_merge_kernel<D, 1>, grid, dim3(D), 0, st, p);
 }
 template <int D, int NG>
-cudaError_t launch(const Params& p, int batch, cudaStream_t st) {
-  return p.G <= 8 ? launch<D, NG, 1>(p, batch, st) : launch<D, NG, 2>(p, batch, st);
+cudaError_t launch(const Params& p, cudaStream_t st) {
+  return p.G <= 8 ? launch<D, NG, 1>(p, st) : launch<D, NG, 2>(p, st);
 }
 
 }  // namespace dattn4
-
-int decode4_device_error(unsigned* code, int reset) {
-  QX_CUDA_TRY(cudaMemcpyFromSymbol(code, dattn4::g_decode4_error, sizeof(unsigned)), "get_device_error: read");
-  if (reset) {
-    const unsigned zero = 0;
-    QX_CUDA_TRY(cudaMemcpyToSymbol(dattn4::g_decode4_error, &zero, sizeof(unsigned)), "get_device_error: reset");
-  }
-  return QX_OK;
-}
-
 }  // namespace qx
 
 using namespace qx;
@@ -583,7 +676,8 @@ extern "C" size_t qx_decode_attention_q4_workspace_size(int batch, int q_heads, 
   if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || (head_dim != 64 && head_dim != 128) ||
       sink < 0 || window < 1 || kv4::capacity(sink, window) >= (int64_t(1) << 30))
     return 0;
-  return dattn4::workspace_for(batch, q_heads, head_dim, dattn4::splits(batch, kv_heads, sink + window));
+  return dattn4::workspace_for(batch, q_heads, kv_heads, head_dim,
+                               dattn4::ctas(batch, q_heads, kv_heads, head_dim, sink, window));
 }
 
 extern "C" int qx_decode_attention_q4(const void* q, const void* k_codes, const void* k_params, const void* v_codes,
@@ -602,10 +696,10 @@ extern "C" int qx_decode_attention_q4(const void* q, const void* k_codes, const 
   QX_REQUIRE(aligned(q, 16) && aligned(k_codes, 16) && aligned(v_codes, 16) && aligned(k_params, 16) &&
                  aligned(v_params, 16) && aligned(out, 16),
              "decode_attention_q4: tensors must be 16-byte aligned");
-  // the split is chosen for what the ring can hold, whether the counts are known here or not: the
-  // same ring always sums in the same order
-  const int nsplit = dattn4::splits(batch, kv_heads, sink + window);
-  const size_t need = dattn4::workspace_for(batch, q_heads, head_dim, nsplit);
+  QX_REQUIRE(dattn4::units_most(batch, kv_heads, sink, window) < (int64_t(1) << 31) && int64_t(batch) * q_heads < (int64_t(1) << 31),
+             "decode_attention_q4: batch x heads x slots too large");
+  const int n = dattn4::ctas(batch, q_heads, kv_heads, head_dim, sink, window);
+  const size_t need = dattn4::workspace_for(batch, q_heads, kv_heads, head_dim, n);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(QX_ERR_WORKSPACE, "decode_attention_q4: workspace needs %zu bytes, 16-byte aligned", need);
   dattn4::Params p{};
@@ -616,7 +710,7 @@ extern "C" int qx_decode_attention_q4(const void* q, const void* k_codes, const 
   p.vp = static_cast<const uint16_t*>(v_params);
   p.out = static_cast<__half*>(out);
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + int64_t(batch) * q_heads * nsplit * head_dim);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t(n) + int64_t(batch) * kv_heads) * (q_heads / kv_heads) * head_dim);
   p.counts = counts;
   p.count = count;
   p.cap = kv4::capacity(sink, window);
@@ -625,28 +719,17 @@ extern "C" int qx_decode_attention_q4(const void* q, const void* k_codes, const 
   p.G = q_heads / kv_heads;
   p.sink = sink;
   p.window = window;
-  p.nsplit = nsplit;
+  p.batch = batch;
+  p.ctas = n;
   p.scale_log2 = (softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf(float(head_dim))) * 1.4426950408889634f;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (head_dim == 64)
-    e = group == 32 ? dattn4::launch<64, 2>(p, batch, st) : dattn4::launch<64, 1>(p, batch, st);
+    e = group == 32 ? dattn4::launch<64, 2>(p, st) : dattn4::launch<64, 1>(p, st);
   else
-    e = group == 32   ? dattn4::launch<128, 4>(p, batch, st)
-        : group == 64 ? dattn4::launch<128, 2>(p, batch, st)
-                      : dattn4::launch<128, 1>(p, batch, st);
+    e = group == 32   ? dattn4::launch<128, 4>(p, st)
+        : group == 64 ? dattn4::launch<128, 2>(p, st)
+                      : dattn4::launch<128, 1>(p, st);
   QX_CUDA_TRY(e, "decode_attention_q4: launch");
-  if (nsplit > 1) {
-    const dim3 grid(unsigned(batch) * unsigned(q_heads));
-    if (head_dim == 64)
-      e = launch_pdl(dattn4::decode_attn_q4_merge_kernel<64>, grid, dim3(32), 0, st,
-                     static_cast<const float*>(p.part_o), static_cast<const float2*>(p.part_ml), p.out, counts, count,
-                     q_heads, nsplit);
-    else
-      e = launch_pdl(dattn4::decode_attn_q4_merge_kernel<128>, grid, dim3(32), 0, st,
-                     static_cast<const float*>(p.part_o), static_cast<const float2*>(p.part_ml), p.out, counts, count,
-                     q_heads, nsplit);
-    QX_CUDA_TRY(e, "decode_attention_q4: merge launch");
-  }
   return check_launch("decode_attention_q4");
 }

@@ -1321,7 +1321,6 @@ int gemm_device_error(unsigned* code, int reset);      // w4a16_gemm.cu
 int nvar_device_error(unsigned* code, int reset);      // nvlink_allreduce.cu
 int attn_device_error(unsigned* code, int reset);      // decode_attn.cu
 int prefill4_device_error(unsigned* code, int reset);  // prefill_attn_q4.cu
-int decode4_device_error(unsigned* code, int reset);   // decode_attn_q4.cu
 }
 
 extern "C" int qx_get_device_error(unsigned* code, int reset) {
@@ -1344,9 +1343,6 @@ extern "C" int qx_get_device_error(unsigned* code, int reset) {
   if (rc != QX_OK) return rc;
   *code |= other;
   rc = qx::prefill4_device_error(&other, reset);
-  if (rc != QX_OK) return rc;
-  *code |= other;
-  rc = qx::decode4_device_error(&other, reset);
   if (rc != QX_OK) return rc;
   *code |= other;
   return QX_OK;

@@ -3,7 +3,7 @@ in 64 bits on the values the cache stands for.
 
 Tolerance of an element, from the roundings: the result once to fp16 (2^-11 of
 it); every softmax weight once to fp16 (2^-11 of the sum of weight x |v|), its
-subnormals after a scaling by 2^14 (2^-39 of the largest weight a key); scores
+subnormals after a scaling by 2^10 or more (2^-35 of the largest weight a key); scores
 summed in fp32 over at most D/16 + 16 accumulations whose terms are at most
 15 steps of a group by |q|, under 4 times the largest sum of |q| |k| (a value's
 group reaches at least 7 steps on one side): each score is off by dS <= 4 size
@@ -46,7 +46,7 @@ def _check(got, ref, keys, D, msg="", apart=0.0):
     ds = 4 * size[..., None] * (D / 16 + 16) * 2.0 ** -23
     vmax = np.nanmax(weight, initial=0.0)
     with np.errstate(invalid="ignore"):
-        bound = (np.abs(out) * 2.0 ** -11 + 2.0 ** -25 + keys * 2.0 ** -39 * vmax +
+        bound = (np.abs(out) * 2.0 ** -11 + 2.0 ** -25 + keys * 2.0 ** -35 * vmax +
                  (keys / 16 + 16) * 2.0 ** -22 * 2.1 * apart +
                  weight * (2.0 ** -11 + np.expm1(2 * ds) + 2.0 ** -20 + (keys / 16 + 16) * 2.0 ** -22))
         bad = np.abs(got - out) > bound
