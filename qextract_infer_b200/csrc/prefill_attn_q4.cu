@@ -75,11 +75,12 @@ struct Params {
   const unsigned char* vc;
   const uint16_t* vp;
   __half* out;
-  float* part_o;    // [nsplit][B][n][Hq][D]
-  float2* part_ml;  // [nsplit][B][n][Hq]
+  float4* part_o;   // [nsplit][B][Hkv][strip][D / 4][32 rows]
+  float2* part_ml;  // [nsplit][B][Hkv][strip][32 rows]
   const int64_t* counts;
   int64_t count, cap;
   int batch, n, hq, hkv, G, sink, window, nsplit;
+  int strips;  // of 32 rows (a softmax warp's): 8 a row block
   float scale_log2;
 };
 
@@ -273,9 +274,9 @@ __device__ float ring_value(const Params& p, int which, int64_t row, int d) {
 
 // A row whose result is not finite, done again by one warp over its visible keys
 // alone: in a tile product a hidden key's weight 0 times an infinite or NaN value
-// is NaN.  Two passes (maximum; weights and sums), plain fp32.
+// is NaN.  Two passes (maximum; weights and sums), plain fp32; writes values [from, to).
 template <int D, int NG>
-__device__ __noinline__ void redo_row(const Params& p, const Ring& ring, int b, int h, int row, int lane) {
+__device__ __noinline__ void redo_row(const Params& p, const Ring& ring, int b, int h, int row, int lane, int from, int to) {
   constexpr int E = D / 32;
   const int kvh = h / p.G;
   const int64_t base = (int64_t(b) * p.hkv + kvh) * p.cap;
@@ -307,7 +308,8 @@ __device__ __noinline__ void redo_row(const Params& p, const Ring& ring, int b, 
     }
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) p.out[at + 32 * e] = __float2half_rn(acc[e] / l);
+  for (int e = 0; e < E; ++e)
+    if (lane + 32 * e >= from && lane + 32 * e < to) p.out[at + 32 * e] = __float2half_rn(acc[e] / l);
 }
 
 // The key tiles that some row of [rmin, rmax] (chunk positions) may see, as
@@ -645,19 +647,19 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
         uint32_t redo = __ballot_sync(0xffffffffu, !fine && fabsf(l) < INFINITY && row < rows);
         for (; redo; redo &= redo - 1) {
           const int r = row0 + x * ROWS + quad * 32 + __ffs(redo) - 1;
-          redo_row<D, NG>(p, ring, b, kvh * p.G + r % p.G, r / p.G, lane);
+          redo_row<D, NG>(p, ring, b, kvh * p.G + r % p.G, r / p.G, lane, 0, D);
         }
       } else {
-        const int64_t part = int64_t(split) * p.batch * p.n * p.hq + orow;
-        if (row < rows) p.part_ml[part] = make_float2(m_used, l);
+        // a lane a row, so that a warp writes 512 bytes in a row (a row a thread, as in the result, took 2.5 us)
+        const int64_t strip = ((int64_t(split) * p.batch + b) * p.hkv + kvh) * p.strips + block * 8 + x * 4 + quad;
+        p.part_ml[strip * 32 + lane] = make_float2(m_used, l);
         if (T > 0) {
 #pragma unroll 1
           for (int j = 0; j < D; j += 32) {
             tmem_ld32(to + j, v);
-            if (row < rows)
 #pragma unroll
-              for (int e = 0; e < 32; e += 4)
-                *reinterpret_cast<float4*>(p.part_o + part * D + j + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            for (int e = 0; e < 32; e += 4)
+              p.part_o[(strip * (D / 4) + (j + e) / 4) * 32 + lane] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
           }
         }
       }
@@ -771,40 +773,68 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
   }
 }
 
-// joins the splits of a row: one warp a row
+// Joins the splits of a strip of 32 rows, 32 of its values a block: a lane a row, a
+// warp four values.
 template <int D, int NG>
-__global__ void __launch_bounds__(128) prefill_attn_q4_merge_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(256) prefill_attn_q4_merge_kernel(const __grid_constant__ Params p) {
   pdl_trigger();
   pdl_wait();
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t total = int64_t(p.batch) * p.n * p.hq;
-  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= total) return;
-  float2 ml = make_float2(-INFINITY, 0.f);
-  if (lane < p.nsplit) ml = p.part_ml[lane * total + row];
-  const float m = warp_max(ml.x);
-  const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-  const float inv = 1.f / warp_sum(w * ml.y);
-  float acc[E];
+  __shared__ unsigned s_redo;
+  const int part = blockIdx.x % (D / 32), strip32 = blockIdx.x / (D / 32);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c4 = part * 8 + warp, kvh = blockIdx.y, b = blockIdx.z;
+  const int64_t of_split = int64_t(p.batch) * p.hkv * p.strips;
+  const int64_t strip = (int64_t(b) * p.hkv + kvh) * p.strips + strip32;
+  if (threadIdx.x == 0) s_redo = 0;
+  __syncthreads();
+  const int row = strip32 * 32 + lane;
+  if (row < p.n * p.G) {
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int AHEAD = 8;  // splits whose loads are in flight together
+    for (int s0 = 0; s0 < p.nsplit; s0 += AHEAD) {
+      float2 ml[AHEAD];
+      float4 v[AHEAD];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int s = 0; s < p.nsplit; ++s) {
-    const float ws = __shfl_sync(0xffffffffu, w, s);
-    if (__shfl_sync(0xffffffffu, ml.x, s) == -INFINITY) continue;  // no key there: its O was not written, or is void
+      for (int i = 0; i < AHEAD; ++i) {
+        const int64_t at = strip + min(s0 + i, p.nsplit - 1) * of_split;
+        ml[i] = p.part_ml[at * 32 + lane];
+        v[i] = p.part_o[(at * (D / 4) + c4) * 32 + lane];
+        if (s0 + i >= p.nsplit) ml[i].x = -INFINITY;
+      }
+      float top = m;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(ws, p.part_o[(s * total + row) * D + 32 * e + lane], acc[e]);
+      for (int i = 0; i < AHEAD; ++i) top = fmaxf(top, ml[i].x);
+      const float w0 = m == -INFINITY ? 0.f : ex2(m - top);
+      m = top;
+      l *= w0;
+      acc.x *= w0, acc.y *= w0, acc.z *= w0, acc.w *= w0;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        if (ml[i].x == -INFINITY) continue;  // no key there: its O was not written, or is void
+        const float w = ex2(ml[i].x - m);
+        l = fmaf(w, ml[i].y, l);
+        acc.x = fmaf(w, v[i].x, acc.x);
+        acc.y = fmaf(w, v[i].y, acc.y);
+        acc.z = fmaf(w, v[i].z, acc.z);
+        acc.w = fmaf(w, v[i].w, acc.w);
+      }
+    }
+    const float inv = 1.f / l;
+    const float a0 = acc.x * inv, a1 = acc.y * inv, a2 = acc.z * inv, a3 = acc.w * inv;
+    const int pos = row / p.G, h = kvh * p.G + row - pos * p.G;
+    *reinterpret_cast<uint2*>(p.out + ((int64_t(b) * p.n + pos) * p.hq + h) * D + 4 * c4) =
+        make_uint2(pack_h2(a0, a1), pack_h2(a2, a3));
+    const bool fine = fabsf(a0) <= 65504.f && fabsf(a1) <= 65504.f && fabsf(a2) <= 65504.f && fabsf(a3) <= 65504.f;
+    if (!fine && fabsf(l) < INFINITY) atomicOr(&s_redo, 1u << lane);  // (a sum that is not finite: the row is NaN already)
   }
-  bool fine = true;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    fine = fine && fabsf(acc[e] * inv) <= 65504.f;
-    p.out[row * D + 32 * e + lane] = __float2half_rn(acc[e] * inv);
-  }
-  if (__any_sync(0xffffffffu, !fine) && fabsf(inv) > 0.f) {  // 1 / l: 0 or NaN where a visible score is not finite
-    const int h = int(row % p.hq), b = int(row / p.hq / p.n), pos = int(row / p.hq % p.n);
-    const Ring ring(kv4::count_of(p.counts, p.count, b), p.sink, p.window);
-    redo_row<D, NG>(p, ring, b, h, pos, lane);
+  __syncthreads();
+  unsigned redo = s_redo;
+  if (redo == 0) return;
+  const Ring ring(kv4::count_of(p.counts, p.count, b), p.sink, p.window);
+  for (int i = 0; redo; redo &= redo - 1, ++i) {
+    if (i % 8 != warp) continue;
+    const int r = strip32 * 32 + __ffs(redo) - 1;
+    redo_row<D, NG>(p, ring, b, kvh * p.G + r % p.G, r / p.G, lane, part * 32, part * 32 + 32);
   }
 }
 
@@ -815,8 +845,10 @@ inline int splits(int batch, int n, int G, int kv_heads, int sink, int window) {
   const int64_t most = (kv4::capacity(sink, window) / KT + (n + KT - 1) / KT) / 2;
   return int(std::max<int64_t>(1, std::min<int64_t>({device_sm_count() / ctas, most, MAX_SPLITS})));
 }
-inline size_t workspace_for(int batch, int n, int q_heads, int head_dim, int nsplit) {
-  return nsplit == 1 ? 0 : size_t(nsplit) * batch * n * q_heads * (size_t(head_dim) * sizeof(float) + sizeof(float2));
+inline int strips_of(int n, int G) { return (n * G + 2 * ROWS - 1) / (2 * ROWS) * 8; }
+inline size_t workspace_for(int batch, int n, int G, int kv_heads, int head_dim, int nsplit) {
+  return nsplit == 1 ? 0
+                     : size_t(nsplit) * batch * kv_heads * strips_of(n, G) * 32 * (size_t(head_dim) * sizeof(float) + sizeof(float2));
 }
 
 template <int D, int NG>
@@ -840,8 +872,8 @@ cudaError_t launch(const Params& p, cudaStream_t st) {
   const cudaError_t e = launch_pdl(prefill_attn_q4_kernel<D, NG>, dim3(unsigned(blocks * p.nsplit), unsigned(p.hkv), unsigned(p.batch)),
                                    dim3(THREADS), Smem<D>::BYTES, st, p);
   if (e != cudaSuccess || p.nsplit == 1) return e;
-  const int64_t rows = int64_t(p.batch) * p.n * p.hq;
-  return launch_pdl(prefill_attn_q4_merge_kernel<D, NG>, dim3(unsigned((rows + 3) / 4)), dim3(128), 0, st, p);
+  return launch_pdl(prefill_attn_q4_merge_kernel<D, NG>, dim3(unsigned((p.n * p.G + 31) / 32 * (D / 32)), unsigned(p.hkv), unsigned(p.batch)),
+                    dim3(256), 0, st, p);
 }
 
 }  // namespace pattn4
@@ -865,7 +897,7 @@ extern "C" size_t qx_prefill_attention_q4_workspace_size(int batch, int n, int q
       q_heads / kv_heads > 16 || (head_dim != 64 && head_dim != 128) || sink < 0 || window < 1 ||
       kv4::capacity(sink, window) >= (int64_t(1) << 30))
     return 0;
-  return pattn4::workspace_for(batch, n, q_heads, head_dim,
+  return pattn4::workspace_for(batch, n, q_heads / kv_heads, kv_heads, head_dim,
                                pattn4::splits(batch, n, q_heads / kv_heads, kv_heads, sink, window));
 }
 
@@ -887,7 +919,7 @@ extern "C" int qx_prefill_attention_q4(const void* q, const void* k_new, const v
                  aligned(v_codes, 16) && aligned(k_params, 16) && aligned(v_params, 16) && aligned(out, 16),
              "prefill_attention_q4: tensors must be 16-byte aligned");
   const int nsplit = pattn4::splits(batch, n, q_heads / kv_heads, kv_heads, sink, window);
-  const size_t need = pattn4::workspace_for(batch, n, q_heads, head_dim, nsplit);
+  const size_t need = pattn4::workspace_for(batch, n, q_heads / kv_heads, kv_heads, head_dim, nsplit);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(QX_ERR_WORKSPACE, "prefill_attention_q4: workspace needs %zu bytes, 16-byte aligned", need);
   pattn4::Params p{};
@@ -899,8 +931,9 @@ extern "C" int qx_prefill_attention_q4(const void* q, const void* k_new, const v
   p.vc = static_cast<const unsigned char*>(v_codes);
   p.vp = static_cast<const uint16_t*>(v_params);
   p.out = static_cast<__half*>(out);
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + int64_t(nsplit) * batch * n * q_heads * head_dim);
+  p.part_o = static_cast<float4*>(workspace);
+  p.strips = pattn4::strips_of(n, q_heads / kv_heads);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + int64_t(nsplit) * batch * kv_heads * p.strips * 32 * (head_dim / 4));
   p.counts = counts;
   p.count = count;
   p.cap = kv4::capacity(sink, window);
