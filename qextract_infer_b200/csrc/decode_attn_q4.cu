@@ -11,22 +11,25 @@
 // through shared memory as fp16, four times their bytes, for a product whose
 // arithmetic is a small part of the time.
 // The codes enter as fp16 subnormals: a mask of a 32-bit word is the pair c 2^-24
-// (or 16 c 2^-24), exact, one instruction a pair; the zero points take part as one
-// more product of the same kind.
-//   S^T = K Q^T   per group, sum q c - z sum q (sum q in two fp16 parts) in one
-//                 accumulator, then times the token's scale in fp32.  The q of the
-//                 codes that come as 16 c are divided by 16.
+// (or 16 c 2^-24), exact, one instruction a pair.
+//   S^T = K Q^T   sum q c per group; then s (sum q c - z sum q) per token in fp32.  The
+//                 q of the codes that come as 16 c are divided by 16.
 //   O^T = V^T P^T the token sits on the K side, so the scale goes to the weight:
-//                 P s in fp16 per group.  P^T comes from S^T's accumulator layout
-//                 by movmatrix.
+//                 P s in fp16 per group, and sum P s z is taken off in fp32.  P^T comes
+//                 from S^T's accumulator layout by movmatrix.
 // The online softmax keeps a running reference and sum per warp and head in fp32.
 // The reference is the largest score, to 2^4, plus the exponent of the largest value
 // scale so far, and P carries 2^10: P s stays below 2^15 and its fp16 subnormals
 // start below 2^-24 of the largest.
 //
-// What bounds it: at 8 sequences and more the instructions (about 250 a warp for
-// 16 tokens of a KV head), not HBM.  Made exact fp16 s (c - z) in registers, with
-// three instructions a pair of V, it took 352.
+// What bounds it: where the work fills the GPU, neither HBM nor one pipe alone (32
+// sequences x 4096 slots: 37.6 us, 3.8 TB/s), but the integer pipe's masks and the
+// mma.sync issue, which together take about 900 of a scheduler's 1000 clocks for a
+// step of 32 tokens.  So the next step's scores are computed next to this step's
+// weights and values (45 -> 44 us for 131072 slots), the zero points' terms run on the
+// FMA pipe (one more product each for them: 40 us), and V is not made exact fp16
+// (three instructions a pair: 46 us).  For one short sequence the two launches and
+// their first loads are the time (8.2 us).
 //
 // Each warp streams its steps of 32 tokens through a ring of its own in shared
 // memory (STAGES deep, cp.async) and reads the fragments from there; the format puts
@@ -69,12 +72,11 @@ template <int D, int NG>
 struct Stage {
   static constexpr int CODES = STEP * D / 2, PARAMS = STEP * NG * 2, BYTES = 2 * (CODES + PARAMS);
 };
-// shared memory: the ring of every warp, or the warps' results
+// shared memory: the ring of every warp, then the warps' results
 template <int D, int NG, int NT>
 struct Smem {
   static constexpr int RING = WARPS * STAGES * Stage<D, NG>::BYTES;
-  static constexpr int JOIN = WARPS * 8 * NT * (D + 1 + 2) * 4;
-  static constexpr int BYTES = RING > JOIN ? RING : JOIN;
+  static constexpr int BYTES = RING + WARPS * 8 * NT * (D + 1 + 2) * 4;
 };
 
 struct Params {
@@ -199,14 +201,26 @@ struct RowParams {
   }
 };
 // the scale of group `grp` from a row's params
+// its zero points, as fp16 (exactly), and one of them
+template <int NG>
+__device__ __forceinline__ void zeros_of(const RowParams<NG>& p, uint32_t (&z)[RowParams<NG>::W]) {
+#pragma unroll
+  for (int i = 0; i < RowParams<NG>::W; ++i) z[i] = hsub2_u32(lop3_and_or(p.w[i], 0x000F000Fu, 0x64006400u), 0x64006400u);
+}
+template <int NG>
+__device__ __forceinline__ float zero_of(const uint32_t (&z)[RowParams<NG>::W], int grp) {
+  const float2 f = h2_to_f2(z[NG == 1 ? 0 : grp >> 1]);
+  return NG > 1 && (grp & 1) ? f.y : f.x;
+}
 template <int NG>
 __device__ __forceinline__ float scale_of(const RowParams<NG>& p, int grp) {
   const uint32_t w = NG == 1 ? p.w[0] : (grp & 1) ? p.w[grp >> 1] >> 16 : p.w[grp >> 1];
   return __half2float(__ushort_as_half(uint16_t(w & 0xFFF0u)));
 }
 
-// what their registers and rings allow
-constexpr int ctas_per_sm(int head_dim, int n_tiles) { return n_tiles > 1 ? 2 : head_dim == 64 ? 4 : 3; }
+// What the registers allow: at D = 128 two CTAs of 240 registers a thread are faster than three of 168 (32 sequences
+// x 4096 slots 37.6 against 40.0 us, one of 131072 42.3 against 46.1).
+constexpr int ctas_per_sm(int head_dim, int n_tiles) { return head_dim == 64 && n_tiles == 1 ? 3 : 2; }
 
 template <int D, int NG, int NT>
 __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_kernel(const __grid_constant__ Params p) {
@@ -216,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
   using St = Stage<D, NG>;
   using Sm = Smem<D, NG, NT>;
   extern __shared__ __align__(128) unsigned char smem[];
-  float (*s_o)[8 * NT][SROW] = reinterpret_cast<float (*)[8 * NT][SROW]>(smem);
+  float (*s_o)[8 * NT][SROW] = reinterpret_cast<float (*)[8 * NT][SROW]>(smem + Sm::RING);
   float (*s_m)[8 * NT] = reinterpret_cast<float (*)[8 * NT]>(s_o + WARPS);
   float (*s_l)[8 * NT] = s_m + WARPS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -262,39 +276,49 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
   const int tg = g ^ ((g >> 1) & 1), odd = c & 1;
   const int at_k = tg * (D / 2) + c * (D / 8), at_p = 2 * St::CODES + tg * NG * 2;
   const int at_v[2] = {St::CODES + (2 * c + odd) * (D / 2) + g * (D / 16), St::CODES + (2 * c + 1 - odd) * (D / 2) + g * (D / 16)};
-  const int at_z = 2 * St::CODES + St::PARAMS + 2 * c * NG * 2;
-  const uint32_t sel_lo = odd ? 0x1054u : 0x5410u, sel_hi = odd ? 0x3276u : 0x7632u;  // a pair of tokens in MMA order
 
-  const uint32_t kz_mask = c == 0 ? 0x000F000Fu : 0u;
-  while (true) {  // a pair (sequence b, KV head kvh), or the part of it that is this CTA's
-  const int kvh = (u - first) / units, off = u - first - kvh * units, len = min(units - off, u_end - u);
-  const int valid = valid_of(p, b), steps = min((valid + STEP - 1) / STEP, (off + len) * WARPS);
-  const int64_t row0 = (int64_t(b) * p.hkv + kvh) * p.cap;
-  int step = off * WARPS + warp;
+  // a pair (sequence b, KV head kvh), or the part of it that is this CTA's: units off .. off + len
+  int kvh, off, len, valid, steps, step;
+  int64_t row0;
+  uint4 q_raw[NT][NI];
+  auto begin = [&] {
+    kvh = (u - first) / units;
+    off = u - first - kvh * units;
+    len = min(units - off, u_end - u);
+    valid = valid_of(p, b);
+    steps = min((valid + STEP - 1) / STEP, (off + len) * WARPS);
+    row0 = (int64_t(b) * p.hkv + kvh) * p.cap;
+    step = off * WARPS + warp;
+    // the queries first: behind the rings' first fill, of every CTA at once, they took 3 us
 #pragma unroll
-  for (int i = 0; i < STAGES; ++i) {
-    if (step + i * WARPS < steps) fetch(i, row0 + int64_t(step + i * WARPS) * STEP);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
-
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        q_raw[nt][i] = nt * 8 + g < p.G
+                           ? __ldg(reinterpret_cast<const uint4*>(
+                                 p.q + ((int64_t(b) * p.hq + int64_t(kvh) * p.G + nt * 8 + g) * D + 32 * i + 8 * c)))
+                           : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) {
+      if (step + i * WARPS < steps) fetch(i, row0 + int64_t(step + i * WARPS) * STEP);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  begin();
+  while (true) {
   // Q^T fragments: head g (of N tile nt), values 32 i + 8 c ..; a head is scaled by
   // the power of two that brings its largest value to [2^4, 2^5), undone in hf: the
   // second pair of each k step is divided by 16, which then costs no bits that count,
   // and the sum over a group stays within fp16.
   uint32_t qb[NT][NI][4];
-  uint32_t qz[NT][NG];  // minus the sum of the scaled q over a group, in two fp16 parts: k = 0, 1 of a product
+  float qz[NT][NG][2];  // minus 2^-24 the sum of the scaled q over a group, of heads 2c, 2c + 1
   float hf[NT][2];      // accumulator -> log2 domain, of heads 2c, 2c + 1
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int h = nt * 8 + g;
-    uint4 v[NI];
     float top = 0.f, sum[NG];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      v[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (h < p.G)
-        v[i] = *reinterpret_cast<const uint4*>(p.q + ((int64_t(b) * p.hq + int64_t(kvh) * p.G + h) * D + 32 * i + 8 * c));
-      const uint32_t d[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      const uint32_t d[4] = {q_raw[nt][i].x, q_raw[nt][i].y, q_raw[nt][i].z, q_raw[nt][i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 f = h2_to_f2(d[e]);
@@ -309,7 +333,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
     for (int n = 0; n < NG; ++n) sum[n] = 0.f;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const uint32_t d[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      const uint32_t d[4] = {q_raw[nt][i].x, q_raw[nt][i].y, q_raw[nt][i].z, q_raw[nt][i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float2 f = h2_to_f2(d[e]);
@@ -323,15 +347,15 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
     for (int n = 0; n < NG; ++n) {
       sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 1);
       sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], 2);
-      const float big = __half2float(__float2half_rn(-sum[n]));
-      qz[nt][n] = c == 0 ? pack_h2(big, -sum[n] - big) : 0u;
+      qz[nt][n][0] = __shfl_sync(0xffffffffu, sum[n], 8 * c) * -0x1p-24f;
+      qz[nt][n][1] = __shfl_sync(0xffffffffu, sum[n], 8 * c + 4) * -0x1p-24f;
     }
     const float k = down * 0x1p24f * p.scale_log2;
     hf[nt][0] = __shfl_sync(0xffffffffu, k, 8 * c);
     hf[nt][1] = __shfl_sync(0xffffffffu, k, 8 * c + 4);
   }
 
-  float o[NI][2][NT][4], oz[NG][NT][4];
+  float o[NI][2][NT][4], oz[NG][NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -339,7 +363,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
 #pragma unroll
       for (int f = 0; f < 2; ++f) o[i][f][nt][0] = o[i][f][nt][1] = o[i][f][nt][2] = o[i][f][nt][3] = 0.f;
 #pragma unroll
-    for (int n = 0; n < NG; ++n) oz[n][nt][0] = oz[n][nt][1] = oz[n][nt][2] = oz[n][nt][3] = 0.f;
+    for (int n = 0; n < NG; ++n) oz[n][nt][0] = oz[n][nt][1] = 0.f;
   }
   // m_r: the score and vexp: the exponent (of its bits, biased) of the value scale that the
   // weights refer to
@@ -347,13 +371,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
   int vexp = 0;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) m_r[nt][0] = m_r[nt][1] = -INFINITY, l_r[nt][0] = l_r[nt][1] = shift[nt][0] = shift[nt][1] = 0.f;
-  for (int st = 0; step < steps; step += WARPS, st = st + 1 == STAGES ? 0 : st + 1) {
-    const int left = valid - step * STEP;  // tokens of this step that exist
-    const unsigned char* at = ring + st * St::BYTES;
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-    __syncwarp();
-    // scores, over hf: rows g, g + 8 (e >> 1) by heads 2c, 2c + 1 (e & 1)
-    float s[2][NT][4];
+  // scores of a stage's step, over hf: rows g, g + 8 (e >> 1) by heads 2c, 2c + 1 (e & 1)
+  auto scores = [&](const unsigned char* at, float (&s)[2][NT][4]) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       uint32_t kc[2][NI];
@@ -363,13 +382,14 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
         load_words<NI>(at + at_k + (u * 16 + 8 * r) * (D / 2), kc[r]);
         kp[r].load(at + at_p + (u * 16 + 8 * r) * NG * 2);
       }
+      uint32_t kz[2][RowParams<NG>::W];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) zeros_of<NG>(kp[r], kz[r]);
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         float acc[NT][4];
-        const uint32_t sel = NG == 1 || !(n & 1) ? 0x1010u : 0x3232u;
-        const uint32_t z0 = prmt(kp[0].w[n >> 1], 0u, sel) & kz_mask, z1 = prmt(kp[1].w[n >> 1], 0u, sel) & kz_mask;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_16816_zc(acc[nt], z0, z1, 0u, 0u, qz[nt][n], 0u);
+        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
 #pragma unroll
         for (int i = n * IPG; i < (n + 1) * IPG; ++i) {
           const uint32_t w0 = kc[0][i], w1 = kc[1][i], h0 = w0 >> 8, h1 = w1 >> 8;
@@ -383,17 +403,29 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float sc = scale_of<NG>(kp[r], n);
+          const float sc = scale_of<NG>(kp[r], n), z = zero_of<NG>(kz[r], n);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int k = 0; k < 2; ++k)
-              s[u][nt][2 * r + k] = n == 0 ? sc * acc[nt][2 * r + k] : fmaf(sc, acc[nt][2 * r + k], s[u][nt][2 * r + k]);
+            {
+              const float a = fmaf(z, qz[nt][n][k], acc[nt][2 * r + k]);
+              s[u][nt][2 * r + k] = n == 0 ? sc * a : fmaf(sc, a, s[u][nt][2 * r + k]);
+            }
         }
       }
     }
+  };
+  float s[2][NT][4];
+  asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+  __syncwarp();
+  scores(ring, s);
+  for (int st = 0, next = 1; step < steps; step += WARPS, st = next, next = next + 1 == STAGES ? 0 : next + 1) {
+    const int left = valid - step * STEP;  // tokens of this step that exist
+    const unsigned char* at = ring + st * St::BYTES;
     // the value scales of tokens g, g + 8, and the exponent of the largest
     float vs[2][2][NG];
+    uint32_t vz[2][2][RowParams<NG>::W];
     uint32_t top = 0;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -405,6 +437,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
         if (left < STEP && u * 16 + tg + 8 * r >= left) vp = RowParams<NG>{};
 #pragma unroll
         for (int n = 0; n < NG; ++n) vs[u][r][n] = scale_of<NG>(vp, n);
+        zeros_of<NG>(vp, vz[u][r]);
 #pragma unroll
         for (int w = 0; w < RowParams<NG>::W; ++w) top = __vmaxu2(top, vp.w[w]);
       }
@@ -456,10 +489,17 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
             o[i][1][nt][e] *= alpha[e & 1];
           }
 #pragma unroll
-          for (int n = 0; n < NG; ++n) oz[n][nt][e] *= alpha[e & 1];
+          for (int n = 0; n < NG; ++n)
+            if (e < 2) oz[n][nt][e] *= alpha[e];
         }
       }
     }
+    // the next step's scores, next to this step's weights and values (past the last step: of whatever the stage
+    // holds, and not used)
+    float s_next[2][NT][4];
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncwarp();
+    scores(ring + next * St::BYTES, s_next);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -474,26 +514,23 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
     // O^T += V^T (P s)^T
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      uint32_t vc[4][NI / 2], vz[2][NG];
+      uint32_t vc[4][NI / 2];
 #pragma unroll
       for (int t = 0; t < 4; ++t) load_words<NI / 2>(at + at_v[t & 1] + (u * 16 + (t >> 1) * 8) * (D / 2), vc[t]);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) load_words<NG>(at + at_z + (u * 16 + t * 8) * NG * 2, vz[t]);
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         uint32_t pb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
-            pb[nt][r] = transpose8x8(pack_h2(s[u][nt][2 * r] * vs[u][r][n], s[u][nt][2 * r + 1] * vs[u][r][n]));
-        // the zero points of this lane's pairs of tokens, as fp16 z 2^-24
-        uint32_t z2[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          z2[t] = prmt(vz[t][n >> 1], NG == 1 ? vz[t][0] >> 16 : vz[t][NG / 2 + (n >> 1)], (n & 1) ? sel_hi : sel_lo) & 0x000F000Fu;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_16816(oz[n][nt], z2[0], z2[0], z2[1], z2[1], pb[nt][0], pb[nt][1]);
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t ps = pack_h2(s[u][nt][2 * r] * vs[u][r][n], s[u][nt][2 * r + 1] * vs[u][r][n]);
+            const float2 f = h2_to_f2(ps);  // the rounded weights, so that c and z meet the same ones
+            const float z = zero_of<NG>(vz[u][r], n);
+            oz[n][nt][0] = fmaf(f.x, z, oz[n][nt][0]);
+            oz[n][nt][1] = fmaf(f.y, z, oz[n][nt][1]);
+            pb[nt][r] = transpose8x8(ps);
+          }
 #pragma unroll
         for (int i = n * IPG; i < (n + 1) * IPG; ++i) {
           const uint32_t sel = (i & 1) ? 0x7632u : 0x5410u;
@@ -511,9 +548,27 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
     __syncwarp();  // every lane has read the stage
     if (step + STAGES * WARPS < steps) fetch(st, row0 + int64_t(step + STAGES * WARPS) * STEP);
     asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u][nt][e] = s_next[u][nt][e];
   }
-  __syncthreads();  // the rings are free
 
+  // the next pair's loads start before this one's results are joined
+  const bool whole = len == units, more = u + len < u_end;
+  const int64_t row = int64_t(b) * p.hq + int64_t(kvh) * p.G;                             // of the result
+  const int64_t piece = (int64_t(blockIdx.x) + int64_t(b) * p.hkv + kvh) * p.G;  // of the partial results
+  u += len;
+  if (more) {
+    if (off + len == units && kvh == p.hkv - 1) {  // the next sequence with tokens
+      first += units * p.hkv;
+      do units = units_of(p, ++b);
+      while (units == 0);
+    }
+    begin();
+  }
   // the warps' results to shared memory, joined per (head, value)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -524,6 +579,12 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
       l += __shfl_xor_sync(0xffffffffu, l, 8);
       l += __shfl_xor_sync(0xffffffffu, l, 16);
       const int h = nt * 8 + 2 * c + k;
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        oz[n][nt][k] += __shfl_xor_sync(0xffffffffu, oz[n][nt][k], 4);
+        oz[n][nt][k] += __shfl_xor_sync(0xffffffffu, oz[n][nt][k], 8);
+        oz[n][nt][k] += __shfl_xor_sync(0xffffffffu, oz[n][nt][k], 16);
+      }
       if (g == 0) s_m[warp][h] = m_r[nt][k] + float(vexp), s_l[warp][h] = l;
 #pragma unroll
       for (int i = 0; i < NI; ++i)
@@ -532,7 +593,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
 #pragma unroll
           for (int r = 0; r < 2; ++r)
             s_o[warp][h][32 * i + 8 * (g >> 1) + 2 * (2 * f + r) + (g & 1)] =
-                fmaf(o[i][f][nt][2 * r + k], r ? 0x1p20f : 0x1p24f, -0x1p24f * oz[i / IPG][nt][k]);
+                fmaf(o[i][f][nt][2 * r + k], r ? 0x1p20f : 0x1p24f, -oz[i / IPG][nt][k]);
     }
   __syncthreads();
   for (int idx = tid; idx < p.G * D; idx += THREADS) {
@@ -548,22 +609,15 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
       acc = fmaf(a, s_o[w][h][d], acc);
       l = fmaf(a, s_l[w][h], l);
     }
-    if (len == units) {
-      p.out[(int64_t(b) * p.hq + int64_t(kvh) * p.G + h) * D + d] = __float2half_rn(acc / l);
+    if (whole) {
+      p.out[(row + h) * D + d] = __float2half_rn(acc / l);
     } else {
-      const int64_t piece = (int64_t(blockIdx.x) + int64_t(b) * p.hkv + kvh) * p.G + h;
-      p.part_o[piece * D + d] = acc;
-      if (d == 0) p.part_ml[piece] = make_float2(m, l);
+      p.part_o[(piece + h) * D + d] = acc;
+      if (d == 0) p.part_ml[piece + h] = make_float2(m, l);
     }
   }
-  u += len;
-  if (u >= u_end) break;
-  if (off + len == units && kvh == p.hkv - 1) {  // the next sequence with tokens
-    first += units * p.hkv;
-    do units = units_of(p, ++b);
-    while (units == 0);
-  }
-  __syncthreads();  // the ring's memory back to the copies
+  if (!more) break;
+  __syncthreads();  // read: the next results may come
   }
 }
 
