@@ -28,24 +28,28 @@
 // step of 32 tokens.  So the next step's scores are computed next to this step's
 // weights and values (45 -> 44 us for 131072 slots), the zero points' terms run on the
 // FMA pipe (one more product each for them: 40 us), and V is not made exact fp16
-// (three instructions a pair: 46 us).  For one short sequence the two launches and
-// their first loads are the time (8.2 us).
+// (three instructions a pair: 46 us).  For one sequence of 4096 slots the launch, the
+// first loads and the join are most of the time (7.0 us).
 //
 // Each warp streams its steps of 32 tokens through a ring of its own in shared
 // memory (STAGES deep, cp.async) and reads the fragments from there; the format puts
 // each lane's share of a row side by side.  (Loaded from global memory straight into
 // the fragments, one step ahead, the bytes in flight hung on the registers: 84 us for
-// one sequence of 131072 slots.  Four bulk copies a step, two of them of 128 bytes,
-// were bound by the number of copies: 47 us for 32 sequences x 4096 slots.)
+// one sequence of 131072 slots.  Four bulk copies a step onto an mbarrier were no
+// faster, 46.8 against 45.5 us for 32 sequences x 4096 slots, and have waits to bound.)
 //
 // The work is cut into units of 128 tokens of one (sequence, KV head), and the CTAs,
 // as many as are resident at once, take equal runs of units in order, whatever pair
-// they belong to: with a grid of (split, KV head, sequence) the last wave of CTAs left
-// SMs idle (41 us for 32 sequences x 4096 slots at the best split).  The warps of a
-// CTA take a unit's four steps and join their results of a pair in the ring's
-// memory; a pair that one CTA did whole is finished there, the others' fp32 results
-// are joined by a second kernel (the results of CTA i for pair j are number i + j:
-// in the order of the runs each next one has a larger i or a larger j).
+// they belong to (a grid of (split, KV head, sequence) at its best split: 41 against
+// 39.9 us for 32 sequences x 4096 slots, 58 against 48 for one of 131072).  The warps of
+// a CTA take a unit's four steps and join their results of a pair in shared memory; a
+// pair that one CTA did whole is finished there, the others' fp32 results are joined
+// by a second kernel (the results of CTA i for pair j are number i + j: in the order
+// of the runs each next one has a larger i or a larger j).
+// Where a cluster of at most 16 CTAs a pair leaves each CTA at most FEW units, the
+// clusters do the pairs instead and join through distributed shared memory: no second
+// kernel, no scratch and no look at the other sequences' counts (one sequence of 4096
+// slots 7.0 against 8.3 us as runs, seven of up to 1005 and 5 heads 5.7 against 8.1).
 //
 // Row g of an MMA is token g ^ (g / 2 & 1) of its eight: neighbouring rows, and the
 // rows that four quads read together, then lie in different halves of the banks.
@@ -66,6 +70,8 @@ constexpr float GROW = 4.f;       // log2 growth of the largest score that the r
 constexpr float PSHIFT = 14.f - GROW;  // what P carries: P s stays below 2^15
 constexpr int UNIT = WARPS * STEP;  // tokens
 constexpr int STAGES = 3;
+constexpr int MAX_CLUSTER = 16;
+constexpr int FEW = 4;            // units of a CTA up to which a pair is a cluster's
 
 // bytes of a stage: codes of K and V, params of K and V
 template <int D, int NG>
@@ -91,7 +97,8 @@ struct Params {
   const int64_t* counts;
   int64_t count, cap;
   int batch, hq, hkv, G, sink, window;
-  int ctas;  // of the first kernel
+  int ctas;     // of the first kernel
+  int cluster;  // CTAs of a pair, where a cluster does it; 0: the CTAs take runs of units
   float scale_log2;
 };
 
@@ -233,29 +240,44 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
   float (*s_o)[8 * NT][SROW] = reinterpret_cast<float (*)[8 * NT][SROW]>(smem + Sm::RING);
   float (*s_m)[8 * NT] = reinterpret_cast<float (*)[8 * NT]>(s_o + WARPS);
   float (*s_l)[8 * NT] = s_m + WARPS;
+  // a cluster's CTA keeps its result for the others where its rings were
+  float* c_o = reinterpret_cast<float*>(smem);
+  float2* c_ml = reinterpret_cast<float2*>(c_o + 8 * NT * D);
+  static_assert(8 * NT * (D + 2) * 4 <= Sm::RING, "the result fits the rings");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, c = lane & 3;
   const unsigned char* ring = smem + warp * STAGES * St::BYTES;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   pdl_wait();
   // this CTA's units [u, u_end), and the sequence and its first unit that u lies in
-  int b, first, total, units = 0;
-  if (p.counts) {
-    place<THREADS>(p, -1, [&](int all) { return first_unit(all, min(int(blockIdx.x), min(p.ctas, all) - 1), min(p.ctas, all)); },
-                   total, b, first);
-  } else {
-    units = units_of(p, 0);
-    total = units * p.hkv * p.batch;
-  }
-  const int n = min(p.ctas, total);  // CTAs with work: none of them has an empty run
-  if (int(blockIdx.x) >= n) return;
-  int u = first_unit(total, blockIdx.x, n);
-  const int u_end = first_unit(total, blockIdx.x + 1, n);
-  if (p.counts) {
+  int b, first, units = 0, u, u_end;
+  if (p.cluster) {
+    const int pair = blockIdx.x / p.cluster, rank = blockIdx.x - pair * p.cluster;
+    b = pair / p.hkv;
+    first = 0;
     units = units_of(p, b);
+    const int at = (pair - b * p.hkv) * units;
+    u = at + units * rank / p.cluster;
+    u_end = at + units * (rank + 1) / p.cluster;
   } else {
-    b = u / (units * p.hkv);
-    first = b * units * p.hkv;
+    int total;
+    if (p.counts) {
+      place<THREADS>(p, -1, [&](int all) { return first_unit(all, min(int(blockIdx.x), min(p.ctas, all) - 1), min(p.ctas, all)); },
+                     total, b, first);
+    } else {
+      units = units_of(p, 0);
+      total = units * p.hkv * p.batch;
+    }
+    const int n = min(p.ctas, total);  // CTAs with work: none of them has an empty run
+    if (int(blockIdx.x) >= n) return;
+    u = first_unit(total, blockIdx.x, n);
+    u_end = first_unit(total, blockIdx.x + 1, n);
+    if (p.counts) {
+      units = units_of(p, b);
+    } else {
+      b = u / (units * p.hkv);
+      first = b * units * p.hkv;
+    }
   }
 
   // a step's rows to stage st, 16 bytes a lane and copy; they all lie in the storage: it has a multiple of 64
@@ -282,14 +304,14 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
   int64_t row0;
   uint4 q_raw[NT][NI];
   auto begin = [&] {
-    kvh = (u - first) / units;
+    kvh = p.cluster ? blockIdx.x / p.cluster - b * p.hkv : (u - first) / units;  // (a cluster's CTA may have no unit)
     off = u - first - kvh * units;
     len = min(units - off, u_end - u);
     valid = valid_of(p, b);
     steps = min((valid + STEP - 1) / STEP, (off + len) * WARPS);
     row0 = (int64_t(b) * p.hkv + kvh) * p.cap;
     step = off * WARPS + warp;
-    // the queries first: behind the rings' first fill, of every CTA at once, they took 3 us
+    // the queries first: the first scores wait for them
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -609,8 +631,11 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
       acc = fmaf(a, s_o[w][h][d], acc);
       l = fmaf(a, s_l[w][h], l);
     }
-    if (whole) {
-      p.out[(row + h) * D + d] = __float2half_rn(acc / l);
+    if (p.cluster > 1) {
+      c_o[idx] = acc;
+      if (d == 0) c_ml[h] = make_float2(m, l);
+    } else if (whole) {
+      p.out[(row + h) * D + d] = __float2half_rn(units > 0 ? acc / l : 0.f);
     } else {
       p.part_o[(piece + h) * D + d] = acc;
       if (d == 0) p.part_ml[piece + h] = make_float2(m, l);
@@ -618,6 +643,39 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
   }
   if (!more) break;
   __syncthreads();  // read: the next results may come
+  }
+  if (p.cluster > 1) {
+    // every CTA of the pair joins its share of the (head, value)s, in rank order
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const int pair = blockIdx.x / p.cluster, rank = blockIdx.x - pair * p.cluster;
+    for (int idx = rank * THREADS + tid; idx < p.G * D; idx += p.cluster * THREADS) {
+      const uint32_t at_o = static_cast<uint32_t>(__cvta_generic_to_shared(c_o + idx));
+      const uint32_t at_m = static_cast<uint32_t>(__cvta_generic_to_shared(c_ml + idx / D));
+      float x[MAX_CLUSTER], m[MAX_CLUSTER], l[MAX_CLUSTER], top = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < MAX_CLUSTER; ++r) {
+        m[r] = -INFINITY, l[r] = x[r] = 0.f;
+        if (r >= p.cluster) continue;
+        uint32_t a, b2;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at_o), "r"(r));
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b2) : "r"(at_m), "r"(r));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[r]) : "r"(a) : "memory");
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m[r]), "=f"(l[r]) : "r"(b2) : "memory");
+      }
+#pragma unroll
+      for (int r = 0; r < MAX_CLUSTER; ++r) top = fmaxf(top, m[r]);
+      const float mb = top == -INFINITY ? 0.f : top;
+      float acc = 0.f, sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < MAX_CLUSTER; ++r) {
+        const float w = ex2(m[r] - mb);
+        acc = fmaf(w, x[r], acc);
+        sum = fmaf(w, l[r], sum);
+      }
+      p.out[(int64_t(b) * p.hq + int64_t(pair - b * p.hkv) * p.G) * D + idx] = __float2half_rn(units > 0 ? acc / sum : 0.f);
+    }
+    // (and none leaves while another reads it)
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
 }
 
@@ -683,7 +741,17 @@ inline int ctas(int batch, int q_heads, int kv_heads, int head_dim, int sink, in
   const int most = device_sm_count() * ctas_per_sm(head_dim, q_heads / kv_heads > 8 ? 2 : 1);
   return int(std::min<int64_t>(most, units_most(batch, kv_heads, sink, window)));
 }
-inline size_t workspace_for(int batch, int q_heads, int kv_heads, int head_dim, int n) {
+// CTAs of a pair where clusters do the pairs, else 0: a power of two, as many as are
+// resident at once for all pairs and have a unit each
+inline int cluster_of(int batch, int q_heads, int kv_heads, int head_dim, int sink, int window) {
+  const int64_t units = (kv4::capacity(sink, window) + UNIT - 1) / UNIT, pairs = int64_t(batch) * kv_heads;
+  const int most = device_sm_count() * ctas_per_sm(head_dim, q_heads / kv_heads > 8 ? 2 : 1);
+  int c = 1;
+  while (c < MAX_CLUSTER && c < units && pairs * (2 * c) <= most) c *= 2;
+  return (units + c - 1) / c <= FEW && pairs * c < (int64_t(1) << 31) ? c : 0;
+}
+inline size_t workspace_for(int batch, int q_heads, int kv_heads, int head_dim, int n, int cluster) {
+  if (cluster) return 0;
   return (size_t(n) + size_t(batch) * kv_heads) * (q_heads / kv_heads) * (size_t(head_dim) * sizeof(float) + sizeof(float2));
 }
 
@@ -701,8 +769,26 @@ cudaError_t launch(const Params& p, cudaStream_t st) {
       const cudaError_t a = cudaFuncSetAttribute(decode_attn_q4_kernel<D, NG, NT>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D, NG, NT>::BYTES);
       if (a != cudaSuccess) return a;
+      const cudaError_t c = cudaFuncSetAttribute(decode_attn_q4_kernel<D, NG, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (c != cudaSuccess) return c;
       done[dev] = true;
     }
+  }
+  if (p.cluster) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(p.batch) * unsigned(p.hkv) * unsigned(p.cluster));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Smem<D, NG, NT>::BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = unsigned(p.cluster);
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = g_pdl_enabled.load(std::memory_order_relaxed) ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, decode_attn_q4_kernel<D, NG, NT>, p);
   }
   const cudaError_t e = launch_pdl(decode_attn_q4_kernel<D, NG, NT>, dim3(unsigned(p.ctas)), dim3(THREADS),
                                    Smem<D, NG, NT>::BYTES, st, p);
@@ -731,7 +817,8 @@ extern "C" size_t qx_decode_attention_q4_workspace_size(int batch, int q_heads, 
       sink < 0 || window < 1 || kv4::capacity(sink, window) >= (int64_t(1) << 30))
     return 0;
   return dattn4::workspace_for(batch, q_heads, kv_heads, head_dim,
-                               dattn4::ctas(batch, q_heads, kv_heads, head_dim, sink, window));
+                               dattn4::ctas(batch, q_heads, kv_heads, head_dim, sink, window),
+                               dattn4::cluster_of(batch, q_heads, kv_heads, head_dim, sink, window));
 }
 
 extern "C" int qx_decode_attention_q4(const void* q, const void* k_codes, const void* k_params, const void* v_codes,
@@ -753,7 +840,8 @@ extern "C" int qx_decode_attention_q4(const void* q, const void* k_codes, const 
   QX_REQUIRE(dattn4::units_most(batch, kv_heads, sink, window) < (int64_t(1) << 31) && int64_t(batch) * q_heads < (int64_t(1) << 31),
              "decode_attention_q4: batch x heads x slots too large");
   const int n = dattn4::ctas(batch, q_heads, kv_heads, head_dim, sink, window);
-  const size_t need = dattn4::workspace_for(batch, q_heads, kv_heads, head_dim, n);
+  const int cluster = dattn4::cluster_of(batch, q_heads, kv_heads, head_dim, sink, window);
+  const size_t need = dattn4::workspace_for(batch, q_heads, kv_heads, head_dim, n, cluster);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(QX_ERR_WORKSPACE, "decode_attention_q4: workspace needs %zu bytes, 16-byte aligned", need);
   dattn4::Params p{};
@@ -775,6 +863,7 @@ extern "C" int qx_decode_attention_q4(const void* q, const void* k_codes, const 
   p.window = window;
   p.batch = batch;
   p.ctas = n;
+  p.cluster = cluster;
   p.scale_log2 = (softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf(float(head_dim))) * 1.4426950408889634f;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;

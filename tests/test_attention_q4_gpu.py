@@ -110,6 +110,27 @@ def test_decode_batch_with_its_own_counts(C, B):
     _decode(C, B, 8, 2, 128, 64, 4, 996, counts, seed=B)
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,D,group,W,counts", [
+    (6, 8, 2, 128, 64, 12000, [0, 13000, 1, 5000, 0, 129]), (4, 6, 3, 64, 32, 12000, 20000),
+    (2, 18, 2, 128, 32, 12000, [12004, 77]), (3, 4, 1, 128, 128, 9000, [0, 0, 0]), (1, 9, 1, 64, 64, 12000, 300),
+    (150, 2, 1, 64, 64, 2000, "mixed"), (300, 1, 1, 64, 32, 700, "mixed")])
+def test_decode_runs(C, B, Hq, Hkv, D, group, W, counts):
+    """Rings wide enough that the CTAs take runs over all pairs (more sequences than a
+    block has threads, too) instead of a cluster a pair."""
+    if counts == "mixed":
+        rng = np.random.default_rng(B)
+        counts = np.where(rng.random(B) < 0.3, 0, rng.integers(0, 2 * W, B))
+    _decode(C, B, Hq, Hkv, D, group, 4, W, np.array(counts) if isinstance(counts, list) else counts, seed=B)
+
+
+@pytest.mark.parametrize("count", [0, 500, 1500])
+def test_decode_runs_that_end_with_pairs(C, count):
+    """As many pairs as CTAs are resident: every pair is one CTA's."""
+    B = 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    _decode(C, B, 1, 1, 128, 64, 0, 1000, count, seed=3)
+    _decode(C, 3, 2, 1, 128, 64, 4, 5, count, seed=4)  # a CTA a pair: a ring of one unit
+
+
 def test_decode_small_rings_scale_and_sizes(C):
     for S, W, count in [(0, 1, 5), (1, 1, 1), (4, 8, 12), (17, 8, 9), (2, 70, 200), (4, 60, 64)]:
         _decode(C, 1, 8, 2, 128, 64, S, W, count, seed=S * 100 + W)
