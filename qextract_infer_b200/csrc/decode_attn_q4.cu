@@ -15,20 +15,24 @@
 //   S^T = K Q^T   sum q c per group; then s (sum q c - z sum q) per token in fp32.  The
 //                 q of the codes that come as 16 c are divided by 16.
 //   O^T = V^T P^T the token sits on the K side, so the scale goes to the weight:
-//                 P s in fp16 per group, and sum P s z is taken off in fp32.  P^T comes
-//                 from S^T's accumulator layout by movmatrix.
+//                 P s in fp16 per group.  The codes come as c - 8 (one more instruction
+//                 a pair, exact), and sum P s (z - 8) is taken off in fp32: with c and z
+//                 the two sums of a long context are far larger than their difference
+//                 (131072 slots: relative error 5.9e-4 instead of 2.8e-4; 37.6 instead
+//                 of 39.5 us for 32 sequences x 4096 slots).  P^T comes from S^T's
+//                 accumulator layout by movmatrix.
 // The online softmax keeps a running reference and sum per warp and head in fp32.
 // The reference is the largest score, to 2^4, plus the exponent of the largest value
 // scale so far, and P carries 2^10: P s stays below 2^15 and its fp16 subnormals
 // start below 2^-24 of the largest.
 //
 // What bounds it: where the work fills the GPU, neither HBM nor one pipe alone (32
-// sequences x 4096 slots: 37.6 us, 3.8 TB/s), but the integer pipe's masks and the
-// mma.sync issue, which together take about 900 of a scheduler's 1000 clocks for a
-// step of 32 tokens.  So the next step's scores are computed next to this step's
-// weights and values (45 -> 44 us for 131072 slots), the zero points' terms run on the
-// FMA pipe (one more product each for them: 40 us), and V is not made exact fp16
-// (three instructions a pair: 46 us).  For one sequence of 4096 slots the launch, the
+// sequences x 4096 slots: 39.5 us, 3.6 TB/s; one of 131072: 43.8 us), but the integer
+// pipe's masks and the mma.sync issue, which together take about 900 of a scheduler's
+// 1000 clocks for a step of 32 tokens.  So the next step's scores are computed next to
+// this step's weights and values (45 -> 44 us for 131072 slots), the zero points' terms
+// run on the FMA pipe (one more product each for them: 40 instead of 37.6 us, both with
+// c unshifted), and V is not made exact fp16 (three instructions a pair: 46 us).  For one sequence of 4096 slots the launch, the
 // first loads and the join are most of the time (7.0 us).
 //
 // Each warp streams its steps of 32 tokens through a ring of its own in shared
@@ -208,12 +212,17 @@ struct RowParams {
   }
 };
 // the scale of group `grp` from a row's params
-// its zero points, as fp16 (exactly), and one of them
-template <int NG>
+// its zero points less OFF, as fp16 (exactly), and one of them
+template <int NG, int OFF>
 __device__ __forceinline__ void zeros_of(const RowParams<NG>& p, uint32_t (&z)[RowParams<NG>::W]) {
 #pragma unroll
-  for (int i = 0; i < RowParams<NG>::W; ++i) z[i] = hsub2_u32(lop3_and_or(p.w[i], 0x000F000Fu, 0x64006400u), 0x64006400u);
+  for (int i = 0; i < RowParams<NG>::W; ++i)
+    z[i] = hsub2_u32(lop3_and_or(p.w[i], 0x000F000Fu, 0x64006400u), 0x64006400u + OFF * 0x10001u);
 }
+// a pair of codes less 8, as fp16 times 2^-24, from the low and from the high four bits of its bytes
+__device__ __forceinline__ uint32_t mid(uint32_t w) { return hsub2_u32(w & 0x000F000Fu, 0x00080008u); }
+__device__ __forceinline__ uint32_t mid16(uint32_t w) { return hsub2_u32(w & 0x00F000F0u, 0x00800080u); }
+
 template <int NG>
 __device__ __forceinline__ float zero_of(const uint32_t (&z)[RowParams<NG>::W], int grp) {
   const float2 f = h2_to_f2(z[NG == 1 ? 0 : grp >> 1]);
@@ -406,7 +415,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
       }
       uint32_t kz[2][RowParams<NG>::W];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) zeros_of<NG>(kp[r], kz[r]);
+      for (int r = 0; r < 2; ++r) zeros_of<NG, 0>(kp[r], kz[r]);
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         float acc[NT][4];
@@ -459,7 +468,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
         if (left < STEP && u * 16 + tg + 8 * r >= left) vp = RowParams<NG>{};
 #pragma unroll
         for (int n = 0; n < NG; ++n) vs[u][r][n] = scale_of<NG>(vp, n);
-        zeros_of<NG>(vp, vz[u][r]);
+        zeros_of<NG, 8>(vp, vz[u][r]);
 #pragma unroll
         for (int w = 0; w < RowParams<NG>::W; ++w) top = __vmaxu2(top, vp.w[w]);
       }
@@ -559,10 +568,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
           const uint32_t a = prmt(vc[0][i / 2], vc[1][i / 2], sel), ah = a >> 8;
           const uint32_t d = prmt(vc[2][i / 2], vc[3][i / 2], sel), dh = d >> 8;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {  // rows g: c 2^-24, rows g + 8: 16 c 2^-24
-            mma_16816(o[i][0][nt], a & 0x000F000Fu, a & 0x00F000F0u, d & 0x000F000Fu, d & 0x00F000F0u, pb[nt][0], pb[nt][1]);
-            mma_16816(o[i][1][nt], ah & 0x000F000Fu, ah & 0x00F000F0u, dh & 0x000F000Fu, dh & 0x00F000F0u, pb[nt][0],
-                      pb[nt][1]);
+          for (int nt = 0; nt < NT; ++nt) {  // rows g: (c - 8) 2^-24, rows g + 8: 16 (c - 8) 2^-24
+            mma_16816(o[i][0][nt], mid(a), mid16(a), mid(d), mid16(d), pb[nt][0], pb[nt][1]);
+            mma_16816(o[i][1][nt], mid(ah), mid16(ah), mid(dh), mid16(dh), pb[nt][0], pb[nt][1]);
           }
         }
       }
