@@ -211,8 +211,7 @@ struct RowParams {
       load_words<W>(p, w);
   }
 };
-// the scale of group `grp` from a row's params
-// its zero points less OFF, as fp16 (exactly), and one of them
+// a row's zero points less OFF, as fp16 (exactly)
 template <int NG, int OFF>
 __device__ __forceinline__ void zeros_of(const RowParams<NG>& p, uint32_t (&z)[RowParams<NG>::W]) {
 #pragma unroll
@@ -223,6 +222,7 @@ __device__ __forceinline__ void zeros_of(const RowParams<NG>& p, uint32_t (&z)[R
 __device__ __forceinline__ uint32_t mid(uint32_t w) { return hsub2_u32(w & 0x000F000Fu, 0x00080008u); }
 __device__ __forceinline__ uint32_t mid16(uint32_t w) { return hsub2_u32(w & 0x00F000F0u, 0x00800080u); }
 
+// one of them, and the scale, of group `grp`
 template <int NG>
 __device__ __forceinline__ float zero_of(const uint32_t (&z)[RowParams<NG>::W], int grp) {
   const float2 f = h2_to_f2(z[NG == 1 ? 0 : grp >> 1]);
@@ -493,7 +493,15 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
         grew = grew || mx[nt][k] > m_r[nt][k] + GROW;
       }
     if (__any_sync(0xffffffffu, grew)) {
-      const int e_new = max(vexp, int(__reduce_max_sync(0xffffffffu, max(top >> 16, top & 0xFFFFu)) >> 10));
+      // (of the finite scales: a NaN's exponent would cost the other groups' weights their bits)
+      float largest = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int n = 0; n < NG; ++n) largest = fmaxf(largest, vs[u][r][n]);
+      const int e_new = max(vexp, int(__reduce_max_sync(0xffffffffu, __float_as_uint(largest)) >> 23) - 112);
       const float e_shift = float(e_new - vexp);
       vexp = e_new;
 #pragma unroll
@@ -805,7 +813,7 @@ cudaError_t launch(const Params& p, cudaStream_t st) {
   const dim3 grid(unsigned(p.batch) * unsigned(p.hq));
   // many pieces a pair (one sequence: 32 and more) are loaded by four groups of threads: 8.3 instead of 9.5 us for
   // one sequence of 4096 slots; a few by one: 512 threads a block and row cost 4 us more at 32 sequences
-  if (p.ctas >= 8 * p.batch * p.hkv)
+  if (p.ctas >= int64_t(8) * p.batch * p.hkv)
     return launch_pdl(decode_attn_q4_merge_kernel<D, 4>, grid, dim3(4 * D), 0, st, p);
   return launch_pdl(decode_attn_q4_merge_kernel<D, 1>, grid, dim3(D), 0, st, p);
 }
@@ -839,7 +847,7 @@ extern "C" int qx_decode_attention_q4(const void* q, const void* k_codes, const 
   QX_REQUIRE(q_heads > 0 && q_heads % kv_heads == 0 && q_heads / kv_heads <= 16,
              "decode_attention_q4: bad heads q=%d kv=%d (a group of 1 to 16)", q_heads, kv_heads);
   QX_REQUIRE(batch <= 65535 && kv_heads <= 65535, "decode_attention_q4: batch or heads too large");
-  QX_REQUIRE(counts || count >= 0, "decode_attention_q4: negative count");
+  QX_REQUIRE(counts || kv4::count_fits(count), "decode_attention_q4: count=%lld", (long long)count);
   if (batch == 0) return QX_OK;
   QX_REQUIRE(q && k_codes && k_params && v_codes && v_params && out, "decode_attention_q4: null pointer");
   QX_REQUIRE(aligned(q, 16) && aligned(k_codes, 16) && aligned(v_codes, 16) && aligned(k_params, 16) &&

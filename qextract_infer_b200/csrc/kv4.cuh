@@ -81,6 +81,9 @@ __device__ __forceinline__ void dequant_word(uint32_t w, const GroupScale& g, ui
   out[3] = hmul2_u32(hsub2_u32(lop3_and_or(h, 0x00F000F0u, 0x54005400u), g.zz4), g.ss);
 }
 
+// what the entry points take as a count of tokens: positions and their sums with a chunk's stay within 64 bits
+inline bool count_fits(int64_t count) { return count >= 0 && count < (int64_t(1) << 62); }
+
 // shared argument checks of the entry points; 0 or an error status
 inline int check_ring(const char* op, int batch, int kv_heads, int head_dim, int group, int sink, int window) {
   if (batch < 0 || kv_heads <= 0)

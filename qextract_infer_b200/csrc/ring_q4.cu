@@ -206,7 +206,7 @@ extern "C" int qx_ring_append_q4(void* k_codes, void* k_params, void* v_codes, v
                                  int sink, int window, int64_t count, const int64_t* counts, qx_stream_t stream) {
   const int rc = kv4::check_ring("ring_append_q4", batch, kv_heads, head_dim, group, sink, window);
   if (rc != QX_OK) return rc;
-  QX_REQUIRE(tokens >= 0 && (counts || count >= 0), "ring_append_q4: tokens=%d count=%lld", tokens, (long long)count);
+  QX_REQUIRE(tokens >= 0 && (counts || kv4::count_fits(count)), "ring_append_q4: tokens=%d count=%lld", tokens, (long long)count);
   if (batch == 0 || tokens == 0) return QX_OK;
   QX_REQUIRE(k_codes && k_params && v_codes && v_params && new_k && new_v, "ring_append_q4: null pointer");
   QX_REQUIRE(aligned(k_codes, 16) && aligned(v_codes, 16) && aligned(k_params, 16) && aligned(v_params, 16) &&
@@ -246,7 +246,7 @@ extern "C" int qx_ring_gather_q4(const void* k_codes, const void* k_params, cons
                                  int window, int64_t count, qx_stream_t stream) {
   const int rc = kv4::check_ring("ring_gather_q4", batch, kv_heads, head_dim, group, sink, window);
   if (rc != QX_OK) return rc;
-  QX_REQUIRE(count >= 0, "ring_gather_q4: negative count");
+  QX_REQUIRE(kv4::count_fits(count), "ring_gather_q4: count=%lld", (long long)count);
   const int valid = kv4::valid_slots(count, sink, window);
   if (batch == 0 || valid == 0) return QX_OK;
   QX_REQUIRE(k_codes && k_params && v_codes && v_params && k_out && v_out, "ring_gather_q4: null pointer");

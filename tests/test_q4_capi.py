@@ -31,7 +31,8 @@ def _prefill(lib, q=P, batch=2, n=3, hq=4, hkv=2, d=128, group=64, sink=4, windo
 
 RING = [(dict(batch=-1), "bad sizes"), (dict(hkv=0), "kv"), (dict(d=96), "head_dim"), (dict(d=256), "head_dim"),
         (dict(group=16), "group"), (dict(d=64, group=128), "group"), (dict(sink=-1), "sink"), (dict(window=0), "window"),
-        (dict(window=(1 << 31) - 8), "too large"), (dict(count=-1), "count")]
+        (dict(window=(1 << 31) - 8), "too large"), (dict(count=-1), "count"),
+        (dict(count=1 << 62), "count")]
 
 
 @pytest.mark.parametrize("call", [_append, _decode, _prefill])
