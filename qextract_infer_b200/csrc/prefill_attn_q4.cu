@@ -35,6 +35,7 @@
 #include <algorithm>
 #include <cmath>
 #include <mutex>
+#include <type_traits>
 
 #include "kv4.cuh"
 #include "qx_b200.h"
@@ -272,46 +273,6 @@ __device__ float ring_value(const Params& p, int which, int64_t row, int d) {
   return __half2float(__ushort_as_half(uint16_t(w & 0xFFF0u))) * float(code - int(w & 15u));
 }
 
-// A row whose result is not finite, done again by one warp over its visible keys
-// alone: in a tile product a hidden key's weight 0 times an infinite or NaN value
-// is NaN.  Two passes (maximum; weights and sums), plain fp32; writes values [from, to).
-template <int D, int NG>
-__device__ __noinline__ void redo_row(const Params& p, const Ring& ring, int b, int h, int row, int lane, int from, int to) {
-  constexpr int E = D / 32;
-  const int kvh = h / p.G;
-  const int64_t base = (int64_t(b) * p.hkv + kvh) * p.cap;
-  const int64_t at = ((int64_t(b) * p.n + row) * p.hq + h) * D + lane;
-  float q[E], acc[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) q[e] = __half2float(p.q[at + 32 * e]) * p.scale_log2, acc[e] = 0.f;
-  for (int pass = 0; pass < 2; ++pass) {
-    for (int t = 0; t <= ring.valid + row; ++t) {
-      const bool old = t < ring.valid;
-      const int j = t - ring.valid;
-      if (old ? !ring.sees(t, row, p.sink, p.window) : !ring.sees_new(j, row, p.window)) continue;
-      const int64_t fresh = ((int64_t(b) * p.n + (old ? 0 : j)) * p.hkv + kvh) * D + lane;
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        s = fmaf(q[e], old ? ring_value<D, NG>(p, 0, base + t, lane + 32 * e) : __half2float(p.kn[fresh + 32 * e]), s);
-      s = warp_sum(s);
-      if (pass == 0) {
-        m = fmaxf(m, s);
-        continue;
-      }
-      const float w = exp2f(s - m);
-      l += w;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        acc[e] = fmaf(w, old ? ring_value<D, NG>(p, 1, base + t, lane + 32 * e) : __half2float(p.vn[fresh + 32 * e]),
-                      acc[e]);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (lane + 32 * e >= from && lane + 32 * e < to) p.out[at + 32 * e] = __float2half_rn(acc[e] / l);
-}
-
 // The key tiles that some row of [rmin, rmax] (chunk positions) may see, as
 // ranges of tile numbers: of the ring's slots the sinks (0), those up to the
 // newest token's (1) and those after it (2: older, where the ring has wrapped),
@@ -374,6 +335,136 @@ __device__ __forceinline__ uint32_t bits(int lo, int hi, int base) {
   return (0xFFFFFFFFu >> (32 - (hi - lo))) << lo;  // hi > lo: lo < 32 and the width is 1 to 32
 }
 
+// the keys k0 + 32 j .. + 31 that the row at `pos` sees, a bit each
+__device__ __forceinline__ uint32_t seen_bits(const Params& p, const Ring& ring, bool of_ring, int k0, int j, int pos) {
+  if (of_ring) {
+    const int sk = p.sink - k0, nw = sk + ring.newest;  // from the tile's first slot: first ring slot, newest
+    const int end = ring.valid - k0;
+    return bits(0, min(sk, end), 32 * j) | bits(max(sk, nw - p.window + 2 + pos), min(nw + 1, end), 32 * j) |
+           bits(max(nw + 1, nw + 2 + pos), end, 32 * j);
+  }
+  return bits(0, min(pos + 1, ring.sinks) - k0, 32 * j) | bits(pos - p.window + 1 - k0, pos + 1 - k0, 32 * j);
+}
+
+// Has a key that the row at `pos` does not see, in its row block's tiles, a value that is
+// not finite, where the row sees no key whose values are all NaN (it is NaN then in
+// any case: the rows of a padded sequence's end)?  By one warp.
+template <int D, int NG>
+__device__ __forceinline__ bool hidden_reached(const Params& p, const Ring& ring, int b, int h, int pos, int lane) {
+  const int kvh = h / p.G, row0 = (pos * p.G + h - kvh * p.G) / (2 * ROWS) * (2 * ROWS);
+  Tiles tiles;
+  tiles.make(ring, row0 / p.G, (min(p.n * p.G, row0 + 2 * ROWS) - 1) / p.G, p.sink, p.window);
+  uint32_t reached = 0, gone = 0;
+#pragma unroll 1
+  for (int k = 0; k < 5; ++k) {
+    const bool of_ring = k < 3;
+    const int end = tiles.end[k] * KT;
+#pragma unroll 1
+    for (int k1 = tiles.start[k] * KT; k1 < end; k1 += 32 * 32) {
+      // of 32 runs of 32 keys, a lane each: those not all seen, and the row's own key's
+      const int mine = k1 + 32 * lane;
+      const bool own = !of_ring && mine <= pos && pos < mine + 32;
+      uint32_t runs = __ballot_sync(0xffffffffu, mine < end && (own || seen_bits(p, ring, of_ring, mine, 0, pos) != 0xFFFFFFFFu));
+#pragma unroll 1
+      for (; runs; runs &= runs - 1) {
+        const int k0 = k1 + 32 * (__ffs(runs) - 1);
+        const uint32_t seen = seen_bits(p, ring, of_ring, k0, 0, pos);
+        const int key = k0 + lane;
+        bool bad = false, nan = false;  // some value, every value
+        if (of_ring && key < ring.valid) {  // a scale that is NaN
+          const uint16_t* w = p.vp + ((int64_t(b) * p.hkv + kvh) * p.cap + key) * NG;
+          nan = true;
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            bad = bad || w[n] >= 0x7C00u;
+            nan = nan && w[n] >= 0x7C00u;
+          }
+        } else if (!of_ring && key < p.n) {
+          const uint4* v = reinterpret_cast<const uint4*>(p.vn + ((int64_t(b) * p.n + key) * p.hkv + kvh) * D);
+          uint32_t top = 0, least = 0x7FFF7FFFu;  // of the magnitudes' bits
+#pragma unroll 4
+          for (int i = 0; i < D / 8; ++i) {
+            const uint4 x = __ldg(v + i);
+            const uint32_t y[4] = {x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu, x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = __vmaxu2(top, y[e]), least = __vminu2(least, y[e]);
+          }
+          bad = max(top >> 16, top & 0xFFFFu) >= 0x7C00u;
+          nan = min(least >> 16, least & 0xFFFFu) > 0x7C00u;
+        }
+        reached |= __ballot_sync(0xffffffffu, bad) & ~seen;
+        gone |= __ballot_sync(0xffffffffu, nan) & seen;
+      }
+    }
+  }
+  return reached && !gone;
+}
+
+// A row whose result is not finite: where a hidden key's NaN or infinity has reached it
+// (in a tile product its weight 0 times that value is NaN), it is done again by one
+// warp over the visible keys alone: two passes (maximum; weights and sums), plain fp32,
+// eight keys at a time; writes values [from, to).  (Every such row done again, whoever's
+// the NaN, took 340 ms for a 2048-token chunk whose second half is NaN; now 0.6.)
+template <int D, int NG>
+__device__ __noinline__ void redo_row(const Params& p, const Ring& ring, int b, int h, int row, int lane, int from, int to) {
+  constexpr int E = D / 32, KEYS = 8;
+  if (!hidden_reached<D, NG>(p, ring, b, h, row, lane)) return;
+  const int kvh = h / p.G;
+  const int64_t base = (int64_t(b) * p.hkv + kvh) * p.cap;
+  const int64_t at = ((int64_t(b) * p.n + row) * p.hq + h) * D + lane;
+  float q[E], acc[E], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) q[e] = __half2float(p.q[at + 32 * e]) * p.scale_log2, acc[e] = 0.f;
+  // the ring's slots, or the chunk's keys up to the row's own
+  auto keys = [&](auto of_ring, bool maximum) {
+    constexpr bool OLD = decltype(of_ring)::value;
+    const int end = OLD ? ring.valid : row + 1;
+    auto value = [&](int which, int t, int e) {
+      if constexpr (OLD)
+        return ring_value<D, NG>(p, which, base + t, lane + 32 * e);
+      else
+        return __half2float((which == 0 ? p.kn : p.vn)[((int64_t(b) * p.n + t) * p.hkv + kvh) * D + lane + 32 * e]);
+    };
+#pragma unroll 1
+    for (int t0 = 0; t0 < end; t0 += KEYS) {
+      float x[KEYS][E], s[KEYS];
+      bool seen[KEYS];
+#pragma unroll
+      for (int u = 0; u < KEYS; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = value(0, min(t0 + u, end - 1), e);
+#pragma unroll
+      for (int u = 0; u < KEYS; ++u) {
+        s[u] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[u] = fmaf(q[e], x[u][e], s[u]);
+        s[u] = warp_sum(s[u]);
+        seen[u] = t0 + u < end && (OLD ? ring.sees(t0 + u, row, p.sink, p.window) : ring.sees_new(t0 + u, row, p.window));
+        if (maximum && seen[u]) m = fmaxf(m, s[u]);
+      }
+      if (maximum) continue;
+#pragma unroll
+      for (int u = 0; u < KEYS; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = value(1, min(t0 + u, end - 1), e);
+#pragma unroll
+      for (int u = 0; u < KEYS; ++u) {
+        const float w = seen[u] ? exp2f(s[u] - m) : 0.f;
+        l += w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, seen[u] ? x[u][e] : 0.f, acc[e]);
+      }
+    }
+  };
+  for (int pass = 0; pass < 2; ++pass) {
+    keys(std::true_type{}, pass == 0);
+    keys(std::false_type{}, pass == 0);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (lane + 32 * e >= from && lane + 32 * e < to) p.out[at + 32 * e] = __float2half_rn(acc[e] / l);
+}
+
 // A loader lane's share of a key tile: a quarter (c) of rows 8 pass + its own, the
 // 8-value blocks 4 i + c, as 16-byte chunks of the swizzled tile.  The rows of
 // a warp's store turn are four apart in pairs, so that eight lanes write eight
@@ -396,7 +487,8 @@ struct RingTile {
     const int c = lane & 3, q = lane >> 2, r8 = (q >> 1) | ((q & 1) << 2);
 #pragma unroll
     for (int s = 0; s < PASSES; ++s) {
-      // a free slot reads the last valid one's row (the tile may end behind the storage)
+      // a free slot reads the last valid one's row (the tile may end behind the storage): with weight 0
+      // a NaN there adds nothing to what that row, in the same tile, brings already
       const int64_t row = base + min(k0 + (s * LOAD_WARPS + warp) * 8 + r8, valid - 1);
       if constexpr (NI == 4) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(codes + row * (D / 2)) + c);
@@ -562,15 +654,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
         if (!full) {  // the keys of the tile that this row sees, a bit each
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            uint32_t seen;
-            if (of_ring) {
-              const int sk = p.sink - k0, nw = sk + ring.newest;  // from the tile's first slot: first ring slot, newest
-              const int end = ring.valid - k0;
-              seen = bits(0, min(sk, end), 32 * j) | bits(max(sk, nw - p.window + 2 + pos), min(nw + 1, end), 32 * j) |
-                     bits(max(nw + 1, nw + 2 + pos), end, 32 * j);
-            } else {
-              seen = bits(0, min(pos + 1, ring.sinks) - k0, 32 * j) | bits(pos - p.window + 1 - k0, pos + 1 - k0, 32 * j);
-            }
+            const uint32_t seen = seen_bits(p, ring, of_ring, k0, j, pos);
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[32 * j + e] = (seen >> e) & 1u ? v[32 * j + e] : -INFINITY;
           }
@@ -911,7 +995,7 @@ extern "C" int qx_prefill_attention_q4(const void* q, const void* k_new, const v
   QX_REQUIRE(n >= 0 && q_heads > 0 && q_heads % kv_heads == 0 && q_heads / kv_heads <= 16,
              "prefill_attention_q4: bad sizes n=%d heads q=%d kv=%d (a group of 1 to 16)", n, q_heads, kv_heads);
   QX_REQUIRE(batch <= 65535 && kv_heads <= 65535 && n < (1 << 26), "prefill_attention_q4: batch, heads or chunk too large");
-  QX_REQUIRE(counts || count >= 0, "prefill_attention_q4: negative count");
+  QX_REQUIRE(counts || kv4::count_fits(count), "prefill_attention_q4: count=%lld", (long long)count);
   if (batch == 0 || n == 0) return QX_OK;
   QX_REQUIRE(q && k_new && v_new && k_codes && k_params && v_codes && v_params && out,
              "prefill_attention_q4: null pointer");

@@ -175,6 +175,23 @@ def test_decode_non_finite_values(C):
     assert np.array_equal(np.isnan(out), nan)
 
 
+@pytest.mark.parametrize("D,group,bad", [(128, 32, 40), (128, 64, 3), (64, 32, 63)])
+def test_decode_a_group_that_reads_as_nan_leaves_the_others_exact(C, D, group, bad):
+    """Small values next to a group whose scale is NaN keep their weights' bits."""
+    rng = np.random.default_rng(D + group)
+    n, S, W = 5, 4, 60
+    k = rng.standard_normal((1, n, 1, D)).astype(np.float16)
+    v = (rng.standard_normal((1, n, 1, D)) * 2.0 ** -9).astype(np.float16)
+    v[0, 2, 0, bad] = np.nan
+    codes, params = C.ring_q4_storage(1, 1, D, S, W, group)
+    C.ring_append_q4(dev_tensor(k), dev_tensor(v), codes, params, 0, S, W)
+    q = rng.standard_normal((1, 4, D)).astype(np.float16)
+    out = to_np(C.decode_attention_q4(dev_tensor(q), codes, params, n, S, W))
+    v64 = kv4_values(v, group)[0]
+    ref = attention64(q, kv4_values(k, group)[0], v64, np.ones((1, n), bool))
+    _check(out, ref, n, D, apart=np.nanmax(np.abs(v64)))
+
+
 def test_decode_cache_object_streams_and_graph(C):
     """One captured step follows its count tensor and its cache; on another stream the same bits."""
     rng = np.random.default_rng(11)
@@ -275,6 +292,59 @@ def test_prefill_evicted_values_do_not_reach_a_row(C):
     out = to_np(C.prefill_attention_q4(q, kn, vn, codes, params, W, S, W))[0]
     # position 20 is visible to row r (position 64 + r) iff 20 > 64 + r - 64
     assert np.isnan(out[:20, :, :64]).all() and np.isfinite(out[20:]).all() and np.isfinite(out[:, :, 64:]).all()
+
+
+@pytest.mark.parametrize("n,W,count", [(700, 4092, 5000), (700, 4092, 100), (90, 4092, 4000)])
+def test_prefill_a_visible_value_that_is_not_finite_costs_no_repair(C, n, W, count):
+    """A NaN value that every row sees makes its column (its group, in the ring) NaN
+    and nothing else, and no row is done again for it: within 20 times the time of
+    the call without it (a repair of every row took hundreds)."""
+    S, H, D = 4, 2, 128
+    rng = np.random.default_rng(n)
+    g = torch.Generator(device="cuda").manual_seed(n)
+
+    def halves(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").half()
+
+    q, k, v = halves(1, n, 8, D), halves(1, n, H, D), halves(1, n, H, D)
+    ring = [C.ring_q4_storage(1, H, D, S, W, 64) for _ in range(2)]
+    ko, vo = halves(1, count, H, D), halves(1, count, H, D)
+    C.ring_append_q4(ko, vo, *ring[0], 0, S, W)
+    vo[0, 1] = float("nan")  # a sink
+    C.ring_append_q4(ko, vo, *ring[1], 0, S, W)
+    times = []
+    for codes, params in ring:
+        for i in range(2):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            out = C.prefill_attention_q4(q, k, v, codes, params, count, S, W)
+            b.record()
+            b.synchronize()
+        times.append(a.elapsed_time(b))
+    assert out.isnan().all()
+    assert times[1] < 20 * times[0] + 0.2, times
+    v[0, 0, 1, 5] = float("inf")  # the chunk's first key: hidden from no row
+    out = C.prefill_attention_q4(q, k, v, *ring[0], count, S, W)
+    fine = out.isfinite()
+    assert not fine[:, :, 4:, 5].any() and fine[:, :, :4].all() and fine[..., :5].all() and fine[..., 6:].all()
+
+
+def test_prefill_free_slots_behind_a_nan(C):
+    """The token in the ring's last slot is NaN and evicted for the later rows; the tile goes on behind it."""
+    S, W, n, D = 0, 70, 100, 64
+    rng = np.random.default_rng(6)
+    count = 70
+    k, v = (rng.standard_normal((1, count, 1, D)).astype(np.float16) for _ in range(2))
+    v[0, 69] = np.nan
+    codes, params = C.ring_q4_storage(1, 1, D, S, W, 32)
+    C.ring_append_q4(dev_tensor(k), dev_tensor(v), codes, params, 0, S, W)
+    # two more tokens put position 70 into slot 0: the ring then starts at slot 2
+    x = dev_tensor(rng.standard_normal((1, 2, 1, D)).astype(np.float16))
+    C.ring_append_q4(x, x, codes, params, count, S, W)
+    q, kn, vn = (dev_tensor(rng.standard_normal((1, n, h, D)).astype(np.float16)) for h in (2, 1, 1))
+    out = to_np(C.prefill_attention_q4(q, kn, vn, codes, params, count + 2, S, W))[0]
+    # position 69 is visible to row r (position 72 + r) iff 69 > 72 + r - 70
+    assert np.isnan(out[:67]).all() and np.isfinite(out[67:]).all()
 
 
 def test_prefill_equals_fp16_prefill_of_the_read_back(C):
