@@ -14,6 +14,9 @@ Differences from the reference, all widening what it accepts:
 * ``RingBufferKVCache.append`` also takes ``[T, H, D]`` and ``[B, T, H, D]``
   chunks, and the cache adds ``decode_attention``.
 
+Added beside them: the same ring held in 4 bits (``RingBufferKVCacheQ4`` and the
+``*_q4`` ops) and ``qk_norm_rope``.
+
 Every op runs on the current torch CUDA stream and raises if the native
 library is missing or the inputs are not CUDA tensors: there is no CPU path.
 """

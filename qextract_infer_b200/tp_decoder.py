@@ -30,7 +30,14 @@ one-shot exchange over NVLink peer memory inside that kernel
 (``nvlink_allreduce.py``); prefill chunks all-reduce with NCCL.  Prefill chunks
 run the same projections with the tensor-core GEMM; their attention (each
 query over the sinks, the previous window and the causal part of its chunk)
-is ``prefill_attention``, which reads the ring in place.
+is ``prefill_attention``, which reads the ring in place, behind
+``qk_norm_rope`` (head norms and rotation in one pass).
+
+With ``kv_bits=4`` the ring holds 4-bit values: a prompt chunk runs
+``prefill_attention_q4`` and the quantising append, a decode step
+``qk_norm_rope``, ``ring_append_q4`` and ``decode_attention_q4`` in place of the
+fused attention (7 launches a layer on one GPU at up to 8 sequences; one more where
+the attention's pieces are joined by a second kernel).
 
 Weights are synthetic: every full tensor comes from a generator seeded by
 (seed, layer, projection) on the device and each rank keeps its shard, so the
