@@ -18,7 +18,7 @@
 //                 P s in fp16 per group.  The codes come as c - 8 (one more instruction
 //                 a pair, exact), and sum P s (z - 8) is taken off in fp32: with c and z
 //                 the two sums of a long context are far larger than their difference
-//                 (131072 slots: relative error 5.9e-4 instead of 2.8e-4; 37.6 instead
+//                 (131072 slots: relative error 5.9e-4 instead of 2.8e-4; it costs 1.9
 //                 of 39.5 us for 32 sequences x 4096 slots).  P^T comes from S^T's
 //                 accumulator layout by movmatrix.
 // The online softmax keeps a running reference and sum per warp and head in fp32.
@@ -27,7 +27,7 @@
 // start below 2^-24 of the largest.
 //
 // What bounds it: where the work fills the GPU, neither HBM nor one pipe alone (32
-// sequences x 4096 slots: 39.5 us, 3.6 TB/s; one of 131072: 43.8 us), but the integer
+// sequences x 4096 slots: 37.2 us, 3.8 TB/s; one of 131072: 41.5 us), but the integer
 // pipe's masks and the mma.sync issue, which together take about 900 of a scheduler's
 // 1000 clocks for a step of 32 tokens.  So the next step's scores are computed next to
 // this step's weights and values (45 -> 44 us for 131072 slots), the zero points' terms
@@ -695,56 +695,83 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT)) decode_attn_q4_ke
   }
 }
 
-// Joins the pieces of one (sequence, query head), PARTS groups of D threads taking
-// every PARTS-th; zeros where a sequence has no token.
-template <int D, int PARTS>
-__global__ void __launch_bounds__(PARTS * D) decode_attn_q4_merge_kernel(const __grid_constant__ Params p) {
+// Joins the pieces of one (sequence, query head): four values a thread, T / (D / 4)
+// parts that take the pieces in turn; zeros where a sequence has no token.  With the
+// count known on the host, which pieces those are is found before the first kernel
+// ends.  (One value a thread, the pieces looked up after it: 39.3 against 37.2 us for 32
+// sequences x 4096 slots, 43.4 against 41.5 for one of 131072, of which the join is now 1.8.)
+template <int D, int T>
+__global__ void __launch_bounds__(T) decode_attn_q4_merge_kernel(const __grid_constant__ Params p) {
+  constexpr int LANES = D / 4, PARTS = T / LANES;
   pdl_trigger();
-  pdl_wait();
-  __shared__ float s_acc[PARTS][D], s_l[PARTS];
-  __shared__ int s_cta[2];
-  const int b = blockIdx.x / p.hq, h = blockIdx.x - b * p.hq, kvh = h / p.G, d = threadIdx.x % D, part = threadIdx.x / D;
-  const int units = units_of(p, b);
-  __half* out = p.out + (int64_t(b) * p.hq + h) * D + d;
-  if (units == 0) {
-    if (part == 0) *out = __float2half_rn(0.f);
-    return;
-  }
-  int first, total, at = b;
+  __shared__ float4 s_acc[PARTS][LANES];
+  __shared__ float2 s_ml[PARTS];
+  const int b = blockIdx.x / p.hq, h = blockIdx.x - b * p.hq, kvh = h / p.G;
+  const int lane = threadIdx.x % LANES, part = threadIdx.x / LANES;
+  int units, first = 0, total = 0, i0 = 0, i1 = 0;
+  auto pieces = [&] {  // the CTAs of the first and of the last unit
+    const int n = min(p.ctas, total);
+    i0 = cta_of(first + kvh * units, total, n);
+    i1 = cta_of(first + kvh * units + units - 1, total, n);
+  };
   if (p.counts) {
-    place<PARTS * D>(p, b, [](int) { return 0; }, total, at, first);
+    pdl_wait();
+    units = units_of(p, b);
+    if (units > 0) {
+      int at = b;
+      place<T>(p, b, [](int) { return 0; }, total, at, first);
+      pieces();
+    }
   } else {
+    units = units_of(p, b);
     total = units * p.hkv * p.batch;
     first = b * units * p.hkv;
+    if (units > 0) pieces();
+    pdl_wait();
   }
-  first += kvh * units;
-  if (threadIdx.x < 2)  // the CTAs of the first and of the last unit
-    s_cta[threadIdx.x] = cta_of(threadIdx.x == 0 ? first : first + units - 1, total, min(p.ctas, total));
-  __syncthreads();
-  const int i0 = s_cta[0], i1 = s_cta[1];
+  uint2* out = reinterpret_cast<uint2*>(p.out + (int64_t(b) * p.hq + h) * D) + lane;
+  if (units == 0) {
+    if (part == 0) *out = make_uint2(0u, 0u);
+    return;
+  }
   if (i0 == i1) return;  // one CTA's: finished there
   const int64_t base = (int64_t(b) * p.hkv + kvh) * p.G + (h - kvh * p.G);  // piece i at base + i G
-  float m = -INFINITY;
-  for (int i = i0 + int(threadIdx.x) % 32; i <= i1; i += 32) m = fmaxf(m, p.part_ml[base + int64_t(i) * p.G].x);
-  m = warp_max(m);
-  const float mb = m == -INFINITY ? 0.f : m;
-  float acc = 0.f, l = 0.f;
-#pragma unroll 8
-  for (int i = i0 + part; i <= i1; i += PARTS) {
-    const float2 ml = p.part_ml[base + int64_t(i) * p.G];
-    const float a = ex2(ml.x - mb);
-    l = fmaf(a, ml.y, l);
-    acc = fmaf(a, p.part_o[(base + int64_t(i) * p.G) * D + d], acc);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float m = -INFINITY, l = 0.f;
+  auto add = [&](float2 ml, float4 v) {
+    const float top = fmaxf(m, ml.x), mb = top == -INFINITY ? 0.f : top;
+    const float a = ex2(m - mb), c = ex2(ml.x - mb);
+    m = top;
+    l = fmaf(l, a, c * ml.y);
+    acc.x = fmaf(acc.x, a, c * v.x);
+    acc.y = fmaf(acc.y, a, c * v.y);
+    acc.z = fmaf(acc.z, a, c * v.z);
+    acc.w = fmaf(acc.w, a, c * v.w);
+  };
+  constexpr int AHEAD = 4;  // pieces whose loads are in flight together
+  for (int i = i0 + part; i <= i1; i += PARTS * AHEAD) {
+    float2 ml[AHEAD];
+    float4 v[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int64_t at = base + int64_t(min(i + k * PARTS, i1)) * p.G;
+      ml[k] = p.part_ml[at];
+      v[k] = reinterpret_cast<const float4*>(p.part_o + at * D)[lane];
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (i + k * PARTS <= i1) add(ml[k], v[k]);
   }
   if constexpr (PARTS > 1) {
-    s_acc[part][d] = acc;
-    if (d == 0) s_l[part] = l;
+    s_acc[part][lane] = acc;
+    if (lane == 0) s_ml[part] = make_float2(m, l);
     __syncthreads();
     if (part > 0) return;
 #pragma unroll
-    for (int k = 1; k < PARTS; ++k) acc += s_acc[k][d], l += s_l[k];
+    for (int k = 1; k < PARTS; ++k) add(s_ml[k], s_acc[k][lane]);
   }
-  *out = __float2half_rn(acc / l);
+  const float inv = 1.f / l;
+  *out = make_uint2(pack_h2(acc.x * inv, acc.y * inv), pack_h2(acc.z * inv, acc.w * inv));
 }
 
 // CTAs of the first kernel: those resident at once, or one a unit of what the ring
@@ -811,11 +838,11 @@ cudaError_t launch(const Params& p, cudaStream_t st) {
   // where the runs end with pairs, known here without per-sequence counts, every pair is one CTA's
   if (e != cudaSuccess || (!p.counts && p.count > 0 && p.batch * p.hkv % p.ctas == 0)) return e;
   const dim3 grid(unsigned(p.batch) * unsigned(p.hq));
-  // many pieces a pair (one sequence: 32 and more) are loaded by four groups of threads: 8.3 instead of 9.5 us for
-  // one sequence of 4096 slots; a few by one: 512 threads a block and row cost 4 us more at 32 sequences
-  if (p.ctas >= int64_t(8) * p.batch * p.hkv)
-    return launch_pdl(decode_attn_q4_merge_kernel<D, 4>, grid, dim3(4 * D), 0, st, p);
-  return launch_pdl(decode_attn_q4_merge_kernel<D, 1>, grid, dim3(D), 0, st, p);
+  // many pieces a pair (one sequence: 32 and more) are shared out to 16 warps; of a few, one warp does a head; past
+  // 128 sequences four, which look through the counts
+  if (p.ctas >= int64_t(8) * p.batch * p.hkv) return launch_pdl(decode_attn_q4_merge_kernel<D, 512>, grid, dim3(512), 0, st, p);
+  if (p.batch > 128) return launch_pdl(decode_attn_q4_merge_kernel<D, 128>, grid, dim3(128), 0, st, p);
+  return launch_pdl(decode_attn_q4_merge_kernel<D, 32>, grid, dim3(32), 0, st, p);
 }
 template <int D, int NG>
 cudaError_t launch(const Params& p, cudaStream_t st) {
