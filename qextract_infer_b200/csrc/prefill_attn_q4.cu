@@ -859,8 +859,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
 }
 
 // Joins the splits of a strip of 32 rows, 32 of its values a block: a lane a row, a
-// warp four values.
-template <int D, int NG>
+// warp four values, AHEAD splits' loads in flight together.
+template <int D, int NG, int AHEAD>
 __global__ void __launch_bounds__(256) prefill_attn_q4_merge_kernel(const __grid_constant__ Params p) {
   pdl_trigger();
   pdl_wait();
@@ -875,7 +875,6 @@ __global__ void __launch_bounds__(256) prefill_attn_q4_merge_kernel(const __grid
   if (row < p.n * p.G) {
     float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int AHEAD = 8;  // splits whose loads are in flight together
     for (int s0 = 0; s0 < p.nsplit; s0 += AHEAD) {
       float2 ml[AHEAD];
       float4 v[AHEAD];
@@ -958,8 +957,12 @@ cudaError_t launch(const Params& p, cudaStream_t st) {
   const cudaError_t e = launch_pdl(prefill_attn_q4_kernel<D, NG>, dim3(unsigned(blocks * p.nsplit), unsigned(p.hkv), unsigned(p.batch)),
                                    dim3(THREADS), Smem<D>::BYTES, st, p);
   if (e != cudaSuccess || p.nsplit == 1) return e;
-  return launch_pdl(prefill_attn_q4_merge_kernel<D, NG>, dim3(unsigned((p.n * p.G + 31) / 32 * (D / 32)), unsigned(p.hkv), unsigned(p.batch)),
-                    dim3(256), 0, st, p);
+  // all splits' loads at once where that is few enough (past the last one they are loaded again for nothing: 2 splits
+  // 22.3 us for the call with room for 2, 23.7 with 8; 17 splits 17.7 with 18, 18.7 with 8)
+  const dim3 grid(unsigned((p.n * p.G + 31) / 32 * (D / 32)), unsigned(p.hkv), unsigned(p.batch));
+  if (p.nsplit <= 2) return launch_pdl(prefill_attn_q4_merge_kernel<D, NG, 2>, grid, dim3(256), 0, st, p);
+  if (p.nsplit <= 6) return launch_pdl(prefill_attn_q4_merge_kernel<D, NG, 6>, grid, dim3(256), 0, st, p);
+  return launch_pdl(prefill_attn_q4_merge_kernel<D, NG, 18>, grid, dim3(256), 0, st, p);
 }
 
 }  // namespace pattn4
