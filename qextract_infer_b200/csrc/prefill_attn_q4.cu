@@ -23,7 +23,9 @@
 //                   maximum grew by more than 2^4, so P carries 2^11 at the
 //                   maximum last used and at most 2^15; both cancel in O / l.
 // The two row tiles alternate: while one's softmax runs, the other's P V and next
-// Q K^T do.  A softmax thread takes its row of S to registers, and P goes over S:
+// Q K^T do, and P V starts on the first 64 keys while the weights of the other 64 are
+// computed (2048-token chunk after 4096 slots 180 -> 172.6 us, 796 TFLOP/s; on the first
+// 32: 176.8, 96: 173.2).  A softmax thread takes its row of S to registers, and P goes over S:
 // TMEM holds S/P of both row tiles (256 columns) and O of both (2 D), the SM's 512
 // at D = 128.  (Steps of 64 keys with an S, P and O apart overlap more on paper,
 // but their products read Q twice as often: shared memory is then the bound, and
@@ -51,13 +53,14 @@ constexpr int THREADS = (SOFTMAX_WARP0 + SOFTMAX_WARPS) * 32;
 constexpr int GROUPS = KT / 8;  // 8-row groups of a key tile, dealt to the loader warps in turn
 constexpr int PASSES = (GROUPS + LOAD_WARPS - 1) / LOAD_WARPS;
 static_assert(SOFTMAX_WARP0 % 4 == 0, "a softmax warp's TMEM lanes are 32 (warp % 4) ..");
+constexpr int FIRST = 64;        // keys of a tile whose P V starts before the other weights are there
 constexpr float GROW = 4.f;      // log2 growth of a row's maximum that O is rescaled for
 constexpr float PSHIFT = 11.f;   // P carries 2^11: at most 2^15 with GROW, subnormal below 2^-25 of the maximum
 constexpr int MAX_SPLITS = 32;
 
 // barriers (8 bytes each)
 enum { FULL_K, EMPTY_K = FULL_K + STAGES, FULL_V = EMPTY_K + STAGES, EMPTY_V = FULL_V + STAGES,
-       S_FULL = EMPTY_V + STAGES, P_FULL = S_FULL + 2, PV_DONE = P_FULL + 2, O_FULL = PV_DONE + 2, Q_FULL = O_FULL + 2, NBARS };
+       S_FULL = EMPTY_V + STAGES, P_FULL = S_FULL + 2, P_HALF = P_FULL + 2, PV_DONE = P_HALF + 2, O_FULL = PV_DONE + 2, Q_FULL = O_FULL + 2, NBARS };
 
 template <int D>
 struct Smem {
@@ -565,6 +568,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
     for (int x = 0; x < 2; ++x) {
       bar_init(bar(S_FULL + x), 1);
       bar_init(bar(P_FULL + x), 4);
+      bar_init(bar(P_HALF + x), 4);
       bar_init(bar(PV_DONE + x), 1);
       bar_init(bar(O_FULL + x), 1);
     }
@@ -696,6 +700,12 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
             pk[e / 2] = pack_h2(w.x, w.y);
           }
           tmem_st16(ts + j / 2, pk);  // over S, which is in registers
+          if (j == FIRST - 32) {  // the products with these keys start
+            tmem_st_wait();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(bar(P_HALF + x));
+          }
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_st_wait();
@@ -817,14 +827,17 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
       }
       __syncwarp();
     };
-    auto values = [&](int x, int it) {  // O_x += P_x V of tile it: 16 keys are 8 columns of P and 16 rows of V
+    // O_x += P_x V of tile it, keys [from, to): 16 keys are 8 columns of P and 16 rows of V
+    auto values = [&](int x, int it, auto from, auto to) {
       const uint32_t vl = v_lo + it % STAGES * (L::TILE >> 4);
       if (elected()) {
 #pragma unroll
-        for (int k = 0; k < KT / 16; ++k)
+        for (int k = from.value / 16; k < to.value / 16; ++k)
           mma_ts(tm + 2 * KT + x * D, tm + KT * x + 8 * k, vl + k * (2048 >> 4), idesc<D, true>(), (it | k) != 0);
-        mma_commit(bar(it + 1 < n ? PV_DONE + x : O_FULL + x));
-        if (x == nx - 1) mma_commit(bar(EMPTY_V + it % STAGES));
+        if (to.value == KT) {
+          mma_commit(bar(it + 1 < n ? PV_DONE + x : O_FULL + x));
+          if (x == nx - 1) mma_commit(bar(EMPTY_V + it % STAGES));
+        }
       }
       __syncwarp();
     };
@@ -838,9 +851,12 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
       const int st = it % STAGES, nst = (it + 1) % STAGES;
       bar_wait(bar(FULL_V + st), (it / STAGES) & 1, gave_up);
       for (int x = 0; x < nx; ++x) {
+        bar_wait(bar(P_HALF + x), it & 1, gave_up);
+        fence_after();
+        values(x, it, std::integral_constant<int, 0>{}, std::integral_constant<int, FIRST>{});
         bar_wait(bar(P_FULL + x), it & 1, gave_up);
         fence_after();
-        values(x, it);
+        values(x, it, std::integral_constant<int, FIRST>{}, std::integral_constant<int, KT>{});
         if (it + 1 == n) continue;
         if (x == 0) bar_wait(bar(FULL_K + nst), ((it + 1) / STAGES) & 1, gave_up);
         // the next S overwrites P: products with different accumulators need not run in the order of their issue
