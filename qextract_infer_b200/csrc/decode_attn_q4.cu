@@ -32,8 +32,9 @@
 // 1000 clocks for a step of 32 tokens.  So the next step's scores are computed next to
 // this step's weights and values (45 -> 44 us for 131072 slots), the zero points' terms
 // run on the FMA pipe (one more product each for them: 40 instead of 37.6 us, both with
-// c unshifted), and V is not made exact fp16 (three instructions a pair: 46 us).  For one sequence of 4096 slots the launch, the
-// first loads and the join are most of the time (7.0 us).
+// c unshifted), and V is not made exact fp16 (three instructions a pair: 46 us).  For one
+// sequence of 4096 slots the launch, the first loads and the join are most of the time
+// (7.2 us).
 //
 // Each warp streams its steps of 32 tokens through a ring of its own in shared
 // memory (STAGES deep, cp.async) and reads the fragments from there; the format puts
@@ -53,7 +54,7 @@
 // Where a cluster of at most 16 CTAs a pair leaves each CTA at most FEW units, the
 // clusters do the pairs instead and join through distributed shared memory: no second
 // kernel, no scratch and no look at the other sequences' counts (one sequence of 4096
-// slots 7.0 against 8.3 us as runs, seven of up to 1005 and 5 heads 5.7 against 8.1).
+// slots 7.2 against 8.3 us as runs, seven of up to 1005 and 5 heads 5.7 against 8.1).
 //
 // Row g of an MMA is token g ^ (g / 2 & 1) of its eight: neighbouring rows, and the
 // rows that four quads read together, then lie in different halves of the banks.
@@ -234,8 +235,8 @@ __device__ __forceinline__ float scale_of(const RowParams<NG>& p, int grp) {
   return __half2float(__ushort_as_half(uint16_t(w & 0xFFF0u)));
 }
 
-// What the registers allow: at D = 128 two CTAs of 240 registers a thread are faster than three of 168 (32 sequences
-// x 4096 slots 37.6 against 40.0 us, one of 131072 42.3 against 46.1).
+// What the registers allow: at D = 128 two CTAs of up to 255 registers a thread are faster than three of 168 (32
+// sequences x 4096 slots 37.6 against 40.0 us, one of 131072 42.3 against 46.1, measured with codes unshifted).
 constexpr int ctas_per_sm(int head_dim, int n_tiles) { return head_dim == 64 && n_tiles == 1 ? 3 : 2; }
 
 template <int D, int NG, int NT>

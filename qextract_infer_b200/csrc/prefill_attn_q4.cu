@@ -30,6 +30,11 @@
 // at D = 128.  (Steps of 64 keys with an S, P and O apart overlap more on paper,
 // but their products read Q twice as often: shared memory is then the bound, and
 // every barrier wait queues behind it: 197 us for the 2048-token chunk.)
+// What bounds it (2048 tokens after 4096 slots, 799 TFLOP/s, 0.48 of the bf16 rate): the
+// exponentials are half of the time on their pipe, the products 45 % on theirs, and with
+// two row tiles, which is what TMEM holds, the chain S - softmax - P V leaves both idle
+// in turn; and 256 CTAs are 1.73 waves.  (Two threads a row: 251 us; some exponentials as
+// polynomials on the FMA pipe: 204 and more, against 180 then.)
 // Few rows (a short chunk after a long context): CTAs split the key tiles and a
 // second kernel joins their fp32 results.
 // Every wait is bounded (kWaitLimitNs, then QX_DEVERR_MBAR_TIMEOUT; the CTA's

@@ -15,7 +15,10 @@
 // the sum is a butterfly over them and the rotation's partner (i +- D/2) sits
 // D / 16 lanes away.  A CTA stays on one token: its cos / sin rows and the norm
 // weights are read once into registers and serve HPL heads per lane group,
-// whose loads are all in flight before the first is used.
+// whose loads are all in flight before the first is used.  2048 tokens of 32 + 2 x 8
+// heads of 128: 12.7 us, 4.1 TB/s (8.0 at the copy rate), by instruction issue (69 %) and
+// load latency; with six heads a lane group 14.5, with 256 threads 14.9, a root and a
+// division for each head in every lane 13.9.  One token: 1.4 us.
 #include <algorithm>
 
 #include "qx_b200.h"
