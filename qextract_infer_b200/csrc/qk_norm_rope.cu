@@ -16,9 +16,10 @@
 // D / 16 lanes away.  A CTA stays on one token: its cos / sin rows and the norm
 // weights are read once into registers and serve HPL heads per lane group,
 // whose loads are all in flight before the first is used.  2048 tokens of 32 + 2 x 8
-// heads of 128: 12.7 us, 4.1 TB/s (8.0 at the copy rate), by instruction issue (69 %) and
-// load latency; with six heads a lane group 14.5, with 256 threads 14.9, a root and a
-// division for each head in every lane 13.9.  One token: 1.4 us.
+// heads of 128: 12.3 us, 4.3 TB/s (8.0 at the copy rate), by instruction issue and load
+// latency.  The norm's products two an instruction, the sine negated once instead of the
+// partner: 12.7 before; with six heads a lane group 14.5, with 256 threads 14.9, a root
+// and a division for each head in every lane 13.9 (before that).  One token: 1.4 us.
 #include <algorithm>
 
 #include "qx_b200.h"
@@ -42,6 +43,16 @@ struct Params {
   int hq, hkv;
   float eps;
 };
+
+// two fp32 products an instruction, each rounded as the scalar one
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{ .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n"
+      "mov.b64 {%0, %1}, x; }"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 
 template <int D, int HPL>
 __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const Params p) {
@@ -70,7 +81,9 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const Params p) {
     c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
     s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
   }
-  const bool lo = l < LPH / 2;  // first half of the head: its partner enters negated
+  if (l < LPH / 2)  // first half of the head: its partner enters negated
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = -s[j];
   const int vfirst = p.hq + p.hkv, warp_h = h0 - (threadIdx.x % 32) / LPH;
   float ss[HPL];
 #pragma unroll
@@ -106,14 +119,15 @@ __global__ void __launch_bounds__(THREADS) qk_norm_rope_kernel(const Params p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 f = h2_to_f2(xd[j]), g = h2_to_f2(wd[j]);
-      const __half2 y = __floats2half2_rn((f.x * r) * g.x, (f.y * r) * g.y);
+      const float2 n = mul2(mul2(f, make_float2(r, r)), g);
+      const __half2 y = __floats2half2_rn(n.x, n.y);
       yd[j] = *reinterpret_cast<const uint32_t*>(&y);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      uint32_t pd = __shfl_xor_sync(0xffffffffu, yd[j], LPH / 2);
-      pd ^= lo ? 0x80008000u : 0u;
+      const uint32_t pd = __shfl_xor_sync(0xffffffffu, yd[j], LPH / 2);
       const float2 y = h2_to_f2(yd[j]), t = h2_to_f2(pd);
+      // (one at a time: two products and a sum of pairs come out fused, with other roundings)
       const __half2 o =
           __floats2half2_rn(__fadd_rn(__fmul_rn(y.x, c[2 * j]), __fmul_rn(t.x, s[2 * j])),
                             __fadd_rn(__fmul_rn(y.y, c[2 * j + 1]), __fmul_rn(t.y, s[2 * j + 1])));
