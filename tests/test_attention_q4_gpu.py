@@ -347,6 +347,73 @@ def test_prefill_free_slots_behind_a_nan(C):
     assert np.isnan(out[:67]).all() and np.isfinite(out[67:]).all()
 
 
+@pytest.mark.parametrize("counted", [False, True])
+def test_calls_at_once_and_captured(C, counted):
+    """Split prefill and decode in runs, eager on two streams at once, then captured as two graphs that are replayed at
+    once: the same bits as one call alone (each call has its own scratch)."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+
+    def halves(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").half()
+
+    B, Hq, H, D, S, W, n = 2, 8, 2, 128, 4, 9000, 37
+    rings, args = [], []
+    for i in range(2):
+        ring = C.ring_q4_storage(B, H, D, S, W, 64)
+        C.ring_append_q4(halves(B, 9004, H, D), halves(B, 9004, H, D), *ring, 0, S, W)
+        rings.append(ring)
+        args.append((halves(B, n, Hq, D), halves(B, n, H, D), halves(B, n, H, D), halves(B, Hq, D)))
+    counts = [torch.tensor(c, device="cuda") for c in ([8000, 301], [12000, 9004])]
+
+    def both(i):
+        q, k, v, one = args[i]
+        count = counts[i] if counted else (8000, 12000)[i]
+        return (C.prefill_attention_q4(q, k, v, *rings[i], count, S, W), C.decode_attention_q4(one, *rings[i], count, S, W))
+
+    want = [both(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append(both(i))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    graphs, outs = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(both(i))
+    for _ in range(5):
+        for o in outs:
+            for t in o:
+                t.zero_()
+        torch.cuda.synchronize()
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_host_count_and_device_count_give_the_same_bits(C):
+    for seed, (B, Hq, H, D, group, W, count) in enumerate([(1, 8, 2, 128, 64, 20000, 15000), (3, 6, 2, 64, 32, 9000, 30000),
+                                                          (2, 18, 2, 128, 128, 500, 400), (140, 2, 1, 64, 64, 700, 600)]):
+        codes, params, _ = _ring(C, np.random.default_rng(seed), 1, H, D, group, 4, W, [count])
+        codes, params = (t.expand(2, B, *t.shape[2:]).contiguous() for t in (codes, params))
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        q = torch.randn(B, Hq, D, generator=g, device="cuda").half()
+        each = torch.full((B,), count, dtype=torch.int64, device="cuda")
+        assert torch.equal(C.decode_attention_q4(q, codes, params, count, 4, W),
+                           C.decode_attention_q4(q, codes, params, each, 4, W))
+        q, k, v = (torch.randn(B, 21, h, D, generator=g, device="cuda").half() for h in (Hq, H, H))
+        assert torch.equal(C.prefill_attention_q4(q, k, v, codes, params, count, 4, W),
+                           C.prefill_attention_q4(q, k, v, codes, params, each, 4, W))
+
+
 def test_prefill_equals_fp16_prefill_of_the_read_back(C):
     """Where the 4-bit ring's read-back is put into an fp16 ring, both attentions
     see the same numbers: equal up to the two kernels' fp32 order and weight rounding."""
