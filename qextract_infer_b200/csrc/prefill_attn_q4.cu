@@ -904,7 +904,7 @@ __global__ void __launch_bounds__(256) prefill_attn_q4_merge_kernel(const __grid
         const int64_t at = strip + min(s0 + i, p.nsplit - 1) * of_split;
         ml[i] = p.part_ml[at * 32 + lane];
         v[i] = p.part_o[(at * (D / 4) + c4) * 32 + lane];
-        if (s0 + i >= p.nsplit) ml[i].x = -INFINITY;
+        if (s0 + i >= p.nsplit) ml[i] = make_float2(-INFINITY, 0.f);
       }
       float top = m;
 #pragma unroll
@@ -915,7 +915,10 @@ __global__ void __launch_bounds__(256) prefill_attn_q4_merge_kernel(const __grid
       acc.x *= w0, acc.y *= w0, acc.z *= w0, acc.w *= w0;
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        if (ml[i].x == -INFINITY) continue;  // no key there: its O was not written, or is void
+        if (ml[i].x == -INFINITY) {  // no key there (l is 0): its O was not written, or is void
+          l += ml[i].y;              // or only scores that are NaN (l is NaN): so is the row
+          continue;
+        }
         const float w = ex2(ml[i].x - m);
         l = fmaf(w, ml[i].y, l);
         acc.x = fmaf(w, v[i].x, acc.x);
