@@ -744,6 +744,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_attn_q4_kernel(const __gri
         }
         // a sum that is not finite has a visible score that is not: the whole row is NaN, and is so already
         uint32_t redo = __ballot_sync(0xffffffffu, !fine && fabsf(l) < INFINITY && row < rows);
+        __syncwarp();  // the rows' own lanes have stored them: what all lanes store now comes after
         for (; redo; redo &= redo - 1) {
           const int r = row0 + x * ROWS + quad * 32 + __ffs(redo) - 1;
           redo_row<D, NG>(p, ring, b, kvh * p.G + r % p.G, r / p.G, lane, 0, D);

@@ -94,7 +94,7 @@ def _same(got, ref, msg=""):
     assert np.array_equal(got[inf], out[inf]) and not np.isinf(got[~inf]).any(), msg
     fine = np.isfinite(out)
     assert np.isfinite(bound[fine]).all()
-    off = np.abs(got - out)[fine] - bound[fine]
+    off = np.abs(got[fine] - out[fine]) - bound[fine]
     assert (off <= 0).all(), (msg, int((off > 0).sum()), np.argwhere(fine)[off.argmax()], off.max(), bound[fine][off.argmax()])
 
 
@@ -125,3 +125,37 @@ def test_a_key_that_is_nan_makes_every_row_that_sees_it_nan(C, D, group, n, W, c
     k[0, chunk_nan, 1, 5] = np.nan
     out, refs = _run(C, q, k, v, old, [count], S, W, group)
     _same(out[0], refs[0])
+
+
+@pytest.mark.parametrize("D,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("B,n,Hq,Hkv,S,W,counts,split", [
+    (2, 60, 6, 2, 4, 100, [30, 400], False),
+    (1, 100, 2, 1, 0, 70, [72], False),          # the ring starts at slot 2, its tile goes on behind slot 69
+    (10, 130, 8, 8, 3, 400, [0, 2, 3, 4, 100, 402, 403, 404, 700, 1999], False),  # enough row blocks to fill the GPU
+    (2, 150, 4, 2, 4, 100, [30, 400], True),
+    (1, 90, 7, 1, 0, 1000, [2500], True),
+    (1, 33, 8, 2, 4, 4092, [5000], True),
+])
+def test_rows_that_hidden_values_reached_equal_the_formula(C, D, group, B, n, Hq, Hkv, S, W, counts, split):
+    """Values of the chunk's later keys and of the ring's oldest tokens that are not finite share a tile with keys that a
+    row sees: the row is done again over its own keys, where the tiles are split and where they are not."""
+    assert _is_split(C, B, n, Hq, Hkv, D, S, W) == split
+    rng = np.random.default_rng(n + D + group)
+    q, k, v = _normal(rng, B, n, Hq, D), _normal(rng, B, n, Hkv, D), _normal(rng, B, n, Hkv, D)
+    old = _normal(rng, B, max(counts), Hkv, D), _normal(rng, B, max(counts), Hkv, D)
+    old[0][..., ::17] *= np.float16(4)
+    k[:, n // 2, 0, 3] = np.inf
+    v[:, n // 2, :, 7] = np.nan
+    v[:, n - 1, :, 9] = -np.inf
+    for b, count in enumerate(counts):
+        first = count - W  # the oldest position held (the first row sees the one after it)
+        if first >= S:
+            old[1][b, first + 3, :, 5] = np.inf
+            old[1][b, first + n // 3, 0, D - 1] = np.nan
+        last = count - 1 - (count - 1 - (W - 1) - S) % W  # the position in the ring's last slot
+        if max(S, first) <= last < first + n:  # not seen by all rows
+            old[1][b, last, -1] = np.nan
+    out, refs = _run(C, q, k, v, old, counts, S, W, group)
+    for b in range(B):
+        _same(out[b], refs[b], f"b={b} count={counts[b]}")
+        assert np.isfinite(refs[b][0]).mean() > 0.125
