@@ -453,7 +453,8 @@ int qx_qk_norm_rope(const void* qkv, int64_t tokens, int q_heads, int kv_heads, 
  *
  * count / counts: tokens written before this call; counts = NULL: `count` for
  * every sequence, else int64 [batch] in device memory, each sequence's own
- * (read when the kernel runs, so a captured graph follows it); >= 0, below 2^62.
+ * (read when the kernel runs, so a captured graph follows it); >= 0, below 2^62
+ * (`count` outside is refused, an entry of counts taken as the nearer end).
  * Every tensor 16-byte aligned.
  * ---------------------------------------------------------------------- */
 int64_t qx_ring_q4_slots(int sink, int window);

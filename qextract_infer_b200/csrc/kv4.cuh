@@ -46,10 +46,16 @@ __host__ __device__ __forceinline__ int valid_slots(int64_t count, int sink, int
   return sink + int(f < window ? f : window);
 }
 
-// tokens written to sequence b: its own count, or the call's
+// what the entry points take as a count of tokens: positions and their sums with a chunk's stay within 64 bits
+constexpr int64_t MAX_COUNT = (int64_t(1) << 62) - 1;
+inline bool count_fits(int64_t count) { return count >= 0 && count <= MAX_COUNT; }
+
+// tokens written to sequence b: its own count, or the call's.  The host does not see a
+// device count: one outside 0 .. MAX_COUNT is taken as the nearer end, so that no position
+// wraps to a slot before the storage.
 __device__ __forceinline__ int64_t count_of(const int64_t* counts, int64_t count, int b) {
   const int64_t c = counts ? counts[b] : count;
-  return c < 0 ? 0 : c;
+  return c < 0 ? 0 : c < MAX_COUNT ? c : MAX_COUNT;
 }
 
 // one halfword pair: bits n of the low half (even values) and of the high half
@@ -80,9 +86,6 @@ __device__ __forceinline__ void dequant_word(uint32_t w, const GroupScale& g, ui
   out[2] = hmul2_u32(hsub2_u32(lop3_and_or(h, 0x000F000Fu, 0x64006400u), g.zz), g.ss);
   out[3] = hmul2_u32(hsub2_u32(lop3_and_or(h, 0x00F000F0u, 0x54005400u), g.zz4), g.ss);
 }
-
-// what the entry points take as a count of tokens: positions and their sums with a chunk's stay within 64 bits
-inline bool count_fits(int64_t count) { return count >= 0 && count < (int64_t(1) << 62); }
 
 // shared argument checks of the entry points; 0 or an error status
 inline int check_ring(const char* op, int batch, int kv_heads, int head_dim, int group, int sink, int window) {
