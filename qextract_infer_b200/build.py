@@ -61,6 +61,13 @@ def _stale(out, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _read(path):
+    if not os.path.exists(path):
+        return None
+    with open(path) as f:
+        return f.read()
+
+
 def build(force: bool = False, verbose: bool = False, extra_flags=None, trace: bool = False) -> str:
     build_dir, lib = (BUILD_TRACE, LIB_TRACE) if trace else (BUILD, LIB)
     os.makedirs(build_dir, exist_ok=True)
@@ -99,13 +106,17 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None, trace: b
 
 
 def build_binding(force: bool = False, verbose: bool = False) -> str:
-    """``_binding.so``, linked against ``libqx_b200.so`` beside it and torch."""
-    src = os.path.join(CSRC, "binding.cpp")
-    if not (force or _stale(BINDING, [src, os.path.join(INCLUDE, "qx_b200.h")])):
-        return BINDING
+    """``_binding.so``, linked against ``libqx_b200.so`` beside it and torch; rebuilt when
+    torch or Python are others than those it was built with, too."""
     import sysconfig
 
     import torch
+    src = os.path.join(CSRC, "binding.cpp")
+    stamp = os.path.join(BUILD, "binding.stamp")
+    made_for = (f"torch {torch.__version__} cuda {torch.version.cuda} cxx11abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)} "
+                f"python {sysconfig.get_config_var('SOABI')}\n")
+    if not (force or _stale(BINDING, [src, os.path.join(INCLUDE, "qx_b200.h")]) or _read(stamp) != made_for):
+        return BINDING
     from torch.utils import cpp_extension
     tmp = BINDING + f".tmp{os.getpid()}"
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
@@ -123,6 +134,9 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, BINDING)
+    os.makedirs(BUILD, exist_ok=True)
+    with open(stamp, "w") as f:
+        f.write(made_for)
     return BINDING
 
 
