@@ -37,12 +37,25 @@ __all__ = ["fused_rmsnorm", "fused_swiglu", "w4a16_gemv", "w4a16_lora_gemv",
            "decode_attention_q4", "prefill_attention_q4"]
 
 _LIB = _lib.load()  # fail at import time if the native library is absent
+
+
+class _NoBinding:
+    """Stands for a ``_binding.so`` that cannot be loaded: the ops that need it raise, the others run."""
+
+    def __init__(self, why: ImportError):
+        self._why = why
+
+    def __getattr__(self, name):
+        raise ImportError(f"qextract_infer_b200: cannot load the native binding, which {name} needs: {self._why}; run "
+                          "`python -m qextract_infer_b200.build`") from self._why
+
+
 try:
     from . import _binding
+    _binding.set_error(_lib.QXError)
 except ImportError as e:
-    raise ImportError(f"qextract_infer_b200: cannot load the native binding: {e}; run "
-                      "`python -m qextract_infer_b200.build`") from e
-_binding.set_error(_lib.QXError)
+    _binding = _NoBinding(e)
+
 _SUPPORTED_RANKS = (8, 16, 32, 48, 64, 128)
 
 
