@@ -613,7 +613,7 @@ def tp_decode_measure(args, world, rank, dev):
     from qextract_infer_b200 import _C
     from qextract_infer_b200.tp_decoder import DecoderConfig, TPDecoder
 
-    cfg = DecoderConfig()
+    cfg = DecoderConfig(kv_bits=args.kv_bits)
     prompt_len, decode_steps, chunk = args.prompt, args.decode, 2048
     batches = [int(b) for b in args.batches.split(",")]
     hbm = measured_peaks()[0]
@@ -638,13 +638,14 @@ def tp_decode_measure(args, world, rank, dev):
         torch.cuda.synchronize(dev)
         prefill_s = max_over_ranks(time.time() - t0)
         count0 = dec.cache.get_total_written()
-        k0, v0 = dec.cache.k.clone(), dec.cache.v.clone()
+        held = (dec.cache.codes, dec.cache.params) if cfg.kv_bits == 4 else (dec.cache.k, dec.cache.v)
+        held0 = [t.clone() for t in held]
         tok = torch.empty_like(nxt)
         st = torch.cuda.Stream(dev)
 
         def restore():
-            dec.cache.k.copy_(k0)
-            dec.cache.v.copy_(v0)
+            for t, t0 in zip(held, held0):
+                t.copy_(t0)
             dec.cache._write_count = count0
             tok.copy_(nxt)
 
@@ -680,7 +681,7 @@ def tp_decode_measure(args, world, rank, dev):
         # shard, and the ring (all layers, this rank's KV heads, every sequence)
         wbytes = sum(L[k].weight_bytes() for L in dec.layers for k in ("qkv", "o", "gate_up", "down"))
         wbytes += dec.lm_head.numel() * 2
-        kvbytes = 2 * cfg.num_layers * B * (cfg.sink + cfg.window) * dec.hkv * cfg.head_dim * 2
+        kvbytes = sum(t.numel() * t.element_size() for t in held)
         per_rank_gbs = (wbytes + kvbytes) / (step_ms / 1e3) / 1e9
         ar_us = None
         if dec.ar is not None:  # one NVLink all-reduce + add + RMSNorm call, device time
@@ -714,7 +715,7 @@ def tp_decode_measure(args, world, rank, dev):
             "ms_per_step": step_ms, "scaling": "strong",
             "config": {"workload": "Qwen3-8B decoder (36 layers, hidden 4096, 32/8 heads, "
                                    "GPTQ int4 g128 + LoRA r16), TP decode",
-                       "prompt": prompt_len, "decode_tokens": decode_steps, "prefill_chunk": chunk,
+                       "prompt": prompt_len, "decode_tokens": decode_steps, "prefill_chunk": chunk, "kv_bits": cfg.kv_bits,
                        "graphs": "one CUDA graph per decode step"},
             "prefill_s": prefill_s, "prefill_tok_s": B * prompt_len / prefill_s,
             "nvlink_allreduce_us": ar_us,
@@ -722,7 +723,7 @@ def tp_decode_measure(args, world, rank, dev):
                          "frac": per_rank_gbs / hbm, "bytes_per_step_per_rank": wbytes + kvbytes}})
         del graphs, g
         dec.close()
-        del dec, k0, v0
+        del dec, held, held0
         torch.cuda.empty_cache()
     return lines
 
@@ -993,6 +994,7 @@ def main():
     ap.add_argument("--batches", default="1,32", help="decode_tp: batch sizes")
     ap.add_argument("--prompt", type=int, default=8192, help="decode_tp: prompt tokens")
     ap.add_argument("--decode", type=int, default=64, help="decode_tp: greedy decode tokens")
+    ap.add_argument("--kv-bits", type=int, choices=[16, 4], default=16, help="decode_tp: bits of the ring's K and V")
     ap.add_argument("--workload", choices=["decode_gemv", "kernels", "prefill_gemm", "decode_tp",
                                            "profile_cases", "profile_decode_step", "timeline"],
                     default="decode_gemv",
