@@ -416,8 +416,8 @@ def _graph_time_us(torch, stream, fn, nsteps, reps=3):
 
 
 def run_kernel_suite(args):
-    """Secondary kernels at the RMSNorm/SwiGLU and ring-cache configurations:
-    one JSON line per (kernel, shape) with us/call, GB/s and HBM fraction.
+    """Secondary kernels at the RMSNorm/SwiGLU and ring-cache configurations and
+    the cases of perf/operators.py: one JSON line per (kernel, shape) with us/call, GB/s and HBM fraction.
     Inputs rotate over buffers totalling > 2x L2 where one call is smaller."""
     import numpy as np
     import torch
@@ -508,6 +508,18 @@ def run_kernel_suite(args):
                           "us_per_call": us, "TFLOP/s": flops / us / 1e6, "bound": "mma.sync"}),
               flush=True)
         del pq, pk, pv, kc, vc
+    # the head norm with rotation and the 4-bit ring's operators: the cases of perf/operators.py
+    from perf import operators
+    operators.own = True
+    for case in operators.listed():
+        w = operators.work(case)
+        states = [operators.prepare(case, seed) for seed in range(nbuf(w["bytes"]))]
+        torch.cuda.synchronize()
+        us = _graph_time_us(torch, st, lambda i: operators.run(states[i % len(states)]),
+                            40 if case["kind"] == "prefill" else steps)
+        emit(case["name"], {n: v for n, v in case.items() if n != "name"}, w["bytes"], us,
+             {"TFLOP/s": w["flops"] / us / 1e6})
+        del states
     return 0
 
 
