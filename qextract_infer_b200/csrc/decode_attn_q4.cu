@@ -7,9 +7,9 @@
 // Both products run on the tensor cores with the cache as the A operand
 // (mma.sync m16n8k16: 16 tokens or 16 head dimensions by 8 query heads), so a
 // KV head's group of up to 8 query heads fills the N side (two N tiles up to
-// 16).  tcgen05 would need 128 rows of M: the cache rows would have to pass
-// through shared memory as fp16, four times their bytes, for a product whose
-// arithmetic is a small part of the time.
+// 16).  tcgen05 takes 128 rows of M: for V^T P^T those are head dimensions, so the
+// cache's rows would have to be turned over in shared memory as fp16, four times their
+// bytes.  For K Q^T they are tokens, and A could come from TMEM, a token a lane: not built.
 // The codes enter as fp16 subnormals: a mask of a 32-bit word is the pair c 2^-24
 // (or 16 c 2^-24), exact, one instruction a pair.
 //   S^T = K Q^T   sum q c per group; then s (sum q c - z sum q) per token in fp32.  The
@@ -26,15 +26,16 @@
 // scale so far, and P carries 2^10: P s stays below 2^15 and its fp16 subnormals
 // start below 2^-24 of the largest.
 //
-// What bounds it: where the work fills the GPU, neither HBM nor one pipe alone (32
-// sequences x 4096 slots: 37.2 us, 3.8 TB/s; one of 131072: 41.5 us), but the integer
-// pipe's masks and the mma.sync issue, which together take about 900 of a scheduler's
-// 1000 clocks for a step of 32 tokens.  So the next step's scores are computed next to
+// What bounds it: where the work fills the GPU (32 sequences x 4096 slots: 37.0 us, 3.9
+// TB/s; one of 131072: 41.2 us), neither HBM nor a pipe is full: issue 59 %, the integer
+// pipe 50 %, the tensor pipe 24 %, DRAM 45 %.  A scheduler has two warps, each a chain of
+// masks, products and exponentials, and they do not cover each other's latencies (of an
+// issue 0.67 waits for a fixed latency, 0.31 for a pipe).  So the next step's scores are computed next to
 // this step's weights and values (45 -> 44 us for 131072 slots), the zero points' terms
 // run on the FMA pipe (one more product each for them: 40 instead of 37.6 us, both with
 // c unshifted), and V is not made exact fp16 (three instructions a pair: 46 us).  For one
 // sequence of 4096 slots the launch, the first loads and the join are most of the time
-// (7.2 us).
+// (7.5 us).
 //
 // Each warp streams its steps of 32 tokens through a ring of its own in shared
 // memory (STAGES deep, cp.async) and reads the fragments from there; the format puts

@@ -24,16 +24,16 @@
 //                   maximum last used and at most 2^15; both cancel in O / l.
 // The two row tiles alternate: while one's softmax runs, the other's P V and next
 // Q K^T do, and P V starts on the first 64 keys while the weights of the other 64 are
-// computed (2048-token chunk after 4096 slots 180 -> 172.6 us, 796 TFLOP/s; on the first
+// computed (2048-token chunk after 4096 slots 180 -> 172.6 us; on the first
 // 32: 176.8, 96: 173.2).  A softmax thread takes its row of S to registers, and P goes over S:
 // TMEM holds S/P of both row tiles (256 columns) and O of both (2 D), the SM's 512
 // at D = 128.  (Steps of 64 keys with an S, P and O apart overlap more on paper,
 // but their products read Q twice as often: shared memory is then the bound, and
 // every barrier wait queues behind it: 197 us for the 2048-token chunk.)
-// What bounds it (2048 tokens after 4096 slots, 799 TFLOP/s, 0.48 of the bf16 rate): the
-// exponentials are half of the time on their pipe, the products 45 % on theirs, and with
-// two row tiles, which is what TMEM holds, the chain S - softmax - P V leaves both idle
-// in turn; and 256 CTAs are 1.73 waves.  (Two threads a row: 251 us; some exponentials as
+// What bounds it (2048 tokens after 4096 slots: 171 us, 804 TFLOP/s, 0.48 of the bf16 rate;
+// on another GPU 178): the exponentials take 46 % of the time on their pipe, the products
+// 45 % on theirs, issue is 47 %, and with two row tiles, which is what TMEM holds, the chain
+// S - softmax - P V leaves each idle in turn; and 256 CTAs are 1.73 waves.  (Two threads a row: 251 us; some exponentials as
 // polynomials on the FMA pipe: 204 and more, against 180 then.)
 // Few rows (a short chunk after a long context): CTAs split the key tiles and a
 // second kernel joins their fp32 results.
@@ -412,7 +412,10 @@ __device__ __forceinline__ bool hidden_reached(const Params& p, const Ring& ring
 // (in a tile product its weight 0 times that value is NaN), it is done again by one
 // warp over the visible keys alone: two passes (maximum; weights and sums), plain fp32,
 // eight keys at a time; writes values [from, to).  (Every such row done again, whoever's
-// the NaN, took 340 ms for a 2048-token chunk whose second half is NaN; now 0.6.)
+// the NaN, took 340 ms for a 2048-token chunk whose second half is NaN; now 0.6.)  It is
+// slow where there are many: a NaN token that the ring evicts during a 2048-token chunk
+// over 4096 slots makes the call 86 ms instead of 0.18, one in the middle of a 64-token
+// chunk over 131072 slots 474 instead of 0.17.
 template <int D, int NG>
 __device__ __noinline__ void redo_row(const Params& p, const Ring& ring, int b, int h, int row, int lane, int from, int to) {
   constexpr int E = D / 32, KEYS = 8;
@@ -949,7 +952,10 @@ __global__ void __launch_bounds__(256) prefill_attn_q4_merge_kernel(const __grid
 
 // CTAs that split the key tiles of a row block: where the row blocks leave SMs
 // idle, as many as fill them with two tiles each, where there are that many (33 tokens
-// after 4096 slots, 33 tiles: 17 CTAs 19.4 us, 16 CTAs, one of them with three tiles, 20.3)
+// after 4096 slots, 33 tiles: 17 CTAs 19.4 us, 16 CTAs, one of them with three tiles, 20.3).
+// Tiles of what the ring can hold, not of what it holds, so that host and device counts
+// sum in the same order: a wide ring's first 33 tokens take 13.3 us, of which 3.8 are
+// splits without a tile (9.5 in a ring of 128 slots).
 inline int splits(int batch, int n, int G, int kv_heads, int sink, int window) {
   const int64_t ctas = (int64_t(n) * G + 2 * ROWS - 1) / (2 * ROWS) * kv_heads * batch;
   const int64_t tiles = (kv4::capacity(sink, window) + KT - 1) / KT + (n + KT - 1) / KT, most = (tiles + 1) / 2;

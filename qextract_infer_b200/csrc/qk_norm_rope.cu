@@ -16,10 +16,10 @@
 // D / 16 lanes away.  A CTA stays on one token: its cos / sin rows and the norm
 // weights are read once into registers and serve HPL heads per lane group,
 // whose loads are all in flight before the first is used.  2048 tokens of 32 + 2 x 8
-// heads of 128: 12.3 us, 4.3 TB/s (8.0 at the copy rate), by instruction issue and load
-// latency.  The norm's products two an instruction, the sine negated once instead of the
+// heads of 128: 12.3 us, 4.3 TB/s (8.0 at the copy rate; 10.5 in a graph of such calls), by
+// load latency and issue (67 %).  The norm's products two an instruction, the sine negated once instead of the
 // partner: 12.7 before; with six heads a lane group 14.5, with 256 threads 14.9, a root
-// and a division for each head in every lane 13.9 (before that).  One token: 1.4 us.
+// and a division for each head in every lane 13.9 (before that).  One token: 1.3 us.
 #include <algorithm>
 
 #include "qx_b200.h"

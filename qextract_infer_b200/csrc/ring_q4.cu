@@ -24,7 +24,7 @@
 // 16 bytes side by side in the cache (8 at D = 64), a group of 32 is one block of
 // each of the four lanes, and a row's loads are all in flight at once.  (With
 // D / 8 lanes a row, one block each, and 64-bit index divisions: append of 2048
-// tokens x 8 heads and read-back of 4096 slots 29.6 us; now 10.3, two kernels that
+// tokens x 8 heads and read-back of 4096 slots 29.6 us; now 10.7, two kernels that
 // each are one wave.)
 #include <algorithm>
 
