@@ -1,6 +1,6 @@
-"""Prefill attention over the 4-bit ring where keys or values are NaN or infinite,
-against the softmax formula in 64 bits over the keys a row sees: NaN and infinities
-exactly where the formula has them, every other element within a finite bound.
+"""Attention over the 4-bit ring where keys or values are NaN or infinite, against the
+softmax formula in 64 bits over the keys a row sees: NaN and infinities exactly where the
+formula has them, every other element within a finite bound.
 
 Bound of an element, from the roundings, per (row, head) and over the finite values
 alone: the result once to fp16 (2^-11 of it, 2^-25 at fp16's end); every weight
@@ -159,3 +159,31 @@ def test_rows_that_hidden_values_reached_equal_the_formula(C, D, group, B, n, Hq
     for b in range(B):
         _same(out[b], refs[b], f"b={b} count={counts[b]}")
         assert np.isfinite(refs[b][0]).mean() > 0.125
+
+
+@pytest.mark.parametrize("D,group,Hq,Hkv", [(128, 64, 8, 2), (64, 32, 5, 5), (128, 32, 18, 2)])
+@pytest.mark.parametrize("B,W,counts,nan_at", [
+    (1, 4092, [5000], [0, 3, 100, 4095]), (2, 1000, [900, 33], [32, 5]), (3, 12000, [12004, 129, 0], [128, 9000]),
+    (1, 60, [40], [39]),
+])
+def test_decode_a_key_that_is_nan_makes_its_heads_nan(C, D, group, Hq, Hkv, B, W, counts, nan_at):
+    """Alone in a step, a warp, a CTA or a piece; the other KV heads and sequences stay as the formula has them."""
+    rng = np.random.default_rng(W + D)
+    S = 4
+    q = _normal(rng, B, Hq, D)
+    k, v = _normal(rng, B, S + W, Hkv, D), _normal(rng, B, S + W, Hkv, D)
+    k[0, nan_at, -1, 5] = np.nan
+    codes, params = C.ring_q4_storage(B, Hkv, D, S, W, group)
+    C.ring_append_q4(dev_tensor(k), dev_tensor(v), codes, params, 0, S, W)
+    arg = counts[0] if B == 1 else dev_tensor(np.asarray(counts, np.int64))
+    out = to_np(C.decode_attention_q4(dev_tensor(q), codes, params, arg, S, W)).astype(np.float64)
+    for b, count in enumerate(counts):
+        held = min(count, S + W)
+        if held == 0:
+            assert (out[b] == 0).all()
+            continue
+        kk, vv = kv4_values(k[b, :held], group), kv4_values(v[b, :held], group)
+        ref, bound = _formula(q[b:b + 1], kk, vv, np.ones((1, held), bool))
+        # codes and zero points are summed apart: each of the steps over the keys is off by 2^-22 x 2.1 max |v| more
+        _same(out[b:b + 1], (ref, bound + (held / 16 + 16) * 2.0 ** -22 * 2.1 * np.abs(vv).max()), f"b={b}")
+        assert np.isnan(ref[0, Hq - Hq // Hkv:]).all() == (b == 0)
