@@ -498,6 +498,55 @@ int qx_prefill_attention_q4(const void* q, const void* k_new, const void* v_new,
                             int window, int64_t count, const int64_t* counts, float softmax_scale,
                             void* workspace, size_t workspace_bytes, qx_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * What each request of a served batch brings of its own: its low-rank adapter
+ * and its sampling settings.  New components (the reference merges one adapter
+ * into a linear's call and leaves sampling to HF).
+ *
+ * qx_multi_lora_add: adapters of many requests beside a shared projection.
+ *   out[b][t] = fp16( y[b][t] + scales[a] (x[b][t] A[a]) B[a] ),  a = adapters[b]
+ *   y, out fp16 [batch, tokens, N]; x fp16 [batch, tokens, K];
+ *   lora_A fp16 [num_adapters, K, P rank]; lora_B fp16 [num_adapters, rank, N];
+ *   adapters int64 [batch], scales fp32 [num_adapters], both on the device and
+ *   read when the kernel runs.  A sequence whose adapter is outside
+ *   0 .. num_adapters - 1 has none: its rows of out equal y.
+ *   splits: host array of num_splits <= 4 widths that sum to N (multiples of
+ *   8), the column blocks of a fused projection; block j uses the ranks
+ *   j rank .. j rank + rank - 1 of lora_A.  num_splits = 0: one block (P = 1).
+ *   Sums in fp32, one rounding.  out may be y (in place); it must not overlap
+ *   anything else.  lora_A, lora_B, scales and adapters must not be written by a kernel
+ *   of this library issued just before on the stream (qx_set_pdl).
+ *   K % 8 == 0, N % 8 == 0, rank % 8 == 0, P rank <= 256; 16-byte aligned.
+ * qx_lm_head_logits: logits fp16 [batch, vocab] = h [batch, hidden] W, W fp16
+ *   [hidden, vocab], fp32 sums; the values whose maximum qx_lm_head_argmax takes.  Any
+ *   batch (32 rows a launch); hidden % 64 == 0, vocab % 8 == 0.
+ * qx_sample_logits: one token for each row of logits fp16 [batch, vocab] from
+ *   u fp32 [batch] in [0, 1).  Tokens stand by their logit, the largest first,
+ *   equal ones by index; w = exp((l - max l) / temperature).  Kept are the
+ *   first top_k (<= 0: all), of these the shortest run from the front with at
+ *   least top_p of their weight (>= 1: all; always one), of these the ones
+ *   with w >= min_p; drawn is the first token at which the running sum of the
+ *   kept weights exceeds u times their sum.  temperature <= 0 or NaN takes
+ *   the first token.  NaN and -inf logits are never drawn; a row without any
+ *   other gives token -1 and logprob -inf.  temperature, top_k, top_p and
+ *   min_p: device arrays [batch] (fp32; top_k int64), or NULL for the *_all
+ *   value; any value is taken (NaN: no limit).  u <= 0 or NaN draws as 0, u >= 1
+ *   the last token kept.  tokens int64 [batch]; logprobs fp32 [batch]: log of
+ *   the token's share of the kept weight.  Weights are summed as integers in
+ *   units of 2^-43 of the largest, so the result does not depend on order.
+ *   vocab <= 524224.
+ * ---------------------------------------------------------------------- */
+int qx_multi_lora_add(const void* y, const void* x, const void* lora_A, const void* lora_B,
+                      const int64_t* adapters, const float* scales, void* out, int batch, int tokens,
+                      int K, int N, int rank, int num_adapters, const int* splits, int num_splits,
+                      qx_stream_t stream);
+int qx_lm_head_logits(const void* h, const void* weight, void* logits, int batch, int hidden, int vocab,
+                      qx_stream_t stream);
+int qx_sample_logits(const void* logits, const float* u, const float* temperature, const int64_t* top_k,
+                     const float* top_p, const float* min_p, float temperature_all, int64_t top_k_all,
+                     float top_p_all, float min_p_all, int64_t* tokens, float* logprobs, int batch,
+                     int vocab, qx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,7 +15,9 @@ Differences from the reference, all widening what it accepts:
   chunks, and the cache adds ``decode_attention``.
 
 Added beside them: the same ring held in 4 bits (``RingBufferKVCacheQ4`` and the
-``*_q4`` ops) and ``qk_norm_rope``.
+``*_q4`` ops), ``qk_norm_rope``, and what each request of a served batch brings of
+its own: its adapter (``multi_lora_add``, ``w4a16_multi_lora_gemv``) and its sampling
+settings (``lm_head_logits``, ``sample_logits``).
 
 Every op runs on the current torch CUDA stream and raises if the native
 library is missing or the inputs are not CUDA tensors: there is no CPU path.
@@ -34,7 +36,8 @@ from . import _lib, _workspace
 __all__ = ["fused_rmsnorm", "fused_swiglu", "w4a16_gemv", "w4a16_lora_gemv",
            "RingBufferKVCache", "decode_attention", "ring_slot_indices", "qk_norm_rope",
            "RingBufferKVCacheQ4", "ring_q4_storage", "ring_append_q4", "ring_gather_q4",
-           "decode_attention_q4", "prefill_attention_q4"]
+           "decode_attention_q4", "prefill_attention_q4", "multi_lora_add", "w4a16_multi_lora_gemv", "lm_head_logits",
+           "sample_logits"]
 
 _LIB = _lib.load()  # fail at import time if the native library is absent
 
@@ -480,6 +483,36 @@ def w4a16_lora_gemv(input, qweight, scales, zeros, lora_A, lora_B, group_size: i
     return _w4a16(input, qweight, scales, zeros, lora_A, lora_B, group_size, scale, zero_offset, out=out)
 
 
+# ---------------------------------------------------- adapters of many requests --
+def multi_lora_add(y: torch.Tensor, x: torch.Tensor, lora_A: torch.Tensor, lora_B: torch.Tensor,
+                   adapters: torch.Tensor, scales: torch.Tensor, *, splits=None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """``fp16(y + scales[a] (x A[a]) B[a])`` with ``a = adapters[b]``, each
+    sequence's adapter beside a shared projection whose output is ``y``: ``y``
+    fp16 ``[B, N]`` or ``[B, T, N]``, ``x`` fp16 ``[B, K]`` or ``[B, T, K]``,
+    ``lora_A`` fp16 ``[n, K, P r]``, ``lora_B`` fp16 ``[n, r, N]``, ``adapters`` int64
+    ``[B]`` and ``scales`` (alpha / r) fp32 ``[n]`` on the device, read when the
+    kernel runs (a captured graph follows them).  A sequence whose adapter is
+    outside ``0 .. n - 1`` has none and keeps ``y``.  ``splits``: the widths of the
+    ``P`` <= 4 column blocks of a fused projection (q | k | v), block ``j`` taking
+    the ranks ``j r ..`` of ``lora_A``; None: one block.  K, N, r and the widths are
+    multiples of 8, ``P r <= 256``.  ``out``: the output, ``y`` itself for in place.
+    New component (the reference's op has one adapter for all rows)."""
+    return _binding.multi_lora_add(y, x, lora_A, lora_B, adapters, scales, splits, out)
+
+
+def w4a16_multi_lora_gemv(input: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
+                          lora_A: torch.Tensor, lora_B: torch.Tensor, adapters: torch.Tensor,
+                          lora_scales: torch.Tensor, group_size: int = 128, *, zero_offset: int = 0, splits=None):
+    """``w4a16_lora_gemv`` for a batch of requests with an adapter each:
+    ``w4a16_gemv(input, ...)`` (``[B, K]`` or ``[B, T, K]``, rounded to fp16), then
+    ``multi_lora_add`` over it."""
+    if isinstance(input, torch.Tensor) and input.dim() not in (2, 3):
+        raise RuntimeError(f"w4a16_multi_lora_gemv: input must be [B, K] or [B, T, K], got {list(input.shape)}")
+    y = _w4a16(input, qweight, scales, zeros, None, None, group_size, 0.0, zero_offset)
+    return multi_lora_add(y, input, lora_A, lora_B, adapters, lora_scales, splits=splits, out=y)
+
+
 # ------------------------------------------------------------- ring cache --
 def ring_slot_indices(count: int, sink: int, window: int, device) -> torch.Tensor:
     """Logical-order slot list for ``count`` written tokens (int32, on device)."""
@@ -579,6 +612,32 @@ def lm_head_argmax(h: torch.Tensor, weight: torch.Tensor, vocab_offset: int = 0)
                                           val.data_ptr(), idx.data_ptr(), ws.data_ptr(), ws.numel(),
                                           st.cuda_stream), "lm_head_argmax")
     return val, idx
+
+
+def lm_head_logits(h: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """Logits ``h @ weight`` in fp16, ``[B, V]``, of ``h`` fp16 ``[B, H]`` and ``weight``
+    fp16 ``[H, V]`` (fp32 sums; H a multiple of 64, V of 8): the values whose
+    maximum ``lm_head_argmax`` takes.  Any B, 32 rows a pass over the weights."""
+    return _binding.lm_head_logits(h, weight)
+
+
+def sample_logits(logits: torch.Tensor, u: torch.Tensor, temperature: float | torch.Tensor = 1.0,
+                  top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
+                  min_p: float | torch.Tensor = 0.0):
+    """One token for each row of ``logits`` fp16 ``[B, V]`` (V <= 524224) from the
+    random numbers ``u`` fp32 ``[B]`` in [0, 1).  Tokens stand by their logit, the
+    largest first, equal ones by index; the weight of one is ``w = exp((l - max l) /
+    temperature)``.  Kept are the first ``top_k`` (<= 0: all), of these the shortest
+    run from the front with at least ``top_p`` of their weight (>= 1: all), of these
+    the ones with ``w >= min_p``.  Drawn is the first token at which the running sum
+    of the kept weights exceeds ``u`` times their sum; ``temperature`` <= 0 takes the
+    first token.  A setting is a number, or each row's own on the device (fp32
+    ``[B]``; ``top_k`` int64 ``[B]``), read when the kernel runs.  Returns (token
+    int64 ``[B]``, log of its share of the kept weight fp32 ``[B]``).  NaN and -inf
+    logits are never drawn; a row with nothing else gives (-1, -inf).  The same
+    inputs give the same tokens (weights are summed as integers).  New component
+    (the reference leaves sampling to HF)."""
+    return _binding.sample_logits(logits, u, temperature, top_k, top_p, min_p)
 
 
 def prefill_attention(q, k_new, v_new, k_cache, v_cache, count: int, sink: int, window: int,

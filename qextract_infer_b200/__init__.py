@@ -18,13 +18,17 @@ try:
         decode_attention_q4,
         fused_rmsnorm,
         fused_swiglu,
+        lm_head_logits,
+        multi_lora_add,
         prefill_attention_q4,
         qk_norm_rope,
         ring_append_q4,
         ring_gather_q4,
         ring_q4_storage,
+        sample_logits,
         w4a16_gemv,
         w4a16_lora_gemv,
+        w4a16_multi_lora_gemv,
     )
     _C_AVAILABLE = True
 except ImportError:

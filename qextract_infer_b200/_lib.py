@@ -101,6 +101,11 @@ SIGNATURES = {
     "qx_prefill_attention_q4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                         c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                         c_int64, c_void_p, c_float, c_void_p, c_size_t, c_void_p]),
+    "qx_multi_lora_add": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                  c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p]),
+    "qx_lm_head_logits": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "qx_sample_logits": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int64, c_float,
+                                 c_float, c_void_p, c_void_p, c_int, c_int, c_void_p]),
 }
 
 

@@ -1,4 +1,5 @@
-// Python binding of the head norm + rotation and of the 4-bit ring's operators:
+// Python binding of the head norm + rotation, of the 4-bit ring's operators and of the
+// adapters, logits and sampling of a served batch:
 // argument checks, outputs and scratch from torch's allocator, the current
 // stream of the tensors' device, then one call of the C ABI (include/qx_b200.h).
 // These operators run once a layer and decode step, on a few microseconds of GPU
@@ -290,6 +291,122 @@ PyObject* prefill_attention_q4(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// y, x, lora_A, lora_B, adapters, scales, splits (a sequence or None), out (a tensor or None) -> out
+PyObject* multi_lora_add(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* what = "multi_lora_add";
+  arguments(what, n, 8);
+  const at::Tensor &y = half(o[0], "y"), &x = half(o[1], "x"), &A = half(o[2], "lora_A"), &B = half(o[3], "lora_B");
+  const at::Tensor &ids = tensor(o[4], "adapters"), &scales = tensor(o[5], "scales");
+  int splits[64], parts = 0;
+  if (o[6] != Py_None) {
+    PyObject* const seq = PySequence_Fast(o[6], "multi_lora_add: splits must be a sequence of widths");
+    if (!seq) throw python_error();
+    const Py_ssize_t m = PySequence_Fast_GET_SIZE(seq);
+    bool fine = m <= 64;
+    for (Py_ssize_t i = 0; fine && i < m; ++i) {
+      const long long v = PyLong_AsLongLong(PySequence_Fast_GET_ITEM(seq, i));
+      fine = !(v == -1 && PyErr_Occurred()) && v >= INT32_MIN && v <= INT32_MAX;
+      splits[i] = int(v);
+    }
+    Py_DECREF(seq);
+    if (PyErr_Occurred()) throw python_error();
+    if (!fine || m == 0) refuse("%s: splits must be a sequence of a few widths", what);
+    parts = int(m);
+  }
+  const int dims = int(y.dim());
+  if ((dims != 2 && dims != 3) || x.dim() != dims || x.size(0) != y.size(0) || (dims == 3 && x.size(1) != y.size(1)))
+    refuse("%s: y must be [B, N] or [B, T, N] and x [B, K] or [B, T, K], got %s and %s", what, shape_of(y).c_str(),
+           shape_of(x).c_str());
+  const int batch = size32(y, 0, what), tokens = dims == 3 ? size32(y, 1, what) : 1;
+  const int K = size32(x, dims - 1, what), N = size32(y, dims - 1, what), P = parts ? parts : 1;
+  if (A.dim() != 3 || B.dim() != 3 || A.size(0) != B.size(0) || A.size(1) != K || B.size(2) != N || A.size(2) != P * B.size(1))
+    refuse("%s: lora_A must be [n, %d, %d r] and lora_B [n, r, %d], got %s and %s", what, K, P, N, shape_of(A).c_str(),
+           shape_of(B).c_str());
+  const int adapters = size32(A, 0, what), rank = size32(B, 1, what);
+  if (ids.scalar_type() != at::kLong || ids.dim() != 1 || ids.size(0) != batch) refuse("%s: adapters must be int64 [%d]", what, batch);
+  if (scales.scalar_type() != at::kFloat || scales.dim() != 1 || scales.size(0) != adapters)
+    refuse("%s: scales must be float32 [%d]", what, adapters);
+  const at::Device dev = y.device();
+  same_device(what, dev, {&x, &A, &B, &ids, &scales});
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor out;
+  if (o[7] == Py_None) {
+    out = empty(y.sizes(), at::kHalf, dev);
+  } else {
+    out = half(o[7], "out");
+    if (out.sizes() != y.sizes()) refuse("%s: out must be like y, got %s", what, shape_of(out).c_str());
+    same_device(what, dev, {&out});
+  }
+  check(qx_multi_lora_add(y.const_data_ptr(), x.const_data_ptr(), A.const_data_ptr(), B.const_data_ptr(),
+                          ids.const_data_ptr<int64_t>(), scales.const_data_ptr<float>(), out.data_ptr(), batch, tokens, K, N,
+                          rank, adapters, parts ? splits : nullptr, parts, stream_of(dev)),
+        what);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// h, weight -> logits
+PyObject* lm_head_logits(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* what = "lm_head_logits";
+  arguments(what, n, 2);
+  const at::Tensor &h = half(o[0], "h"), &w = half(o[1], "weight");
+  if (h.dim() != 2 || w.dim() != 2 || w.size(0) != h.size(1))
+    refuse("%s: h must be [B, H] and weight [H, V], got %s and %s", what, shape_of(h).c_str(), shape_of(w).c_str());
+  const at::Device dev = h.device();
+  same_device(what, dev, {&w});
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor out = empty({h.size(0), w.size(1)}, at::kHalf, dev);
+  check(qx_lm_head_logits(h.const_data_ptr(), w.const_data_ptr(), out.data_ptr(), size32(h, 0, what), size32(h, 1, what),
+                          size32(w, 1, what), stream_of(dev)),
+        what);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// a number for all rows, or a tensor with each row's own
+const void* setting(PyObject* o, const char* name, at::ScalarType type, int64_t rows, at::Device dev, double* all) {
+  if (!THPVariable_Check(o)) {
+    *all = type == at::kLong ? double(integer(o)) : PyFloat_AsDouble(o);
+    if (*all == -1.0 && PyErr_Occurred()) throw python_error();
+    return nullptr;
+  }
+  const at::Tensor& t = tensor(o, name);
+  if (t.scalar_type() != type || t.dim() != 1 || t.size(0) != rows)
+    refuse("sample_logits: %s must be a number or %s [%lld]", name, type == at::kLong ? "int64" : "float32", (long long)rows);
+  same_device("sample_logits", dev, {&t});
+  return t.const_data_ptr();
+}
+
+// logits, u, temperature, top_k, top_p, min_p -> (tokens, logprobs)
+PyObject* sample_logits(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* what = "sample_logits";
+  arguments(what, n, 6);
+  const at::Tensor &l = half(o[0], "logits"), &u = tensor(o[1], "u");
+  if (l.dim() != 2) refuse("%s: logits must be [B, V], got %s", what, shape_of(l).c_str());
+  const int64_t rows = l.size(0);
+  if (u.scalar_type() != at::kFloat || u.dim() != 1 || u.size(0) != rows) refuse("%s: u must be float32 [%lld]", what, (long long)rows);
+  const at::Device dev = l.device();
+  same_device(what, dev, {&u});
+  double t_all = 0, k_all = 0, p_all = 0, m_all = 0;
+  const void* t = setting(o[2], "temperature", at::kFloat, rows, dev, &t_all);
+  const void* k = setting(o[3], "top_k", at::kLong, rows, dev, &k_all);
+  const void* p = setting(o[4], "top_p", at::kFloat, rows, dev, &p_all);
+  const void* m = setting(o[5], "min_p", at::kFloat, rows, dev, &m_all);
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor tokens = empty({rows}, at::kLong, dev), logprobs = empty({rows}, at::kFloat, dev);
+  check(qx_sample_logits(l.const_data_ptr(), u.const_data_ptr<float>(), static_cast<const float*>(t),
+                         static_cast<const int64_t*>(k), static_cast<const float*>(p), static_cast<const float*>(m),
+                         float(t_all), int64_t(std::min(k_all, 9e18)), float(p_all), float(m_all),
+                         tokens.data_ptr<int64_t>(), logprobs.data_ptr<float>(), size32(l, 0, what), size32(l, 1, what),
+                         stream_of(dev)),
+        what);
+  return wrap({tokens, logprobs});
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* set_error(PyObject*, PyObject* cls) {
   Py_INCREF(cls);
   Py_XDECREF(g_error);
@@ -299,7 +416,8 @@ PyObject* set_error(PyObject*, PyObject* cls) {
 
 #define QX_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {QX_FAST(qk_norm_rope),        QX_FAST(ring_append_q4),       QX_FAST(ring_gather_q4),
-                         QX_FAST(decode_attention_q4), QX_FAST(prefill_attention_q4), {"set_error", set_error, METH_O, nullptr},
+                         QX_FAST(decode_attention_q4), QX_FAST(prefill_attention_q4), QX_FAST(multi_lora_add),
+                         QX_FAST(lm_head_logits),      QX_FAST(sample_logits),        {"set_error", set_error, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -10,6 +10,9 @@
 // per-row maximum with its smallest index is written to the workspace.
 // Kernel 2: one warp per row reduces the CTAs' candidates in index order
 // (ties go to the smallest index) and adds the slice's vocabulary offset.
+//
+// Whole logits (qx_lm_head_logits): kernel 1 with the fp16 values stored instead of
+// compared, 32 rows a launch.  Bound by the weights' bytes like the greedy head.
 #include <algorithm>
 #include <cfloat>
 #include <mutex>
@@ -67,10 +70,11 @@ __device__ __forceinline__ bool better(float v, int i, float bv, int bi) {
   return v > bv || (v == bv && i < bi);
 }
 
-template <int MT>
-__global__ void __launch_bounds__(THREADS) logits_argmax_kernel(const __half* __restrict__ h,
-                                                               const __half* __restrict__ W, int B, int H,
-                                                               int V, Cand* __restrict__ part) {
+// STORE: the logits go to `out` [B, V]; else the CTA's candidates to `part`
+template <int MT, bool STORE>
+__global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restrict__ h, const __half* __restrict__ W,
+                                                        int B, int H, int V, Cand* __restrict__ part,
+                                                        __half* __restrict__ out) {
   pdl_trigger();
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Cand s_best[WARPS][MAXB];
@@ -142,6 +146,22 @@ __global__ void __launch_bounds__(THREADS) logits_argmax_kernel(const __half* __
   }
   cp_async_wait<0>();
 
+  if constexpr (STORE) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int hr = 0; hr < 2; ++hr) {  // rows g and g + 8 of the m-tile
+        const int row = m * 16 + g + hr * 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int col = n0 + warp * 64 + j * 8 + 2 * c;
+          if (row < B && col < V)  // V % 8 == 0: both columns or none
+            *reinterpret_cast<__half2*>(out + size_t(row) * V + col) =
+                __floats2half2_rn(acc[m][j][hr * 2], acc[m][j][hr * 2 + 1]);
+        }
+      }
+    return;
+  }
   // per row: the fp16-rounded logits' maximum and its smallest index
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -217,6 +237,21 @@ __global__ void __launch_bounds__(128) argmax_finish_kernel(const Cand* __restri
   }
 }
 
+// shared-memory limits of the kernels on the current device, once
+int prepare(const char* what) {
+  static std::mutex mu;
+  static bool done[64] = {};
+  int dev = 0;
+  QX_CUDA_TRY(cudaGetDevice(&dev), what);
+  QX_REQUIRE(dev >= 0 && dev < 64, "%s: device index %d unsupported", what, dev);
+  std::lock_guard<std::mutex> lk(mu);
+  if (done[dev]) return QX_OK;
+  for (auto kernel : {logits_kernel<1, false>, logits_kernel<2, false>, logits_kernel<1, true>, logits_kernel<2, true>})
+    QX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM), what);
+  done[dev] = true;
+  return QX_OK;
+}
+
 }  // namespace lmh
 }  // namespace qx
 
@@ -238,38 +273,42 @@ extern "C" int qx_lm_head_argmax(const void* h, const void* weight, int batch, i
   const size_t need = qx_lm_head_argmax_workspace_size(vocab);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
     return fail(QX_ERR_WORKSPACE, "lm_head_argmax: workspace needs %zu bytes, 16-byte aligned", need);
-  {
-    static std::mutex mu;
-    static bool done[64] = {};
-    int dev = 0;
-    QX_CUDA_TRY(cudaGetDevice(&dev), "lm_head_argmax: cudaGetDevice");
-    QX_REQUIRE(dev >= 0 && dev < 64, "lm_head_argmax: device index %d unsupported", dev);
-    std::lock_guard<std::mutex> lk(mu);
-    if (!done[dev]) {
-      QX_CUDA_TRY(cudaFuncSetAttribute(lmh::logits_argmax_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       lmh::SMEM),
-                  "lm_head_argmax: set smem limit");
-      QX_CUDA_TRY(cudaFuncSetAttribute(lmh::logits_argmax_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       lmh::SMEM),
-                  "lm_head_argmax: set smem limit");
-      done[dev] = true;
-    }
-  }
+  if (const int rc = lmh::prepare("lm_head_argmax"); rc != QX_OK) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int nblk = (vocab + lmh::COLS - 1) / lmh::COLS;
   auto H = static_cast<const __half*>(h);
   auto Wt = static_cast<const __half*>(weight);
   auto part = static_cast<lmh::Cand*>(workspace);
-  if (batch <= 16)
-    QX_CUDA_TRY(launch_pdl(lmh::logits_argmax_kernel<1>, dim3(nblk), dim3(lmh::THREADS), lmh::SMEM, st, H, Wt,
-                           batch, hidden, vocab, part),
-                "lm_head_argmax: launch");
-  else
-    QX_CUDA_TRY(launch_pdl(lmh::logits_argmax_kernel<2>, dim3(nblk), dim3(lmh::THREADS), lmh::SMEM, st, H, Wt,
-                           batch, hidden, vocab, part),
-                "lm_head_argmax: launch");
+  QX_CUDA_TRY(launch_pdl(batch <= 16 ? lmh::logits_kernel<1, false> : lmh::logits_kernel<2, false>, dim3(nblk),
+                         dim3(lmh::THREADS), lmh::SMEM, st, H, Wt, batch, hidden, vocab, part,
+                         static_cast<__half*>(nullptr)),
+              "lm_head_argmax: launch");
   QX_CUDA_TRY(launch_pdl(lmh::argmax_finish_kernel, dim3((batch + 3) / 4), dim3(128), 0, st,
                          static_cast<const lmh::Cand*>(part), nblk, batch, vocab_offset, out_val, out_idx),
               "lm_head_argmax: finish launch");
   return check_launch("lm_head_argmax");
+}
+
+extern "C" int qx_lm_head_logits(const void* h, const void* weight, void* logits, int batch, int hidden, int vocab,
+                                 qx_stream_t stream) {
+  QX_REQUIRE(batch >= 0, "lm_head_logits: batch=%d", batch);
+  QX_REQUIRE(hidden > 0 && hidden % lmh::KT == 0, "lm_head_logits: hidden=%d must be a multiple of %d", hidden,
+             lmh::KT);
+  QX_REQUIRE(vocab > 0 && vocab % 8 == 0, "lm_head_logits: vocab=%d must be a multiple of 8", vocab);
+  if (batch == 0) return QX_OK;
+  QX_REQUIRE(h && weight && logits, "lm_head_logits: null pointer");
+  QX_REQUIRE(aligned(h, 16) && aligned(weight, 16) && aligned(logits, 4),
+             "lm_head_logits: h and weight must be 16-byte aligned, logits 4-byte");
+  if (const int rc = lmh::prepare("lm_head_logits"); rc != QX_OK) return rc;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int nblk = (vocab + lmh::COLS - 1) / lmh::COLS;
+  for (int64_t r = 0; r < batch; r += lmh::MAXB) {
+    const int rows = int(std::min<int64_t>(lmh::MAXB, batch - r));
+    QX_CUDA_TRY(launch_pdl(rows <= 16 ? lmh::logits_kernel<1, true> : lmh::logits_kernel<2, true>, dim3(nblk),
+                           dim3(lmh::THREADS), lmh::SMEM, st, static_cast<const __half*>(h) + r * hidden,
+                           static_cast<const __half*>(weight), rows, hidden, vocab, static_cast<lmh::Cand*>(nullptr),
+                           static_cast<__half*>(logits) + r * vocab),
+                "lm_head_logits: launch");
+  }
+  return check_launch("lm_head_logits");
 }
