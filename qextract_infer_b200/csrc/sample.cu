@@ -16,9 +16,11 @@
 //
 // A cluster of C CTAs takes a row.  Each CTA counts a slice of it in its own histogram
 // (16-bit counters, 128 KB of shared memory), then owns 1 / C of the values: it adds
-// their counters of all CTAs through distributed shared memory, and the prefix sums run
-// over threads, warps and CTAs.  Whoever owns the border in question (the k-th token,
-// top_p of the weight, u of the weight) tells all CTAs.
+// their counters of all CTAs through distributed shared memory (only those that are
+// not empty: each CTA tells the others which of its groups of 8 counters are in use),
+// and the prefix sums run over threads, warps and CTAs.  Whoever owns the border in question
+// (the k-th token, top_p of the weight, u of the weight) tells all CTAs: its warp looks
+// at the thread's values again, a lane a value.
 #include <mutex>
 
 #include "qx_b200.h"
@@ -30,7 +32,8 @@ namespace smp {
 constexpr int THREADS = 1024, WARPS = THREADS / 32;
 constexpr int VALUES = 65536;
 constexpr int HIST_BYTES = VALUES * 2;
-constexpr int SLICE_MAX = 65528;  // logits of a CTA: a 16-bit counter holds them all
+constexpr int SLICE_MAX = 47104;  // logits of a CTA: they stay in shared memory, and a 16-bit counter holds them all
+constexpr int VOCAB_MAX = 524224;
 constexpr int FRAC = 43;
 constexpr unsigned NONE = ~0u;
 typedef unsigned long long u64;
@@ -47,19 +50,30 @@ struct Params {
   int vocab, slice;
 };
 
+constexpr int RUNS = SLICE_MAX / 256;  // of 256 logits in the largest slice
+
+enum Exchange { USED, TOTALS, TOP_K, LIMITS, PICK, EXCHANGES };
+
 template <int C>
 struct Shared {
+  u64 done[EXCHANGES];  // mbarriers: what the cluster sends for this exchange has arrived
+  // written by the cluster's CTAs
+  alignas(16) u64 total[C][2];  // tokens and weight of each CTA's values
+  alignas(16) u64 p_run[2];     // tokens and weight of the run that top_p leaves
+  alignas(16) u64 m_run[C][2];  // those before the first value of each CTA that is too light for min_p
+  u64 k_mass, pick;
+  unsigned used[C][VALUES / 8 / C / 32];  // of each CTA: which groups of 8 of this CTA's values occur
+  unsigned top[C];
+  // this CTA's
   u64 warp_mass[WARPS];
   unsigned warp_count[WARPS];
-  // written by the cluster's CTAs
-  unsigned top[C], count[C];
-  u64 mass[C];
-  u64 k_mass, p_mass, m_mass[C];
-  unsigned p_n, m_n[C];
-  unsigned pick, pick_nth;
-  // this CTA's
-  unsigned top_here, m_here, found;
+  unsigned top_here, m_here, found, found_nth;
+  unsigned run[RUNS];
 };
+
+// Sticky device-side error word of this file's kernel (QX_DEVERR_* bits), merged into
+// qx_get_device_error.
+static __device__ unsigned g_sample_error = 0;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ uint32_t at_rank(const void* p, int rank) {
@@ -67,18 +81,50 @@ __device__ __forceinline__ uint32_t at_rank(const void* p, int rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void tell(const unsigned* p, int rank, unsigned v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at_rank(p, rank)), "r"(v) : "memory");
+// Sends to CTA `rank` and counts the bytes on its barrier there: an exchange costs a
+// store's way and no barrier of the cluster (which took up to 2 us here).
+__device__ __forceinline__ void send(const u64* p, const u64* done, int rank, u64 a) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(at_rank(p, rank)),
+               "l"(a), "r"(at_rank(done, rank))
+               : "memory");
 }
-__device__ __forceinline__ void tell(const u64* p, int rank, u64 v) {
-  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at_rank(p, rank)), "l"(v) : "memory");
+__device__ __forceinline__ void send(const unsigned* p, const u64* done, int rank, unsigned a) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(at_rank(p, rank)),
+               "r"(a), "r"(at_rank(done, rank))
+               : "memory");
+}
+__device__ __forceinline__ void send(const u64* p, const u64* done, int rank, u64 a, u64 b) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(at_rank(p, rank)),
+               "l"(a), "l"(b), "r"(at_rank(done, rank))
+               : "memory");
+}
+__device__ __forceinline__ void expect(const u64* done, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(done)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool arrived(uint32_t bar) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred P; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], 0; selp.u32 %0, 1, 0, P; }"
+      : "=r"(ok)
+      : "r"(bar)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void wait_for(const u64* done) {  // at most kWaitLimitNs
+  const uint32_t bar = smem_u32(done);
+  if (arrived(bar)) return;
+  uint64_t t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  while (!arrived(bar)) {
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    if (t - t0 > kWaitLimitNs) {
+      atomicOr(&g_sample_error, QX_DEVERR_MBAR_TIMEOUT);
+      return;
+    }
+  }
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_sync() {
-  cluster_arrive();
-  cluster_wait();
-}
 
 // the place of a logit's bits among all values, the largest first; NaN and -inf: NONE
 __device__ __forceinline__ unsigned place_of(unsigned bits) {
@@ -91,91 +137,239 @@ __device__ __forceinline__ double value_at(unsigned place) {
   return double(__half2float(__ushort_as_half(static_cast<unsigned short>(bits))));
 }
 
+// Weights of a row's values.  exp((v - top) / T) = 2^n e^f with n the nearest integer to
+// (v - top) log2(e) / T and |f| <= ln(2) / 2; e^f by its Taylor series to f^12 (the
+// next term is below 2^-52).  Conversions between doubles and integers are slow: both
+// here are a sum with a number that is so large that the integer stands in the sum's
+// low bits, rounded to the nearest.
+// A thread's values are neighbours and equally spaced, so their weights are a
+// geometric sequence: two exponentials, then a product each (measured at 32 values a
+// thread: an exponential each 8300 cycles a row).  Every use of a weight makes it by the
+// same products, so its integer is the same everywhere.
 struct Weights {
-  double top, temperature;
+  double top, scale;
   unsigned place;
-  bool top_is_inf;
-  // logarithm of a value's weight
-  __device__ __forceinline__ double log_of(unsigned d) const {
-    if (d == place) return 0.0;
-    return top_is_inf ? -INFINITY : (value_at(d) - top) / temperature;
+
+  // 2^y, 0 below half a unit of the sums
+  static __device__ __forceinline__ double power(double y) {
+    constexpr double BIG = 6755399441055744.0;  // 1.5 x 2^52
+    if (!(y > -45.0)) return 0.0;
+    const double big = y + BIG;
+    const double f = (y - (big - BIG)) * 0.69314718055994530942;
+    double e = 1.0 / 479001600.0;
+    e = fma(e, f, 1.0 / 39916800.0);
+    e = fma(e, f, 1.0 / 3628800.0);
+    e = fma(e, f, 1.0 / 362880.0);
+    e = fma(e, f, 1.0 / 40320.0);
+    e = fma(e, f, 1.0 / 5040.0);
+    e = fma(e, f, 1.0 / 720.0);
+    e = fma(e, f, 1.0 / 120.0);
+    e = fma(e, f, 1.0 / 24.0);
+    e = fma(e, f, 1.0 / 6.0);
+    e = fma(e, f, 0.5);
+    e = fma(e, f, 1.0);
+    e = fma(e, f, 1.0);
+    return __hiloint2double(__double2hiint(e) + __double2loint(big) * (1 << 20), __double2loint(e));  // e 2^n
   }
-  __device__ __forceinline__ double of(unsigned d) const { return exp(log_of(d)); }
+  // the weight of the first of a thread's values that is not above the top (only those occur), and
+  // what each of the values behind it has of the one before it
+  __device__ __forceinline__ void start(unsigned first, double& w, double& ratio) const {
+    const unsigned d = max(first, place);
+    w = d == place ? 1.0 : power((value_at(d) - top) * scale);
+    ratio = power((value_at(first + 1) - value_at(first)) * scale);
+  }
+  // w: the weight of place d - 1 (or what start gave) -> that of place d
+  __device__ __forceinline__ void next(unsigned first, unsigned d, double ratio, double& w) const {
+    if (d > first && d > place) w *= ratio;
+  }
 };
-__device__ __forceinline__ u64 fixed(double w) { return u64(__double2ull_rn(w * double(u64(1) << FRAC))); }
+__device__ __forceinline__ u64 fixed(double w) {  // w 2^FRAC <= 2^43
+  constexpr double BIG = 4503599627370496.0;  // 2^52
+  return u64(__double_as_longlong(fma(w, double(u64(1) << FRAC), BIG))) & ((u64(1) << 52) - 1);
+}
+
+// A row as aligned groups of 8 logits; places outside the row read as -inf
+struct Row {
+  const unsigned short* at;  // the first logit
+  int shift;                 // its place in its aligned group
+  int vocab;
+  // starts the copy of group i into shared memory
+  __device__ __forceinline__ void fetch(int i, uint4* to) const {
+    const int first = 8 * i - shift;
+    if (first >= 0 && first + 8 <= vocab) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(at + first) : "memory");
+      return;
+    }
+    unsigned short* const v = reinterpret_cast<unsigned short*>(to);
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+      const int k = first + e;
+      v[e] = k >= 0 && k < vocab ? __ldcg(at + k) : 0xFC00u;
+    }
+  }
+};
+__device__ __forceinline__ uint32_t hadd2_u32(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t hmax2_u32(uint32_t a, uint32_t b) {  // the number, where one is NaN
+  uint32_t d;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// the larger half of a pair and its place
+__device__ __forceinline__ unsigned top_of(uint32_t pair) {
+  const uint32_t m = hmax2_u32(pair, pair >> 16);
+  return place_of(m & 0xFFFFu);
+}
 
 template <int C>
-__global__ void __launch_bounds__(THREADS, 1) sample_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, 1) sample_kernel(const __grid_constant__ Params p) {
   constexpr int OWN = VALUES / (C * THREADS);  // values of a thread
   extern __shared__ __align__(16) unsigned char smem[];
   unsigned* const hist = reinterpret_cast<unsigned*>(smem);
-  Shared<C>& s = *reinterpret_cast<Shared<C>*>(smem + HIST_BYTES);
+  uint4* const slice = reinterpret_cast<uint4*>(smem + HIST_BYTES);
+  Shared<C>& s = *reinterpret_cast<Shared<C>*>(smem + HIST_BYTES + 2 * p.slice);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row = blockIdx.x / C, rank = blockIdx.x % C;
   pdl_trigger();
 
-  for (int i = tid; i < HIST_BYTES / 16; i += THREADS) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0u, 0u, 0u, 0u);
   if (tid == 0) {
-    s.pick = s.top_here = s.m_here = s.p_n = NONE;
-    for (int r = 0; r < C; ++r) s.m_n[r] = NONE;
+    s.top_here = s.m_here = NONE;
+    for (int i = 0; i < EXCHANGES; ++i)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&s.done[i])) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
   cluster_arrive();
   pdl_wait();
+  Row logits;
+  logits.at = reinterpret_cast<const unsigned short*>(p.logits) + int64_t(row) * p.vocab;
+  logits.shift = int(uint32_t(reinterpret_cast<uintptr_t>(logits.at)) & 15u) >> 1;
+  logits.vocab = p.vocab;
+  const int first_group = rank * (p.slice / 8);
+  const int groups = max(0, min(p.slice / 8, (p.vocab + logits.shift + 7) / 8 - first_group));
+  // the slice, a thread's own groups (nobody else reads them before a barrier)
+  for (int i = tid; i < groups; i += THREADS) logits.fetch(first_group + i, slice + i);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  const float u_row = p.u[row], t_row = p.temperature ? p.temperature[row] : p.temperature_all;
+  const float p_row = p.top_p ? p.top_p[row] : p.top_p_all, m_row = p.min_p ? p.min_p[row] : p.min_p_all;
+  const bool greedy = !(t_row > 0.f);
+  const int64_t k_row = greedy ? 1 : p.top_k ? p.top_k[row] : p.top_k_all;
+  const double min_p = !greedy && m_row > 0.f ? fmin(double(m_row), 1.0) : 0.0;
+  Weights weights;
+  weights.scale = greedy ? 1.0 : 1.44269504088896340736 / double(t_row);
+
+  for (int i = tid; i < HIST_BYTES / 16; i += THREADS) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0u, 0u, 0u, 0u);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
 
   // ---- count the slice
-  const unsigned short* const slice = reinterpret_cast<const unsigned short*>(p.logits) + int64_t(row) * p.vocab + int64_t(rank) * p.slice;
-  const int len = max(0, min(p.slice, p.vocab - rank * p.slice));
-  unsigned top = NONE;
-  auto count = [&](unsigned bits) {
-    const unsigned d = place_of(bits);
-    if (d == NONE) return;
-    atomicAdd(hist + (d >> 1), d & 1 ? 0x10000u : 1u);
-    top = min(top, d);
-  };
-  const int head = min(len, int((16u - (uint32_t(reinterpret_cast<uintptr_t>(slice)) & 15u)) & 15u) >> 1);
-  const int vectors = (len - head) >> 3;
-  for (int i = tid; i < vectors; i += THREADS) {
-    const uint4 v = __ldcg(reinterpret_cast<const uint4*>(slice + head) + i);
-    const unsigned w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      count(w[e] & 0xFFFFu);
-      count(w[e] >> 16);
+  // A slice's logits matter only up to its own k-th largest, and that is not below the
+  // k-th largest of the threads' largest ones: a search over places, a count of the block
+  // each of 16 steps.  Without top_p nothing lighter than min_p matters (beside the slice's
+  // largest, all the more beside the row's).  Either leaves few logits to count.
+  unsigned last = 0xFBFFu;  // the last place that is counted
+  const bool by_k = k_row > 0 && k_row <= THREADS / 2, by_min = min_p > 0.0 && !(p_row < 1.f);
+  if (by_k || by_min) {
+    uint32_t best = 0xFC00FC00u;
+    for (int i = tid; i < groups; i += THREADS) {
+      const uint4 v = slice[i];
+      best = hmax2_u32(best, hmax2_u32(hmax2_u32(v.x, v.y), hmax2_u32(v.z, v.w)));
     }
-  }
-  const int rest = len - 8 * vectors;  // the ends that no aligned vector covers
-  if (tid < rest) count(__ldcg(slice + (tid < head ? tid : tid + 8 * vectors)));
-  top = __reduce_min_sync(0xffffffffu, top);
-  if (lane == 0) atomicMin(&s.top_here, top);
-  __syncthreads();
-  cluster_wait();  // every CTA has started
-  if (tid < C) tell(&s.top[rank], tid, s.top_here);
-  cluster_sync();
-
-  // ---- the counters of the values that this CTA owns, of all CTAs
-  const unsigned first = unsigned(rank * THREADS + tid) * OWN;
-  unsigned c[OWN];
-#pragma unroll
-  for (int i = 0; i < OWN; ++i) c[i] = 0;
-#pragma unroll
-  for (int r = 0; r < C; ++r) {
-    const uint32_t at = at_rank(hist + first / 2, (rank + r) % C);
-#pragma unroll
-    for (int i = 0; i < OWN; i += 8) {
-      uint32_t w[4];
-      asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                   : "r"(at + 2 * i)
-                   : "memory");
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        c[i + 2 * e] += w[e] & 0xFFFFu;
-        c[i + 2 * e + 1] += w[e] >> 16;
+    const unsigned mine = top_of(best);
+    if (by_k) {
+      unsigned low = 0;  // the least place with k_row threads whose top is not behind it
+#pragma unroll 1
+      for (unsigned bit = 0x8000u; bit; bit >>= 1)
+        if (__syncthreads_count(mine < low + bit) < int(k_row)) low += bit;
+      last = min(last, low);
+    }
+    if (by_min) {
+      const unsigned warp_top = __reduce_min_sync(0xffffffffu, mine);
+      if (lane == 0) atomicMin(&s.top_here, warp_top);
+      __syncthreads();
+      const unsigned seen = s.top_here;
+      if (seen > 0x3FFu && seen != NONE) {
+        const float seen_at = float(value_at(seen)), down = t_row * -__logf(float(min_p));
+        const float rounded = seen_at - down - 1e-3f * (1.f + fabsf(seen_at) + down);
+        last = min(last, place_of(__half_as_ushort(__float2half_rd(rounded))));  // (NONE where it is -inf)
       }
     }
   }
-  Weights weights;
+  uint32_t best = 0xFC00FC00u;
+  {
+    const unsigned span = last - 0x3FFu;  // places before 0x3FF (+inf) are NaN, those behind 0xFBFF -inf and NaN
+#pragma unroll 1
+    for (int i = tid; i < groups; i += THREADS) {
+      const uint4 v = slice[i];
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      const uint32_t all = hmax2_u32(hmax2_u32(v.x, v.y), hmax2_u32(v.z, v.w));
+      best = hmax2_u32(best, all);
+      if ((by_k || by_min) && top_of(all) > last) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = hadd2_u32(w[e], 0u);  // the zeros are one value
+        const uint32_t d = x ^ (~prmt(x, 0u, 0xBB99u) & 0x7FFF7FFFu);  // place_of of both halves
+        const unsigned lo = d & 0xFFFFu, hi = d >> 16;
+        if (lo - 0x3FFu <= span) atomicAdd(hist + (lo >> 1), lo & 1 ? 0x10000u : 1u);
+        if (hi - 0x3FFu <= span) atomicAdd(hist + (hi >> 1), hi & 1 ? 0x10000u : 1u);
+      }
+    }
+  }
+  const unsigned warp_top = __reduce_min_sync(0xffffffffu, top_of(best));
+  if (lane == 0) atomicMin(&s.top_here, warp_top);
+  __syncthreads();
+  cluster_wait();  // every CTA has started
+  // what was counted before the __syncthreads is seen by whoever receives from these threads
+  if (lane == 0 || tid < C) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  if (tid == 0) expect(&s.done[USED], C * 4 + VALUES / 64);
+  if (tid < C) send(&s.top[rank], &s.done[USED], tid, s.top_here);
+#pragma unroll
+  for (int i = 0; i < VALUES / 8 / THREADS; ++i) {
+    constexpr int WORDS = VALUES / 8 / C / 32;  // of a CTA's values
+    const uint4 v = reinterpret_cast<const uint4*>(hist)[i * THREADS + tid];
+    const unsigned used = __ballot_sync(0xffffffffu, (v.x | v.y | v.z | v.w) != 0u);
+    const int word = i * WARPS + warp;
+    if (lane == 0) send(&s.used[rank][word % WORDS], &s.done[USED], word / WORDS, used);
+  }
+  wait_for(&s.done[USED]);
+
+  // ---- the counters of the values that this CTA owns, of all CTAs
+  const unsigned first = unsigned(rank * THREADS + tid) * OWN;
+  constexpr int WORDS16 = OWN < 8 ? 1 : OWN / 8, WIDE = OWN < 8 ? OWN / 2 : 4;  // loads of a CTA's counters, words of one
+  uint32_t there[C][WORDS16][WIDE];
+#pragma unroll
+  for (int r = 0; r < C; ++r) {
+    const uint32_t at = at_rank(hist + first / 2, r);
+#pragma unroll
+    for (int i = 0; i < WORDS16; ++i) {
+#pragma unroll
+      for (int e = 0; e < WIDE; ++e) there[r][i][e] = 0u;
+      const int group = (tid * OWN) / 8 + i;
+      if (s.used[r][group >> 5] >> (group & 31) & 1) {
+        if constexpr (WIDE == 4)
+          asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(there[r][i][0]), "=r"(there[r][i][1]), "=r"(there[r][i][2]), "=r"(there[r][i][3])
+                       : "r"(at + 16 * i)
+                       : "memory");
+        else
+          asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(there[r][i][0]), "=r"(there[r][i][1]) : "r"(at) : "memory");
+      }
+    }
+  }
+  unsigned c[OWN];
+#pragma unroll
+  for (int i = 0; i < OWN / 2; ++i) {
+    c[2 * i] = c[2 * i + 1] = 0u;
+#pragma unroll
+    for (int r = 0; r < C; ++r) {
+      const uint32_t w = there[r][i / WIDE][i % WIDE];
+      c[2 * i] += w & 0xFFFFu;
+      c[2 * i + 1] += w >> 16;
+    }
+  }
   weights.place = s.top[0];
   for (int r = 1; r < C; ++r) weights.place = min(weights.place, s.top[r]);
   if (weights.place == NONE) {  // nothing to draw from
@@ -183,26 +377,30 @@ __global__ void __launch_bounds__(THREADS, 1) sample_kernel(const Params p) {
       p.tokens[row] = -1;
       p.logprobs[row] = -INFINITY;
     }
-    cluster_sync();  // nobody reads this CTA's histogram any more
+    cluster_arrive();  // nobody reads this CTA's histogram any more
+    cluster_wait();
     return;
   }
   weights.top = value_at(weights.place);
-  weights.top_is_inf = isinf(weights.top);
-  const float t_row = p.temperature ? p.temperature[row] : p.temperature_all;
-  const bool greedy = !(t_row > 0.f);
-  weights.temperature = greedy ? 1.0 : double(t_row);
-  const float p_row = p.top_p ? p.top_p[row] : p.top_p_all, m_row = p.min_p ? p.min_p[row] : p.min_p_all;
-  const double min_p = m_row > 0.f ? fmin(double(m_row), 1.0) : 0.0;
+  // (beside +inf nothing has weight, whatever the temperature)
+  if (isinf(weights.top)) weights.top = 1e300, weights.scale = 1.0;
 
-  // ---- prefix sums of counts and weights
-  unsigned n_here = 0;
-  u64 mass_here = 0;
+  // ---- prefix sums of counts and weights; of those heavy enough for min_p, and whether some are not
+  unsigned n_here = 0, n_heavy = 0;
+  u64 mass_here = 0, mass_heavy = 0;
+  bool light = false;
+  double w, ratio;
+  weights.start(first, w, ratio);
 #pragma unroll
-  for (int i = 0; i < OWN; ++i)
+  for (int i = 0; i < OWN; ++i) {
+    weights.next(first, first + i, ratio, w);
     if (c[i]) {
       n_here += c[i];
-      mass_here += c[i] * fixed(weights.of(first + i));
+      mass_here += c[i] * fixed(w);
+      light |= !(w >= min_p);
+      if (!light) n_heavy = n_here, mass_heavy = mass_here;
     }
+  }
   unsigned n_before = n_here;
   u64 before = mass_here;
 #pragma unroll
@@ -221,202 +419,306 @@ __global__ void __launch_bounds__(THREADS, 1) sample_kernel(const Params p) {
   n_before -= n_here;
   before -= mass_here;
   __syncthreads();
-  {
-    unsigned n = s.warp_count[lane], n_all = n;
-    u64 m = s.warp_mass[lane], m_all = m;
-    if (lane >= warp) n = 0, m = 0;
+  if (warp == 0) {
+    const unsigned n_own = lane < WARPS ? s.warp_count[lane] : 0u;
+    const u64 m_own = lane < WARPS ? s.warp_mass[lane] : 0u;
+    unsigned n = n_own;
+    u64 m = m_own;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      n += __shfl_xor_sync(0xffffffffu, n, o);
-      m += __shfl_xor_sync(0xffffffffu, m, o);
-      n_all += __shfl_xor_sync(0xffffffffu, n_all, o);
-      m_all += __shfl_xor_sync(0xffffffffu, m_all, o);
+    for (int o = 1; o < WARPS; o <<= 1) {
+      const unsigned n2 = __shfl_up_sync(0xffffffffu, n, o);
+      const u64 m2 = __shfl_up_sync(0xffffffffu, m, o);
+      if (lane >= o) {
+        n += n2;
+        m += m2;
+      }
     }
-    n_before += n;
-    before += m;
-    if (tid < C) {
-      tell(&s.count[rank], tid, n_all);
-      tell(&s.mass[rank], tid, m_all);
+    if (lane < WARPS) {
+      s.warp_count[lane] = n - n_own;
+      s.warp_mass[lane] = m - m_own;
     }
+    n = __shfl_sync(0xffffffffu, n, WARPS - 1);
+    m = __shfl_sync(0xffffffffu, m, WARPS - 1);
+    if (lane == 0) expect(&s.done[TOTALS], C * 16);
+    if (lane < C) send(s.total[rank], &s.done[TOTALS], lane, n, m);
   }
-  cluster_sync();
+  __syncthreads();
+  n_before += s.warp_count[warp];
+  before += s.warp_mass[warp];
+  wait_for(&s.done[TOTALS]);
   unsigned kept = 0;
   u64 kept_mass = 0;
+#pragma unroll
   for (int r = 0; r < C; ++r) {
     if (r < rank) {
-      n_before += s.count[r];
-      before += s.mass[r];
+      n_before += unsigned(s.total[r][0]);
+      before += s.total[r][1];
     }
-    kept += s.count[r];
-    kept_mass += s.mass[r];
+    kept += unsigned(s.total[r][0]);
+    kept_mass += s.total[r][1];
   }
 
-  // ---- top-k (every thread of the cluster takes the same branches)
-  const int64_t k_row = greedy ? 1 : p.top_k ? p.top_k[row] : p.top_k_all;
-  if (k_row > 0 && k_row < int64_t(kept)) {
-    kept = unsigned(k_row);
-    if (n_before < kept && kept <= n_before + n_here) {
-      unsigned left = kept - n_before;
-      u64 m = before;
+  // Three borders: of the first top_k tokens, of top_p of their weight, of u of the weight
+  // kept.  Each lies among the values of one thread of the cluster; in its warp, lane i < OWN
+  // looks at the thread's value i, and the one that has the border tells all CTAs.  (One
+  // loop and not three pieces of code: every instruction is fetched for one use.)
+  const bool cut_k = k_row > 0 && k_row < int64_t(kept), cut_p = !greedy && p_row < 1.f;
+  if (cut_k) kept = unsigned(k_row);
+#pragma unroll 1
+  for (int border = TOP_K; border <= PICK; ++border) {
+    u64 want = 0;  // the border lies behind this much weight (TOP_K: behind kept - 1 tokens)
+    if (border == TOP_K) {
+      if (!cut_k) continue;
+      if (tid == 0) expect(&s.done[TOP_K], 8);
+    } else if (border == LIMITS) {
+      if (!cut_p && !(min_p > 0.0)) continue;
+      if (tid == 0) expect(&s.done[LIMITS], (cut_p ? 16 : 0) + (min_p > 0.0 ? 16 * C : 0));
+      want = max(u64(1), min(kept_mass, u64(ceil(fmax(double(p_row), 0.0) * double(kept_mass))))) - 1;
+      if (min_p > 0.0) {  // where the first value stands that is too light
+        const unsigned n = light ? n_before + n_heavy : NONE;
+        const unsigned least = __reduce_min_sync(0xffffffffu, n);
+        if (lane == 0) atomicMin(&s.m_here, least);
+        __syncthreads();
+        if (s.m_here == NONE ? tid == 0 : light && n == s.m_here)
+#pragma unroll 1
+          for (int r = 0; r < C; ++r) send(s.m_run[rank], &s.done[LIMITS], r, n, before + mass_heavy);
+      }
+    } else {
+      if (tid == 0) expect(&s.done[PICK], 8);
+      const double x = u_row > 0.f ? double(u_row) * double(kept_mass) : 0.0;
+      want = x < double(kept_mass) ? min(u64(x), kept_mass - 1) : kept_mass - 1;
+    }
+    bool here = before <= want && want < before + mass_here;
+    if (border == TOP_K) here = n_before < kept && kept <= n_before + n_here;
+    if (border == LIMITS) here = here && cut_p;
+    const unsigned who = __ballot_sync(0xffffffffu, here);
+    if (who) {
+      const int o = __ffs(who) - 1;
+      const unsigned from = __shfl_sync(0xffffffffu, first, o);
+      unsigned count = 0;
+      double w, ratio;
+      weights.start(from, w, ratio);
 #pragma unroll
       for (int i = 0; i < OWN; ++i) {
-        const unsigned take = min(left, c[i]);
-        if (take) m += take * fixed(weights.of(first + i));
-        left -= take;
+        const unsigned t = __shfl_sync(0xffffffffu, c[i], o);
+        if (lane == i) count = t;
+        if (i <= lane) weights.next(from, from + i, ratio, w);
       }
-      for (int r = 0; r < C; ++r) tell(&s.k_mass, r, m);
-    }
-    cluster_sync();
-    kept_mass = s.k_mass;
-  }
-
-  // ---- top-p and min-p
-  if (!greedy && (p_row < 1.f || min_p > 0.0)) {
-    if (p_row < 1.f) {
-      const u64 want = max(u64(1), min(kept_mass, u64(ceil(fmax(double(p_row), 0.0) * double(kept_mass)))));
-      if (before < want && want <= before + mass_here) {
-        unsigned n = n_before;
-        u64 m = before;
-        bool found = false;
+      const u64 each = count ? fixed(w) : 0;
+      unsigned n = count;
+      u64 m = count * each;
 #pragma unroll
-        for (int i = 0; i < OWN; ++i)
-          if (c[i] && !found) {
-            const u64 w = fixed(weights.of(first + i));
-            found = want <= m + c[i] * w;
-            const unsigned take = found ? unsigned((want - m + w - 1) / w) : c[i];
-            n += take;
-            m += take * w;
-          }
-        for (int r = 0; r < C; ++r) {
-          tell(&s.p_n, r, n);
-          tell(&s.p_mass, r, m);
+      for (int i = 1; i < OWN; i <<= 1) {
+        const unsigned n2 = __shfl_up_sync(0xffffffffu, n, i);
+        const u64 m2 = __shfl_up_sync(0xffffffffu, m, i);
+        if (lane >= i) {
+          n += n2;
+          m += m2;
         }
       }
-    }
-    if (min_p > 0.0) {  // where the first value stands that is too light
-      unsigned n = n_before;
-      u64 m = before;
-      bool found = false;
+      n += __shfl_sync(0xffffffffu, n_before, o) - count;  // before this lane's value
+      m += __shfl_sync(0xffffffffu, before, o) - count * each;
+      const bool found = border == TOP_K ? n < kept && kept <= n + count : m <= want && want < m + count * each;
+      const int f = __ffs(__ballot_sync(0xffffffffu, found)) - 1;
+      // the tokens of the value before the border: want less m in units of its weight (a count
+      // is below 2^19, so the quotient in fp32 is off by one at most)
+      unsigned nth = kept - n;
+      if (border != TOP_K && found) {
+        const u64 x = want - m;
+        nth = unsigned(__fdividef(float(x), float(each)));
+        if (nth * each > x) --nth;
+        if ((nth + 1) * each <= x) ++nth;
+      }
+      const unsigned place = from + f;
+      n = __shfl_sync(0xffffffffu, n, f);
+      nth = __shfl_sync(0xffffffffu, nth, f);
+      const u64 upto = __shfl_sync(0xffffffffu, m + nth * each, f), one = __shfl_sync(0xffffffffu, each, f);
+      // lane r tells CTA r
+      if (border == TOP_K) {
+        if (lane < C) send(&s.k_mass, &s.done[TOP_K], lane, upto);
+      } else if (border == LIMITS) {
+        if (lane < C) send(s.p_run, &s.done[LIMITS], lane, n + nth + 1, upto + one);
+      } else {  // the CTA that holds the token learns which, the others that it is not theirs
+        uint32_t mine = 0;
+        if (lane < C) {
+          asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(mine) : "r"(at_rank(hist + (place >> 1), lane)) : "memory");
+          mine = place & 1 ? mine >> 16 : mine & 0xFFFFu;
+        }
+        unsigned all = mine;
 #pragma unroll
-      for (int i = 0; i < OWN; ++i)
-        if (c[i] && !found) {
-          const double w = weights.of(first + i);
-          found = !(w >= min_p);
-          if (!found) {
-            n += c[i];
-            m += c[i] * fixed(w);
-          }
+        for (int i = 1; i < C; i <<= 1) {
+          const unsigned t = __shfl_up_sync(0xffffffffu, all, i);
+          if (lane >= i) all += t;
         }
-      if (!found) n = NONE;
-      const unsigned least = __reduce_min_sync(0xffffffffu, n);
-      if (lane == 0) atomicMin(&s.m_here, least);
-      __syncthreads();
-      if (found && n == s.m_here)
-        for (int r = 0; r < C; ++r) {
-          tell(&s.m_n[rank], r, n);
-          tell(&s.m_mass[rank], r, m);
+        const bool holds = all - mine <= nth && nth < all;
+        if (lane < C) send(&s.pick, &s.done[PICK], lane, holds ? u64(nth - (all - mine)) << 32 | place : u64(NONE));
+        if (lane == 0) {
+          const double away = place == weights.place ? 0.0 : (value_at(place) - weights.top) * weights.scale * 0.69314718055994530942;
+          p.logprobs[row] = float(away - log(double(kept_mass) / double(u64(1) << FRAC)));
         }
-    }
-    cluster_sync();
-    if (s.p_n < kept) kept = s.p_n, kept_mass = s.p_mass;
-    for (int r = 0; r < C; ++r)
-      if (s.m_n[r] < kept) kept = s.m_n[r], kept_mass = s.m_mass[r];
-  }
-
-  // ---- draw: whoever owns the border finds the value, its number among the equal
-  // ones, and the CTA whose slice holds it
-  {
-    const float u_row = p.u[row];
-    const double x = u_row > 0.f ? double(u_row) * double(kept_mass) : 0.0;
-    const u64 want = x < double(kept_mass) ? min(u64(x), kept_mass - 1) : kept_mass - 1;
-    if (before <= want && want < before + mass_here) {
-      u64 m = before;
-      unsigned place = 0, nth = 0;
-      bool found = false;
-#pragma unroll
-      for (int i = 0; i < OWN; ++i)
-        if (c[i] && !found) {
-          const u64 w = fixed(weights.of(first + i));
-          if (want < m + c[i] * w) {
-            found = true;
-            place = first + i;
-            nth = unsigned((want - m) / w);
-          }
-          m += c[i] * w;
-        }
-      p.logprobs[row] = float(weights.log_of(place) - log(double(kept_mass) / double(u64(1) << FRAC)));
-      for (int r = 0; r < C; ++r) {
-        uint32_t w;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(w) : "r"(at_rank(hist + (place >> 1), r)) : "memory");
-        const unsigned there = place & 1 ? w >> 16 : w & 0xFFFFu;
-        if (nth < there) {
-          tell(&s.pick_nth, r, nth);
-          tell(&s.pick, r, place);
-          break;
-        }
-        nth -= there;
       }
     }
+    if (border == PICK) break;
+    wait_for(&s.done[border]);
+    if (border == TOP_K) kept_mass = s.k_mass;
+    if (border == LIMITS) {
+      if (cut_p && s.p_run[0] < kept) kept = unsigned(s.p_run[0]), kept_mass = s.p_run[1];
+      if (min_p > 0.0)
+#pragma unroll 1
+        for (int r = 0; r < C; ++r)
+          if (s.m_run[r][0] < kept) kept = unsigned(s.m_run[r][0]), kept_mass = s.m_run[r][1];
+    }
   }
-  cluster_sync();
-  const unsigned pick = s.pick;
+  wait_for(&s.done[PICK]);
+  const unsigned pick = unsigned(s.pick);
   if (pick == NONE) return;
-  // ---- the pick_nth-th logit of that value in the slice, in index order: a warp counts a
-  // run of it, the warp that holds the one looks again
-  const unsigned nth = s.pick_nth;
-  const int run = (len + THREADS - 1) / THREADS * 32;
-  const int begin = min(len, warp * run), end = min(len, begin + run);
-  unsigned n = 0;
-  for (int i = begin + lane; i < end; i += 32) n += place_of(__ldcg(slice + i)) == pick;
-  n = __reduce_add_sync(0xffffffffu, n);
+  // ---- the logit of that value and number in the slice, in index order: counted in runs
+  // of 256 logits (a load of a warp), then within the run that holds it
+  const unsigned bits = (pick & 0x8000u) ? pick : 0x7FFFu - pick;
+  const unsigned pattern = bits | bits << 16, ignore = bits ? ~0u : 0x7FFF7FFFu;  // the zeros' sign does not count
+  auto matches = [&](int group) {
+    const uint4 v = slice[group];
+    const unsigned w[4] = {v.x, v.y, v.z, v.w};
+    unsigned mask = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const unsigned t = (w[e] & ignore) ^ pattern;
+      mask |= (t & 0xFFFFu ? 0u : 1u << 2 * e) | (t >> 16 ? 0u : 2u << 2 * e);
+    }
+    return mask;
+  };
+#pragma unroll 2
+  for (int i = tid; i - lane < groups; i += THREADS) {
+    const unsigned n = __reduce_add_sync(0xffffffffu, i < groups ? __popc(matches(i)) : 0u);
+    if (lane == 0) s.run[i / 32] = n;
+  }
   __syncthreads();
-  if (lane == 0) s.warp_count[warp] = n;
+  const int runs = (groups + 31) / 32;
+  if (warp == 0) {
+    unsigned left = unsigned(s.pick >> 32);
+    for (int i = 0; i < runs; i += 32) {
+      unsigned upto = i + lane < runs ? s.run[i + lane] : 0u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned t = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += t;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, left < upto);
+      if (past) {
+        const int r = __ffs(past) - 1;
+        const unsigned ahead = r ? __shfl_sync(0xffffffffu, upto, r ? r - 1 : 0) : 0u;
+        if (lane == 0) {
+          s.found = i + r;
+          s.found_nth = left - ahead;
+        }
+        break;
+      }
+      left -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
   __syncthreads();
-  unsigned ahead = 0;
-  for (int w = 0; w < warp; ++w) ahead += s.warp_count[w];
-  if (nth < ahead || nth >= ahead + n) return;
-  for (int i = begin; i < end; i += 32) {
-    const bool is = i + lane < end && place_of(__ldcg(slice + i + lane)) == pick;
-    const unsigned all = __ballot_sync(0xffffffffu, is);
-    if (is && ahead + __popc(all & ((1u << lane) - 1)) == nth) p.tokens[row] = int64_t(rank) * p.slice + i + lane;
-    ahead += __popc(all);
+  if (warp != 0) return;
+  const int group = int(s.found) * 32 + lane;
+  unsigned mask = group < groups ? matches(group) : 0u;
+  unsigned upto = __popc(mask);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned t = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += t;
+  }
+  const unsigned ahead = upto - __popc(mask), nth = s.found_nth;
+  if (nth >= ahead && nth < upto) {
+    for (unsigned k = ahead; k < nth; ++k) mask &= mask - 1;
+    p.tokens[row] = 8 * int64_t(first_group + group) - logits.shift + __ffs(mask) - 1;
   }
 }
 
 template <int C>
-int launch(const Params& p, int batch, cudaStream_t st) {
-  constexpr int SMEM = HIST_BYTES + int(sizeof(Shared<C>));
+constexpr int smem_bytes(int slice) {
+  return HIST_BYTES + 2 * slice + int(sizeof(Shared<C>));
+}
+inline int slice_of(int vocab, int c) {  // (a row may begin up to 7 places into a group of 8)
+  return ((vocab + 7 + c - 1) / c + 255) / 256 * 256;
+}
+
+struct Launch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+};
+template <int C>
+void configure(Launch& l, int slice, int batch, cudaStream_t st) {
+  l.cfg.gridDim = dim3(unsigned(batch) * C);
+  l.cfg.blockDim = dim3(THREADS);
+  l.cfg.dynamicSmemBytes = size_t(smem_bytes<C>(slice));
+  l.cfg.stream = st;
+  l.at[0].id = cudaLaunchAttributeClusterDimension;
+  l.at[0].val.clusterDim.x = C;
+  l.at[0].val.clusterDim.y = l.at[0].val.clusterDim.z = 1;
+  l.at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  l.at[1].val.programmaticStreamSerializationAllowed = 1;
+  l.cfg.attrs = l.at;
+  l.cfg.numAttrs = g_pdl_enabled.load(std::memory_order_relaxed) ? 2 : 1;
+}
+
+// Prepares the kernel on the current device, once; how many clusters run on it at the same time.
+template <int C>
+int prepare(int* clusters) {
+  static_assert(smem_bytes<C>(SLICE_MAX) <= 227 * 1024, "shared memory of the largest slice");
   static std::mutex mu;
-  static bool done[64] = {};
+  static int fit[64] = {};
   int dev = 0;
   QX_CUDA_TRY(cudaGetDevice(&dev), "sample_logits: cudaGetDevice");
   QX_REQUIRE(dev >= 0 && dev < 64, "sample_logits: device index %d unsupported", dev);
-  {
-    std::lock_guard<std::mutex> lk(mu);
-    if (!done[dev]) {
-      QX_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM),
-                  "sample_logits: set smem limit");
-      done[dev] = true;
-    }
+  std::lock_guard<std::mutex> lk(mu);
+  if (fit[dev] == 0) {
+    QX_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<C>(SLICE_MAX)),
+                "sample_logits: set smem limit");
+    if (C > 8)
+      QX_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<C>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+                  "sample_logits: allow clusters of 16");
+    Launch l;
+    configure<C>(l, SLICE_MAX, 1, nullptr);
+    l.cfg.numAttrs = 1;
+    QX_CUDA_TRY(cudaOccupancyMaxActiveClusters(&fit[dev], sample_kernel<C>, &l.cfg), "sample_logits: clusters on the device");
+    if (fit[dev] == 0) fit[dev] = -1;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(batch) * C);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = g_pdl_enabled.load(std::memory_order_relaxed) ? 2 : 1;
-  QX_CUDA_TRY(cudaLaunchKernelEx(&cfg, sample_kernel<C>, p), "sample_logits: launch");
+  *clusters = fit[dev];
+  return QX_OK;
+}
+
+template <int C>
+int launch(Params& p, int batch, cudaStream_t st) {
+  p.slice = slice_of(p.vocab, C);
+  Launch l;
+  configure<C>(l, p.slice, batch, st);
+  QX_CUDA_TRY(cudaLaunchKernelEx(&l.cfg, sample_kernel<C>, p), "sample_logits: launch");
   return check_launch("sample_logits");
 }
 
+// The largest cluster with which the whole batch runs at once (7 rows by 16 CTAs, 15 by 8, 32 by 4 on a B200 of 148
+// SMs), else 4.  Measured at 151936 tokens, us by 16 / 8 / 4 CTAs: 1 row 13.6 / 14.3 / 17.4,
+// 8 rows 25.6 / 14.9 / 18.1, 16 rows 38 / 27 / 18.3, 64 rows 123 / 65 / 36.
+int choose(Params& p, int batch, cudaStream_t st) {
+  int at16 = 0, at8 = 0, at4 = 0;
+  if (const int rc = prepare<16>(&at16); rc != QX_OK) return rc;
+  if (const int rc = prepare<8>(&at8); rc != QX_OK) return rc;
+  if (const int rc = prepare<4>(&at4); rc != QX_OK) return rc;
+  if (batch <= at16 || slice_of(p.vocab, 8) > SLICE_MAX) return launch<16>(p, batch, st);
+  if (batch <= at8 || slice_of(p.vocab, 4) > SLICE_MAX) return launch<8>(p, batch, st);
+  return launch<4>(p, batch, st);
+}
+
 }  // namespace smp
+
+int sample_device_error(unsigned* code, int reset) {
+  QX_CUDA_TRY(cudaMemcpyFromSymbol(code, smp::g_sample_error, sizeof(unsigned)), "get_device_error: read");
+  if (reset) {
+    const unsigned zero = 0;
+    QX_CUDA_TRY(cudaMemcpyToSymbol(smp::g_sample_error, &zero, sizeof(unsigned)), "get_device_error: reset");
+  }
+  return QX_OK;
+}
+
 }  // namespace qx
 
 using namespace qx;
@@ -425,10 +727,9 @@ extern "C" int qx_sample_logits(const void* logits, const float* u, const float*
                                 const float* top_p, const float* min_p, float temperature_all, int64_t top_k_all,
                                 float top_p_all, float min_p_all, int64_t* tokens, float* logprobs, int batch, int vocab,
                                 qx_stream_t stream) {
-  constexpr int C = 8;
   QX_REQUIRE(batch >= 0 && vocab > 0, "sample_logits: bad sizes batch=%d vocab=%d", batch, vocab);
-  QX_REQUIRE(vocab <= C * smp::SLICE_MAX, "sample_logits: vocab=%d is above %d", vocab, C * smp::SLICE_MAX);
-  QX_REQUIRE(int64_t(batch) * C <= 0x7fffffffLL, "sample_logits: batch=%d is too large", batch);
+  QX_REQUIRE(vocab <= smp::VOCAB_MAX, "sample_logits: vocab=%d is above %d", vocab, smp::VOCAB_MAX);
+  QX_REQUIRE(batch <= 0x7fffffff / 16, "sample_logits: batch=%d is too large", batch);
   if (batch == 0) return QX_OK;
   QX_REQUIRE(logits && u && tokens && logprobs, "sample_logits: null pointer");
   QX_REQUIRE(aligned(logits, 2) && aligned(u, 4) && aligned(temperature, 4) && aligned(top_k, 8) && aligned(top_p, 4) &&
@@ -448,6 +749,5 @@ extern "C" int qx_sample_logits(const void* logits, const float* u, const float*
   p.tokens = tokens;
   p.logprobs = logprobs;
   p.vocab = vocab;
-  p.slice = ((vocab + C - 1) / C + 7) / 8 * 8;
-  return smp::launch<C>(p, batch, reinterpret_cast<cudaStream_t>(stream));
+  return smp::choose(p, batch, reinterpret_cast<cudaStream_t>(stream));
 }
