@@ -1322,6 +1322,7 @@ int nvar_device_error(unsigned* code, int reset);      // nvlink_allreduce.cu
 int attn_device_error(unsigned* code, int reset);      // decode_attn.cu
 int prefill4_device_error(unsigned* code, int reset);  // prefill_attn_q4.cu
 int sample_device_error(unsigned* code, int reset);    // sample.cu
+int lora_device_error(unsigned* code, int reset);      // multi_lora.cu
 }
 
 extern "C" int qx_get_device_error(unsigned* code, int reset) {
@@ -1347,6 +1348,9 @@ extern "C" int qx_get_device_error(unsigned* code, int reset) {
   if (rc != QX_OK) return rc;
   *code |= other;
   rc = qx::sample_device_error(&other, reset);
+  if (rc != QX_OK) return rc;
+  *code |= other;
+  rc = qx::lora_device_error(&other, reset);
   if (rc != QX_OK) return rc;
   *code |= other;
   return QX_OK;
