@@ -41,6 +41,7 @@ struct Params {
   int edge[MAX_PARTS + 1];  // first column of each block, then N
   int chunks;               // clusters of a sequence: the chunks that may start in it
   int k_slice, k_step;      // K of a CTA, and of one of its steps (multiples of 16)
+  int width;                // columns of a CTA
   int a_pitch;              // bytes of a staged row of A: an odd number of 16-byte units
 };
 
@@ -171,36 +172,48 @@ __device__ __forceinline__ int part_of(const Params& p, int column) {
 // 8 rows a chunk.  h^T [P r][8] = A^T x^T by mma.sync with A as the 16-row operand (its
 // rows are the ranks) and the chunk's rows as the 8 columns: an instruction covers
 // 16 ranks x 16 of K for every row.  Then thread by thread 4 columns of a row in fp32.
+// Bound by the weights' bytes where every row has its own adapter, else by the chain of
+// latencies: adapters, A, x, the exchange, y.
 namespace few {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int ROWS = 8;
 constexpr int A_BYTES = 25600;   // a step's rows of A
-constexpr int B_BYTES = 16384;   // a step's columns of B
+constexpr int B_BYTES = 32768;   // a step's columns of B
 constexpr int MAX_STEP = 512;    // K of a step
 
 struct Layout {
-  int a, x, b, part, recv, h, total;  // byte offsets
-  int x_pitch, b_columns, steps;
+  int a, a_step, x, x_step, b[2], part, recv, h, done, total;  // byte offsets, bytes of a buffer
+  int x_pitch, steps, a_shift, b_shift;  // a row of A in 2^a_shift threads; a step of B has 2^b_shift 4-column pieces
 };
-__host__ __device__ inline Layout layout(const Params& p) {
+__host__ __device__ inline int log2_up(int v) {
+  int s = 0;
+  while (1 << s < v) ++s;
+  return s;
+}
+inline Layout layout(const Params& p) {
   Layout l;
   l.steps = (p.k_slice + p.k_step - 1) / p.k_step;
   l.x_pitch = p.k_step * 2 + 16;
-  l.b_columns = B_BYTES / (2 * p.rank) / 8 * 8;
+  l.a_shift = log2_up(p.ranks / 8);
+  l.b_shift = std::min(log2_up(B_BYTES / (8 * p.rank) + 1) - 1, log2_up(p.width / 4));  // the largest that fits and is of use
   const int buffers = l.steps > 1 ? 2 : 1;
   int at = 0;
-  l.a = at, at += buffers * (p.k_step * p.a_pitch + 16);  // + 16: the last tile of 16 ranks may end past the last row
-  l.x = at, at += buffers * ROWS * l.x_pitch;
-  l.b = at, at += 2 * B_BYTES;
-  l.part = at, at += 8 * 16 * ROWS * 4 > p.ranks * 2 * ROWS * 4 ? 8 * 16 * ROWS * 4 : p.ranks * 2 * ROWS * 4;
+  l.a = at, l.a_step = p.k_step * p.a_pitch + 16;  // + 16: the last tile of 16 ranks may end past the last row
+  // when h is done, A's place takes every other step of B
+  l.b[1] = at, at += buffers * l.a_step > B_BYTES ? buffers * l.a_step : B_BYTES;
+  l.b[0] = at, at += B_BYTES;
+  l.x = at, l.x_step = ROWS * l.x_pitch, at += buffers * l.x_step;
+  l.part = at, at += 8 * 16 * ROWS * 4 > p.ranks * ROWS * 4 ? 8 * 16 * ROWS * 4 : p.ranks * ROWS * 4;
   l.recv = at, at += C * p.ranks * ROWS * 4;
   l.h = at, at += p.ranks * ROWS * 4;
+  l.done = at, at += 16;
   l.total = at;
   return l;
 }
 
-__global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __grid_constant__ Params p,
+                                                                     const __grid_constant__ Layout l) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int rows[ROWS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -214,8 +227,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
     return;
   }
   // this CTA's columns
-  const int width = ((p.N + C - 1) / C + 7) / 8 * 8;
-  const int n0 = min(p.N, rank * width), n1 = min(p.N, n0 + width);
+  const int n0 = min(p.N, rank * p.width), n1 = min(p.N, n0 + p.width);
   if (a < 0) {  // no adapter: the rows as they are
     pdl_wait();
     for (int m = 0; m < n; ++m) {
@@ -225,47 +237,58 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
     }
     return;
   }
-  cluster_arrive();
-  const Layout l = layout(p);
   const uint32_t base = smem_u32(smem);
-  const int k0 = rank * p.k_slice;
+  if (tid == 0) {
+    bar_init(base + l.done);
+    bar_expect(base + l.done, C * p.ranks * ROWS * 4);
+  }
+  __syncthreads();
+  cluster_arrive();
+  const int k0 = rank * p.k_slice, k_end = min(p.K, k0 + p.k_slice);
   const int units = p.ranks / 8;  // 16-byte units of a row of A
   auto load_a = [&](int step) {
-    if (step >= l.steps) return;
-    const uint32_t to = base + l.a + (step & 1) * (p.k_step * p.a_pitch + 16);
+    const int c = tid & ((1 << l.a_shift) - 1);
+    if (step >= l.steps || c >= units) return;
+    int kk = tid >> l.a_shift;
     const int k = k0 + step * p.k_step;
-    const __half* from = p.A + (a * p.K + k) * p.ranks;
-    for (int i = tid; i < p.k_step * units; i += THREADS) {
-      const int kk = i / units, c = i - kk * units;
-      const bool ok = k + kk < p.K && step * p.k_step + kk < p.k_slice;
-      copy16(to + kk * p.a_pitch + c * 16, ok ? from + i * 8 : p.A, ok);
+    uint32_t to = base + l.a + (step & 1) * l.a_step + kk * p.a_pitch + c * 16;
+    const __half* from = p.A + (a * p.K + k + kk) * p.ranks + c * 8;
+    const int down = THREADS >> l.a_shift;
+    for (; kk < p.k_step; kk += down) {
+      const bool ok = k + kk < k_end;
+      copy16(to, ok ? from : p.A, ok);
+      to += down * p.a_pitch;
+      from += down * p.ranks;
     }
   };
-  auto load_x = [&](int step) {
+  auto load_x = [&](int step) {  // a warp a row
     if (step >= l.steps) return;
-    const uint32_t to = base + l.x + (step & 1) * ROWS * l.x_pitch;
-    const int k = k0 + step * p.k_step, per_row = p.k_step / 8;
-    for (int i = tid; i < ROWS * per_row; i += THREADS) {
-      const int m = i / per_row, c = i - m * per_row;
-      const bool ok = m < n && k + 8 * c < p.K && step * p.k_step + 8 * c < p.k_slice;
-      copy16(to + m * l.x_pitch + c * 16, ok ? p.x + int64_t(rows[m]) * p.K + k + 8 * c : p.x, ok);
+    const int k = k0 + step * p.k_step;
+    const uint32_t to = base + l.x + (step & 1) * l.x_step + warp * l.x_pitch;
+    const __half* from = p.x + int64_t(rows[warp]) * p.K + k;
+    for (int c = lane * 8; c < p.k_step; c += 256) {
+      const bool ok = warp < n && k + c < k_end;
+      copy16(to + c * 2, ok ? from + c : p.x, ok);
     }
   };
-  const int b_steps = (n1 - n0 + l.b_columns - 1) / l.b_columns;
+  const int columns = 4 << l.b_shift;  // of a step of B
   auto load_b = [&](int step) {
-    if (step >= b_steps) return;
-    const uint32_t to = base + l.b + (step & 1) * B_BYTES;
-    const int c0 = n0 + step * l.b_columns, per_row = min(l.b_columns, n1 - c0) / 8;
-    const __half* from = p.B + a * p.rank * p.N + c0;
-    for (int i = tid; i < p.rank * per_row; i += THREADS) {
-      const int j = i / per_row, c = i - j * per_row;
-      copy16(to + (j * l.b_columns + c * 8) * 2, from + int64_t(j) * p.N + c * 8, true);
+    const int eighths = l.b_shift - 1;  // log2 of 8-column pieces
+    const int c = tid & ((1 << eighths) - 1), column = n0 + step * columns + c * 8;
+    if (column >= n1) return;
+    int j = tid >> eighths;
+    uint32_t to = base + l.b[step & 1] + (j * columns + c * 8) * 2;
+    const __half* from = p.B + (a * p.rank + j) * p.N + column;
+    const int down = THREADS >> eighths;  // (a step has at most 256 pieces of 8: its ranks are 8 or more)
+    for (; j < p.rank; j += down) {
+      copy16(to, from, true);
+      to += down * columns * 2;
+      from += int64_t(down) * p.N;
     }
   };
   load_a(0);
   load_a(1);
   load_b(0);
-  load_b(1);
   copy_commit();
   const float scale = p.scales[a];
   pdl_wait();
@@ -282,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
   for (int step = 0; step < l.steps; ++step) {
     copy_wait<1>();
     __syncthreads();
-    const uint32_t as = base + l.a + (step & 1) * (p.k_step * p.a_pitch + 16), xs = base + l.x + (step & 1) * ROWS * l.x_pitch;
+    const uint32_t as = base + l.a + (step & 1) * l.a_step, xs = base + l.x + (step & 1) * l.x_step;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int item = warp + WARPS * i, tile = item % tiles, share = item / tiles;
@@ -304,6 +327,10 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
     }
     copy_commit();
   }
+  // a step of B that has landed stays where it is; the next takes A's place
+  const int b_steps = (n1 - n0 + columns - 1) / columns;
+  load_b(1);
+  copy_commit();
   float* const part = reinterpret_cast<float*>(smem + l.part);  // [share][ranks][8]
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -325,13 +352,18 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
       const float4 o = reinterpret_cast<const float4*>(part)[s * p.ranks * 2 + v];
       sum.x += o.x, sum.y += o.y, sum.z += o.z, sum.w += o.w;
     }
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
                      at_rank(base + l.recv + (rank * p.ranks * 2 + v) * 16, r)),
-                 "f"(sum.x), "f"(sum.y), "f"(sum.z), "f"(sum.w)
+                 "f"(sum.x), "f"(sum.y), "f"(sum.z), "f"(sum.w), "r"(at_rank(base + l.done, r))
                  : "memory");
   }
-  cluster_arrive();
-  cluster_wait();
+  // thread's first piece of the columns: item (row, 4 columns) of a step
+  auto read_y = [&](int step, int item) {
+    const int m = item >> l.b_shift, c = n0 + step * columns + (item & ((1 << l.b_shift) - 1)) * 4;
+    return m < n && c < n1 ? __ldcg(reinterpret_cast<const uint2*>(p.y + int64_t(rows[m]) * p.N + c)) : make_uint2(0u, 0u);
+  };
+  uint2 y = read_y(0, tid);
+  bar_wait(base + l.done);
   float* const h = reinterpret_cast<float*>(smem + l.h);  // [ranks][8]
   {
     const float* recv = reinterpret_cast<const float*>(smem + l.recv);
@@ -346,31 +378,36 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
   for (int step = 0; step < b_steps; ++step) {
     copy_wait<1>();
     __syncthreads();
-    const __half* const w = reinterpret_cast<const __half*>(smem + l.b + (step & 1) * B_BYTES);
-    const int c0 = n0 + step * l.b_columns, fours = min(l.b_columns, n1 - c0) / 4;
-    for (int i = tid; i < fours * n; i += THREADS) {
-      const int m = i / fours, c = (i - m * fours) * 4;
-      const int64_t at = int64_t(rows[m]) * p.N + c0 + c;
-      const uint2 yv = __ldcg(reinterpret_cast<const uint2*>(p.y + at));
-      const float* hm = h + part_of(p, c0 + c) * p.rank * ROWS + m;
+    const __half* const w = reinterpret_cast<const __half*>(smem + l.b[step & 1]);
+    const int items = n << l.b_shift;
+    for (int i = tid; i < items; i += THREADS) {
+      const uint2 yv = y;
+      y = i + THREADS < items ? read_y(step, i + THREADS) : read_y(step + 1, tid);
+      const int m = i >> l.b_shift, c = (i & ((1 << l.b_shift) - 1)) * 4, column = n0 + step * columns + c;
+      if (column >= n1) continue;
+      const float* hm = h + part_of(p, column) * p.rank * ROWS + m;
+      const __half* wc = w + c;
       float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll 8
       for (int j = 0; j < p.rank; ++j) {
-        const uint2 bw = *reinterpret_cast<const uint2*>(w + j * l.b_columns + c);
+        const uint2 bw = *reinterpret_cast<const uint2*>(wc);
         const float2 b01 = h2_to_f2(bw.x), b23 = h2_to_f2(bw.y);
         const float hv = hm[j * ROWS];
         s0 = fmaf(hv, b01.x, s0);
         s1 = fmaf(hv, b01.y, s1);
         s2 = fmaf(hv, b23.x, s2);
         s3 = fmaf(hv, b23.y, s3);
+        wc += columns;
       }
       const float2 y01 = h2_to_f2(yv.x), y23 = h2_to_f2(yv.y);
       const __half2 o01 = __floats2half2_rn(y01.x + s0, y01.y + s1), o23 = __floats2half2_rn(y23.x + s2, y23.y + s3);
-      *reinterpret_cast<uint2*>(p.out + at) =
+      *reinterpret_cast<uint2*>(p.out + int64_t(rows[m]) * p.N + column) =
           make_uint2(*reinterpret_cast<const uint32_t*>(&o01), *reinterpret_cast<const uint32_t*>(&o23));
     }
-    __syncthreads();
-    if (step + 2 < b_steps) load_b(step + 2);
+    if (step + 2 < b_steps) {
+      __syncthreads();
+      load_b(step + 2);
+    }
     copy_commit();
   }
 }
@@ -453,8 +490,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
   pdl_wait();
   if (n == 0) return;  // (every CTA of the cluster)
   if (a < 0) {         // no adapter: the rows as they are
-    const int width = ((p.N + C - 1) / C + 7) / 8 * 8;
-    const int n0 = min(p.N, rank * width), n1 = min(p.N, n0 + width);
+    const int n0 = min(p.N, rank * p.width), n1 = min(p.N, n0 + p.width);
     for (int m = warp; m < n; m += WARPS) {
       const int64_t at = int64_t(rows[m]) * p.N;
       for (int c = n0 + 8 * lane; c < n1; c += 8 * 32)
@@ -825,7 +861,8 @@ bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
 constexpr int FEW_TOKENS = 8;  // tokens of a sequence up to which 8-row chunks do them
 
 // one cluster of C CTAs for every chunk that may start in a sequence
-int launch(void (*kernel)(Params), int threads, const Params& p, int smem, cudaStream_t st) {
+template <typename... Args>
+int launch(void (*kernel)(Args...), int threads, const Params& p, int smem, cudaStream_t st, Args... args) {
   static std::mutex mu;
   static bool done[64] = {};
   int dev = 0;
@@ -835,11 +872,13 @@ int launch(void (*kernel)(Params), int threads, const Params& p, int smem, cudaS
     std::lock_guard<std::mutex> lk(mu);
     if (!done[dev]) {
       using namespace many;
-      for (auto k : {few::multi_lora_rows_kernel, multi_lora_tile_kernel<0, 64>, multi_lora_tile_kernel<1, 64>,
-                     multi_lora_tile_kernel<2, 64>, multi_lora_tile_kernel<4, 64>, multi_lora_tile_kernel<1, 32>,
-                     multi_lora_tile_kernel<2, 32>, multi_lora_tile_kernel<4, 32>})
-        QX_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM),
-                    "multi_lora_add: set smem limit");
+      const char* what = "multi_lora_add: set smem limit";
+      constexpr cudaFuncAttribute limit = cudaFuncAttributeMaxDynamicSharedMemorySize;
+      QX_CUDA_TRY(cudaFuncSetAttribute(few::multi_lora_rows_kernel, limit, MAX_SMEM), what);
+      for (auto k : {multi_lora_tile_kernel<0, 64>, multi_lora_tile_kernel<1, 64>, multi_lora_tile_kernel<2, 64>,
+                     multi_lora_tile_kernel<4, 64>, multi_lora_tile_kernel<1, 32>, multi_lora_tile_kernel<2, 32>,
+                     multi_lora_tile_kernel<4, 32>})
+        QX_CUDA_TRY(cudaFuncSetAttribute(k, limit, MAX_SMEM), what);
       done[dev] = true;
     }
   }
@@ -859,22 +898,22 @@ int launch(void (*kernel)(Params), int threads, const Params& p, int smem, cudaS
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = g_pdl_enabled.load(std::memory_order_relaxed) ? 2 : 1;
-  QX_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p), "multi_lora_add: launch");
+  QX_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...), "multi_lora_add: launch");
   return check_launch("multi_lora_add");
 }
 
 int launch_few(Params& p, cudaStream_t st) {
   using namespace few;
   p.chunks = (p.tokens + ROWS - 1) / ROWS;
-  p.k_slice = ((p.K + C - 1) / C + 15) / 16 * 16;
   const int most = std::min(MAX_STEP, A_BYTES / p.a_pitch / 16 * 16);
   const int steps = (p.k_slice + most - 1) / most;
   p.k_step = ((p.k_slice + steps - 1) / steps + 15) / 16 * 16;
-  return launch(multi_lora_rows_kernel, THREADS, p, layout(p).total, st);
+  const Layout l = layout(p);
+  return launch(multi_lora_rows_kernel, THREADS, p, l.total, st, p, l);
 }
 
 // Rows up to which chunks of 64 are 18 clusters at most, so that an SM has one CTA: then
-// chunks of 32.  Measured at 999 rows (rank 8, 2560 x 9728): 22.7 us with 64, LORA32 with 32.
+// chunks of 32.  Measured at 999 rows (rank 8, 2560 x 9728): 22.7 us with 64, 15.8 with 32.
 constexpr int SMALL_ROWS = 18 * 64;
 
 int launch_many(Params& p, cudaStream_t st) {
@@ -882,7 +921,6 @@ int launch_many(Params& p, cudaStream_t st) {
   const int ks = (p.rank + 15) / 16;
   const int rows = int64_t(p.batch) * p.tokens <= SMALL_ROWS && ks <= 4 ? 32 : 64;
   p.chunks = (p.tokens + rows - 1) / rows;
-  p.k_slice = ((p.K + C - 1) / C + 15) / 16 * 16;
   const int here = std::min(RANKS, p.ranks);
   p.a_pitch = here * 2 + (here / 8 % 2 ? 0 : 16);
   void (*kernel)(Params);
@@ -893,7 +931,7 @@ int launch_many(Params& p, cudaStream_t st) {
              : ks == 2 ? multi_lora_tile_kernel<2, 64>
              : ks <= 4 ? multi_lora_tile_kernel<4, 64>
                        : multi_lora_tile_kernel<0, 64>;
-  return launch(kernel, THREADS, p, layout(p, rows).total, st);
+  return launch(kernel, THREADS, p, layout(p, rows).total, st, p);
 }
 
 }  // namespace mlora
@@ -964,6 +1002,8 @@ extern "C" int qx_multi_lora_add(const void* y, const void* x, const void* lora_
   p.ranks = rank * p.parts;
   p.n = num_adapters;
   p.a_pitch = p.ranks * 2 + (p.ranks / 8 % 2 ? 0 : 16);
+  p.k_slice = ((K + C - 1) / C + 15) / 16 * 16;
+  p.width = ((N + C - 1) / C + 7) / 8 * 8;
   return tokens <= FEW_TOKENS ? launch_few(p, reinterpret_cast<cudaStream_t>(stream))
                               : launch_many(p, reinterpret_cast<cudaStream_t>(stream));
 }
