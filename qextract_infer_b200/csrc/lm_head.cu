@@ -2,9 +2,9 @@
 // this rank's vocabulary slice) and, per row, the largest logit and its index,
 // in two launches instead of a library GEMV, a reduction and an index add.
 //
-// Kernel 1: a CTA owns 256 vocabulary columns (4 warps x 64) for every row
+// Kernel 1: a CTA owns 128 vocabulary columns (4 warps x 32) for every row
 // (batch <= 32, one or two 16-row m-tiles).  64-row K tiles of W and of h are
-// staged by cp.async (double buffered); W fragments come from ldmatrix.trans,
+// staged by cp.async (three of them: 62 KB, three CTAs an SM); W fragments come from ldmatrix.trans,
 // h fragments from ldmatrix; mma.sync m16n8k16 with fp32 accumulation.  The
 // logits are rounded to fp16 (the values a fp16 GEMV stores), and the CTA's
 // per-row maximum with its smallest index is written to the workspace.
@@ -12,7 +12,14 @@
 // (ties go to the smallest index) and adds the slice's vocabulary offset.
 //
 // Whole logits (qx_lm_head_logits): kernel 1 with the fp16 values stored instead of
-// compared, 32 rows a launch.  Bound by the weights' bytes like the greedy head.
+// compared, 32 rows a launch.
+//
+// Bound by the weights' bytes.  Measured for 1 / 32 rows of 4096 x 151936 and 1 row of
+// 4096 x 37984 (us, tiles K x columns): 64 x 256 in two stages 189 / 222 / 59, 32 x 256 in
+// four 208 / 238 / 66, 64 x 128 in two 172 / 196 / 59, in three 171 / 188 / 54 (kept; 7.3
+// TB/s), in four (two CTAs an SM) 190 / 208 / 63.  The next kernel is let in at the end:
+// earlier, its CTAs fill the slots as they come free, three on one SM and one on another
+// (the slice: 54 us, 48 without).
 #include <algorithm>
 #include <cfloat>
 #include <mutex>
@@ -25,15 +32,17 @@ namespace lmh {
 
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
-constexpr int COLS = 256;                  // vocabulary columns per CTA
+constexpr int COLS = 128;                  // vocabulary columns per CTA
+constexpr int WCOLS = COLS / WARPS, NJ = WCOLS / 8;  // of a warp, in tiles of 8
 constexpr int KT = 64;                     // K rows per tile
 constexpr int MAXB = 32;                   // rows (two m-tiles)
-constexpr int WROW = COLS * 2;             // bytes of one W tile row (512)
-constexpr int W_TILE = KT * WROW;          // 32 KB
+constexpr int WROW = COLS * 2;             // bytes of one W tile row (256)
+constexpr int W_TILE = KT * WROW;          // 16 KB
 constexpr int HROW = KT * 2 + 16;          // bytes of one staged h row (+16: conflict-free ldmatrix)
 constexpr int H_TILE = MAXB * HROW;        // 4.5 KB
 constexpr int STAGE = W_TILE + H_TILE;
-constexpr int SMEM = 2 * STAGE;            // 2 stages
+constexpr int STAGES = 3;
+constexpr int SMEM = STAGES * STAGE;
 
 struct Cand {
   float v;
@@ -75,7 +84,6 @@ template <int MT, bool STORE>
 __global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restrict__ h, const __half* __restrict__ W,
                                                         int B, int H, int V, Cand* __restrict__ part,
                                                         __half* __restrict__ out) {
-  pdl_trigger();
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Cand s_best[WARPS][MAXB];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -86,10 +94,10 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restric
 
   auto issue = [&](int kt, int stage) {
     const uint32_t ws = sbase + stage * STAGE, hs = ws + W_TILE;
-    // W: 64 rows x 32 chunks of 16 B = 2048 chunks, 16 per thread
+    // W: 64 rows x 16 chunks of 16 B = 1024 chunks, 8 per thread
 #pragma unroll
     for (int i = 0; i < (KT * (COLS / 8)) / THREADS; ++i) {
-      const int idx = i * THREADS + tid, r = idx >> 5, ch = idx & 31;
+      const int idx = i * THREADS + tid, r = idx / (COLS / 8), ch = idx % (COLS / 8);
       const int col = n0 + ch * 8;
       const bool ok = col < V;  // V % 8 == 0: a chunk is all in or all out
       const __half* src = W + (size_t(kt) * KT + r) * V + (ok ? col : 0);
@@ -105,21 +113,23 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restric
     cp_async_commit();
   };
 
-  float acc[MT][8][4];
+  float acc[MT][NJ][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
+    for (int j = 0; j < NJ; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
 
   pdl_wait();  // h comes from the previous kernel
-  issue(0, 0);
-  if (ktiles > 1) issue(1, 1);
-  else cp_async_commit();
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) {
+    if (i < ktiles) issue(i, i);
+    else cp_async_commit();
+  }
   const int mi = lane >> 3, ri = lane & 7;
   for (int kt = 0; kt < ktiles; ++kt) {
-    cp_async_wait<1>();
+    cp_async_wait<STAGES - 1>();
     __syncthreads();
-    const uint32_t ws = sbase + (kt & 1) * STAGE, hs = ws + W_TILE;
+    const uint32_t ws = sbase + (kt % STAGES) * STAGE, hs = ws + W_TILE;
 #pragma unroll
     for (int ks = 0; ks < KT / 16; ++ks) {
       // A fragments (h rows m*16.., k ks*16..): matrices (rows 0-7 | 8-15) x (k 0-7 | 8-15)
@@ -127,11 +137,11 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restric
 #pragma unroll
       for (int m = 0; m < MT; ++m)
         ldsm_x4(a[m], hs + (m * 16 + (mi & 1) * 8 + ri) * HROW + (ks * 16 + (mi >> 1) * 8) * 2);
-      // B fragments: k16 x n8 of W for this warp's 8 n-tiles (two per ldmatrix.x4.trans)
+      // B fragments: k16 x n8 of W for this warp's n-tiles (two per ldmatrix.x4.trans)
 #pragma unroll
-      for (int jj = 0; jj < 4; ++jj) {
+      for (int jj = 0; jj < NJ / 2; ++jj) {
         uint32_t bw[4];
-        const int ch = (warp * 64 + jj * 16) / 8 + (mi >> 1);
+        const int ch = (warp * WCOLS + jj * 16) / 8 + (mi >> 1);
         ldsm_x4_t(bw, ws + wswz(ks * 16 + (mi & 1) * 8 + ri, ch));
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -141,10 +151,11 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restric
       }
     }
     __syncthreads();
-    if (kt + 2 < ktiles) issue(kt + 2, kt & 1);
+    if (kt + STAGES < ktiles) issue(kt + STAGES, kt % STAGES);
     else cp_async_commit();
   }
   cp_async_wait<0>();
+  pdl_trigger();
 
   if constexpr (STORE) {
 #pragma unroll
@@ -153,8 +164,8 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restric
       for (int hr = 0; hr < 2; ++hr) {  // rows g and g + 8 of the m-tile
         const int row = m * 16 + g + hr * 8;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int col = n0 + warp * 64 + j * 8 + 2 * c;
+        for (int j = 0; j < NJ; ++j) {
+          const int col = n0 + warp * WCOLS + j * 8 + 2 * c;
           if (row < B && col < V)  // V % 8 == 0: both columns or none
             *reinterpret_cast<__half2*>(out + size_t(row) * V + col) =
                 __floats2half2_rn(acc[m][j][hr * 2], acc[m][j][hr * 2 + 1]);
@@ -171,10 +182,10 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restric
       float bv = -FLT_MAX;
       int bi = 0x7fffffff;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < NJ; ++j) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int col = n0 + warp * 64 + j * 8 + 2 * c + e;
+          const int col = n0 + warp * WCOLS + j * 8 + 2 * c + e;
           const float v = __half2float(__float2half_rn(acc[m][j][hr * 2 + e]));
           if (col < V && better(v, col, bv, bi)) {
             bv = v;
