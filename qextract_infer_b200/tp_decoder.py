@@ -39,6 +39,12 @@ With ``kv_bits=4`` the ring holds 4-bit values: a prompt chunk runs
 fused attention (7 launches a layer on one GPU at up to 8 sequences; one more where
 the attention's pieces are joined by a second kernel).
 
+With ``cfg.adapters`` every linear holds that many LoRA adapters and each
+sequence names its own (``adapter_ids``): the projection's shared part, then the
+adapters' addition (``multi_lora_add``), and SwiGLU on its own.  With a
+``Sampling`` a step draws its tokens from the whole logits instead of taking the
+largest (of more than one rank: the vocabulary slices' logits gathered first).
+
 Weights are synthetic: every full tensor comes from a generator seeded by
 (seed, layer, projection) on the device and each rank keeps its shard, so the
 model is the same for every tensor-parallel size.
@@ -53,7 +59,7 @@ import torch
 import torch.distributed as dist
 
 from . import _C
-from .tp_shard import merge_greedy, shard_quant_linear, shard_vocab
+from .tp_shard import gather_logits, merge_greedy, shard_adapters, shard_quant_linear, shard_vocab
 
 
 @dataclass
@@ -75,6 +81,21 @@ class DecoderConfig:
     init_std: float = 0.02  # embeddings, norms, lm_head ~ N(0, std)
     kv_bits: int = 16  # the ring's K and V: fp16, or 4 bits with a scale and zero point
     kv_group: int = 64  # for every kv_group values of a head
+    adapters: int = 0  # LoRA adapters held beside every linear, each sequence with its own; 0: one, merged
+
+
+@dataclass
+class Sampling:
+    """How a batch's next tokens are drawn (``_C.sample_logits``): ``u`` fp32 ``[B]``
+    random numbers in [0, 1) on the device, a new one for each step; the settings a
+    number or each sequence's own on the device (fp32 ``[B]``; ``top_k`` int64 ``[B]``).
+    A step leaves the logarithms of the drawn tokens' probabilities in ``logprobs``."""
+    u: torch.Tensor
+    temperature: float | torch.Tensor = 1.0
+    top_k: int | torch.Tensor = 0
+    top_p: float | torch.Tensor = 1.0
+    min_p: float | torch.Tensor = 0.0
+    logprobs: torch.Tensor | None = None
 
 
 class ShardedQuantLinear:
@@ -106,6 +127,38 @@ class ShardedQuantLinear:
         """bytes of the operands one call reads (int4 weights, scales, qzeros, LoRA A and B)"""
         return sum(t.numel() * t.element_size()
                    for t in (self.qweight, self.scales, self.qzeros, self.lora_A, self.lora_B))
+
+
+class AdapterLinear:
+    """One rank's shard of GPTQ int4 linears that read the same input, side by
+    side, with ``cfg.adapters`` LoRA adapters: A side by side along the ranks ``[n,
+    K, parts r]``, B compact ``[n, r, N]`` (``_C.w4a16_multi_lora_gemv``)."""
+
+    def __init__(self, K: int, widths: list, cfg: DecoderConfig, seeds: list, device, rank: int, world: int,
+                 split: str):
+        parts = [ShardedQuantLinear(K, n, cfg, seed, device, rank, world, split) for n, seed in zip(widths, seeds)]
+        self.K, self.splits = parts[0].K, [p.N for p in parts]
+        self.N, self.group, n, r = sum(self.splits), cfg.group_size, cfg.adapters, cfg.lora_rank
+        self.qweight, self.scales, self.qzeros = (torch.cat([getattr(p, name) for p in parts], 1).contiguous()
+                                                  for name in ("qweight", "scales", "qzeros"))
+        factors = []
+        for p, width, seed in zip(parts, widths, seeds):
+            g = torch.Generator(device=device).manual_seed(seed + 500009)
+            A = (torch.randn(n, K, r, generator=g, device=device) * 0.02).half()
+            B = (torch.randn(n, r, width, generator=g, device=device) * 0.02).half()
+            factors.append(shard_adapters(A, B, split, rank, world))
+        self.lora_A = torch.cat([A for A, _ in factors], 2).contiguous()
+        self.lora_B = torch.cat([B for _, B in factors], 2).contiguous()
+        self.lora_scales = torch.full((n,), float(np.float32(cfg.lora_alpha) / np.float32(r)), device=device)
+
+    def __call__(self, x: torch.Tensor, adapters: torch.Tensor) -> torch.Tensor:
+        """``x`` ``[B, K]`` or ``[B, T, K]``, ``adapters`` int64 ``[B]``"""
+        return _C.w4a16_multi_lora_gemv(x, self.qweight, self.scales, self.qzeros, self.lora_A, self.lora_B, adapters,
+                                        self.lora_scales, self.group, splits=self.splits)
+
+    def weight_bytes(self) -> int:
+        """bytes of the shared operands one call reads (each adapter in use adds its own)"""
+        return sum(t.numel() * t.element_size() for t in (self.qweight, self.scales, self.qzeros))
 
 
 class FusedQuantLinear:
@@ -207,14 +260,24 @@ class TPDecoder:
         self.layers = []
         for li in range(cfg.num_layers):
             base = seed * 1000003 + 100 + li * 16
+            L = dict(in_norm=normal((H,), base), post_norm=normal((H,), base + 1),
+                     q_norm=normal((D,), base + 2), k_norm=normal((D,), base + 3))
+            if cfg.adapters:
+                def linear(K, widths, offsets, split):
+                    return AdapterLinear(K, widths, cfg, [base + i for i in offsets], dev, r, w, split)
+
+                L.update(qkv=linear(H, [cfg.num_q_heads * D, cfg.num_kv_heads * D, cfg.num_kv_heads * D], (4, 5, 6), "col"),
+                         o=linear(cfg.num_q_heads * D, [H], (7,), "row"),
+                         gate_up=linear(H, [cfg.intermediate] * 2, (8, 9), "col"),
+                         down=linear(cfg.intermediate, [H], (10,), "row"))
+                self.layers.append(L)
+                continue
             q = ShardedQuantLinear(H, cfg.num_q_heads * D, cfg, base + 4, dev, r, w, "col")
             k = ShardedQuantLinear(H, cfg.num_kv_heads * D, cfg, base + 5, dev, r, w, "col")
             v = ShardedQuantLinear(H, cfg.num_kv_heads * D, cfg, base + 6, dev, r, w, "col")
             gate = ShardedQuantLinear(H, cfg.intermediate, cfg, base + 8, dev, r, w, "col")
             up = ShardedQuantLinear(H, cfg.intermediate, cfg, base + 9, dev, r, w, "col")
-            L = dict(
-                in_norm=normal((H,), base), post_norm=normal((H,), base + 1),
-                q_norm=normal((D,), base + 2), k_norm=normal((D,), base + 3),
+            L.update(
                 qkv=FusedQuantLinear([q, k, v], _padded_rank(3 * cfg.lora_rank)),
                 o=ShardedQuantLinear(cfg.num_q_heads * D, H, cfg, base + 7, dev, r, w, "row"),
                 gate_up=FusedQuantLinear([gate, up], _padded_rank(2 * cfg.lora_rank)).interleave_gate_up(),
@@ -230,6 +293,8 @@ class TPDecoder:
         else:
             self.cache = _C.RingBufferKVCache(cfg.num_layers, self.hkv, D, cfg.sink, cfg.window,
                                               batch=batch, device=dev)
+        # the sequences' adapters (cfg.adapters of them; -1: none); write into it, captured steps follow
+        self.adapter_ids = torch.zeros(batch, dtype=torch.int64, device=dev) if cfg.adapters else None
         # q/k norm + RoPE + append fused into the attention kernel for a few
         # sequences (one launch fewer per layer, same time); for many, the
         # separate append kernel is faster (32 sequences: 86 vs 96 us per layer)
@@ -271,14 +336,28 @@ class TPDecoder:
             return self.ar.add_rmsnorm(partial, x, w, self.cfg.rms_eps)
         return _C.add_rmsnorm(x, self._allreduce(partial), w, self.cfg.rms_eps)
 
+    def _linear(self, lin, x: torch.Tensor) -> torch.Tensor:
+        """``lin`` of ``x`` ``[B n, K]``, with the sequences' adapters where the decoder holds them"""
+        if self.adapter_ids is None:
+            return lin(x)
+        if x.size(0) != self.batch:
+            return lin(x.view(self.batch, -1, x.size(1)), self.adapter_ids).view(x.size(0), -1)
+        return lin(x, self.adapter_ids)
+
+    def _gate_up(self, L, h: torch.Tensor) -> torch.Tensor:
+        """silu(gate) * up of ``h``"""
+        if self.adapter_ids is None:
+            return L["gate_up"].swiglu(h)
+        return _C.swiglu_packed(self._linear(L["gate_up"], h))  # the adapters come before SwiGLU
+
     def _mlp(self, L, h: torch.Tensor) -> torch.Tensor:
-        return self._allreduce(L["down"](L["gate_up"].swiglu(h)))
+        return self._allreduce(self._linear(L["down"], self._gate_up(L, h)))
 
     # ------------------------------------------------------------------ decode
-    def decode_step(self, tokens: torch.Tensor, return_hidden: bool = False):
-        """One greedy step for the batch: ``tokens`` int64 [B] (device) -> next
-        tokens int64 [B] (and the final hidden state [B, H] if asked).  The
-        position is the cache's token count."""
+    def decode_step(self, tokens: torch.Tensor, return_hidden: bool = False, sampling: Sampling | None = None):
+        """One step for the batch, greedy or drawn by ``sampling``: ``tokens`` int64
+        [B] (device) -> next tokens int64 [B] (and the final hidden state [B, H] if
+        asked).  The position is the cache's token count."""
         cfg, B, D = self.cfg, self.batch, self.cfg.head_dim
         eps = cfg.rms_eps
         pos = self.cache.get_total_written()
@@ -289,7 +368,8 @@ class TPDecoder:
         # one GPU and a few rows: the residual add + RMSNorm before the MLP and
         # before the next layer's q|k|v run as those projections' prologue (5
         # launches per layer); the residual alternates between two buffers
-        fuse = self.world == 1 and B <= 8
+        # (not with adapters: they read the normed rows, which stay inside the projection there)
+        fuse = self.world == 1 and B <= 8 and self.adapter_ids is None
         xo = torch.empty_like(x) if fuse else None
         dn = None
         for li, L in enumerate(self.layers):
@@ -297,7 +377,7 @@ class TPDecoder:
                 qkv = L["qkv"].addnorm(x, dn, L["in_norm"], eps, xo)  # x + down of the layer before
                 x, xo = xo, x
             else:
-                qkv = L["qkv"](h)
+                qkv = self._linear(L["qkv"], h)
             if cfg.kv_bits == 4:
                 q, k, v = _C.qk_norm_rope(qkv.view(B, 1, -1), self.hq, self.hkv, L["q_norm"], L["k_norm"], eps,
                                           cos, sin)
@@ -314,7 +394,7 @@ class TPDecoder:
                                            pos)
                 att = _C.decode_attention(q, self.cache.k[li], self.cache.v[li], pos + 1, cfg.sink,
                                           cfg.window, after_append=True)
-            o = L["o"](att.view(B, self.hq * D))
+            o = self._linear(L["o"], att.view(B, self.hq * D))
             if fuse:
                 gu = L["gate_up"].addnorm(x, o, L["post_norm"], eps, xo, swiglu=True)  # x + o
                 x, xo = xo, x
@@ -323,12 +403,23 @@ class TPDecoder:
                     h = _C.add_rmsnorm(x, dn, self.final_norm, eps)  # x += down; the final RMSNorm
                 continue
             h = self._reduce_add_norm(o, x, L["post_norm"])  # x += o
-            dn = L["down"](L["gate_up"].swiglu(h))
+            dn = self._linear(L["down"], self._gate_up(L, h))
             nxt_w = self.layers[li + 1]["in_norm"] if li + 1 < n else self.final_norm
             h = self._reduce_add_norm(dn, x, nxt_w)  # x += down; the next RMSNorm
         self.cache.advance(1)
-        nxt = self._greedy_normed(h)
+        nxt = self._next(h, sampling)
         return (nxt, x) if return_hidden else nxt
+
+    def _next(self, h: torch.Tensor, sampling: Sampling | None) -> torch.Tensor:
+        """next tokens from the final-normed hidden state"""
+        if sampling is None:
+            return self._greedy_normed(h)
+        logits = _C.lm_head_logits(h, self.lm_head)
+        if self.world > 1:  # every rank draws from the whole row, with the same numbers
+            logits = gather_logits(logits, self.world, self.group)
+        tokens, sampling.logprobs = _C.sample_logits(logits, sampling.u, sampling.temperature, sampling.top_k,
+                                                     sampling.top_p, sampling.min_p)
+        return tokens.clamp_(min=0)  # (-1: a row without a finite logit; the next step embeds some token)
 
     def _greedy_logits(self, x: torch.Tensor) -> torch.Tensor:
         """this rank's vocabulary slice of the logits [B, V / tp] (fp16; tests only)"""
@@ -350,9 +441,10 @@ class TPDecoder:
         return idx
 
     # ----------------------------------------------------------------- prefill
-    def prefill(self, tokens: torch.Tensor, chunk: int = 2048, return_hidden: bool = False):
-        """``tokens`` int64 [B, T] (device); returns the greedy next tokens [B]
-        (and the last position's hidden state [B, H] if asked)."""
+    def prefill(self, tokens: torch.Tensor, chunk: int = 2048, return_hidden: bool = False,
+                sampling: Sampling | None = None):
+        """``tokens`` int64 [B, T] (device); returns the next tokens [B], greedy or
+        drawn by ``sampling`` (and the last position's hidden state [B, H] if asked)."""
         cfg, B, D = self.cfg, self.batch, self.cfg.head_dim
         T = tokens.size(1)
         x_last = None
@@ -364,7 +456,7 @@ class TPDecoder:
             x = self.embed.index_select(0, tc.reshape(-1)).view(B * n, cfg.hidden)
             for li, L in enumerate(self.layers):
                 h = _C.fused_rmsnorm(x, L["in_norm"], cfg.rms_eps)
-                q, k, v = _C.qk_norm_rope(L["qkv"](h).view(B, n, -1), self.hq, self.hkv, L["q_norm"], L["k_norm"],
+                q, k, v = _C.qk_norm_rope(self._linear(L["qkv"], h).view(B, n, -1), self.hq, self.hkv, L["q_norm"], L["k_norm"],
                                           cfg.rms_eps, cos, sin)
                 # the chunk over the ring (read in place) and its own keys, then the append
                 if cfg.kv_bits == 4:
@@ -375,9 +467,9 @@ class TPDecoder:
                                                cfg.sink, cfg.window)  # [B, n, hq, D]
                 self.cache.append(k, v, li)
                 att = att.reshape(B * n, self.hq * D)
-                x = x + self._allreduce(L["o"](att))
+                x = x + self._allreduce(self._linear(L["o"], att))
                 h = _C.fused_rmsnorm(x, L["post_norm"], cfg.rms_eps)
                 x = x + self._mlp(L, h)
             x_last = x.view(B, n, cfg.hidden)[:, -1].contiguous()
-        nxt = self._greedy(x_last)
+        nxt = self._next(_C.fused_rmsnorm(x_last, self.final_norm, cfg.rms_eps), sampling)
         return (nxt, x_last) if return_hidden else nxt

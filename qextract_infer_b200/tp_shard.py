@@ -18,7 +18,10 @@ each a GPTQ int4 weight (``qweight int32 [K/8, N]``, ``scales [K/g, N]``,
 * vocabulary-parallel lm_head: rank ``i`` keeps vocabulary columns
   ``[i V/tp, (i+1) V/tp)``; greedy decoding gathers every rank's
   (max logit, global index) and keeps the largest (lowest rank on ties, which
-  is the lowest index: the first maximum, as ``argmax`` over the full row).
+  is the lowest index: the first maximum, as ``argmax`` over the full row);
+  sampling gathers the slices' logits, so that every rank draws from the whole row.
+* adapters of many requests (``A [n, K, r]``, ``B [n, r, N]``): split like the one
+  adapter of a linear, ``B`` by columns or ``A`` by rows.
 
 The functions take and return torch tensors on any device (the decoder calls
 them on the GPU; the CPU test suite checks them over ``gloo`` ranks).
@@ -27,8 +30,9 @@ them on the GPU; the CPU test suite checks them over ``gloo`` ranks).
 from __future__ import annotations
 
 import torch
+import torch.distributed as dist
 
-__all__ = ["shard_quant_linear", "shard_vocab", "merge_greedy"]
+__all__ = ["shard_quant_linear", "shard_adapters", "shard_vocab", "merge_greedy", "gather_logits"]
 
 
 def shard_quant_linear(qweight, scales, qzeros, lora_A, lora_B, split, rank: int, world: int,
@@ -56,6 +60,20 @@ def shard_quant_linear(qweight, scales, qzeros, lora_A, lora_B, split, rank: int
     raise ValueError(f"unknown split {split!r}")
 
 
+def shard_adapters(lora_A, lora_B, split: str, rank: int, world: int):
+    """This rank's ``(A, B)`` of adapters ``A [n, K, r]``, ``B [n, r, N]`` beside a
+    linear split by "col" or "row".  Views; the caller makes them contiguous."""
+    if world <= 1:
+        return lora_A, lora_B
+    if split == "col":
+        n = lora_B.size(2) // world
+        return lora_A, lora_B[:, :, rank * n:(rank + 1) * n]
+    if split == "row":
+        k = lora_A.size(1) // world
+        return lora_A[:, rank * k:(rank + 1) * k], lora_B
+    raise ValueError(f"unknown split {split!r}")
+
+
 def shard_vocab(lm_head: torch.Tensor, rank: int, world: int) -> torch.Tensor:
     """This rank's vocabulary columns of ``lm_head [H, V]``."""
     V = lm_head.size(1)
@@ -70,3 +88,11 @@ def merge_greedy(vals: torch.Tensor, idxs: torch.Tensor) -> torch.Tensor:
     vocabulary index -> the greedy token ``[B]`` (first rank on ties)."""
     best = vals.argmax(dim=0)
     return idxs.gather(0, best[None, :])[0]
+
+
+def gather_logits(logits: torch.Tensor, world: int, group=None) -> torch.Tensor:
+    """The whole rows ``[B, V]`` of every rank's slice ``[B, V / world]``, in rank
+    order (collective; the same on every rank)."""
+    parts = [torch.empty_like(logits) for _ in range(world)]
+    dist.all_gather(parts, logits, group=group)
+    return torch.cat(parts, 1)
