@@ -508,18 +508,20 @@ def run_kernel_suite(args):
                           "us_per_call": us, "TFLOP/s": flops / us / 1e6, "bound": "mma.sync"}),
               flush=True)
         del pq, pk, pv, kc, vc
-    # the head norm with rotation and the 4-bit ring's operators: the cases of perf/operators.py
-    from perf import operators
-    operators.own = True
-    for case in operators.listed():
-        w = operators.work(case)
-        states = [operators.prepare(case, seed) for seed in range(nbuf(w["bytes"]))]
-        torch.cuda.synchronize()
-        us = _graph_time_us(torch, st, lambda i: operators.run(states[i % len(states)]),
-                            40 if case["kind"] == "prefill" else steps)
-        emit(case["name"], {n: v for n, v in case.items() if n != "name"}, w["bytes"], us,
-             {"TFLOP/s": w["flops"] / us / 1e6})
-        del states
+    # the head norm with rotation and the 4-bit ring's operators, then the adapters, logits and sampling
+    # of a served batch: the cases of perf/operators.py and perf/more_operators.py
+    from perf import more_operators, operators
+    for module in (operators, more_operators):
+        module.own = True
+        for case in module.listed():
+            w = module.work(case)
+            states = [module.prepare(case, seed) for seed in range(nbuf(w["bytes"]))]
+            torch.cuda.synchronize()
+            us = _graph_time_us(torch, st, lambda i: module.run(states[i % len(states)]),
+                                40 if case["kind"] in ("prefill", "head") else steps)
+            emit(case["name"], {n: v for n, v in case.items() if n != "name"}, w["bytes"], us,
+                 {"TFLOP/s": w["flops"] / us / 1e6})
+            del states
     return 0
 
 
@@ -623,9 +625,9 @@ def tp_decode_measure(args, world, rank, dev):
     import torch
     import torch.distributed as dist
     from qextract_infer_b200 import _C
-    from qextract_infer_b200.tp_decoder import DecoderConfig, TPDecoder
+    from qextract_infer_b200.tp_decoder import DecoderConfig, Sampling, TPDecoder
 
-    cfg = DecoderConfig(kv_bits=args.kv_bits)
+    cfg = DecoderConfig(kv_bits=args.kv_bits, adapters=args.adapters)
     prompt_len, decode_steps, chunk = args.prompt, args.decode, 2048
     batches = [int(b) for b in args.batches.split(",")]
     hbm = measured_peaks()[0]
@@ -642,6 +644,12 @@ def tp_decode_measure(args, world, rank, dev):
         dec = TPDecoder(cfg, batch=B, device=dev, seed=4)
         prompt = torch.randint(0, cfg.vocab, (B, prompt_len), generator=torch.Generator().manual_seed(4))
         prompt = prompt.to(dev)
+        if cfg.adapters:  # each sequence its own, as far as there are that many
+            dec.adapter_ids.copy_(torch.arange(B) % cfg.adapters)
+        sampling = None
+        if args.sample:
+            u = torch.rand(B, generator=torch.Generator().manual_seed(5)).to(dev)
+            sampling = Sampling(u, temperature=0.7, top_k=50, top_p=0.9)
         torch.cuda.synchronize(dev)
         if world > 1:
             dist.barrier()
@@ -663,14 +671,14 @@ def tp_decode_measure(args, world, rank, dev):
 
         with torch.cuda.stream(st):
             restore()
-            tok.copy_(dec.decode_step(tok))  # eager step: plans, workspaces, lazy state
+            tok.copy_(dec.decode_step(tok, sampling=sampling))  # eager step: plans, workspaces, lazy state
             restore()
         st.synchronize()
         graphs, pool = [], torch.cuda.graph_pool_handle()
         for _ in range(decode_steps):
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g, pool=pool, stream=st):
-                tok.copy_(dec.decode_step(tok))
+                tok.copy_(dec.decode_step(tok, sampling=sampling))
             graphs.append(g)
         for rep in range(2):  # rep 0 uploads the graphs; rep 1 is timed
             with torch.cuda.stream(st):
@@ -693,6 +701,9 @@ def tp_decode_measure(args, world, rank, dev):
         # shard, and the ring (all layers, this rank's KV heads, every sequence)
         wbytes = sum(L[k].weight_bytes() for L in dec.layers for k in ("qkv", "o", "gate_up", "down"))
         wbytes += dec.lm_head.numel() * 2
+        if cfg.adapters:  # those in use
+            wbytes += sum(t[0].numel() * t.element_size() * min(B, cfg.adapters) for L in dec.layers
+                          for k in ("qkv", "o", "gate_up", "down") for t in (L[k].lora_A, L[k].lora_B))
         kvbytes = sum(t.numel() * t.element_size() for t in held)
         per_rank_gbs = (wbytes + kvbytes) / (step_ms / 1e3) / 1e9
         ar_us = None
@@ -728,6 +739,7 @@ def tp_decode_measure(args, world, rank, dev):
             "config": {"workload": "Qwen3-8B decoder (36 layers, hidden 4096, 32/8 heads, "
                                    "GPTQ int4 g128 + LoRA r16), TP decode",
                        "prompt": prompt_len, "decode_tokens": decode_steps, "prefill_chunk": chunk, "kv_bits": cfg.kv_bits,
+                       "adapters": cfg.adapters, "sampled": bool(args.sample),
                        "graphs": "one CUDA graph per decode step"},
             "prefill_s": prefill_s, "prefill_tok_s": B * prompt_len / prefill_s,
             "nvlink_allreduce_us": ar_us,
@@ -1007,6 +1019,9 @@ def main():
     ap.add_argument("--prompt", type=int, default=8192, help="decode_tp: prompt tokens")
     ap.add_argument("--decode", type=int, default=64, help="decode_tp: greedy decode tokens")
     ap.add_argument("--kv-bits", type=int, choices=[16, 4], default=16, help="decode_tp: bits of the ring's K and V")
+    ap.add_argument("--adapters", type=int, default=0,
+                    help="decode_tp: LoRA adapters beside every linear, each sequence with its own (0: one, merged)")
+    ap.add_argument("--sample", action="store_true", help="decode_tp: draw the tokens instead of taking the largest logit")
     ap.add_argument("--workload", choices=["decode_gemv", "kernels", "prefill_gemm", "decode_tp",
                                            "profile_cases", "profile_decode_step", "timeline"],
                     default="decode_gemv",

@@ -516,7 +516,8 @@ int qx_prefill_attention_q4(const void* q, const void* k_new, const void* v_new,
  *   Sums in fp32, one rounding.  out may be y (in place); it must not overlap
  *   anything else.  lora_A, lora_B, scales and adapters must not be written by a kernel
  *   of this library issued just before on the stream (qx_set_pdl).
- *   K % 8 == 0, N % 8 == 0, rank % 8 == 0, P rank <= 256; 16-byte aligned.
+ *   K % 8 == 0, N % 8 == 0, rank % 8 == 0, P rank <= 256, batch <= 32768 (the time
+ *   of a call grows with its square beyond some thousands); 16-byte aligned.
  * qx_lm_head_logits: logits fp16 [batch, vocab] = h [batch, hidden] W, W fp16
  *   [hidden, vocab], fp32 sums; the values whose maximum qx_lm_head_argmax takes.  Any
  *   batch (32 rows a launch); hidden % 64 == 0, vocab % 8 == 0.

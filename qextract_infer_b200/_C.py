@@ -496,7 +496,7 @@ def multi_lora_add(y: torch.Tensor, x: torch.Tensor, lora_A: torch.Tensor, lora_
     outside ``0 .. n - 1`` has none and keeps ``y``.  ``splits``: the widths of the
     ``P`` <= 4 column blocks of a fused projection (q | k | v), block ``j`` taking
     the ranks ``j r ..`` of ``lora_A``; None: one block.  K, N, r and the widths are
-    multiples of 8, ``P r <= 256``.  ``out``: the output, ``y`` itself for in place.
+    multiples of 8, ``P r <= 256``, B <= 32768.  ``out``: the output, ``y`` itself for in place.
     New component (the reference's op has one adapter for all rows)."""
     return _binding.multi_lora_add(y, x, lora_A, lora_B, adapters, scales, splits, out)
 

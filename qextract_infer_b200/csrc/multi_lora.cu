@@ -30,6 +30,7 @@ namespace mlora {
 constexpr int C = 8;  // CTAs of a cluster
 constexpr int MAX_PARTS = 4;
 constexpr int MAX_RANKS = 256;  // P r
+constexpr int MAX_BATCH = 32768;  // a cluster looks through the sequences before its own
 constexpr int MAX_SMEM = 225 * 1024;  // dynamic; the rest of 227 KB for the static arrays
 
 struct Params {
@@ -956,6 +957,8 @@ extern "C" int qx_multi_lora_add(const void* y, const void* x, const void* lora_
   using namespace mlora;
   QX_REQUIRE(batch >= 0 && tokens >= 0 && K > 0 && N > 0 && num_adapters >= 0,
              "multi_lora_add: bad sizes batch=%d tokens=%d K=%d N=%d adapters=%d", batch, tokens, K, N, num_adapters);
+  QX_REQUIRE(batch <= MAX_BATCH, "multi_lora_add: batch=%d is above %d (rows of one adapter go together as [batch, tokens])",
+             batch, MAX_BATCH);
   QX_REQUIRE(K % 8 == 0 && N % 8 == 0, "multi_lora_add: K=%d and N=%d must be multiples of 8", K, N);
   QX_REQUIRE(num_splits >= 0 && num_splits <= MAX_PARTS && (num_splits == 0 || splits),
              "multi_lora_add: %d column blocks (at most %d)", num_splits, MAX_PARTS);

@@ -679,8 +679,12 @@ int prepare(int* clusters) {
     Launch l;
     configure<C>(l, SLICE_MAX, 1, nullptr);
     l.cfg.numAttrs = 1;
-    QX_CUDA_TRY(cudaOccupancyMaxActiveClusters(&fit[dev], sample_kernel<C>, &l.cfg), "sample_logits: clusters on the device");
-    if (fit[dev] == 0) fit[dev] = -1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, sample_kernel<C>, &l.cfg) != cudaSuccess) {
+      cudaGetLastError();  // a device that has no room for clusters of this size: none of them
+      n = 0;
+    }
+    fit[dev] = n > 0 ? n : -1;
   }
   *clusters = fit[dev];
   return QX_OK;

@@ -26,7 +26,7 @@ def _lora(lib, y=Y, x=X, a=A, b=B, ids=IDS, scales=SCALES, out=OUT, batch=2, tok
     (dict(rank=4), "rank"), (dict(rank=12), "rank"), (dict(rank=264), "rank"), (dict(rank=72, splits=[16] * 4), "rank"),
     (dict(splits=[8] * 5), "column blocks"), (dict(splits=[32, 36]), "columns"), (dict(splits=[64, 0]), "columns"),
     (dict(splits=[32, 24]), "cover"), (dict(splits=[64, 8]), "exceed"), (dict(splits=[-64, 128]), "columns"),
-    (dict(batch=1 << 20, tokens=1 << 20), "too many"), (dict(y=None), "null"), (dict(x=None), "null"),
+    (dict(batch=1 << 14, tokens=1 << 20), "too many"), (dict(batch=32769), "32768"), (dict(y=None), "null"), (dict(x=None), "null"),
     (dict(a=None), "null"), (dict(b=None), "null"), (dict(ids=None), "null"), (dict(scales=None), "null"),
     (dict(out=None), "null"), (dict(y=Y + 8), "aligned"), (dict(x=X + 2), "aligned"), (dict(a=A + 8), "aligned"),
     (dict(b=B + 8), "aligned"), (dict(out=OUT + 8), "aligned"), (dict(ids=IDS + 4), "aligned"),
