@@ -16,7 +16,8 @@
 // then it does an eighth of the columns (its part of B).
 //
 // A row's result depends on no other row: the sums are split in the same way wherever a
-// row stands.  Everything that does not come from the kernel before (adapters, A, B,
+// row stands.  Where there are few chunks, several clusters take one, each a share of the
+// columns.  Everything that does not come from the kernel before (adapters, A, B,
 // scales) is requested before the wait for it.
 #include <algorithm>
 #include <mutex>
@@ -40,7 +41,8 @@ struct Params {
   __half* out;
   int batch, tokens, K, N, rank, ranks, n, parts;
   int edge[MAX_PARTS + 1];  // first column of each block, then N
-  int chunks;               // clusters of a sequence: the chunks that may start in it
+  int chunks;               // chunks that may start in a sequence
+  int fan;                  // clusters of a chunk: each makes h, and does its share of the columns
   int k_slice, k_step;      // K of a CTA, and of one of its steps (multiples of 16)
   int width;                // columns of a CTA
   int a_pitch;              // bytes of a staged row of A: an odd number of 16-byte units
@@ -218,7 +220,8 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int rows[ROWS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = blockIdx.x % C, chunk = blockIdx.x / C;
+  const int rank = blockIdx.x % C, cluster = blockIdx.x / C, chunk = cluster / p.fan;
+  const int cut = (cluster - chunk * p.fan) * C + rank;  // of the columns
   const int b = chunk / p.chunks;
   pdl_trigger();
   const int64_t a = adapter_of(p, b);
@@ -228,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
     return;
   }
   // this CTA's columns
-  const int n0 = min(p.N, rank * p.width), n1 = min(p.N, n0 + p.width);
+  const int n0 = min(p.N, cut * p.width), n1 = min(p.N, n0 + p.width);
   if (a < 0) {  // no adapter: the rows as they are
     pdl_wait();
     for (int m = 0; m < n; ++m) {
@@ -484,14 +487,15 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
   __shared__ int rows[ROWS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, q = lane & 3;
-  const int rank = blockIdx.x % C, chunk = blockIdx.x / C;
+  const int rank = blockIdx.x % C, cluster = blockIdx.x / C, chunk = cluster / p.fan;
+  const int cut = (cluster - chunk * p.fan) * C + rank;  // of the columns
   const int b = chunk / p.chunks;
   const int64_t a = adapter_of(p, b);
   const int n = a < 0 && p.out == p.y ? 0 : find_rows<ROWS, THREADS>(p, b, chunk - b * p.chunks, a, rows);
   pdl_wait();
   if (n == 0) return;  // (every CTA of the cluster)
   if (a < 0) {         // no adapter: the rows as they are
-    const int n0 = min(p.N, rank * p.width), n1 = min(p.N, n0 + p.width);
+    const int n0 = min(p.N, cut * p.width), n1 = min(p.N, n0 + p.width);
     for (int m = warp; m < n; m += WARPS) {
       const int64_t at = int64_t(rows[m]) * p.N;
       for (int c = n0 + 8 * lane; c < n1; c += 8 * 32)
@@ -612,10 +616,10 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
     __syncthreads();  // the ring is free
   }
 
-  // ---- this CTA's columns: an eighth of the 32-column blocks (a block is of one part)
+  // ---- this CTA's columns: its share of the 32-column blocks (a block is of one part)
   int total = 0;
   for (int i = 0; i < p.parts; ++i) total += (p.edge[i + 1] - p.edge[i] + 31) / 32;
-  const int first = int(int64_t(total) * rank / C), last = int(int64_t(total) * (rank + 1) / C);
+  const int first = int(int64_t(total) * cut / (C * p.fan)), last = int(int64_t(total) * (cut + 1) / (C * p.fan));
   const int groups = (last - first + GROUP - 1) / GROUP;
   // this warp's block of a group: its part, first column and number of columns (0: none)
   struct Block {
@@ -861,7 +865,17 @@ bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
 
 constexpr int FEW_TOKENS = 8;  // tokens of a sequence up to which 8-row chunks do them
 
-// one cluster of C CTAs for every chunk that may start in a sequence
+// Clusters of a chunk: doubled while a CTA has more than `columns` columns, up to 8 and up to
+// the 32 in all that run at once.  Measured (rank 16, K 4096, 24576 columns, us by 1 / 8
+// clusters a chunk): 8 tokens 15.9 / 6.0, 16 tokens 20.0 / 9.6, 128 tokens 23.3 / 13.1; one token
+// and 6144 columns: 4.9 with 1, 5.0 with 2, 5.1 with 4.
+void spread(Params& p, int columns) {
+  p.fan = 1;
+  while (p.fan < 8 && int64_t(p.batch) * p.chunks * p.fan * 2 <= 32 && p.N / (C * p.fan) > columns) p.fan *= 2;
+  p.width = ((p.N + C * p.fan - 1) / (C * p.fan) + 7) / 8 * 8;
+}
+
+// C CTAs for every cluster of every chunk that may start in a sequence
 template <typename... Args>
 int launch(void (*kernel)(Args...), int threads, const Params& p, int smem, cudaStream_t st, Args... args) {
   static std::mutex mu;
@@ -884,7 +898,7 @@ int launch(void (*kernel)(Args...), int threads, const Params& p, int smem, cuda
     }
   }
   QX_REQUIRE(smem <= MAX_SMEM, "multi_lora_add: %d bytes of shared memory needed", smem);
-  const int64_t ctas = int64_t(p.batch) * p.chunks * C;
+  const int64_t ctas = int64_t(p.batch) * p.chunks * p.fan * C;
   QX_REQUIRE(ctas <= 0x7fffffffLL, "multi_lora_add: %d sequences of %d tokens are too many", p.batch, p.tokens);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(ctas));
@@ -909,6 +923,7 @@ int launch_few(Params& p, cudaStream_t st) {
   const int most = std::min(MAX_STEP, A_BYTES / p.a_pitch / 16 * 16);
   const int steps = (p.k_slice + most - 1) / most;
   p.k_step = ((p.k_slice + steps - 1) / steps + 15) / 16 * 16;
+  spread(p, 1024 / int(std::min<int64_t>(ROWS, int64_t(p.batch) * p.tokens)));
   const Layout l = layout(p);
   return launch(multi_lora_rows_kernel, THREADS, p, l.total, st, p, l);
 }
@@ -922,6 +937,7 @@ int launch_many(Params& p, cudaStream_t st) {
   const int ks = (p.rank + 15) / 16;
   const int rows = int64_t(p.batch) * p.tokens <= SMALL_ROWS && ks <= 4 ? 32 : 64;
   p.chunks = (p.tokens + rows - 1) / rows;
+  spread(p, 256);
   const int here = std::min(RANKS, p.ranks);
   p.a_pitch = here * 2 + (here / 8 % 2 ? 0 : 16);
   void (*kernel)(Params);
@@ -1006,7 +1022,6 @@ extern "C" int qx_multi_lora_add(const void* y, const void* x, const void* lora_
   p.n = num_adapters;
   p.a_pitch = p.ranks * 2 + (p.ranks / 8 % 2 ? 0 : 16);
   p.k_slice = ((K + C - 1) / C + 15) / 16 * 16;
-  p.width = ((N + C - 1) / C + 7) / 8 * 8;
   return tokens <= FEW_TOKENS ? launch_few(p, reinterpret_cast<cudaStream_t>(stream))
                               : launch_many(p, reinterpret_cast<cudaStream_t>(stream));
 }
