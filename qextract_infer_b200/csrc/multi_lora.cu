@@ -659,6 +659,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
   // lane (g, q): columns column + 8 q .. + 7 of rows 16 t + g and + 8; in shared memory a lane's
   // pieces are a run of the warp's
   constexpr int AHEAD = blocks_ahead(KS * 16);
+  constexpr int TILES = ROWS / 16;  // of a block, a commit each
   auto ask_y = [&](const Block& at, int t, int buffer) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -674,7 +675,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
       const Block at = block_of(i);
       load_b(i, i);
 #pragma unroll
-      for (int t = 0; t < ROWS / 16; ++t) {
+      for (int t = 0; t < TILES; ++t) {
         ask_y(at, t, i);
         copy_commit();
       }
@@ -796,8 +797,8 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
     if constexpr (KS > 0) {
       const Block later = block_of(group + AHEAD);
       const int buffer = AHEAD == 1 ? 0 : group & 1;
-      // a commit a tile: AHEAD blocks of them are on their way behind the one that is waited for
-      copy_wait<4 * AHEAD - 1>();
+      // AHEAD blocks of commits are on their way behind the one that is waited for
+      copy_wait<TILES * AHEAD - 1>();
       __syncwarp();
       const int ks = l.padded / 16;
       uint32_t w[KS > 0 ? KS : 1][4][2];
@@ -808,8 +809,8 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
       __syncwarp();
       load_b(group + AHEAD, buffer);
 #pragma unroll
-      for (int t = 0; t < ROWS / 16; ++t) {
-        copy_wait<4 * AHEAD - 1>();  // a lane reads its own copies
+      for (int t = 0; t < TILES; ++t) {
+        copy_wait<TILES * AHEAD - 1>();  // a lane reads its own copies
         uint4 y[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e)

@@ -235,3 +235,15 @@ def test_refusals(C):
                   lora_A=torch.zeros(3, 64, 4, dtype=torch.float16, device="cuda")), "rank")]:
         with pytest.raises((RuntimeError, TypeError), match=msg):
             C.multi_lora_add(**{**d, **change})
+
+
+@pytest.mark.parametrize("r", [16, 32, 64])
+@pytest.mark.parametrize("b,t", [(36, 32), (30, 20), (7, 9)])
+def test_cold_y_behind_a_short_product(C, r, b, t):
+    """short chunks with many blocks of columns, y and B not in L2: each block has to wait for its own copies"""
+    splits = (1024, 6144)
+    d = inputs(b, t, 64, splits, r, 5, seed=r + b)
+    flush = torch.empty(1 << 26, dtype=torch.int64, device="cuda")
+    for i in range(3):
+        flush.fill_(i)
+        check(C.multi_lora_add(**d, splits=splits), d, splits)
