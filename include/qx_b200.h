@@ -514,8 +514,8 @@ int qx_prefill_attention_q4(const void* q, const void* k_new, const void* v_new,
  *   8), the column blocks of a fused projection; block j uses the ranks
  *   j rank .. j rank + rank - 1 of lora_A.  num_splits = 0: one block (P = 1).
  *   Sums in fp32, one rounding.  out may be y (in place); it must not overlap
- *   anything else.  lora_A, lora_B, scales and adapters must not be written by a kernel
- *   of this library issued just before on the stream (qx_set_pdl).
+ *   anything else.  lora_A and lora_B must not be written by a kernel of this
+ *   library issued just before on the stream (qx_set_pdl); adapters and scales may be.
  *   K % 8 == 0, N % 8 == 0, rank % 8 == 0, P rank <= 256, batch <= 32768 (the time
  *   of a call grows with its square beyond some thousands); 16-byte aligned.
  * qx_lm_head_logits: logits fp16 [batch, vocab] = h [batch, hidden] W, W fp16

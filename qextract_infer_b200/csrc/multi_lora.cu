@@ -7,7 +7,7 @@
 //
 // Sequences with the same adapter are a group, and their tokens in order are the
 // group's rows.  A cluster of 8 CTAs takes a chunk of a group's rows: 8 rows where
-// sequences have few tokens (a decode step), 64 else (a prompt).  Nothing is sorted or
+// sequences have few tokens (a decode step), 32 or 64 else (a prompt).  Nothing is sorted or
 // prepared: the cluster of sequence b counts the sequences before it that share its
 // adapter, which says whether a chunk starts in b, and looks up those after it that
 // fill the chunk; clusters without a chunk end at once.  The group's weights are read
@@ -17,8 +17,7 @@
 //
 // A row's result depends on no other row: the sums are split in the same way wherever a
 // row stands.  Where there are few chunks, several clusters take one, each a share of the
-// columns.  Everything that does not come from the kernel before (adapters, A, B,
-// scales) is requested before the wait for it.
+// columns.
 #include <algorithm>
 #include <mutex>
 
@@ -77,9 +76,6 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
                : "r"(at)
                : "memory");
 }
-__device__ __forceinline__ void ldsm2_t(uint32_t (&r)[2], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at) : "memory");
-}
 __device__ __forceinline__ uint32_t lds32(uint32_t at) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
@@ -120,48 +116,90 @@ __device__ __forceinline__ void bar_wait(uint32_t bar) {
 }
 
 // the adapter of sequence b, -1 where it has none
-__device__ __forceinline__ int64_t adapter_of(const Params& p, int b) {
-  const int64_t a = p.adapters[b];
+__device__ __forceinline__ int64_t adapter_of(const Params& p, int b, bool fresh) {
+  const int64_t a = fresh ? __ldcg(p.adapters + b) : p.adapters[b];
   return a >= 0 && a < p.n ? a : -1;
 }
 
-// The chunk of ROWS rows that cluster (b, j) takes of its group: row indexes into
-// x, y and out; returns their number, 0 where it has no chunk.
+// The chunk of ROWS rows that cluster (b, j) takes of its group.  With `guess` it is found
+// while the kernel before may still be writing the adapters: find() reads them, the loads
+// of weights that follow from them start, and after the wait for that kernel ask_again()
+// reads them once more; changed() compares, behind the work that hides these loads and
+// before anything leaves the CTA.  If it says so, find() and all after it is done again.
+// Whatever find() reads, its results are the same in all threads, and its rows and adapter
+// exist.  (A decode step's launch of one token takes 5.3 us so, 6.9 with the wait first, 4.9 if the
+// second look is left out; of 32 tokens with an adapter each 11.7, 13.2 and 11.0.)
 template <int ROWS, int THREADS>
-__device__ __forceinline__ int find_rows(const Params& p, int b, int j, int64_t mine, int (&rows)[ROWS]) {
-  constexpr int WARPS = THREADS / 32;
-  __shared__ int s_seq[ROWS + 1], s_count[WARPS];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, T = p.tokens;
-  const int need = (ROWS - 1) / T + 2;  // sequences that a chunk can reach into, at most ROWS + 1
-  int before = 0, found = 0;
-  for (int i = 0; i < p.batch && (i <= b || found < need); i += THREADS) {
-    const int q = i + tid;
-    const bool same = q < p.batch && adapter_of(p, q) == mine;
-    const unsigned after = __ballot_sync(0xffffffffu, same && q >= b);
-    if (lane == 0) s_count[warp] = __popc(after);
-    before += __syncthreads_count(same && q < b);
-    int at = found;
-    for (int w = 0; w < WARPS; ++w) {
-      if (w == warp && same && q >= b) {
-        const int n = at + __popc(after & ((1u << lane) - 1));
-        if (n < need) s_seq[n] = q;
+struct Chunk {
+  int64_t a;       // the adapter, -1: none
+  int n;           // rows, 0: no chunk
+  bool settled;    // the kernel before has ended
+  unsigned seen;   // a bit for each of up to 32 steps of THREADS sequences: this thread's one has the adapter
+  int end;         // sequences looked at
+  int64_t again;   // this thread's one of the first step, read again
+  bool differs;    // of the others
+
+  __device__ __forceinline__ Chunk(const Params& p, bool guess) : settled(!guess || p.batch > 32 * THREADS) {
+    if (settled) pdl_wait();
+  }
+  __device__ __forceinline__ bool any() const { return n > 0 && a >= 0; }
+
+  // rows: row indexes into x, y and out
+  __device__ __forceinline__ void find(const Params& p, int b, int j, int (&rows)[ROWS]) {
+    constexpr int WARPS = THREADS / 32;
+    __shared__ int s_seq[ROWS + 1], s_count[WARPS];
+    __shared__ int64_t s_adapter;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, T = p.tokens;
+    const int need = (ROWS - 1) / T + 2;  // sequences that a chunk can reach into, at most ROWS + 1
+    const int64_t mine = adapter_of(p, b, settled);
+    int before = 0, found = 0, i = 0;
+    seen = 0;
+    for (; i < p.batch && (i <= b || found < need); i += THREADS) {
+      const int q = i + tid;
+      const bool same = q < p.batch && (q == b || adapter_of(p, q, settled) == mine);
+      if (q == b) s_adapter = mine;
+      seen = seen << 1 | same;
+      const unsigned after = __ballot_sync(0xffffffffu, same && q >= b);
+      if (lane == 0) s_count[warp] = __popc(after);
+      before += __syncthreads_count(same && q < b);
+      int at = found;
+      for (int w = 0; w < WARPS; ++w) {
+        if (w == warp && same && q >= b) {
+          const int n = at + __popc(after & ((1u << lane) - 1));
+          if (n < need) s_seq[n] = q;
+        }
+        at += s_count[w];
       }
-      at += s_count[w];
+      found = at;
+      __syncthreads();
     }
-    found = at;
+    end = i;
+    a = s_adapter;
+    const int64_t first = (int64_t(before) * T + ROWS - 1) / ROWS * ROWS + int64_t(j) * ROWS;
+    const int64_t here = first - int64_t(before) * T;  // of sequence b's tokens
+    n = here >= T ? 0 : int(min(int64_t(ROWS), int64_t(min(found, need)) * T - here));
+    if (tid < ROWS && n > 0) {
+      const int g = int(here) + min(tid, n - 1);
+      rows[tid] = s_seq[g / T] * T + g % T;
+    }
     __syncthreads();
   }
-  const int64_t first = (int64_t(before) * T + ROWS - 1) / ROWS * ROWS + int64_t(j) * ROWS;
-  const int64_t here = first - int64_t(before) * T;  // of sequence b's tokens
-  if (here >= T) return 0;
-  const int64_t n = min(int64_t(ROWS), int64_t(min(found, need)) * T - here);
-  if (tid < ROWS) {
-    const int g = int(here) + min(tid, int(n) - 1);
-    rows[tid] = s_seq[g / T] * T + g % T;
+  __device__ __forceinline__ void ask_again(const Params& p) {
+    if (settled) return;
+    const int tid = threadIdx.x;
+    if (tid < p.batch) again = __ldcg(p.adapters + tid);
+    differs = false;
+    for (int i = end - THREADS, step = 0; i > 0; i -= THREADS, ++step)
+      differs |= (i + tid < p.batch && adapter_of(p, i + tid, true) == a) != bool(seen >> step & 1);
   }
-  __syncthreads();
-  return int(n);
-}
+  __device__ __forceinline__ bool changed(const Params& p) {  // a barrier
+    const bool same = int(threadIdx.x) < p.batch && (again >= 0 && again < p.n ? again : -1) == a;
+    const bool then = seen >> (end / THREADS - 1) & 1;
+    const bool now = __syncthreads_or(!settled && (differs || same != then));
+    settled = true;
+    return now;
+  }
+};
 
 // the column block that a column is in
 __device__ __forceinline__ int part_of(const Params& p, int column) {
@@ -224,30 +262,15 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
   const int cut = (cluster - chunk * p.fan) * C + rank;  // of the columns
   const int b = chunk / p.chunks;
   pdl_trigger();
-  const int64_t a = adapter_of(p, b);
-  const int n = a < 0 && p.out == p.y ? 0 : find_rows<ROWS, THREADS>(p, b, chunk - b * p.chunks, a, rows);
-  if (n == 0) {  // (every CTA of the cluster)
-    pdl_wait();
-    return;
-  }
-  // this CTA's columns
-  const int n0 = min(p.N, cut * p.width), n1 = min(p.N, n0 + p.width);
-  if (a < 0) {  // no adapter: the rows as they are
-    pdl_wait();
-    for (int m = 0; m < n; ++m) {
-      const int64_t at = int64_t(rows[m]) * p.N;
-      for (int c = n0 + 8 * tid; c < n1; c += 8 * THREADS)
-        *reinterpret_cast<uint4*>(p.out + at + c) = __ldcg(reinterpret_cast<const uint4*>(p.y + at + c));
-    }
-    return;
-  }
   const uint32_t base = smem_u32(smem);
   if (tid == 0) {
     bar_init(base + l.done);
     bar_expect(base + l.done, C * p.ranks * ROWS * 4);
   }
-  __syncthreads();
   cluster_arrive();
+  Chunk<ROWS, THREADS> at(p, true);
+  // this CTA's columns, and its part of K
+  const int n0 = min(p.N, cut * p.width), n1 = min(p.N, n0 + p.width);
   const int k0 = rank * p.k_slice, k_end = min(p.K, k0 + p.k_slice);
   const int units = p.ranks / 8;  // 16-byte units of a row of A
   auto load_a = [&](int step) {
@@ -256,7 +279,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
     int kk = tid >> l.a_shift;
     const int k = k0 + step * p.k_step;
     uint32_t to = base + l.a + (step & 1) * l.a_step + kk * p.a_pitch + c * 16;
-    const __half* from = p.A + (a * p.K + k + kk) * p.ranks + c * 8;
+    const __half* from = p.A + (at.a * p.K + k + kk) * p.ranks + c * 8;
     const int down = THREADS >> l.a_shift;
     for (; kk < p.k_step; kk += down) {
       const bool ok = k + kk < k_end;
@@ -271,7 +294,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
     const uint32_t to = base + l.x + (step & 1) * l.x_step + warp * l.x_pitch;
     const __half* from = p.x + int64_t(rows[warp]) * p.K + k;
     for (int c = lane * 8; c < p.k_step; c += 256) {
-      const bool ok = warp < n && k + c < k_end;
+      const bool ok = warp < at.n && k + c < k_end;
       copy16(to + c * 2, ok ? from + c : p.x, ok);
     }
   };
@@ -282,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
     if (column >= n1) return;
     int j = tid >> eighths;
     uint32_t to = base + l.b[step & 1] + (j * columns + c * 8) * 2;
-    const __half* from = p.B + (a * p.rank + j) * p.N + column;
+    const __half* from = p.B + (at.a * p.rank + j) * p.N + column;
     const int down = THREADS >> eighths;  // (a step has at most 256 pieces of 8: its ranks are 8 or more)
     for (; j < p.rank; j += down) {
       copy16(to, from, true);
@@ -290,64 +313,87 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
       from += int64_t(down) * p.N;
     }
   };
-  load_a(0);
-  load_a(1);
-  load_b(0);
-  copy_commit();
-  const float scale = p.scales[a];
-  pdl_wait();
-  load_x(0);
-  copy_commit();
-  load_x(1);
-  copy_commit();
-
   // a warp's tiles of 16 ranks, and which of the 16-wide steps along K are its own
   const int tiles = (p.ranks + 15) / 16;
   const int shares = tiles == 1 ? 8 : tiles == 2 ? 4 : tiles <= 4 ? 2 : 1;
-  float acc[2][4] = {};
   const int g = lane >> 2, q = lane & 3;
-  for (int step = 0; step < l.steps; ++step) {
-    copy_wait<1>();
-    __syncthreads();
-    const uint32_t as = base + l.a + (step & 1) * l.a_step, xs = base + l.x + (step & 1) * l.x_step;
+  float* const part = reinterpret_cast<float*>(smem + l.part);  // [share][ranks][8]
+  float scale = 0.f;
+  for (;;) {
+    at.find(p, b, chunk - b * p.chunks, rows);
+    if (at.any()) {
+      load_a(0);
+      load_a(1);
+      load_b(0);
+    }
+    copy_commit();
+    pdl_wait();
+    if (at.any()) {
+      load_x(0);
+      copy_commit();
+      load_x(1);
+      copy_commit();
+    }
+    at.ask_again(p);
+    if (at.any()) {
+      scale = __ldcg(p.scales + at.a);
+      float acc[2][4] = {};
+      for (int step = 0; step < l.steps; ++step) {
+        copy_wait<1>();
+        __syncthreads();
+        const uint32_t as = base + l.a + (step & 1) * l.a_step, xs = base + l.x + (step & 1) * l.x_step;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int item = warp + WARPS * i, tile = item % tiles, share = item / tiles;
-      if (share < shares) {
-        // matrices: (k 0-7, ranks 0-7), (k 0-7, ranks 8-15), (k 8-15, ranks 0-7), (k 8-15, ranks 8-15)
-        const uint32_t at = as + ((lane & 7) + 8 * (lane >> 4)) * p.a_pitch + tile * 32 + ((lane >> 3) & 1) * 16;
-        const uint32_t xt = xs + g * l.x_pitch + q * 4;
-        for (int k = share * 16; k < p.k_step; k += shares * 16) {
-          uint32_t w[4];
-          ldsm4_t(w, at + k * p.a_pitch);
-          mma_16816(acc[i], w[0], w[1], w[2], w[3], lds32(xt + k * 2), lds32(xt + k * 2 + 16));
+        for (int i = 0; i < 2; ++i) {
+          const int item = warp + WARPS * i, tile = item % tiles, share = item / tiles;
+          if (share < shares) {
+            // matrices: (k 0-7, ranks 0-7), (k 0-7, ranks 8-15), (k 8-15, ranks 0-7), (k 8-15, ranks 8-15)
+            const uint32_t at = as + ((lane & 7) + 8 * (lane >> 4)) * p.a_pitch + tile * 32 + ((lane >> 3) & 1) * 16;
+            const uint32_t xt = xs + g * l.x_pitch + q * 4;
+            for (int k = share * 16; k < p.k_step; k += shares * 16) {
+              uint32_t w[4];
+              ldsm4_t(w, at + k * p.a_pitch);
+              mma_16816(acc[i], w[0], w[1], w[2], w[3], lds32(xt + k * 2), lds32(xt + k * 2 + 16));
+            }
+          }
+        }
+        __syncthreads();
+        if (step + 2 < l.steps) {
+          load_a(step + 2);
+          load_x(step + 2);
+        }
+        copy_commit();
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int item = warp + WARPS * i, tile = item % tiles, share = item / tiles;
+        const int j = tile * 16 + g;
+        if (share < shares) {
+          float* to = part + (share * p.ranks + j) * ROWS + 2 * q;
+          if (j < p.ranks) *reinterpret_cast<float2*>(to) = make_float2(acc[i][0], acc[i][1]);
+          if (j + 8 < p.ranks) *reinterpret_cast<float2*>(to + 8 * ROWS) = make_float2(acc[i][2], acc[i][3]);
         }
       }
     }
+    if (!at.changed(p)) break;
+    copy_wait<0>();
     __syncthreads();
-    if (step + 2 < l.steps) {
-      load_a(step + 2);
-      load_x(step + 2);
+  }
+  const int n = at.n;
+  cluster_wait();  // every CTA has started
+  if (n == 0) return;  // (every CTA of the cluster)
+  if (at.a < 0) {      // no adapter: the rows as they are
+    if (p.out == p.y) return;
+    for (int m = 0; m < n; ++m) {
+      const int64_t row = int64_t(rows[m]) * p.N;
+      for (int c = n0 + 8 * tid; c < n1; c += 8 * THREADS)
+        *reinterpret_cast<uint4*>(p.out + row + c) = __ldcg(reinterpret_cast<const uint4*>(p.y + row + c));
     }
-    copy_commit();
+    return;
   }
   // a step of B that has landed stays where it is; the next takes A's place
   const int b_steps = (n1 - n0 + columns - 1) / columns;
   load_b(1);
   copy_commit();
-  float* const part = reinterpret_cast<float*>(smem + l.part);  // [share][ranks][8]
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int item = warp + WARPS * i, tile = item % tiles, share = item / tiles;
-    const int j = tile * 16 + g;
-    if (share < shares) {
-      float* to = part + (share * p.ranks + j) * ROWS + 2 * q;
-      if (j < p.ranks) *reinterpret_cast<float2*>(to) = make_float2(acc[i][0], acc[i][1]);
-      if (j + 8 < p.ranks) *reinterpret_cast<float2*>(to + 8 * ROWS) = make_float2(acc[i][2], acc[i][3]);
-    }
-  }
-  __syncthreads();
-  cluster_wait();  // every CTA has started
   // this CTA's partial h to every CTA: thread (4 values, CTA)
   for (int i = tid; i < p.ranks * 2 * C; i += THREADS) {
     const int v = i / C, r = i % C;
@@ -490,19 +536,6 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
   const int rank = blockIdx.x % C, cluster = blockIdx.x / C, chunk = cluster / p.fan;
   const int cut = (cluster - chunk * p.fan) * C + rank;  // of the columns
   const int b = chunk / p.chunks;
-  const int64_t a = adapter_of(p, b);
-  const int n = a < 0 && p.out == p.y ? 0 : find_rows<ROWS, THREADS>(p, b, chunk - b * p.chunks, a, rows);
-  pdl_wait();
-  if (n == 0) return;  // (every CTA of the cluster)
-  if (a < 0) {         // no adapter: the rows as they are
-    const int n0 = min(p.N, cut * p.width), n1 = min(p.N, n0 + p.width);
-    for (int m = warp; m < n; m += WARPS) {
-      const int64_t at = int64_t(rows[m]) * p.N;
-      for (int c = n0 + 8 * lane; c < n1; c += 8 * 32)
-        *reinterpret_cast<uint4*>(p.out + at + c) = __ldcg(reinterpret_cast<const uint4*>(p.y + at + c));
-    }
-    return;
-  }
   const Layout l = layout(p, ROWS);
   const uint32_t base = smem_u32(smem);
   if (tid == 0) {
@@ -513,7 +546,23 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
   }
   __syncthreads();
   cluster_arrive();
-  const float scale = p.scales[a];
+  Chunk<ROWS, THREADS> at(p, false);
+  at.find(p, b, chunk - b * p.chunks, rows);
+  const int n = at.n;
+  const int64_t a = at.a;
+  if (n == 0 || a < 0) {  // (every CTA of the cluster)
+    cluster_wait();
+    if (n == 0 || p.out == p.y) return;
+    // no adapter: the rows as they are
+    const int n0 = min(p.N, cut * p.width), n1 = min(p.N, n0 + p.width);
+    for (int m = warp; m < n; m += WARPS) {
+      const int64_t row = int64_t(rows[m]) * p.N;
+      for (int c = n0 + 8 * lane; c < n1; c += 8 * 32)
+        *reinterpret_cast<uint4*>(p.out + row + c) = __ldcg(reinterpret_cast<const uint4*>(p.y + row + c));
+    }
+    return;
+  }
+  const float scale = __ldcg(p.scales + a);
 
   // ---- h of this CTA's part of K
   const int k0 = min(p.K, rank * p.k_slice), k1 = min(p.K, k0 + p.k_slice);
@@ -615,7 +664,6 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
     }
     __syncthreads();  // the ring is free
   }
-
   // ---- this CTA's columns: its share of the 32-column blocks (a block is of one part)
   int total = 0;
   for (int i = 0; i < p.parts; ++i) total += (p.edge[i + 1] - p.edge[i] + 31) / 32;
@@ -864,17 +912,19 @@ bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
   return p < q + uintptr_t(b_bytes) && q < p + uintptr_t(a_bytes);
 }
 
-constexpr int FEW_TOKENS = 8;  // tokens of a sequence up to which 8-row chunks do them
-
 // Clusters of a chunk: doubled while a CTA has more than `columns` columns, up to 8 and up to
-// the 32 in all that run at once.  Measured (rank 16, K 4096, 24576 columns, us by 1 / 8
+// those in all that run at once.  Measured (rank 16, K 4096, 24576 columns, us by 1 / 8
 // clusters a chunk): 8 tokens 15.9 / 6.0, 16 tokens 20.0 / 9.6, 128 tokens 23.3 / 13.1; one token
 // and 6144 columns: 4.9 with 1, 5.0 with 2, 5.1 with 4.
-void spread(Params& p, int columns) {
+void spread(Params& p, int columns, int at_once) {
   p.fan = 1;
-  while (p.fan < 8 && int64_t(p.batch) * p.chunks * p.fan * 2 <= 32 && p.N / (C * p.fan) > columns) p.fan *= 2;
+  while (p.fan < 8 && int64_t(p.batch) * p.chunks * p.fan * 2 <= at_once && p.N / (C * p.fan) > columns) p.fan *= 2;
   p.width = ((p.N + C * p.fan - 1) / (C * p.fan) + 7) / 8 * 8;
 }
+
+// Clusters that run at once where two CTAs fit an SM, and where one does (148 SMs)
+constexpr int AT_ONCE_BY_TWO = 32, AT_ONCE = 15;
+constexpr int HALF_SMEM = 115000;  // dynamic shared memory of which an SM has room for two
 
 // C CTAs for every cluster of every chunk that may start in a sequence
 template <typename... Args>
@@ -918,15 +968,28 @@ int launch(void (*kernel)(Args...), int threads, const Params& p, int smem, cuda
   return check_launch("multi_lora_add");
 }
 
-int launch_few(Params& p, cudaStream_t st) {
+// 8-row chunks, for sequences of up to FEW_TOKENS.  Where only one of their CTAs fits an SM (128
+// ranks in all and more) the other kernel does them, unless a block has more than 64 ranks, which
+// it takes piece by piece.  Measured (a decode step of 1 / 8 / 32 sequences with an adapter each,
+// us here / there): 3 x 32 ranks and 6144 columns 8.7 / 12.6, 10.0 / 16.9, 15.8 / 21.8; 2 x 64
+// and 24576 12.5 / 14.8, 24 / 23.4, 73 / 43; 2 x 128 25.9 / 34.9, 59 / 84, 179 / 245.
+constexpr int FEW_TOKENS = 8;
+
+bool plan_few(Params& p, few::Layout* l) {
   using namespace few;
+  if (p.tokens > FEW_TOKENS) return false;
   p.chunks = (p.tokens + ROWS - 1) / ROWS;
   const int most = std::min(MAX_STEP, A_BYTES / p.a_pitch / 16 * 16);
   const int steps = (p.k_slice + most - 1) / most;
   p.k_step = ((p.k_slice + steps - 1) / steps + 15) / 16 * 16;
-  spread(p, 1024 / int(std::min<int64_t>(ROWS, int64_t(p.batch) * p.tokens)));
-  const Layout l = layout(p);
-  return launch(multi_lora_rows_kernel, THREADS, p, l.total, st, p, l);
+  const int columns = 1024 / int(std::min<int64_t>(ROWS, int64_t(p.batch) * p.tokens));
+  spread(p, columns, AT_ONCE_BY_TWO);
+  *l = layout(p);
+  if (l->total <= HALF_SMEM) return true;
+  if (p.rank <= many::RANKS) return false;
+  spread(p, columns, AT_ONCE);
+  *l = layout(p);
+  return true;
 }
 
 // Rows up to which chunks of 64 are 18 clusters at most, so that an SM has one CTA: then
@@ -938,9 +1001,10 @@ int launch_many(Params& p, cudaStream_t st) {
   const int ks = (p.rank + 15) / 16;
   const int rows = int64_t(p.batch) * p.tokens <= SMALL_ROWS && ks <= 4 ? 32 : 64;
   p.chunks = (p.tokens + rows - 1) / rows;
-  spread(p, 256);
   const int here = std::min(RANKS, p.ranks);
   p.a_pitch = here * 2 + (here / 8 % 2 ? 0 : 16);
+  const int smem = layout(p, rows).total;
+  spread(p, 256, smem > HALF_SMEM ? AT_ONCE : AT_ONCE_BY_TWO);
   void (*kernel)(Params);
   if (rows == 32)
     kernel = ks == 1 ? multi_lora_tile_kernel<1, 32> : ks == 2 ? multi_lora_tile_kernel<2, 32> : multi_lora_tile_kernel<4, 32>;
@@ -949,7 +1013,7 @@ int launch_many(Params& p, cudaStream_t st) {
              : ks == 2 ? multi_lora_tile_kernel<2, 64>
              : ks <= 4 ? multi_lora_tile_kernel<4, 64>
                        : multi_lora_tile_kernel<0, 64>;
-  return launch(kernel, THREADS, p, layout(p, rows).total, st, p);
+  return launch(kernel, THREADS, p, smem, st, p);
 }
 
 }  // namespace mlora
@@ -976,7 +1040,8 @@ extern "C" int qx_multi_lora_add(const void* y, const void* x, const void* lora_
              "multi_lora_add: bad sizes batch=%d tokens=%d K=%d N=%d adapters=%d", batch, tokens, K, N, num_adapters);
   QX_REQUIRE(batch <= MAX_BATCH, "multi_lora_add: batch=%d is above %d (rows of one adapter go together as [batch, tokens])",
              batch, MAX_BATCH);
-  QX_REQUIRE(K % 8 == 0 && N % 8 == 0, "multi_lora_add: K=%d and N=%d must be multiples of 8", K, N);
+  QX_REQUIRE(K % 8 == 0 && N % 8 == 0 && K <= 1 << 30 && N <= 1 << 30,
+             "multi_lora_add: K=%d and N=%d must be multiples of 8 and at most 2^30", K, N);
   QX_REQUIRE(num_splits >= 0 && num_splits <= MAX_PARTS && (num_splits == 0 || splits),
              "multi_lora_add: %d column blocks (at most %d)", num_splits, MAX_PARTS);
   Params p{};
@@ -1023,6 +1088,8 @@ extern "C" int qx_multi_lora_add(const void* y, const void* x, const void* lora_
   p.n = num_adapters;
   p.a_pitch = p.ranks * 2 + (p.ranks / 8 % 2 ? 0 : 16);
   p.k_slice = ((K + C - 1) / C + 15) / 16 * 16;
-  return tokens <= FEW_TOKENS ? launch_few(p, reinterpret_cast<cudaStream_t>(stream))
-                              : launch_many(p, reinterpret_cast<cudaStream_t>(stream));
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  few::Layout l;
+  if (plan_few(p, &l)) return launch(few::multi_lora_rows_kernel, few::THREADS, p, l.total, st, p, l);
+  return launch_many(p, st);
 }

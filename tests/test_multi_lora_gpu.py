@@ -247,3 +247,36 @@ def test_cold_y_behind_a_short_product(C, r, b, t):
     for i in range(3):
         flush.fill_(i)
         check(C.multi_lora_add(**d, splits=splits), d, splits)
+
+
+@pytest.mark.parametrize("b,t", [(1, 1), (7, 1), (300, 1), (600, 2), (9000, 1), (3, 40), (300, 12)])
+def test_adapters_written_by_the_kernel_before(C, b, t):
+    """a kernel that lets the next one in while it runs writes the ids: the ones that count are the new ones"""
+    import ctypes
+    from qextract_infer_b200 import _lib
+    lib, splits = _lib.load(), (40, 24)
+    d = inputs(b, t, 136, splits, 8, 11, seed=b + t)
+    logits = [torch.randn(b, 13, generator=torch.Generator(device="cuda").manual_seed(i), device="cuda").half() for i in range(3)]
+    want = []
+    for l in logits:
+        ids = C.sample_logits(l, torch.zeros(b, device="cuda"), 0.0)[0]
+        assert torch.equal(ids, l.float().argmax(1))
+        want.append(C.multi_lora_add(**{**d, "adapters": ids}, splits=splits))
+    torch.cuda.synchronize()
+    u, lp, ids = torch.zeros(b, device="cuda"), torch.empty(b, device="cuda"), torch.zeros(b, dtype=torch.int64, device="cuda")
+    d["adapters"] = ids
+    outs = [torch.empty_like(d["y"]) for _ in range(12)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        st = torch.cuda.current_stream().cuda_stream
+        for i, out in enumerate(outs):
+            _lib.check(lib.qx_sample_logits(logits[i % 3].data_ptr(), u.data_ptr(), None, None, None, None, 0.0, 0, 1.0, 0.0,
+                                            ids.data_ptr(), lp.data_ptr(), b, 13, ctypes.c_void_p(st)), "sample_logits")
+            C.multi_lora_add(**d, splits=splits, out=out)
+    for _ in range(3):
+        for out in outs:
+            out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want[i % 3]) for i, out in enumerate(outs))
+    C.check_device_error()

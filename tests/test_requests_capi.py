@@ -22,7 +22,7 @@ def _lora(lib, y=Y, x=X, a=A, b=B, ids=IDS, scales=SCALES, out=OUT, batch=2, tok
 
 @pytest.mark.parametrize("bad,msg", [
     (dict(batch=-1), "bad sizes"), (dict(tokens=-1), "bad sizes"), (dict(k=0), "bad sizes"), (dict(n=0), "bad sizes"),
-    (dict(adapters=-1), "bad sizes"), (dict(k=60), "multiples of 8"), (dict(n=60), "multiples of 8"),
+    (dict(adapters=-1), "bad sizes"), (dict(k=60), "multiples of 8"), (dict(k=(1 << 30) + 8), "2^30"), (dict(n=60), "multiples of 8"),
     (dict(rank=4), "rank"), (dict(rank=12), "rank"), (dict(rank=264), "rank"), (dict(rank=72, splits=[16] * 4), "rank"),
     (dict(splits=[8] * 5), "column blocks"), (dict(splits=[32, 36]), "columns"), (dict(splits=[64, 0]), "columns"),
     (dict(splits=[32, 24]), "cover"), (dict(splits=[64, 8]), "exceed"), (dict(splits=[-64, 128]), "columns"),
