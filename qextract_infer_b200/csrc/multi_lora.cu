@@ -214,7 +214,11 @@ __device__ __forceinline__ int part_of(const Params& p, int column) {
 // rows are the ranks) and the chunk's rows as the 8 columns: an instruction covers
 // 16 ranks x 16 of K for every row.  Then thread by thread 4 columns of a row in fp32.
 // Bound by the weights' bytes where every row has its own adapter, else by the chain of
-// latencies: adapters, A, x, the exchange, y.
+// latencies: adapters, A, x, the exchange, y.  Measured: one token of 4096 x 6144, 3 x 16
+// ranks, 5.3 us (its bytes alone 0.1); 32 tokens with an adapter each, 4096 x 24576, 2 x 16
+// ranks, 11.5 us, 3.2 TB/s (5.6); there the two phases' loads take turns, as A's place takes
+// B's second step: all of B ahead leaves an SM one CTA, asked into L2 ahead 11.6, by bulk copies 11.7
+// (10.9 then).
 namespace few {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
@@ -470,10 +474,18 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
 // time.  CTA i of the cluster adds the partial sums of its eighth of the rows and gives them
 // to all as two fp16 numbers, high and low (22 bits), of h 2^-e with e from the row's
 // largest of that column block: any fp32 range, and a second product instead of a rounding
-// of h to 11 bits.  Then a warp takes 32 columns at a time for all rows; the y of the next one or two blocks of columns is on its way
-// into shared memory meanwhile (a lane's own 16-byte pieces, refilled as they are used).
-// Within the 32 columns the product's columns stand in the order in which a thread gets 8
-// neighbouring ones, so y and out move 16 bytes a lane.
+// of h to 11 bits.  Then a warp takes 32 columns at a time for all rows; the y of the next
+// one or two blocks of columns is on its way into shared memory meanwhile (a lane's own
+// 16-byte pieces, refilled as they are used).  Within the 32 columns the product's columns
+// stand in the order in which a thread gets 8 neighbouring ones, so y and out move 16 bytes
+// a lane.
+//
+// Measured: 2048 tokens of 12288 x 4096, 64 ranks, 37.5 us, 2.3 TB/s (its bytes alone 13.1).
+// Of a CTA's 64K cycles h takes 31K (its loads alone 26K: A comes from L2 for each chunk;
+// its products alone 17K, 12K of them the rate of mma.sync), waiting for the cluster's
+// slowest CTA 9K (256 CTAs on 148 SMs), the columns 12K.  Chunks of 128 rows leave an SM one
+// CTA, and of 16 such clusters 15 run at once: 72 us.  999 tokens of 2560 x 9728, 8 ranks:
+// 15.7 us, 2.8 TB/s (6.8): launch, five steps along K, the two exchanges, then the columns.
 //
 // It launches nothing early: with the next call's clusters waiting on the SMs a 2048-token
 // chunk took 55.7 us instead of 40.6.  Two CTAs an SM: of clusters of 8 with an SM a CTA

@@ -21,6 +21,12 @@
 // and the prefix sums run over threads, warps and CTAs.  Whoever owns the border in question
 // (the k-th token, top_p of the weight, u of the weight) tells all CTAs: its warp looks
 // at the thread's values again, a lane a value.
+//
+// Bound by a chain of latencies, not by bytes: measured 12.6 to 14.1 us for one row of 151936
+// (16 CTAs), 12.9 for 7 rows of 32003, 18.1 to 19.9 for 32 rows of 151936 (4 CTAs a row, 0.5
+// TB/s; their bytes alone 1.5).  Of the 32 rows' time a quarter is loading and counting, then
+// come the counters through distributed shared memory, the weights, and a border 1.5 us each:
+// the owner's warp, a send, and the wait of all.
 #include <mutex>
 
 #include "qx_b200.h"
@@ -703,8 +709,8 @@ int launch(Params& p, int batch, cudaStream_t st) {
 }
 
 // The largest cluster with which the whole batch runs at once (7 rows by 16 CTAs, 15 by 8, 32 by 4 on a B200 of 148
-// SMs), else 4.  Measured at 151936 tokens, us by 16 / 8 / 4 CTAs: 1 row 13.6 / 14.3 / 17.4,
-// 8 rows 25.6 / 14.9 / 18.1, 16 rows 38 / 27 / 18.3, 64 rows 123 / 65 / 36.
+// SMs), else 4.  Measured at 151936 tokens with 1024 threads a CTA, us by 16 / 8 / 4 CTAs: 1 row
+// 13.6 / 14.3 / 17.4, 8 rows 25.6 / 14.9 / 18.1, 16 rows 38 / 27 / 18.3, 64 rows 123 / 65 / 36.
 int choose(Params& p, int batch, cudaStream_t st) {
   int at16 = 0, at8 = 0, at4 = 0;
   if (const int rc = prepare<16>(&at16); rc != QX_OK) return rc;
