@@ -280,3 +280,15 @@ def test_adapters_written_by_the_kernel_before(C, b, t):
         torch.cuda.synchronize()
         assert all(torch.equal(out, want[i % 3]) for i, out in enumerate(outs))
     C.check_device_error()
+
+
+@pytest.mark.parametrize("r,splits", [(8, (264,)), (64, (136, 256)), (24, (40, 600, 72)), (128, (264,))])
+@pytest.mark.parametrize("t", [1, 5, 9, 100])
+def test_a_row_has_the_same_bits_in_any_batch(C, r, splits, t):
+    """few and many rows a call: other chunks, other clusters a chunk, the same sums"""
+    b = 24
+    d = inputs(b, t, 520, splits, r, 3, seed=r + t)
+    whole = C.multi_lora_add(**d, splits=splits)
+    for i in (0, 11, 23):
+        one = {n: v[i:i + 1].contiguous() if n in ("x", "y", "adapters") else v for n, v in d.items()}
+        assert torch.equal(C.multi_lora_add(**one, splits=splits)[0], whole[i])
