@@ -14,12 +14,15 @@
 // Whole logits (qx_lm_head_logits): kernel 1 with the fp16 values stored instead of
 // compared, 32 rows a launch.
 //
-// Bound by the weights' bytes.  Measured for 1 / 32 rows of 4096 x 151936 and 1 row of
-// 4096 x 37984 (us, tiles K x columns): 64 x 256 in two stages 189 / 222 / 59, 32 x 256 in
-// four 208 / 238 / 66, 64 x 128 in two 172 / 196 / 59, in three 171 / 188 / 54 (kept; 7.3
-// TB/s), in four (two CTAs an SM) 190 / 208 / 63.  The next kernel is let in at the end:
-// earlier, its CTAs fill the slots as they come free, three on one SM and one on another
-// (the slice: 54 us, 48 without).
+// Bound by the weights' bytes: 1 / 17 / 32 rows of 4096 x 151936 take 173 / 180 / 184 us (7.2 to
+// 6.8 TB/s), of 4096 x 37984 46.8 / 55.1 / 56.4 (297 CTAs: one SM has three, the others two).  With
+// more than 16 rows a tile's time counts: addresses that only move on, instead of each piece's own
+// (198 instructions a warp and tile, 81 of them for the second 16 rows), took 32 rows from 194 to 184 us.
+// Measured before that for 1 / 32 rows of 4096 x 151936 and 1 row of 4096 x 37984 (us,
+// tiles K x columns): 64 x 256 in two stages 189 / 222 / 59, 32 x 256 in four 208 / 238 / 66, 64 x
+// 128 in two 172 / 196 / 59, in three 171 / 188 / 54 (kept), in four (two CTAs an SM) 190 / 208 /
+// 63; eight warps of 16 columns 175 / 197 / 51 (48 with four).  The next kernel is let in at the end: earlier, its CTAs
+// fill the slots as they come free, three on one SM and one on another (the slice: 54 us, 48 without).
 #include <algorithm>
 #include <cfloat>
 #include <mutex>
@@ -92,23 +95,28 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restric
   const uint32_t sbase = smem_u32(smem);
   const int ktiles = H / KT;
 
-  auto issue = [&](int kt, int stage) {
-    const uint32_t ws = sbase + stage * STAGE, hs = ws + W_TILE;
-    // W: 64 rows x 16 chunks of 16 B = 1024 chunks, 8 per thread
+  // a thread's 16-byte pieces of a tile: W rows tid / 16 + 8 i (64 x 16 pieces in all; those past V and rows past B
+  // read as zero), h rows tid / 8 + 16 i (8 pieces each)
+  static_assert(THREADS == COLS && THREADS == 16 * (KT / 8), "a thread's pieces stand under one another");
+  const int w_col = n0 + (tid % 16) * 8, h_row = tid / 8;
+  const int w_bytes = w_col < V ? 16 : 0;  // V % 8 == 0: a piece is all in or all out
+  const __half* w_from = W + size_t(tid / 16) * V + (w_bytes ? w_col : 0);
+  const size_t w_down = size_t(8) * V;
+  const __half* h_from[MT];
 #pragma unroll
-    for (int i = 0; i < (KT * (COLS / 8)) / THREADS; ++i) {
-      const int idx = i * THREADS + tid, r = idx / (COLS / 8), ch = idx % (COLS / 8);
-      const int col = n0 + ch * 8;
-      const bool ok = col < V;  // V % 8 == 0: a chunk is all in or all out
-      const __half* src = W + (size_t(kt) * KT + r) * V + (ok ? col : 0);
-      cp_async16(ws + wswz(r, ch), src, ok ? 16 : 0);
+  for (int m = 0; m < MT; ++m) h_from[m] = h + size_t(h_row + 16 * m < B ? h_row + 16 * m : 0) * H + (tid % 8) * 8;
+  const uint32_t w_to = sbase + wswz(tid / 16, tid % 16), h_to = sbase + W_TILE + h_row * HROW + (tid % 8) * 16;
+  auto issue = [&](int stage) {  // the next tile along K
+    const uint32_t at = stage * STAGE;
+#pragma unroll
+    for (int i = 0; i < KT / 8; ++i) {
+      cp_async16(w_to + at + i * 8 * WROW, w_from, w_bytes);
+      w_from += w_down;
     }
-    // h: B rows x 8 chunks (rows past B read as zero)
-    for (int idx = tid; idx < MT * 16 * 8; idx += THREADS) {
-      const int r = idx >> 3, ch = idx & 7;
-      const bool ok = r < B;
-      const __half* src = h + size_t(ok ? r : 0) * H + size_t(kt) * KT + ch * 8;
-      cp_async16(hs + r * HROW + ch * 16, src, ok ? 16 : 0);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      cp_async16(h_to + at + m * 16 * HROW, h_from[m], h_row + 16 * m < B ? 16 : 0);
+      h_from[m] += KT;
     }
     cp_async_commit();
   };
@@ -122,27 +130,30 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restric
   pdl_wait();  // h comes from the previous kernel
 #pragma unroll
   for (int i = 0; i < STAGES; ++i) {
-    if (i < ktiles) issue(i, i);
+    if (i < ktiles) issue(i);
     else cp_async_commit();
   }
   const int mi = lane >> 3, ri = lane & 7;
+  // a lane's rows of the fragments: h (rows 0-7 | 8-15) x (k 0-7 | 8-15), W (k 0-7 | 8-15) x (columns 0-7 | 8-15)
+  const uint32_t a_at = sbase + W_TILE + ((mi & 1) * 8 + ri) * HROW + (mi >> 1) * 16;
+  uint32_t b_at[NJ / 2];
+#pragma unroll
+  for (int jj = 0; jj < NJ / 2; ++jj)
+    b_at[jj] = sbase + ((mi & 1) * 8 + ri) * WROW + (((warp * WCOLS + jj * 16) / 8 + (mi >> 1)) ^ ri) * 16;
+  int stage = 0;
   for (int kt = 0; kt < ktiles; ++kt) {
     cp_async_wait<STAGES - 1>();
     __syncthreads();
-    const uint32_t ws = sbase + (kt % STAGES) * STAGE, hs = ws + W_TILE;
+    const uint32_t at = stage * STAGE;
 #pragma unroll
     for (int ks = 0; ks < KT / 16; ++ks) {
-      // A fragments (h rows m*16.., k ks*16..): matrices (rows 0-7 | 8-15) x (k 0-7 | 8-15)
       uint32_t a[MT][4];
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-        ldsm_x4(a[m], hs + (m * 16 + (mi & 1) * 8 + ri) * HROW + (ks * 16 + (mi >> 1) * 8) * 2);
-      // B fragments: k16 x n8 of W for this warp's n-tiles (two per ldmatrix.x4.trans)
+      for (int m = 0; m < MT; ++m) ldsm_x4(a[m], a_at + at + m * 16 * HROW + ks * 32);
 #pragma unroll
       for (int jj = 0; jj < NJ / 2; ++jj) {
         uint32_t bw[4];
-        const int ch = (warp * WCOLS + jj * 16) / 8 + (mi >> 1);
-        ldsm_x4_t(bw, ws + wswz(ks * 16 + (mi & 1) * 8 + ri, ch));
+        ldsm_x4_t(bw, b_at[jj] + at + ks * 16 * WROW);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           mma_16816(acc[m][2 * jj], a[m][0], a[m][1], a[m][2], a[m][3], bw[0], bw[1]);
@@ -151,8 +162,9 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restric
       }
     }
     __syncthreads();
-    if (kt + STAGES < ktiles) issue(kt + STAGES, kt % STAGES);
+    if (kt + STAGES < ktiles) issue(stage);
     else cp_async_commit();
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
   }
   cp_async_wait<0>();
   pdl_trigger();
