@@ -272,6 +272,10 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
     bar_expect(base + l.done, C * p.ranks * ROWS * 4);
   }
   cluster_arrive();
+  // The first columns of B are asked for at once by a few clusters, by more of them behind x, so that the
+  // products do not wait for B's bytes too (us, B first / behind, rank 16, K 4096: one token, 6144
+  // columns 5.3 / 5.6; 32 tokens with an adapter each, 4096 columns 9.8 / 9.1, 8192 9.4 / 8.7, 24576 11.6 / 11.4).
+  const bool late = gridDim.x > 8 * C;
   Chunk<ROWS, THREADS> at(p, true);
   // this CTA's columns, and its part of K
   const int n0 = min(p.N, cut * p.width), n1 = min(p.N, n0 + p.width);
@@ -328,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
     if (at.any()) {
       load_a(0);
       load_a(1);
-      load_b(0);
+      if (!late) load_b(0);
     }
     copy_commit();
     pdl_wait();
@@ -337,13 +341,16 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
       copy_commit();
       load_x(1);
       copy_commit();
+      if (late) load_b(0);
+      copy_commit();
     }
     at.ask_again(p);
     if (at.any()) {
       scale = __ldcg(p.scales + at.a);
       float acc[2][4] = {};
       for (int step = 0; step < l.steps; ++step) {
-        copy_wait<1>();
+        if (step < 2) copy_wait<2>();  // all but the next step and B
+        else copy_wait<1>();
         __syncthreads();
         const uint32_t as = base + l.a + (step & 1) * l.a_step, xs = base + l.x + (step & 1) * l.x_step;
 #pragma unroll
