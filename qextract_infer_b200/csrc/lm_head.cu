@@ -14,10 +14,12 @@
 // Whole logits (qx_lm_head_logits): kernel 1 with the fp16 values stored instead of
 // compared, 32 rows a launch.
 //
-// Bound by the weights' bytes: 1 / 17 / 32 rows of 4096 x 151936 take 173 / 180 / 184 us (7.2 to
-// 6.8 TB/s), of 4096 x 37984 46.8 / 55.1 / 56.4 (297 CTAs: one SM has three, the others two).  With
-// more than 16 rows a tile's time counts: addresses that only move on, instead of each piece's own
-// (198 instructions a warp and tile, 81 of them for the second 16 rows), took 32 rows from 194 to 184 us.
+// Bound by the weights' bytes: 1 / 17 / 32 rows of 4096 x 151936 take 172 / 177 / 181 us (7.2 to
+// 6.9 TB/s), of 4096 x 37984 48.2 / 51.6 / 52.8 (297 CTAs: one SM has three, the others two).  With
+// more rows a tile's own time counts: addresses that only move on, instead of each piece's own
+// (198 instructions a warp and tile at 17 rows, 117 at 16), took 32 rows from 194 to 184 us; h through
+// L1, where an SM's CTAs meet and not all CTAs at the same lines of L2, from 184 to 181, of the slice from
+// 56.4 to 52.8.
 // Measured before that for 1 / 32 rows of 4096 x 151936 and 1 row of 4096 x 37984 (us,
 // tiles K x columns): 64 x 256 in two stages 189 / 222 / 59, 32 x 256 in four 208 / 238 / 66, 64 x
 // 128 in two 172 / 196 / 59, in three 171 / 188 / 54 (kept), in four (two CTAs an SM) 190 / 208 /
@@ -57,6 +59,10 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int src_bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes));
+}
+// the same through L1: the SM's CTAs read the same rows of h at about the same time
+__device__ __forceinline__ void cp_async16_l1(uint32_t dst, const void* src, int src_bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes));
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;"); }
 template <int N>
@@ -115,7 +121,7 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restric
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      cp_async16(h_to + at + m * 16 * HROW, h_from[m], h_row + 16 * m < B ? 16 : 0);
+      cp_async16_l1(h_to + at + m * 16 * HROW, h_from[m], h_row + 16 * m < B ? 16 : 0);
       h_from[m] += KT;
     }
     cp_async_commit();
