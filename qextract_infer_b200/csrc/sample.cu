@@ -40,7 +40,9 @@ namespace smp {
 constexpr int threads_of(int c) { return c >= 8 ? 512 : 1024; }
 constexpr int VALUES = 65536;
 constexpr int HIST_BYTES = VALUES * 2;
-constexpr int SLICE_MAX = 47104;  // logits of a CTA: they stay in shared memory, and a 16-bit counter holds them all
+constexpr int GROUP = 8, GROUPS = VALUES / GROUP, WORDS = GROUPS / 32;  // values that are counted, joined and weighed together
+// logits of a CTA: they stay in shared memory, and a 16-bit counter holds them all
+constexpr int slice_max(int c) { return c == 16 ? 32768 : c == 8 ? 43008 : 45056; }
 constexpr int VOCAB_MAX = 524224;
 constexpr int FRAC = 43;
 constexpr unsigned NONE = ~0u;
@@ -58,7 +60,7 @@ struct Params {
   int vocab, slice;
 };
 
-constexpr int RUNS = SLICE_MAX / 256;  // of 256 logits in the largest slice
+constexpr int RUNS = slice_max(4) / 256;  // of 256 logits in the largest slice
 
 enum Exchange { USED, TOTALS, TOP_K, LIMITS, PICK, EXCHANGES };
 
@@ -70,9 +72,13 @@ struct Shared {
   alignas(16) u64 p_run[2];     // tokens and weight of the run that top_p leaves
   alignas(16) u64 m_run[C][2];  // those before the first value of each CTA that is too light for min_p
   u64 k_mass, pick;
-  unsigned used[C][VALUES / 8 / C / 32];  // of each CTA: which groups of 8 of this CTA's values occur
+  alignas(16) unsigned used[C][WORDS];  // of each CTA: which groups occur
   unsigned top[C];
   // this CTA's
+  alignas(16) unsigned mine[WORDS];  // its row of `used`
+  unsigned any[WORDS];               // the groups that occur in the row
+  unsigned short upto[WORDS];        // how many of them up to a word's end
+  unsigned short words_upto[WORDS / 32];
   u64 warp_mass[threads_of(C) / 32];
   unsigned warp_count[threads_of(C) / 32];
   unsigned top_here, m_here, found, found_nth;
@@ -104,6 +110,11 @@ __device__ __forceinline__ void send(const unsigned* p, const u64* done, int ran
 __device__ __forceinline__ void send(const u64* p, const u64* done, int rank, u64 a, u64 b) {
   asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(at_rank(p, rank)),
                "l"(a), "l"(b), "r"(at_rank(done, rank))
+               : "memory");
+}
+__device__ __forceinline__ void send(const unsigned* p, const u64* done, int rank, const uint4& a) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at_rank(p, rank)),
+               "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(at_rank(done, rank))
                : "memory");
 }
 __device__ __forceinline__ void expect(const u64* done, unsigned bytes) {
@@ -235,7 +246,8 @@ __device__ __forceinline__ unsigned top_of(uint32_t pair) {
 template <int C>
 __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_constant__ Params p) {
   constexpr int THREADS = threads_of(C), WARPS = THREADS / 32;
-  constexpr int OWN = VALUES / (C * THREADS);  // values of a thread
+  constexpr int Q = GROUPS / (C * THREADS), OWN = Q * GROUP;  // groups and values of a thread, at most
+  static_assert(Q >= 1 && OWN <= 32 && THREADS >= WORDS, "a thread's share");
   extern __shared__ __align__(16) unsigned char smem[];
   unsigned* const hist = reinterpret_cast<unsigned*>(smem);
   uint4* const slice = reinterpret_cast<uint4*>(smem + HIST_BYTES);
@@ -276,8 +288,8 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
 
   // ---- count the slice
   // A slice's logits matter only up to its own k-th largest, and that is not below the
-  // k-th largest of the threads' largest ones: a search over places, a count of the block
-  // each of 16 steps.  Without top_p nothing lighter than min_p matters (beside the slice's
+  // k-th largest of the threads' largest ones: a search over places, 16 of them together, a
+  // count of the block each of 12 steps.  Without top_p nothing lighter than min_p matters (beside the slice's
   // largest, all the more beside the row's).  Either leaves few logits to count.
   unsigned last = 0xFBFFu;  // the last place that is counted
   const bool by_k = k_row > 0 && k_row <= THREADS / 2, by_min = min_p > 0.0 && !(p_row < 1.f);
@@ -289,11 +301,11 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
     }
     const unsigned mine = top_of(best);
     if (by_k) {
-      unsigned low = 0;  // the least place with k_row threads whose top is not behind it
+      unsigned low = 0;  // the first of the 16 places that the k_row-th of the threads' tops is among
 #pragma unroll 1
-      for (unsigned bit = 0x8000u; bit; bit >>= 1)
+      for (unsigned bit = 0x8000u; bit >= 16; bit >>= 1)
         if (__syncthreads_count(mine < low + bit) < int(k_row)) low += bit;
-      last = min(last, low);
+      last = min(last, low + 15);
     }
     if (by_min) {
       const unsigned warp_top = __reduce_min_sync(0xffffffffu, mine);
@@ -331,54 +343,20 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
   if (lane == 0) atomicMin(&s.top_here, warp_top);
   __syncthreads();
   cluster_wait();  // every CTA has started
-  // what was counted before the __syncthreads is seen by whoever receives from these threads
-  if (lane == 0 || tid < C) asm volatile("fence.acq_rel.cluster;" ::: "memory");
-  if (tid == 0) expect(&s.done[USED], C * 4 + VALUES / 64);
-  if (tid < C) send(&s.top[rank], &s.done[USED], tid, s.top_here);
+  if (tid == 0) expect(&s.done[USED], C * (4 + 4 * WORDS));
 #pragma unroll
-  for (int i = 0; i < VALUES / 8 / THREADS; ++i) {
-    constexpr int WORDS = VALUES / 8 / C / 32;  // of a CTA's values
+  for (int i = 0; i < GROUPS / THREADS; ++i) {
     const uint4 v = reinterpret_cast<const uint4*>(hist)[i * THREADS + tid];
     const unsigned used = __ballot_sync(0xffffffffu, (v.x | v.y | v.z | v.w) != 0u);
-    const int word = i * WARPS + warp;
-    if (lane == 0) send(&s.used[rank][word % WORDS], &s.done[USED], word / WORDS, used);
+    if (lane == 0) s.mine[i * WARPS + warp] = used;
   }
+  __syncthreads();
+  // what was counted before the __syncthreads is seen by whoever receives from these threads
+  if (tid < C * (WORDS / 4)) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  if (tid < C) send(&s.top[rank], &s.done[USED], tid, s.top_here);
+  for (int i = tid; i < C * (WORDS / 4); i += THREADS)
+    send(&s.used[rank][i % (WORDS / 4) * 4], &s.done[USED], i / (WORDS / 4), reinterpret_cast<const uint4*>(s.mine)[i % (WORDS / 4)]);
   wait_for(&s.done[USED]);
-
-  // ---- the counters of the values that this CTA owns, of all CTAs
-  const unsigned first = unsigned(rank * THREADS + tid) * OWN;
-  constexpr int WORDS16 = OWN < 8 ? 1 : OWN / 8, WIDE = OWN < 8 ? OWN / 2 : 4;  // loads of a CTA's counters, words of one
-  uint32_t there[C][WORDS16][WIDE];
-#pragma unroll
-  for (int r = 0; r < C; ++r) {
-    const uint32_t at = at_rank(hist + first / 2, r);
-#pragma unroll
-    for (int i = 0; i < WORDS16; ++i) {
-#pragma unroll
-      for (int e = 0; e < WIDE; ++e) there[r][i][e] = 0u;
-      const int group = (tid * OWN) / 8 + i;
-      if (s.used[r][group >> 5] >> (group & 31) & 1) {
-        if constexpr (WIDE == 4)
-          asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(there[r][i][0]), "=r"(there[r][i][1]), "=r"(there[r][i][2]), "=r"(there[r][i][3])
-                       : "r"(at + 16 * i)
-                       : "memory");
-        else
-          asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(there[r][i][0]), "=r"(there[r][i][1]) : "r"(at) : "memory");
-      }
-    }
-  }
-  unsigned c[OWN];
-#pragma unroll
-  for (int i = 0; i < OWN / 2; ++i) {
-    c[2 * i] = c[2 * i + 1] = 0u;
-#pragma unroll
-    for (int r = 0; r < C; ++r) {
-      const uint32_t w = there[r][i / WIDE][i % WIDE];
-      c[2 * i] += w & 0xFFFFu;
-      c[2 * i + 1] += w >> 16;
-    }
-  }
   weights.place = s.top[0];
   for (int r = 1; r < C; ++r) weights.place = min(weights.place, s.top[r]);
   if (weights.place == NONE) {  // nothing to draw from
@@ -394,20 +372,95 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
   // (beside +inf nothing has weight, whatever the temperature)
   if (isinf(weights.top)) weights.top = 1e300, weights.scale = 1.0;
 
+  // ---- the groups that occur, dealt out in order, the same number to each CTA: one to a thread, Q where
+  // they are more than its threads.  (By equal shares of all values one CTA had most of those that occur.)
+  if (tid < WORDS) {
+    unsigned any = 0;
+#pragma unroll
+    for (int r = 0; r < C; ++r) any |= s.used[r][tid];
+    s.any[tid] = any;
+    unsigned n = __popc(any);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned t = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) n += t;
+    }
+    s.upto[tid] = n;
+    if (lane == 31) s.words_upto[warp] = n;
+  }
+  __syncthreads();
+  unsigned occur = 0, words_before[WORDS / 32];
+#pragma unroll
+  for (int i = 0; i < WORDS / 32; ++i) words_before[i] = occur, occur += s.words_upto[i];
+  const unsigned deal = (occur + C - 1) / C;  // to a CTA
+  const int share = Q > 1 && deal > THREADS ? Q : 1;
+  unsigned first[Q];  // values of the thread's groups
+  unsigned c[OWN];
+#pragma unroll
+  for (int k = 0; k < Q; ++k) {
+    const unsigned nth = tid * share + k, slot = rank * deal + nth;
+    first[k] = 0;
+#pragma unroll
+    for (int i = 0; i < GROUP; ++i) c[k * GROUP + i] = 0;
+    if (k >= share || nth >= deal || slot >= occur) continue;
+    // the word: of 32 words together, then of those
+    unsigned block = 0, left = slot;
+#pragma unroll
+    for (int i = 1; i < WORDS / 32; ++i)
+      if (slot >= words_before[i]) block = i, left = slot - words_before[i];
+    unsigned word = 0;  // the first with more than `left` up to its end
+#pragma unroll
+    for (int i = 16; i; i >>= 1)
+      if (s.upto[block * 32 + word + i - 1] <= left) word += i;
+    if (word) left -= s.upto[block * 32 + word - 1];
+    word += block * 32;
+    unsigned bits = s.any[word], bit = 0;
+#pragma unroll
+    for (int i = 16; i; i >>= 1) {
+      const unsigned low = __popc(bits & ((1u << i) - 1));
+      if (left >= low) left -= low, bits >>= i, bit += i;
+    }
+    first[k] = (word * 32 + bit) * GROUP;
+    // its counters of all CTAs
+    uint32_t there[C][4];
+#pragma unroll
+    for (int r = 0; r < C; ++r) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) there[r][e] = 0u;
+      if (s.used[r][word] >> bit & 1)
+        asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(there[r][0]), "=r"(there[r][1]), "=r"(there[r][2]), "=r"(there[r][3])
+                     : "r"(at_rank(hist + first[k] / 2, r))
+                     : "memory");
+    }
+#pragma unroll
+    for (int i = 0; i < GROUP / 2; ++i)
+#pragma unroll
+      for (int r = 0; r < C; ++r) {
+        c[k * GROUP + 2 * i] += there[r][i] & 0xFFFFu;
+        c[k * GROUP + 2 * i + 1] += there[r][i] >> 16;
+      }
+  }
+
   // ---- prefix sums of counts and weights; of those heavy enough for min_p, and whether some are not
   unsigned n_here = 0, n_heavy = 0;
   u64 mass_here = 0, mass_heavy = 0;
   bool light = false;
-  double w, ratio;
-  weights.start(first, w, ratio);
 #pragma unroll
-  for (int i = 0; i < OWN; ++i) {
-    weights.next(first, first + i, ratio, w);
-    if (c[i]) {
-      n_here += c[i];
-      mass_here += c[i] * fixed(w);
-      light |= !(w >= min_p);
-      if (!light) n_heavy = n_here, mass_heavy = mass_here;
+  for (int k = 0; k < Q; ++k) {
+    if (Q > 1 && k >= share) break;
+    double w, ratio;
+    weights.start(first[k], w, ratio);
+#pragma unroll
+    for (int i = 0; i < GROUP; ++i) {
+      const unsigned n = c[k * GROUP + i];
+      weights.next(first[k], first[k] + i, ratio, w);
+      if (n) {
+        n_here += n;
+        mass_here += n * fixed(w);
+        light |= !(w >= min_p);
+        if (!light) n_heavy = n_here, mass_heavy = mass_here;
+      }
     }
   }
   unsigned n_before = n_here;
@@ -503,7 +556,11 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
     const unsigned who = __ballot_sync(0xffffffffu, here);
     if (who) {
       const int o = __ffs(who) - 1;
-      const unsigned from = __shfl_sync(0xffffffffu, first, o);
+      unsigned from = __shfl_sync(0xffffffffu, first[0], o);
+      if (Q > 1) {
+        const unsigned second = __shfl_sync(0xffffffffu, first[Q - 1], o);
+        if (lane >= GROUP) from = second;
+      }
       unsigned count = 0;
       double w, ratio;
       weights.start(from, w, ratio);
@@ -511,7 +568,7 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
       for (int i = 0; i < OWN; ++i) {
         const unsigned t = __shfl_sync(0xffffffffu, c[i], o);
         if (lane == i) count = t;
-        if (i <= lane) weights.next(from, from + i, ratio, w);
+        if (i < GROUP && i <= (lane & (GROUP - 1))) weights.next(from, from + i, ratio, w);
       }
       const u64 each = count ? fixed(w) : 0;
       unsigned n = count;
@@ -538,7 +595,7 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
         if (nth * each > x) --nth;
         if ((nth + 1) * each <= x) ++nth;
       }
-      const unsigned place = from + f;
+      const unsigned place = __shfl_sync(0xffffffffu, from + (lane & (GROUP - 1)), f);
       n = __shfl_sync(0xffffffffu, n, f);
       nth = __shfl_sync(0xffffffffu, nth, f);
       const u64 upto = __shfl_sync(0xffffffffu, m + nth * each, f), one = __shfl_sync(0xffffffffu, each, f);
@@ -672,7 +729,7 @@ void configure(Launch& l, int slice, int batch, cudaStream_t st) {
 // Prepares the kernel on the current device, once; how many clusters run on it at the same time.
 template <int C>
 int prepare(int* clusters) {
-  static_assert(smem_bytes<C>(SLICE_MAX) <= 227 * 1024, "shared memory of the largest slice");
+  static_assert(smem_bytes<C>(slice_max(C)) <= 227 * 1024, "shared memory of the largest slice");
   static std::mutex mu;
   static int fit[64] = {};
   int dev = 0;
@@ -680,13 +737,13 @@ int prepare(int* clusters) {
   QX_REQUIRE(dev >= 0 && dev < 64, "sample_logits: device index %d unsupported", dev);
   std::lock_guard<std::mutex> lk(mu);
   if (fit[dev] == 0) {
-    QX_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<C>(SLICE_MAX)),
+    QX_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<C>(slice_max(C))),
                 "sample_logits: set smem limit");
     if (C > 8)
       QX_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<C>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
                   "sample_logits: allow clusters of 16");
     Launch l;
-    configure<C>(l, SLICE_MAX, 1, nullptr);
+    configure<C>(l, slice_max(C), 1, nullptr);
     l.cfg.numAttrs = 1;
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, sample_kernel<C>, &l.cfg) != cudaSuccess) {
@@ -716,8 +773,8 @@ int choose(Params& p, int batch, cudaStream_t st) {
   if (const int rc = prepare<16>(&at16); rc != QX_OK) return rc;
   if (const int rc = prepare<8>(&at8); rc != QX_OK) return rc;
   if (const int rc = prepare<4>(&at4); rc != QX_OK) return rc;
-  if (batch <= at16 || slice_of(p.vocab, 8) > SLICE_MAX) return launch<16>(p, batch, st);
-  if (batch <= at8 || slice_of(p.vocab, 4) > SLICE_MAX) return launch<8>(p, batch, st);
+  if (batch <= at16 || slice_of(p.vocab, 8) > slice_max(8)) return launch<16>(p, batch, st);
+  if (batch <= at8 || slice_of(p.vocab, 4) > slice_max(4)) return launch<8>(p, batch, st);
   return launch<4>(p, batch, st);
 }
 
