@@ -640,18 +640,16 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
   if (pick == NONE) return;
   // ---- the logit of that value and number in the slice, in index order: counted in runs
   // of 256 logits (a load of a warp), then within the run that holds it
-  const unsigned bits = (pick & 0x8000u) ? pick : 0x7FFFu - pick;
-  const unsigned pattern = bits | bits << 16, ignore = bits ? ~0u : 0x7FFF7FFFu;  // the zeros' sign does not count
-  auto matches = [&](int group) {
+  const __half value = __ushort_as_half(static_cast<unsigned short>((pick & 0x8000u) ? pick : 0x7FFFu - pick));
+  const __half2 pattern = __halves2half2(value, value);
+  auto matches = [&](int group) {  // equal as numbers: the zeros' sign does not count
     const uint4 v = slice[group];
     const unsigned w[4] = {v.x, v.y, v.z, v.w};
     unsigned mask = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const unsigned t = (w[e] & ignore) ^ pattern;
-      mask |= (t & 0xFFFFu ? 0u : 1u << 2 * e) | (t >> 16 ? 0u : 2u << 2 * e);
-    }
-    return mask;
+    for (int e = 0; e < 4; ++e)
+      mask |= __heq2_mask(*reinterpret_cast<const __half2*>(&w[e]), pattern) & (1u << 2 * e | 0x20000u << 2 * e);
+    return (mask | mask >> 16) & 0xFFu;
   };
 #pragma unroll 2
   for (int i = tid; i - lane < groups; i += THREADS) {

@@ -262,3 +262,17 @@ def test_a_run_as_a_served_batch_makes_it(C):
     assert torch.equal(logits.float().amax(-1), C.lm_head_argmax(h, head)[0])
     u = torch.rand(12, generator=gen(4), device="cuda")
     check(C, logits, u, temperature=torch.linspace(0, 2, 12, device="cuda"), top_k=40, top_p=0.95)
+
+
+@pytest.mark.parametrize("b,v", [(1, 1000), (16, 40000), (40, 3001)])
+@pytest.mark.parametrize("top_k", [0, 3, 200])
+def test_subnormal_logits_many_alike(C, b, v, top_k):
+    """logits of a few steps of 2^-24, zeros of both signs among them: all weights near one, the order by index counts"""
+    g = torch.Generator(device="cuda").manual_seed(v + top_k)
+    steps = torch.randint(-20, 21, (b, v), generator=g, device="cuda")
+    logits = (steps * 2.0 ** -24).half()
+    logits[steps == 0] = torch.where(torch.rand(int((steps == 0).sum()), generator=g, device="cuda") < 0.5, 0.0, -0.0).half()
+    u = torch.rand(b, generator=g, device="cuda")
+    check(C, logits, u, 1e-6, top_k)
+    greedy = C.sample_logits(logits, u, 0.0)[0]
+    assert torch.equal(greedy, logits.float().argmax(1))
