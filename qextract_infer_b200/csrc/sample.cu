@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
 #pragma unroll
   for (int k = 0; k < Q; ++k) {
     start[k] = ratio[k] = 0.0;
-    if (Q > 1 && k >= share) break;
+    if (first[k] == 0) continue;  // no group (the first one's places are NaN and do not occur)
     weights.start(first[k], start[k], ratio[k]);
     double w = start[k];
 #pragma unroll
