@@ -15,18 +15,18 @@
 // largest weight for each token before it, and 2^19 of them stay below 2^62.
 //
 // A cluster of C CTAs takes a row.  Each CTA counts a slice of it in its own histogram
-// (16-bit counters, 128 KB of shared memory), then owns 1 / C of the values: it adds
-// their counters of all CTAs through distributed shared memory (only those that are
-// not empty: each CTA tells the others which of its groups of 8 counters are in use),
-// and the prefix sums run over threads, warps and CTAs.  Whoever owns the border in question
+// (16-bit counters, 128 KB of shared memory) and tells all which groups of 8 values occur.
+// The groups that occur anywhere are dealt out in order, as many to each CTA, one to a
+// thread, which adds their counters of all CTAs through distributed shared memory; the
+// prefix sums run over threads, warps and CTAs.  Whoever owns the border in question
 // (the k-th token, top_p of the weight, u of the weight) tells all CTAs: its warp looks
 // at the thread's values again, a lane a value.
 //
-// Bound by a chain of latencies, not by bytes: measured 12.6 to 14.1 us for one row of 151936
-// (16 CTAs), 12.9 for 7 rows of 32003, 18.1 to 19.9 for 32 rows of 151936 (4 CTAs a row, 0.5
-// TB/s; their bytes alone 1.5).  Of the 32 rows' time a quarter is loading and counting, then
-// come the counters through distributed shared memory, the weights, and a border 1.5 us each:
-// the owner's warp, a send, and the wait of all.
+// Bound by a chain of latencies, not by bytes: measured 11.7 us for one row of 151936 (16
+// CTAs), 12.0 for 7 rows of 32003, 17.2 to 18.1 for 32 rows of 151936 (4 CTAs a row, 0.56
+// TB/s; their bytes alone 1.5).  Of the 32 rows' time a third is loading and counting, then
+// come the exchange of what occurs, the counters and weights, and a border 1 to 1.5 us each: the
+// owner's warp, a send, and the wait of all.
 #include <mutex>
 
 #include "qx_b200.h"
@@ -774,9 +774,9 @@ int launch(Params& p, int batch, cudaStream_t st) {
   return check_launch("sample_logits");
 }
 
-// The largest cluster with which the whole batch runs at once (7 rows by 16 CTAs, 15 by 8, 32 by 4 on a B200 of 148
-// SMs), else 4.  Measured at 151936 tokens with 1024 threads a CTA, us by 16 / 8 / 4 CTAs: 1 row
-// 13.6 / 14.3 / 17.4, 8 rows 25.6 / 14.9 / 18.1, 16 rows 38 / 27 / 18.3, 64 rows 123 / 65 / 36.
+// The largest cluster with which the whole batch runs at once (7 rows by 16 CTAs, 15 by 8, 32 by 4 on a B200 of
+// 148 SMs), else 4.  Measured at 151936 tokens, us by 16 / 8 / 4 CTAs: 1 row 12.6 / 12.7 / 15.6, 7 rows
+// 12.2 / 13.1 / 16.0, 8 rows 22.4 / 13.2 / 15.9, 16 rows 33 / 24 / 16.1, 64 rows 108 / 58 / 32.
 int choose(Params& p, int batch, cudaStream_t st) {
   int at16 = 0, at8 = 0, at4 = 0;
   if (const int rc = prepare<16>(&at16); rc != QX_OK) return rc;
