@@ -329,19 +329,22 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
   float scale = 0.f;
   for (;;) {
     at.find(p, b, chunk - b * p.chunks, rows);
-    if (at.any()) {
-      load_a(0);
-      load_a(1);
-      if (!late) load_b(0);
-    }
-    copy_commit();
-    pdl_wait();
-    if (at.any()) {
-      load_x(0);
-      copy_commit();
-      load_x(1);
-      copy_commit();
-      if (late) load_b(0);
+    // (loops, not copies: each instruction here is fetched for one use)
+#pragma unroll 1
+    for (int when = 0; when < 2; ++when) {
+      if (when == 1) pdl_wait();
+      if (at.any()) {
+#pragma unroll 1
+        for (int step = 0; step < 2; ++step) {
+          if (when == 0) {
+            load_a(step);
+          } else {
+            load_x(step);
+            copy_commit();
+          }
+        }
+        if (late == (when == 1)) load_b(0);
+      }
       copy_commit();
     }
     at.ask_again(p);
