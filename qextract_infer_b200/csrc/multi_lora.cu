@@ -216,7 +216,7 @@ __device__ __forceinline__ int part_of(const Params& p, int column) {
 // Bound by the weights' bytes where every row has its own adapter, else by the chain of
 // latencies: adapters, A, x, the exchange, y.  Measured: one token of 4096 x 6144, 3 x 16
 // ranks, 5.3 us (its bytes alone 0.1); 32 tokens with an adapter each, 4096 x 24576, 2 x 16
-// ranks, 11.2 us, 3.3 TB/s (5.6); there the two phases' loads take turns, as A's place takes
+// ranks, 11.1 us, 3.3 TB/s (5.6); there the two phases' loads take turns, as A's place takes
 // B's second step: all of B ahead leaves an SM one CTA, asked into L2 ahead 11.6, by bulk copies 11.7
 // (10.9 then).
 namespace few {
@@ -935,17 +935,20 @@ bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
 }
 
 // Clusters of a chunk: doubled while a CTA has more than `columns` columns, up to 8 and up to
-// those in all that run at once.  Measured (rank 16, K 4096, 24576 columns, us by 1 / 8
-// clusters a chunk): 8 tokens 15.9 / 6.0, 16 tokens 20.0 / 9.6, 128 tokens 23.3 / 13.1; one token
-// and 6144 columns: 4.9 with 1, 5.0 with 2, 5.1 with 4.
+// `at_once` in all.  Measured (rank 16, K 4096, 24576 columns, us by 1 / 8 clusters a chunk): 8
+// tokens 15.9 / 6.0, 16 tokens 20.0 / 9.6, 128 tokens 23.3 / 13.1; one token and 6144 columns: 4.9
+// with 1, 5.0 with 2, 5.1 with 4.
 void spread(Params& p, int columns, int at_once) {
   p.fan = 1;
   while (p.fan < 8 && int64_t(p.batch) * p.chunks * p.fan * 2 <= at_once && p.N / (C * p.fan) > columns) p.fan *= 2;
   p.width = ((p.N + C * p.fan - 1) / (C * p.fan) + 7) / 8 * 8;
 }
 
-// Clusters that run at once where two CTAs fit an SM, and where one does (148 SMs)
-constexpr int AT_ONCE_BY_TWO = 32, AT_ONCE = 15;
+// In all: of the tile kernel those that run at once where two CTAs fit an SM, and where one does
+// (148 SMs).  Of the other 8: with more, a decode step's next projection, which streams its weights
+// meanwhile, finds its SMs taken (the decoder's tok/s with 8 sequences and 8 / 16 / 32 clusters a
+// call: 1848 / 1811 / 1759; 16 sequences and 16 / 32: 2470 / 2334; one sequence and 1 / 8: 364 / 368).
+constexpr int AT_ONCE_BY_TWO = 32, AT_ONCE = 15, AT_ONCE_FEW = 8;
 constexpr int HALF_SMEM = 115000;  // dynamic shared memory of which an SM has room for two
 
 // C CTAs for every cluster of every chunk that may start in a sequence
@@ -1005,13 +1008,9 @@ bool plan_few(Params& p, few::Layout* l) {
   const int steps = (p.k_slice + most - 1) / most;
   p.k_step = ((p.k_slice + steps - 1) / steps + 15) / 16 * 16;
   const int columns = 1024 / int(std::min<int64_t>(ROWS, int64_t(p.batch) * p.tokens));
-  spread(p, columns, AT_ONCE_BY_TWO);
+  spread(p, columns, AT_ONCE_FEW);
   *l = layout(p);
-  if (l->total <= HALF_SMEM) return true;
-  if (p.rank <= many::RANKS) return false;
-  spread(p, columns, AT_ONCE);
-  *l = layout(p);
-  return true;
+  return l->total <= HALF_SMEM || p.rank > many::RANKS;
 }
 
 // Rows up to which chunks of 64 are 18 clusters at most, so that an SM has one CTA: then
