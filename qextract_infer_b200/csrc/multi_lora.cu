@@ -216,7 +216,7 @@ __device__ __forceinline__ int part_of(const Params& p, int column) {
 // Bound by the weights' bytes where every row has its own adapter, else by the chain of
 // latencies: adapters, A, x, the exchange, y.  Measured: one token of 4096 x 6144, 3 x 16
 // ranks, 5.3 us (its bytes alone 0.1); 32 tokens with an adapter each, 4096 x 24576, 2 x 16
-// ranks, 11.1 us, 3.3 TB/s (5.6); there the two phases' loads take turns, as A's place takes
+// ranks, 10.9 us, 3.4 TB/s (5.6); there the two phases' loads take turns, as A's place takes
 // B's second step: all of B ahead leaves an SM one CTA, asked into L2 ahead 11.6, by bulk copies 11.7
 // (10.9 then).
 namespace few {
