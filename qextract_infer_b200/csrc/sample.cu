@@ -313,7 +313,8 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
       __syncthreads();
       const unsigned seen = s.top_here;
       if (seen > 0x3FFu && seen != NONE) {
-        const float seen_at = float(value_at(seen)), down = t_row * -__logf(float(min_p));
+        // (logf and not __logf, whose error beside 1 is absolute: high temperatures would multiply it past the margin)
+        const float seen_at = float(value_at(seen)), down = t_row * -logf(float(min_p));
         const float rounded = seen_at - down - 1e-3f * (1.f + fabsf(seen_at) + down);
         last = min(last, place_of(__half_as_ushort(__float2half_rd(rounded))));  // (NONE where it is -inf)
       }
