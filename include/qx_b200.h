@@ -373,7 +373,8 @@ int qx_decode_attention_qkv(const void* qkv, const void* q_norm_w, const void* k
 /* Greedy head: logits = h W for h [batch, hidden] fp16 and W [hidden, vocab]
  * fp16 (a rank's vocabulary slice, vocab contiguous), rounded to fp16, and per
  * row the largest logit (as fp32) and its index + vocab_offset (the smallest
- * index among equal maxima).  batch <= 32, hidden % 64 == 0, vocab % 8 == 0.
+ * index among equal maxima; NaN is never the largest, a row of nothing else
+ * gives -inf and index 0).  batch <= 32, hidden % 64 == 0, vocab % 8 == 0.
  * Workspace: qx_lm_head_argmax_workspace_size(vocab) bytes, no
  * initialisation.  New component (the reference leaves the lm_head to HF). */
 size_t qx_lm_head_argmax_workspace_size(int vocab);

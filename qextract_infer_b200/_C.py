@@ -593,7 +593,7 @@ def lm_head_argmax(h: torch.Tensor, weight: torch.Tensor, vocab_offset: int = 0)
     """Greedy head: ``h`` fp16 ``[B, H]`` (B <= 32), ``weight`` fp16 ``[H, V]``
     (a vocabulary slice).  Returns (max logit fp32 ``[B]``, index int64 ``[B]``
     + ``vocab_offset``) of the fp16 logits ``h @ weight``; ties go to the
-    smallest index."""
+    smallest index, NaN is never the largest (a row of nothing else: -inf, index 0)."""
     for t, n in ((h, "h"), (weight, "weight")):
         _check_input(t, n)
         _check_fp16(t, n)

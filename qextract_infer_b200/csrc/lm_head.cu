@@ -26,7 +26,6 @@
 // 63; eight warps of 16 columns 175 / 197 / 51 (48 with four).  The next kernel is let in at the end: earlier, its CTAs
 // fill the slots as they come free, three on one SM and one on another (the slice: 54 us, 48 without).
 #include <algorithm>
-#include <cfloat>
 #include <mutex>
 
 #include "qx_b200.h"
@@ -83,7 +82,9 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ uint32_t wswz(int r, int ch) {
   return uint32_t(r * WROW + ((ch ^ (r & 7)) << 4));
 }
-// larger value wins; equal values: the smaller index
+// larger value wins (never a NaN); equal values: the smaller index.  A row that is all NaN ends as (-inf,
+// NOWHERE), which becomes the first index: whoever embeds the token next stays inside the vocabulary
+constexpr int NOWHERE = 0x7fffffff;
 __device__ __forceinline__ bool better(float v, int i, float bv, int bi) {
   return v > bv || (v == bv && i < bi);
 }
@@ -197,8 +198,8 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const __half* __restric
 #pragma unroll
     for (int hr = 0; hr < 2; ++hr) {  // rows g and g + 8 of the m-tile
       const int row = m * 16 + g + hr * 8;
-      float bv = -FLT_MAX;
-      int bi = 0x7fffffff;
+      float bv = -INFINITY;
+      int bi = NOWHERE;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
 #pragma unroll
@@ -242,8 +243,8 @@ __global__ void __launch_bounds__(128) argmax_finish_kernel(const Cand* __restri
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = blockIdx.x * 4 + warp;
   if (row >= B) return;
-  float bv = -FLT_MAX;
-  int bi = 0x7fffffff;
+  float bv = -INFINITY;
+  int bi = NOWHERE;
   for (int k = lane; k < nblk; k += 32) {
     const Cand o = part[size_t(k) * MAXB + row];
     if (better(o.v, o.i, bv, bi)) {
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(128) argmax_finish_kernel(const Cand* __restri
   }
   if (lane == 0) {
     out_val[row] = bv;
-    out_idx[row] = int64_t(bi) + offset;
+    out_idx[row] = int64_t(bi == NOWHERE ? 0 : bi) + offset;
   }
 }
 
