@@ -548,6 +548,13 @@ int qx_sample_logits(const void* logits, const float* u, const float* temperatur
                      const float* top_p, const float* min_p, float temperature_all, int64_t top_k_all,
                      float top_p_all, float min_p_all, int64_t* tokens, float* logprobs, int batch,
                      int vocab, qx_stream_t stream);
+/* For tests of the error path of qx_multi_lora_add and qx_sample_logits, whose CTAs exchange messages within a
+ * cluster: of the calls that follow (process-wide), the waits for the exchanges in the mask give up at once, in the
+ * CTA of that rank of each cluster (-1: in all of them), and the others after 20 ms instead of 2 s.  Such a call ends,
+ * sets QX_DEVERR_MBAR_TIMEOUT and leaves parts of out unwritten (qx_multi_lora_add) or gives token -1
+ * and logprob -inf (qx_sample_logits), as a call does whose messages do not come in time.  Exchanges: bits 0 and 1 of
+ * qx_multi_lora_add, 0 to 4 of qx_sample_logits.  0 ends the test. */
+int qx_test_waits(unsigned exchanges, int cta);
 
 #ifdef __cplusplus
 }

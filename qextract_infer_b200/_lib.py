@@ -104,6 +104,7 @@ SIGNATURES = {
     "qx_multi_lora_add": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                   c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p]),
     "qx_lm_head_logits": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "qx_test_waits": (c_int, [ctypes.c_uint, c_int]),
     "qx_sample_logits": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int64, c_float,
                                  c_float, c_void_p, c_void_p, c_int, c_int, c_void_p]),
 }

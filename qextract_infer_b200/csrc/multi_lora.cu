@@ -45,6 +45,7 @@ struct Params {
   int k_slice, k_step;      // K of a CTA, and of one of its steps (multiples of 16)
   int width;                // columns of a CTA
   int a_pitch;              // bytes of a staged row of A: an odd number of 16-byte units
+  unsigned test_waits;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -92,29 +93,6 @@ __device__ __forceinline__ void bar_init(uint32_t bar) {  // one arrival, that o
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ bool bar_try(uint32_t bar) {
-  uint32_t ok;
-  asm volatile(
-      "{ .reg .pred P; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], 0; selp.u32 %0, 1, 0, P; }"
-      : "=r"(ok)
-      : "r"(bar)
-      : "memory");
-  return ok != 0;
-}
-// what the cluster sends here has arrived (at most kWaitLimitNs)
-__device__ __forceinline__ void bar_wait(uint32_t bar) {
-  if (bar_try(bar)) return;
-  uint64_t t0, t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  while (!bar_try(bar)) {
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (t - t0 > kWaitLimitNs) {
-      atomicOr(&g_lora_error, QX_DEVERR_MBAR_TIMEOUT);
-      return;
-    }
-  }
-}
-
 // the adapter of sequence b, -1 where it has none
 __device__ __forceinline__ int64_t adapter_of(const Params& p, int b, bool fresh) {
   const int64_t a = fresh ? __ldcg(p.adapters + b) : p.adapters[b];
@@ -427,7 +405,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
     return m < n && c < n1 ? __ldcg(reinterpret_cast<const uint2*>(p.y + int64_t(rows[m]) * p.N + c)) : make_uint2(0u, 0u);
   };
   uint2 y = read_y(0, tid);
-  bar_wait(base + l.done);
+  const bool have_sums = exchange_wait(base + l.done, p.test_waits, 0, rank, &g_lora_error);
   float* const h = reinterpret_cast<float*>(smem + l.h);  // [ranks][8]
   {
     const float* recv = reinterpret_cast<const float*>(smem + l.recv);
@@ -439,9 +417,16 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
     }
   }
 
+  copy_wait<1>();
+  if (__syncthreads_or(!have_sums)) {  // out stays unwritten
+    cluster_leave_late();
+    return;
+  }
   for (int step = 0; step < b_steps; ++step) {
-    copy_wait<1>();
-    __syncthreads();
+    if (step > 0) {
+      copy_wait<1>();
+      __syncthreads();
+    }
     const __half* const w = reinterpret_cast<const __half*>(smem + l.b[step & 1]);
     const int items = n << l.b_shift;
     for (int i = tid; i < items; i += THREADS) {
@@ -781,7 +766,13 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
     load_b(1, 1);
     copy_commit();
   }
-  bar_wait(base + l.done + 8 * SUMS);  // the partial sums of this CTA's rows are here
+  auto have = [&](int exchange) {
+    return exchange_wait(base + l.done + 8 * exchange, p.test_waits, exchange, rank, &g_lora_error);
+  };
+  if (!have(SUMS)) {  // the partial sums of this CTA's rows; out stays unwritten (no barrier of the CTA lies behind)
+    cluster_leave_late();
+    return;
+  }
 
   // ---- add them up: a warp a row, a lane 4 ranks
   for (int own = warp; own < OWN; own += WARPS) {
@@ -850,7 +841,10 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
                      : "memory");
     }
   }
-  bar_wait(base + l.done + 8 * LOW_RANK);
+  if (!have(LOW_RANK)) {
+    cluster_leave_late();
+    return;
+  }
 
   // ---- the columns
   const float* const factor = reinterpret_cast<const float*>(smem + l.factor);
@@ -1151,6 +1145,7 @@ extern "C" int qx_multi_lora_add(const void* y, const void* x, const void* lora_
   p.rank = rank;
   p.ranks = rank * p.parts;
   p.n = num_adapters;
+  p.test_waits = g_test_waits.load(std::memory_order_relaxed);
   p.a_pitch = p.ranks * 2 + (p.ranks / 8 % 2 ? 0 : 16);
   p.k_slice = ((K + C - 1) / C + 15) / 16 * 16;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -53,6 +53,8 @@ std::mutex g_trace_mu;
 TraceTarget g_trace[2];  // QX_TRACE_GEMV, QX_TRACE_DECODE_ATTENTION
 }  // namespace
 
+std::atomic<unsigned> g_test_waits{0};
+
 unsigned long long* trace_next(int kernel, int* launch) {
 #ifdef QX_TRACE
   std::lock_guard<std::mutex> lk(g_trace_mu);
@@ -84,6 +86,12 @@ extern "C" int qx_trace_launches(int kernel, void* buf, int launches) {
                   "trace: this library was built without tracing (profiling build: "
                   "python -m qextract_infer_b200.build --trace)");
 #endif
+}
+
+extern "C" int qx_test_waits(unsigned exchanges, int cta) {
+  QX_REQUIRE(exchanges <= 0xFFu && cta >= -1 && cta < 16, "test_waits: exchanges=%u cta=%d", exchanges, cta);
+  qx::g_test_waits.store(exchanges ? exchanges | unsigned(cta + 1) << 8 : 0u, std::memory_order_relaxed);
+  return QX_OK;
 }
 
 extern "C" const char* qx_last_error(void) { return qx::g_last_error; }

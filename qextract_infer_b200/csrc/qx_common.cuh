@@ -44,6 +44,7 @@ inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_
 // with other processes does not trip it; a wait that runs out sets an error
 // bit read by qx_get_device_error and the kernel returns.
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;
+constexpr unsigned long long kWaitLimitTestNs = 20000000ull;  // of qx_test_waits: 20 ms
 
 __device__ __forceinline__ uint4 ldg_stream_v4(const void* p) {
   // weights are read exactly once per call: do not keep them in L1
@@ -176,6 +177,61 @@ __device__ __forceinline__ void trace_stamp(unsigned long long* b, int slot, boo
   (void)who;
 #endif
 }
+
+// ---------------------------------------------------- messages in a cluster --
+// A kernel whose CTAs send one another messages by st.async: an exchange is an mbarrier of
+// the receiver (phase 0) that counts their bytes.  Its wait is bounded like every other.  A warp
+// that waited in vain sends nothing and reads nothing of other CTAs any more, and ends by
+// cluster_leave_late(): its CTA stays until all others of the cluster have ended or are there too.
+// They are, at last: each of their waits is bounded, and a cluster barrier does not wait for threads
+// that have ended.  Other warps of its CTA may go on where no barrier of the CTA lies before their
+// end; where one does, the CTA decides as a whole (__syncthreads_or).
+//
+// Bits of qx_test_waits, as the kernels get them: exchange e gives up without a look (bit e), in
+// one CTA (its rank + 1 from bit 8) or, 0 there, in all of them.  0: no test.
+__device__ __forceinline__ bool exchange_here(uint32_t bar) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred P; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], 0; selp.u32 %0, 1, 0, P; }"
+      : "=r"(ok)
+      : "r"(bar)
+      : "memory");
+  return ok != 0;
+}
+// A whole warp asks, waits and gives up together: its threads never part before a barrier.  (Kept
+// apart: code that few calls run is not fetched between that which all do.)
+static __device__ __noinline__ bool exchange_wait_on(uint32_t bar, unsigned test, int exchange, int rank, unsigned* error) {
+  const bool skip = (test >> exchange & 1u) && (test >> 8 == 0 || int(test >> 8) == rank + 1);
+  const unsigned long long limit = skip ? 0ull : test ? kWaitLimitTestNs : kWaitLimitNs;
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  for (;;) {
+    if (__all_sync(0xffffffffu, !skip && exchange_here(bar))) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    if (__any_sync(0xffffffffu, t - t0 >= limit)) break;
+  }
+  atomicOr(error, unsigned(QX_DEVERR_MBAR_TIMEOUT));
+  return false;
+}
+// whether the messages are here
+__device__ __forceinline__ bool exchange_wait(uint32_t bar, unsigned test, int exchange, int rank, unsigned* error) {
+  if (__all_sync(0xffffffffu, test == 0 && exchange_here(bar))) return true;
+  return exchange_wait_on(bar, test, exchange, rank, error);
+}
+// By whole warps.  Messages that were sent before their sender ended may still be on their way (a
+// few microseconds): they land in this CTA's memory, so it stays a millisecond longer.
+static __device__ __noinline__ void cluster_leave_late() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  do {
+    __nanosleep(1000);
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  } while (t - t0 < 1000000ull);
+}
+extern std::atomic<unsigned> g_test_waits;  // qx_capi.cu (qx_test_waits)
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

@@ -58,6 +58,7 @@ struct Params {
   int64_t* tokens;
   float* logprobs;
   int vocab, slice;
+  unsigned test_waits;
 };
 
 constexpr int RUNS = slice_max(4) / 256;  // of 256 logits in the largest slice
@@ -119,28 +120,6 @@ __device__ __forceinline__ void send(const unsigned* p, const u64* done, int ran
 }
 __device__ __forceinline__ void expect(const u64* done, unsigned bytes) {
   asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(done)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool arrived(uint32_t bar) {
-  uint32_t ok;
-  asm volatile(
-      "{ .reg .pred P; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], 0; selp.u32 %0, 1, 0, P; }"
-      : "=r"(ok)
-      : "r"(bar)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ void wait_for(const u64* done) {  // at most kWaitLimitNs
-  const uint32_t bar = smem_u32(done);
-  if (arrived(bar)) return;
-  uint64_t t0, t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  while (!arrived(bar)) {
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (t - t0 > kWaitLimitNs) {
-      atomicOr(&g_sample_error, QX_DEVERR_MBAR_TIMEOUT);
-      return;
-    }
-  }
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -243,6 +222,15 @@ __device__ __forceinline__ unsigned top_of(uint32_t pair) {
   return place_of(m & 0xFFFFu);
 }
 
+// A message did not come in time: the row's token is undefined and says so.
+static __device__ __noinline__ void give_up(int64_t* token, float* logprob) {
+  cluster_leave_late();
+  if (threadIdx.x == 0) {
+    *token = -1;
+    *logprob = -INFINITY;
+  }
+}
+
 template <int C>
 __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_constant__ Params p) {
   constexpr int THREADS = threads_of(C), WARPS = THREADS / 32;
@@ -255,9 +243,15 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int row = blockIdx.x / C, rank = blockIdx.x % C;
   pdl_trigger();
+  auto wait_for = [&](int exchange) {
+    return exchange_wait(smem_u32(&s.done[exchange]), p.test_waits, exchange, rank, &g_sample_error);
+  };
+  // whether any warp of the CTA has waited in vain
+  auto late = [&](int exchange) { return __syncthreads_or(!wait_for(exchange)); };
 
   if (tid == 0) {
     s.top_here = s.m_here = NONE;
+    s.found = s.found_nth = 0;
     for (int i = 0; i < EXCHANGES; ++i)
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&s.done[i])) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -357,18 +351,9 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
   if (tid < C) send(&s.top[rank], &s.done[USED], tid, s.top_here);
   for (int i = tid; i < C * (WORDS / 4); i += THREADS)
     send(&s.used[rank][i % (WORDS / 4) * 4], &s.done[USED], i / (WORDS / 4), reinterpret_cast<const uint4*>(s.mine)[i % (WORDS / 4)]);
-  wait_for(&s.done[USED]);
+  const bool have_used = wait_for(USED);
   weights.place = s.top[0];
   for (int r = 1; r < C; ++r) weights.place = min(weights.place, s.top[r]);
-  if (weights.place == NONE) {  // nothing to draw from
-    if (rank == 0 && tid == 0) {
-      p.tokens[row] = -1;
-      p.logprobs[row] = -INFINITY;
-    }
-    cluster_arrive();  // nobody reads this CTA's histogram any more
-    cluster_wait();
-    return;
-  }
   weights.top = value_at(weights.place);
   // (beside +inf nothing has weight, whatever the temperature)
   if (isinf(weights.top)) weights.top = 1e300, weights.scale = 1.0;
@@ -389,7 +374,19 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
     s.upto[tid] = n;
     if (lane == 31) s.words_upto[warp] = n;
   }
-  __syncthreads();
+  if (__syncthreads_or(!have_used)) {
+    give_up(p.tokens + row, p.logprobs + row);
+    return;
+  }
+  if (weights.place == NONE) {  // nothing to draw from
+    if (rank == 0 && tid == 0) {
+      p.tokens[row] = -1;
+      p.logprobs[row] = -INFINITY;
+    }
+    cluster_arrive();  // nobody reads this CTA's histogram any more
+    cluster_wait();
+    return;
+  }
   unsigned occur = 0, words_before[WORDS / 32];
 #pragma unroll
   for (int i = 0; i < WORDS / 32; ++i) words_before[i] = occur, occur += s.words_upto[i];
@@ -510,7 +507,10 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
   __syncthreads();
   n_before += s.warp_count[warp];
   before += s.warp_mass[warp];
-  wait_for(&s.done[TOTALS]);
+  if (late(TOTALS)) {
+    give_up(p.tokens + row, p.logprobs + row);
+    return;
+  }
   unsigned kept = 0;
   u64 kept_mass = 0;
 #pragma unroll
@@ -637,7 +637,10 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
       }
     }
     if (border == PICK) break;
-    wait_for(&s.done[border]);
+    if (late(border)) {
+      give_up(p.tokens + row, p.logprobs + row);
+      return;
+    }
     if (border == TOP_K) kept_mass = s.k_mass;
     if (border == LIMITS) {
       if (cut_p && s.p_run[0] < kept) kept = unsigned(s.p_run[0]), kept_mass = s.p_run[1];
@@ -647,7 +650,10 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
           if (s.m_run[r][0] < kept) kept = unsigned(s.m_run[r][0]), kept_mass = s.m_run[r][1];
     }
   }
-  wait_for(&s.done[PICK]);
+  if (late(PICK)) {
+    give_up(p.tokens + row, p.logprobs + row);
+    return;
+  }
   const unsigned pick = unsigned(s.pick);
   if (pick == NONE) return;
   // ---- the logit of that value and number in the slice, in index order: counted in runs
@@ -695,7 +701,7 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
   __syncthreads();
   if (warp != 0) return;
   const int group = int(s.found) * 32 + lane;
-  unsigned mask = group < groups ? matches(group) : 0u;
+  unsigned mask = unsigned(group) < unsigned(groups) ? matches(group) : 0u;
   unsigned upto = __popc(mask);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -829,5 +835,6 @@ extern "C" int qx_sample_logits(const void* logits, const float* u, const float*
   p.tokens = tokens;
   p.logprobs = logprobs;
   p.vocab = vocab;
+  p.test_waits = g_test_waits.load(std::memory_order_relaxed);
   return smp::choose(p, batch, reinterpret_cast<cudaStream_t>(stream));
 }
