@@ -426,9 +426,6 @@ class TPDecoder:
         h = _C.fused_rmsnorm(x, self.final_norm, self.cfg.rms_eps)
         return h @ self.lm_head
 
-    def _greedy(self, x: torch.Tensor) -> torch.Tensor:
-        return self._greedy_normed(_C.fused_rmsnorm(x, self.final_norm, self.cfg.rms_eps))
-
     def _greedy_normed(self, h: torch.Tensor) -> torch.Tensor:
         """greedy tokens from the final-normed hidden state"""
         val, idx = _C.lm_head_argmax(h, self.lm_head, self.rank * self.lm_head.size(1))
