@@ -66,13 +66,13 @@ def shard_adapters(lora_A, lora_B, split: str, rank: int, world: int):
     if world <= 1:
         return lora_A, lora_B
     if split == "col":
-        if lora_B.size(2) % world or (lora_B.size(2) // world) % 8:
-            raise ValueError(f"column split of N={lora_B.size(2)} over {world} ranks needs N/tp % 8 == 0")
+        if lora_B.size(2) % world:
+            raise ValueError(f"column split of N={lora_B.size(2)} needs a multiple of {world} ranks")
         n = lora_B.size(2) // world
         return lora_A, lora_B[:, :, rank * n:(rank + 1) * n]
     if split == "row":
-        if lora_A.size(1) % world or (lora_A.size(1) // world) % 8:
-            raise ValueError(f"row split of K={lora_A.size(1)} over {world} ranks needs K/tp % 8 == 0")
+        if lora_A.size(1) % world:
+            raise ValueError(f"row split of K={lora_A.size(1)} needs a multiple of {world} ranks")
         k = lora_A.size(1) // world
         return lora_A[:, rank * k:(rank + 1) * k], lora_B
     raise ValueError(f"unknown split {split!r}")
