@@ -982,11 +982,12 @@ void spread(Params& p, int columns, int at_once) {
   p.width = ((p.N + C * p.fan - 1) / (C * p.fan) + 7) / 8 * 8;
 }
 
-// In all: of the tile kernel those that run at once where two CTAs fit an SM, and where one does
-// (148 SMs).  Of the other 8: with more, a decode step's next projection, which streams its weights
+// In all: of the tile kernel those that run at once on a B200 (148 SMs, clusters of 8 CTAs within a GPC) where two
+// CTAs fit an SM, and where one does: 33 chunks of 32 rows take 15.7 us, 34 26.2 (rank 8, 2560 x 9728); 15 of
+// 3 x 64 ranks 35.2 us, 16 67.9.  Of the other 8: with more, a decode step's next projection, which streams its weights
 // meanwhile, finds its SMs taken (the decoder's tok/s with 8 sequences and 8 / 16 / 32 clusters a
 // call: 1848 / 1811 / 1759; 16 sequences and 16 / 32: 2470 / 2334; one sequence and 1 / 8: 364 / 368).
-constexpr int AT_ONCE_BY_TWO = 32, AT_ONCE = 15, AT_ONCE_FEW = 8;
+constexpr int AT_ONCE_BY_TWO = 33, AT_ONCE = 15, AT_ONCE_FEW = 8;
 constexpr int HALF_SMEM = 115000;  // dynamic shared memory of which an SM has room for two
 
 // C CTAs for every cluster of every chunk that may start in a sequence
@@ -1051,17 +1052,30 @@ bool plan_few(Params& p, few::Layout* l) {
   return l->total <= HALF_SMEM || p.rank > many::RANKS;
 }
 
-// Rows up to which chunks of 64 are 18 clusters at most, so that an SM has one CTA: then
-// chunks of 32.  Measured at 999 rows (rank 8, 2560 x 9728): 22.7 us with 64, 15.8 with 32.
-constexpr int SMALL_ROWS = 18 * 64;
+// Up to SMALL_ROWS rows in all, chunks of 32 rows where they take no more waves of clusters than chunks of 64
+// (each sequence counted by itself).  Measured, us by 32 / 64 (2560 x 9728 rank 8 | 4096 x 24576 rank 16 | 12288 x
+// 4096 rank 64): one sequence of 320 tokens 11.2 / 12.6 | 18.3 / 19.0 | 20.9 / 22.7, of 1056 15.7 / 21.9 | 29.1 / 43.7
+// | 25.6 / 36.4, of 1088 26.2 / 22.0 | 47.3 / 43.7 | 40.2 / 36.5; 100 of 10 tokens with an adapter each 48.2 / 57.7 | 83.7 /
+// 100.4 | 79.8 / 106.0, with one 27.4 / 27.3 | 42.4 / 47.7 | 39.1 / 41.8; 20 of 40 with an adapter each 25.8 / 19.8 | 44.4 / 37.2 |
+// 40.0 / 33.9.  With more rows sequences that share adapters fill chunks of 64: 48 of 32 tokens, 8 adapters, 29.9 / 25.0 |
+// 54.8 / 46.6 | 47.4 / 39.7.
+constexpr int SMALL_ROWS = 1152;
+
+// waves of the tile kernel's clusters with chunks of `rows`
+int64_t waves(const Params& p, int rows) {
+  const int64_t chunks = int64_t(p.batch) * ((p.tokens + rows - 1) / rows);
+  const int at_once = many::layout(p, rows).total > HALF_SMEM ? AT_ONCE : AT_ONCE_BY_TWO;
+  return (chunks + at_once - 1) / at_once;
+}
 
 int launch_many(Params& p, cudaStream_t st) {
   using namespace many;
   const int ks = (p.rank + 15) / 16;
-  const int rows = int64_t(p.batch) * p.tokens <= SMALL_ROWS && ks <= 4 ? 32 : 64;
-  p.chunks = (p.tokens + rows - 1) / rows;
   const int here = std::min(RANKS, p.ranks);
   p.a_pitch = here * 2 + (here / 8 % 2 ? 0 : 16);
+  const bool small = int64_t(p.batch) * p.tokens <= SMALL_ROWS && ks <= 4;
+  const int rows = small && waves(p, 32) <= waves(p, 64) ? 32 : 64;
+  p.chunks = (p.tokens + rows - 1) / rows;
   const int smem = layout(p, rows).total;
   spread(p, 256, smem > HALF_SMEM ? AT_ONCE : AT_ONCE_BY_TWO);
   void (*kernel)(Params);
