@@ -467,12 +467,11 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
 // 64 rows a chunk, 32 where that leaves an SM a CTA.  h = x A by mma.sync (a warp: 32 rows,
 // a quarter of each step of 64 along K, of 32-row chunks half of the ranks), 64 ranks at a
 // time.  CTA i of the cluster adds the partial sums of its eighth of the rows and gives them
-// to all as two fp16 numbers, high and low (22 bits), of h 2^-e with e from the row's
-// largest of that column block: any fp32 range, and a second product instead of a rounding
-// of h to 11 bits.  A value that is too small beside the largest (or finite beside an infinity)
-// is a zero in both that keeps its sign, for the infinities of B: a warp whose block of B
-// holds one takes such a value as the smallest number of its sign, and multiplies the low part by zeros in the
-// infinities' place (0 and a low part of the other sign would make them NaN).  Then a warp takes 32 columns at a time for all rows; the y of the next
+// to all as the sum of two fp16 numbers, high (rounded towards zero) and low, of h 2^-e with e
+// from the row's largest of that column block: 21 bits (2^-32 of the largest at least) over any fp32
+// range, and a second product instead of a rounding of h to 11 bits.  Both have h's sign, and neither
+// is zero where h is not: beside an infinity of B the two products are the same infinity (a zero, or a
+// low part of the other sign, would make it NaN).  Then a warp takes 32 columns at a time for all rows; the y of the next
 // one or two blocks of columns is on its way into shared memory meanwhile (a lane's own
 // 16-byte pieces, refilled as they are used).  Within the 32 columns the product's columns
 // stand in the order in which a thread gets 8 neighbouring ones, so y and out move 16 bytes
@@ -532,27 +531,23 @@ __host__ __device__ inline Layout layout(const Params& p, int ROWS) {
   l.total = at;
   return l;
 }
-// the larger of each half, without the signs
-__device__ __forceinline__ void largest(const uint32_t (&w)[4][2], uint32_t& top) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) asm("max.xorsign.abs.f16x2 %0, %0, %1;" : "+r"(top) : "r"(w[i][e]));
-}
-__device__ __forceinline__ bool is_infinite(uint32_t pair) {  // either half
-  return (pair & 0x7FFFu) == 0x7C00u || (pair & 0x7FFF0000u) == 0x7C000000u;
-}
-// zeros in the place of infinities
-__device__ __forceinline__ uint32_t without_infinities(uint32_t pair) {
-  if ((pair & 0x7FFFu) == 0x7C00u) pair &= 0xFFFF0000u;
-  if ((pair & 0x7FFF0000u) == 0x7C000000u) pair &= 0xFFFFu;
-  return pair;
-}
-// low-rank values' high parts with the smallest number of its sign for each that is marked as too small
-__device__ __forceinline__ uint32_t with_small(uint32_t hi, uint32_t lo) {
-  if (!(hi & 0x7FFFu)) hi |= (hi | lo) >> 15 & 1u;
-  if (!(hi & 0x7FFF0000u)) hi |= (hi | lo) >> 15 & 0x10000u;
-  return hi;
+// Two values as (high, low) halves; `plain`: within +-2^10, else (a row with an infinity or NaN) only those count
+__device__ __forceinline__ void split(float v0, float v1, float down, bool plain, uint32_t& hi, uint32_t& lo) {
+  const float s0 = plain ? v0 * down : isfinite(v0) ? 0.f : v0, s1 = plain ? v1 * down : isfinite(v1) ? 0.f : v1;
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(s1), "f"(s0));
+  const float2 back = h2_to_f2(hi);
+  const __half2 rest = __floats2half2_rn(plain ? s0 - back.x : s0, plain ? s1 - back.y : s1);
+  lo = *reinterpret_cast<const uint32_t*>(&rest);
+  // what is not zero is at least the smallest number of its sign in both
+  const uint32_t sign = (__float_as_uint(v0) >> 16 & 0x8000u) | (__float_as_uint(v1) & 0x80000000u);
+  if (v0 != 0.f) {
+    if (!(hi & 0x7FFFu)) hi |= (sign & 0x8000u) | 1u;
+    if (!(lo & 0x7FFFu)) lo |= (sign & 0x8000u) | 1u;
+  }
+  if (v1 != 0.f) {
+    if (!(hi & 0x7FFF0000u)) hi |= (sign & 0x80000000u) | 0x10000u;
+    if (!(lo & 0x7FFF0000u)) lo |= (sign & 0x80000000u) | 0x10000u;
+  }
 }
 // KS: a column block's ranks in steps of 16 (1, 2, up to 4): its B stays in registers for all
 // row tiles.  0: more than 64 ranks, 64 at a time, the sums of 64 rows in registers
@@ -806,18 +801,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
         if (j < l.padded) {
           uint32_t hi[2], lo[2];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float s0 = finite || !isfinite(v[i][2 * k]) ? v[i][2 * k] * down : copysignf(0.f, v[i][2 * k]);
-            const float s1 = finite || !isfinite(v[i][2 * k + 1]) ? v[i][2 * k + 1] * down : copysignf(0.f, v[i][2 * k + 1]);
-            const __half2 h = __floats2half2_rn(s0, s1);
-            const float2 back = __half22float2(h);
-            const __half2 rest = finite ? __floats2half2_rn(s0 - back.x, s1 - back.y) : __floats2half2_rn(0.f, 0.f);
-            hi[k] = *reinterpret_cast<const uint32_t*>(&h);
-            lo[k] = *reinterpret_cast<const uint32_t*>(&rest);
-            // too small for `hi`: negative ones have -0 there, positive ones -0 in `lo`
-            if (v[i][2 * k] > 0.f && !(hi[k] & 0x7FFFu)) lo[k] |= 0x8000u;
-            if (v[i][2 * k + 1] > 0.f && !(hi[k] & 0x7FFF0000u)) lo[k] |= 0x80000000u;
-          }
+          for (int k = 0; k < 2; ++k) split(v[i][2 * k], v[i][2 * k + 1], down, finite, hi[k], lo[k]);
           const uint32_t at = m * l.h_pitch + (part * l.padded + j) * 2;
 #pragma unroll
           for (int r = 0; r < C; ++r) {
@@ -872,21 +856,11 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
     }
   };
   // 16 rows x 16 ranks (from rank `j`, padded, of all) x 32 columns
-  auto multiply = [&](int t, int j, const uint32_t (&w)[4][2], float (&acc)[4][4], bool infinite) {
+  auto multiply = [&](int t, int j, const uint32_t (&w)[4][2], float (&acc)[4][4]) {
     const uint32_t at = (t * 16 + (lane & 15)) * l.h_pitch + (j + 8 * (lane >> 4)) * 2;
     uint32_t hi[4], lo[4];
     ldsm4(hi, base + l.hi + at);
     ldsm4(lo, base + l.lo + at);
-    if (infinite) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) hi[i] = with_small(hi[i], lo[i]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        mma_16816(acc[i], hi[0], hi[1], hi[2], hi[3], w[i][0], w[i][1]);
-        mma_16816(acc[i], lo[0], lo[1], lo[2], lo[3], without_infinities(w[i][0]), without_infinities(w[i][1]));
-      }
-      return;
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       mma_16816(acc[i], hi[0], hi[1], hi[2], hi[3], w[i][0], w[i][1]);
@@ -903,15 +877,11 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
       copy_wait<TILES * AHEAD - 1>();
       __syncwarp();
       const int ks = l.padded / 16;
-      uint32_t w[KS > 0 ? KS : 1][4][2], top = 0u;
+      uint32_t w[KS > 0 ? KS : 1][4][2];
       if (now.columns > 0)
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-          if (k < ks) {
-            weights(base + buffer * l.b_rows * l.b_pitch + warp * 64, k, w[k]);
-            largest(w[k], top);
-          }
-      const bool infinite = __any_sync(0xffffffffu, is_infinite(top));
+          if (k < ks) weights(base + buffer * l.b_rows * l.b_pitch + warp * 64, k, w[k]);
       __syncwarp();
       load_b(group + AHEAD, buffer);
 #pragma unroll
@@ -927,7 +897,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
           float acc[4][4] = {};
 #pragma unroll
           for (int k = 0; k < KS; ++k)
-            if (k < ks) multiply(t, now.part * l.padded + k * 16, w[k], acc, infinite);
+            if (k < ks) multiply(t, now.part * l.padded + k * 16, w[k], acc);
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             if (mine && t * 16 + e * 8 + g < n) write(now, t, e, y[e], acc);
@@ -941,12 +911,10 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_tile_kernel(const __gri
         __syncwarp();
         if (now.columns > 0)
           for (int k = 0; k < min(RANKS, l.padded - piece * RANKS) / 16; ++k) {
-            uint32_t w[4][2], top = 0u;
+            uint32_t w[4][2];
             weights(base + (step & 1) * l.b_rows * l.b_pitch + warp * 64, k, w);
-            largest(w, top);
-            const bool infinite = __any_sync(0xffffffffu, is_infinite(top));
 #pragma unroll
-            for (int t = 0; t < ROWS / 16; ++t) multiply(t, now.part * l.padded + piece * RANKS + k * 16, w, acc[t], infinite);
+            for (int t = 0; t < ROWS / 16; ++t) multiply(t, now.part * l.padded + piece * RANKS + k * 16, w, acc[t]);
           }
         __syncwarp();
         load_b(step + 2, step & 1);
