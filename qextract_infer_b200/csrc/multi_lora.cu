@@ -417,16 +417,13 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
     }
   }
 
-  copy_wait<1>();
   if (__syncthreads_or(!have_sums)) {  // out stays unwritten
     cluster_leave_late();
     return;
   }
   for (int step = 0; step < b_steps; ++step) {
-    if (step > 0) {
-      copy_wait<1>();
-      __syncthreads();
-    }
+    copy_wait<1>();
+    __syncthreads();
     const __half* const w = reinterpret_cast<const __half*>(smem + l.b[step & 1]);
     const int items = n << l.b_shift;
     for (int i = tid; i < items; i += THREADS) {
