@@ -514,7 +514,8 @@ int qx_prefill_attention_q4(const void* q, const void* k_new, const void* v_new,
  *   splits: host array of num_splits <= 4 widths that sum to N (multiples of
  *   8), the column blocks of a fused projection; block j uses the ranks
  *   j rank .. j rank + rank - 1 of lora_A.  num_splits = 0: one block (P = 1).
- *   Sums in fp32, one rounding.  out may be y (in place); it must not overlap
+ *   Sums in fp32, one rounding; where sequences have more than 8 tokens (or about 100 ranks in all and
+ *   more, at most 64 a block), x A is held in 21 bits, and to 2^-32 of the row's largest of that block.  out may be y (in place); it must not overlap
  *   anything else.  lora_A and lora_B must not be written by a kernel of this
  *   library issued just before on the stream (qx_set_pdl); adapters and scales may be.
  *   K % 8 == 0, N % 8 == 0, rank % 8 == 0, P rank <= 256, batch <= 32768 (the time

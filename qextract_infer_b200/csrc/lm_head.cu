@@ -14,8 +14,9 @@
 // Whole logits (qx_lm_head_logits): kernel 1 with the fp16 values stored instead of
 // compared, 32 rows a launch.
 //
-// Bound by the weights' bytes: 1 / 17 / 32 rows of 4096 x 151936 take 172 / 177 / 181 us (7.2 to
-// 6.9 TB/s), of 4096 x 37984 48.2 / 51.6 / 52.8 (297 CTAs: one SM has three, the others two).  With
+// Bound by the weights' bytes: 1 / 17 / 32 rows of 4096 x 151936 take 173 / 177 / 181 us (7.2 to
+// 6.9 TB/s; a kernel that only reads them 173; 32 rows among calls of other kernels 189 to 200), of 4096 x 37984
+// 48 / 52 / 53 (297 CTAs: one SM has three, the others two); 33 rows and more read them again, 64 rows 372.  With
 // more rows a tile's own time counts: addresses that only move on, instead of each piece's own
 // (198 instructions a warp and tile at 17 rows, 117 at 16), took 32 rows from 194 to 184 us; h through
 // L1, where an SM's CTAs meet and not all CTAs at the same lines of L2, from 184 to 181, of the slice from

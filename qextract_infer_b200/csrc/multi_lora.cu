@@ -11,13 +11,13 @@
 // prepared: the cluster of sequence b counts the sequences before it that share its
 // adapter, which says whether a chunk starts in b, and looks up those after it that
 // fill the chunk; clusters without a chunk end at once.  The group's weights are read
-// once a chunk, and each of the 8 CTAs reads an eighth of them: it multiplies an eighth
+// once a cluster, and each of the 8 CTAs reads an eighth of them: it multiplies an eighth
 // of K (its part of A), the partial h = x A meet through distributed shared memory, and
 // then it does an eighth of the columns (its part of B).
 //
 // A row's result depends on no other row: the sums are split in the same way wherever a
-// row stands.  Where there are few chunks, several clusters take one, each a share of the
-// columns.
+// row stands.  Where there are few chunks, several clusters take one: each reads all of A
+// and makes h, then does its share of the columns.
 #include <algorithm>
 #include <mutex>
 
@@ -105,8 +105,8 @@ __device__ __forceinline__ int64_t adapter_of(const Params& p, int b, bool fresh
 // reads them once more; changed() compares, behind the work that hides these loads and
 // before anything leaves the CTA.  If it says so, find() and all after it is done again.
 // Whatever find() reads, its results are the same in all threads, and its rows and adapter
-// exist.  (A decode step's launch of one token takes 5.3 us so, 6.9 with the wait first, 4.9 if the
-// second look is left out; of 32 tokens with an adapter each 11.7, 13.2 and 11.0.)
+// exist.  (When it was chosen: a launch of one token 5.3 us so, 6.9 with the wait first, 4.9 if the second
+// look is left out; of 32 tokens with an adapter each 11.7, 13.2 and 11.0.)
 template <int ROWS, int THREADS>
 struct Chunk {
   int64_t a;       // the adapter, -1: none
@@ -194,9 +194,8 @@ __device__ __forceinline__ int part_of(const Params& p, int column) {
 // Bound by the weights' bytes where every row has its own adapter, else by the chain of
 // latencies: adapters, A, x, the exchange, y.  Measured: one token of 4096 x 6144, 3 x 16
 // ranks, 5.3 us (its bytes alone 0.1); 32 tokens with an adapter each, 4096 x 24576, 2 x 16
-// ranks, 10.9 us, 3.4 TB/s (5.6); there the two phases' loads take turns, as A's place takes
-// B's second step: all of B ahead leaves an SM one CTA, asked into L2 ahead 11.6, by bulk copies 11.7
-// (10.9 then).
+// ranks, 10.9 us, 3.4 TB/s (5.2); there the two phases' loads take turns, as A's place takes
+// B's second step: all of B ahead leaves an SM one CTA; asked into L2 ahead, or by bulk copies, it took 7 % more.
 namespace few {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
@@ -251,7 +250,7 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
   }
   cluster_arrive();
   // The first columns of B are asked for at once by a few clusters, by more of them behind x, so that the
-  // products do not wait for B's bytes too (us, B first / behind, rank 16, K 4096: one token, 6144
+  // products do not wait for B's bytes too (when it was chosen, us, B first / behind, rank 16, K 4096: one token, 6144
   // columns 5.3 / 5.6; 32 tokens with an adapter each, 4096 columns 9.8 / 9.1, 8192 9.4 / 8.7, 24576 11.6 / 11.4).
   const bool late = gridDim.x > 8 * C;
   Chunk<ROWS, THREADS> at(p, true);
@@ -474,12 +473,12 @@ __global__ void __launch_bounds__(THREADS, 2) multi_lora_rows_kernel(const __gri
 // stand in the order in which a thread gets 8 neighbouring ones, so y and out move 16 bytes
 // a lane.
 //
-// Measured: 2048 tokens of 12288 x 4096, 64 ranks, 37.5 us, 2.3 TB/s (its bytes alone 13.1).
+// Measured: 2048 tokens of 12288 x 4096, 64 ranks, 37.6 us, 2.3 TB/s (its bytes alone 12.4).
 // Of a CTA's 64K cycles h takes 31K (its loads alone 26K: A comes from L2 for each chunk;
 // its products alone 17K, 12K of them the rate of mma.sync), waiting for the cluster's
 // slowest CTA 9K (256 CTAs on 148 SMs), the columns 12K.  Chunks of 128 rows leave an SM one
 // CTA, and of 16 such clusters 15 run at once: 72 us.  999 tokens of 2560 x 9728, 8 ranks:
-// 15.7 us, 2.8 TB/s (6.8): launch, five steps along K, the two exchanges, then the columns.
+// 15.9 us, 2.8 TB/s (6.7): launch, five steps along K, the two exchanges, then the columns.
 //
 // It launches nothing early: with the next call's clusters waiting on the SMs a 2048-token
 // chunk took 55.7 us instead of 40.6.  Two CTAs an SM: of clusters of 8 with an SM a CTA
@@ -940,7 +939,9 @@ bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
 // Clusters of a chunk: doubled while a CTA has more than `columns` columns, up to 8 and up to
 // `at_once` in all.  Measured (rank 16, K 4096, 24576 columns, us by 1 / 8 clusters a chunk): 8
 // tokens 15.9 / 6.0, 16 tokens 20.0 / 9.6, 128 tokens 23.3 / 13.1; one token and 6144 columns: 4.9
-// with 1, 5.0 with 2, 5.1 with 4.
+// with 1, 5.0 with 2, 5.1 with 4.  The chunks counted are those that may start.  Sequences that share an
+// adapter make fewer, and those are not spread: 8 sequences of one token on one adapter take 16.2 us, with an adapter
+// each 6.8; 32 on one 19.2, on 4 21.7, with an adapter each 10.9; 64 on 1, 2 or 4 26.
 void spread(Params& p, int columns, int at_once) {
   p.fan = 1;
   while (p.fan < 8 && int64_t(p.batch) * p.chunks * p.fan * 2 <= at_once && p.N / (C * p.fan) > columns) p.fan *= 2;
@@ -1000,8 +1001,8 @@ int launch(void (*kernel)(Args...), int threads, const Params& p, int smem, cuda
 // 8-row chunks, for sequences of up to FEW_TOKENS.  Where only one of their CTAs fits an SM (128
 // ranks in all and more) the other kernel does them, unless a block has more than 64 ranks, which
 // it takes piece by piece.  Measured (a decode step of 1 / 8 / 32 sequences with an adapter each,
-// us here / there): 3 x 32 ranks and 6144 columns 8.7 / 12.6, 10.0 / 16.9, 15.8 / 21.8; 2 x 64
-// and 24576 12.5 / 14.8, 24 / 23.4, 73 / 43; 2 x 128 25.9 / 34.9, 59 / 84, 179 / 245.
+// us here / there): 3 x 32 ranks and 6144 columns 8.8 / 12.6, 9.9 / 16.9, 20 / 21.8; 2 x 64
+// and 24576 12.5 / 14.2, 24 / 23.7, 73 / 43.5; 2 x 128 26.5 / 34.9, 60.5 / 84, 182 / 245.
 constexpr int FEW_TOKENS = 8;
 
 bool plan_few(Params& p, few::Layout* l) {

@@ -22,9 +22,9 @@
 // (the k-th token, top_p of the weight, u of the weight) tells all CTAs: its warp looks
 // at the thread's values again, a lane a value.
 //
-// Bound by a chain of latencies, not by bytes: measured 11.7 us for one row of 151936 (16
-// CTAs), 12.0 for 7 rows of 32003, 17.2 to 18.1 for 32 rows of 151936 (4 CTAs a row, 0.56
-// TB/s; their bytes alone 1.5).  Of the 32 rows' time a third is loading and counting, then
+// Bound by a chain of latencies, not by bytes: measured 11.8 us for one row of 151936 (16
+// CTAs), 12.2 for 7 rows of 32003, 16.7 to 17.4 for 32 rows of 151936 (4 CTAs a row, 0.58
+// TB/s; their bytes alone 1.35); of these 0.2 to 0.6 for the CTA's decision after each exchange.  Of the 32 rows' time a third is loading and counting, then
 // come the exchange of what occurs, the counters and weights, and a border 1 to 1.5 us each: the
 // owner's warp, a send, and the wait of all.
 #include <mutex>
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(threads_of(C), 1) sample_kernel(const __grid_c
         if (lane >= GROUP) from = second;
       }
       double w, r;
-      // (kept from the sums: one row of 151936 11.8 us instead of 12.2, 7 of 32003 12.0 instead of 12.7; where a
+      // (kept from the sums, when it was chosen: one row of 151936 11.8 us instead of 12.2, 7 of 32003 12.0 instead of 12.7; where a
       // thread has 64 registers, made again: 32 rows 17.4 instead of 17.7)
       if constexpr (THREADS <= 512) {
         w = __shfl_sync(0xffffffffu, start[0], o), r = __shfl_sync(0xffffffffu, ratio[0], o);
@@ -782,7 +782,7 @@ int launch(Params& p, int batch, cudaStream_t st) {
 }
 
 // The largest cluster with which the whole batch runs at once (7 rows by 16 CTAs, 15 by 8, 32 by 4 on a B200 of
-// 148 SMs), else 4.  Measured at 151936 tokens, us by 16 / 8 / 4 CTAs: 1 row 12.6 / 12.7 / 15.6, 7 rows
+// 148 SMs), else 4.  Measured when it was chosen, at 151936 tokens, us by 16 / 8 / 4 CTAs: 1 row 12.6 / 12.7 / 15.6, 7 rows
 // 12.2 / 13.1 / 16.0, 8 rows 22.4 / 13.2 / 15.9, 16 rows 33 / 24 / 16.1, 64 rows 108 / 58 / 32.
 int choose(Params& p, int batch, cudaStream_t st) {
   int at16 = 0, at8 = 0, at4 = 0;
